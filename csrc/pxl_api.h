@@ -290,6 +290,28 @@ int pxl_dsa_index_prep(void* q_idx, int64_t ldq, const void* kv, int64_t ldkv, i
 int pxl_store_rows(const void* src, int64_t ld, const int64_t* slots, void* cache, int T, int D,
                    int64_t num_slots, int* status, pxl_stream_t stream);
 
+// ---- mx4.cu: microscaled 4-bit numbers. A matrix [rows, K], K % 32 == 0: codes uint8 [rows, K / 2] (e2m1, the first of a byte's two
+// in its low half; base on 16 bytes) and scales uint8 [rows, K / 32] (powers of two, bias 127, 255 = NaN).
+// Rows of x (bf16 or fp32, `ld` elements apart) -> codes and scales: the smallest power of two that keeps a group's largest value
+// within 6, the nearest number, ties to the even code.
+int pxl_mx4_quant_rows(const void* x, int is_f32, int64_t ld, void* codes, void* scales, int64_t T, int K, pxl_stream_t stream);
+// ... and back: bf16 [T, K]
+int pxl_mx4_expand_rows(const void* codes, const void* scales, void* out, int64_t T, int K, pxl_stream_t stream);
+// C[M, N] = x W^T (+ bias [N]) (+ residual), or the gated forms PXL_EPI_SILU_MUL / PXL_EPI_CLIP_GLU (N / 2 columns; N % 128 == 0, W rows
+// in groups of 64 gate and 64 up). x bf16, 16-byte rows. w: laid out in blocks of 128 x 128 (see mx4.cu), row_scale fp32 [N up to 128].
+int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
+                 const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, int* status, pxl_stream_t stream);
+// Expert-sorted rows (lists of pxl_moe_align) times E stacked weights; fp32 results with out_f32. bias [E * N].
+int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, int out_f32,
+                         const void* bias, int P, int E, int N, int K, const int* mt_expert, const int* mt_row0, const int* mt_row_end,
+                         const int* num_mt, int max_m_tiles, int epi, float limit, int* status, pxl_stream_t stream);
+// Both operands as codes and scales: C[M, N] bf16 = X W^T (+ bias) (+ residual).
+int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc, const void* bias,
+                      const void* residual, int64_t ldr, int M, int N, int K, int* status, pxl_stream_t stream);
+// pxl_moe_combine of fp32 rows
+int pxl_moe_combine_f32(const float* y, const int* pos_of, const float* w, const void* base, void* out, int T, int k, int H,
+                        pxl_stream_t stream);
+
 // ---- gemm_fp8.cu: block-scaled e4m3 GEMM (1x128 activation groups, weight scales per 64 rows x 128 cols)
 // C[M,N] bf16 = sum over 128-wide K blocks of a_s[m,kb] * w_s[n/64,kb] * (A_kb W_kb^T). K % 128 == 0,
 // N % 128 == 0. epi: PXL_EPI_NONE / PXL_EPI_RESIDUAL / PXL_EPI_SILU_MUL (W rows interleaved as for bf16).

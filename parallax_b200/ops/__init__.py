@@ -12,12 +12,14 @@ import torch
 from . import reference
 from .reference import NORM_LAYER, NORM_RMS
 from ._lib import EPI_CLIP_GLU, EPI_F32, EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, KernelError
+from .mx4 import Mx4Weight
 
 _NAMES = [
     "linear", "rmsnorm", "qk_norm_rope_cache", "reshape_and_cache", "act_mul", "gather_rows",
     "add_inplace", "patch_ids", "attn_decode", "attn_prefill", "argmax", "apply_penalties", "sample", "moe_route", "moe_ffn",
     "mla_kv_prep", "mla_q_absorb", "mla_attn", "mla_unabsorb", "mla_prefill", "store_rows", "dsa_index_prep", "dsa_index_scores", "topk_select",
-    "quant_fp8_rows", "linear_fp8", "moe_ffn_fp8", "causal_conv1d_silu", "gated_delta_rule", "sigmoid_gate_mul", "gate_mul_grouped", "row_dot", "msa_block_scores", "msa_select",
+    "quant_fp8_rows", "linear_fp8", "moe_ffn_fp8",
+    "quant_mx4_rows", "expand_mx4_rows", "linear_mx4", "linear_mx4_rows", "moe_ffn_mx4", "causal_conv1d_silu", "gated_delta_rule", "sigmoid_gate_mul", "gate_mul_grouped", "row_dot", "msa_block_scores", "msa_select",
     "embed_rows", "to_low", "residual_norm", "row_norm", "latent_prep", "head_linear", "latent_attn",
     "glu_linear", "routed_ffn", "residual_add", "conv_qkv_prep", "gated_rows", "lightning_attn",
     "latent_rows", "latent_queries", "act_linear", "tanh_norm", "residual_step", "matrix_memory",
@@ -63,5 +65,5 @@ for _n in _NAMES:
 build_cos_sin = reference.build_cos_sin
 interleave_gate_up = reference.interleave_gate_up
 
-__all__ = _NAMES + ["build_cos_sin", "interleave_gate_up", "reference", "KernelError", "NORM_LAYER", "NORM_RMS", "EPI_CLIP_GLU",
+__all__ = _NAMES + ["build_cos_sin", "interleave_gate_up", "reference", "KernelError", "Mx4Weight", "NORM_LAYER", "NORM_RMS", "EPI_CLIP_GLU",
                     "EPI_NONE", "EPI_RESIDUAL", "EPI_SILU_MUL", "EPI_F32"]

@@ -1,0 +1,166 @@
+"""Microscaled 4-bit matrices: the weights' layout, and the checks that the kernels' wrappers and the CPU forms share.
+
+A microscaled matrix ``[rows, K]`` (K a multiple of 32) is held as ``codes`` uint8 ``[rows, K / 2]``, two e2m1 numbers per byte with
+the first in the low half, and ``scales`` uint8 ``[rows, K / 32]``, a power of two (e8m0, bias 127, 255 for NaN) per 32 values of a
+row: the format of GPT-OSS's ``*_blocks`` (flattened) and ``*_scales``, which the reference hands to its GPU backends untouched
+(``src/parallax/sglang/model_runner.py:358-366``).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._lib import EPI_CLIP_GLU, EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, KernelError
+
+TILE = 128                       # rows and columns of a block of the layout
+CODE_BYTES = TILE * TILE // 2
+BLOCK_BYTES = CODE_BYTES + TILE * 4
+_SLOTS = ((15, 8, 7, 6), (12, 5, 4, 3), (9, 2, 1, 0), (14, 11, 10, 13))     # bits of sign, two of exponent, mantissa in a half word
+_CHUNK = 1 << 24                 # values that are laid out at a time
+
+
+def require(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def check_codes(codes: torch.Tensor, scales: torch.Tensor, what: str) -> tuple[int, int]:
+    """Rows and columns of a microscaled matrix."""
+    require(isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype == torch.uint8
+            and scales.dtype == torch.uint8, f"{what}: codes and scales are uint8 tensors")
+    require(codes.dim() == 2 and scales.dim() == 2 and codes.shape[0] == scales.shape[0] and codes.shape[1] == 16 * scales.shape[1]
+            and scales.shape[1] > 0, f"{what}: codes [rows, K / 2] {tuple(codes.shape)} need scales [rows, K / 32] {tuple(scales.shape)}")
+    require(codes.device == scales.device, f"{what}: codes and scales are on different devices")
+    return codes.shape[0], 2 * codes.shape[1]
+
+
+class Mx4Weight:
+    """Microscaled weights ``[experts * rows, K]`` as :func:`ops.linear_mx4` and :func:`ops.moe_ffn_mx4` read them, laid out once by
+    :meth:`pack`.
+
+    ``data``: per expert, blocks of 128 rows x 128 columns, those of a row of blocks one behind the other. A block holds its codes
+    ``[column group of 32][row][16 bytes]`` and then a byte of power per ``[row][column group]``; rows and columns are filled up to
+    a whole block with zeros. Eight neighbouring codes share a 32-bit word, the even ones in its low half, the odd ones in its high
+    half, with their bits where two at a time become bf16 with few instructions (see ``csrc/mx4.cu``).
+    ``row_scale`` fp32 ``[experts, rows filled up]``: factors of the rows, powers of two (1 where no scale of the row exceeds 128; a
+    row with a larger one is stored relative to it, and values 2^128 times smaller than the row's largest scale become 0), NaN where
+    the row has a scale of 255."""
+
+    __slots__ = ("data", "row_scale", "rows", "cols", "experts")
+
+    def __init__(self, data: torch.Tensor, row_scale: torch.Tensor, rows: int, cols: int, experts: int = 1):
+        self.data, self.row_scale, self.rows, self.cols, self.experts = data, row_scale, rows, cols, experts
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def tensors(self) -> list[torch.Tensor]:
+        return [self.data, self.row_scale]
+
+    def expert_slice(self, lo: int, hi: int) -> "Mx4Weight":
+        """Experts ``[lo, hi)``, as views of this weight."""
+        n = self.data.numel() // self.experts
+        return Mx4Weight(self.data[lo * n:hi * n], self.row_scale[lo:hi], self.rows, self.cols, hi - lo)
+
+    @classmethod
+    def pack(cls, codes: torch.Tensor, scales: torch.Tensor, experts: int = 1) -> "Mx4Weight":
+        """``codes [experts * rows, K / 2]``, ``scales [experts * rows, K / 32]`` -> laid out. Gate and up rows of a gated weight come
+        in alternating groups of 64 per expert (:func:`ops.interleave_gate_up`)."""
+        total, K = check_codes(codes, scales, "Mx4Weight.pack")
+        require(experts > 0 and total > 0 and total % experts == 0, f"Mx4Weight.pack: {total} rows do not divide by {experts} experts")
+        N = total // experts
+        dev, nt, kt = codes.device, -(-N // TILE), -(-K // TILE)
+        data = torch.empty(experts * nt * kt * BLOCK_BYTES, dtype=torch.uint8, device=dev)
+        blocks = data.view(experts, nt, kt, BLOCK_BYTES)
+        row_scale = torch.ones((experts, nt * TILE), dtype=torch.float32, device=dev)
+        codes, scales = codes.view(experts, N, K // 2), scales.view(experts, N, K // 32)
+        step = max(1, _CHUNK // (kt * TILE * TILE))
+        for e in range(experts):
+            for t0 in range(0, nt, step):
+                t1 = min(nt, t0 + step)
+                n = min(N, t1 * TILE) - t0 * TILE
+                pad = torch.nn.functional.pad
+                c = pad(codes[e, t0 * TILE:t0 * TILE + n], (0, kt * 64 - K // 2, 0, (t1 - t0) * TILE - n))
+                s = pad(scales[e, t0 * TILE:t0 * TILE + n], (0, kt * 4 - K // 32, 0, (t1 - t0) * TILE - n)).int()
+                nan = s == 255
+                over = (torch.where(nan, torch.zeros_like(s), s).amax(-1) - 128).clamp_min(0)
+                row_scale[e, t0 * TILE:t1 * TILE] = torch.where(nan.any(-1), torch.full_like(over, float("nan"), dtype=torch.float32),
+                                                                 torch.exp2(over.float()))
+                rel = s - over[:, None]
+                power = torch.where(nan, torch.full_like(s, 255), rel.clamp_min(0) + 126).to(torch.uint8)
+                halves = torch.stack([c & 15, c >> 4], -1).view(-1, kt * 4, 32)
+                halves = torch.where((rel < 0)[..., None], torch.zeros_like(halves), halves)
+                v = halves.view(t1 - t0, TILE, kt, 4, 4, 4, 2).int()       # [.., block, group, word, slot, half]
+                word = torch.zeros(v.shape[:-2] + (2,), dtype=torch.int32, device=dev)
+                for i, bits in enumerate(_SLOTS):
+                    for j, b in enumerate(bits):
+                        word |= ((v[..., i, :] >> (3 - j)) & 1) << b
+                by = torch.stack([word & 255, word >> 8], -1).to(torch.uint8)                  # [.., block, group, word, half, byte]
+                out = blocks[e, t0:t1]
+                out[..., :CODE_BYTES] = by.reshape(t1 - t0, TILE, kt, 4, 16).permute(0, 2, 3, 1, 4).reshape(t1 - t0, kt, CODE_BYTES)
+                out[..., CODE_BYTES:] = power.view(t1 - t0, TILE, kt, 4).permute(0, 2, 1, 3).reshape(t1 - t0, kt, TILE * 4)
+        return cls(data, row_scale, N, K, experts)
+
+    def unpack(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The codes and scales that :meth:`pack` was given (``[experts * rows, ...]``)."""
+        E, N, K = self.experts, self.rows, self.cols
+        nt, kt = -(-N // TILE), -(-K // TILE)
+        blocks = self.data.view(E, nt, kt, BLOCK_BYTES)
+        by = blocks[..., :CODE_BYTES].reshape(E, nt, kt, 4, TILE, 4, 2, 2).int()               # [.., group, row, word, half, byte]
+        word = by[..., 0] | (by[..., 1] << 8)
+        v = torch.stack([sum(((word >> b) & 1) << (3 - j) for j, b in enumerate(bits)) for bits in _SLOTS], -2)   # [.., word, slot, half]
+        c = (v[..., 0] | (v[..., 1] << 4)).to(torch.uint8).reshape(E, nt, kt, 4, TILE, 16)
+        c = c.permute(0, 1, 4, 2, 3, 5).reshape(E, nt * TILE, kt * 64)[:, :N, :K // 2]
+        power = blocks[..., CODE_BYTES:].reshape(E, nt, kt, TILE, 4).permute(0, 1, 3, 2, 4).reshape(E, nt * TILE, kt * 4)
+        over = torch.log2(torch.nan_to_num(self.row_scale, nan=1.0)).int()[..., None]
+        s = torch.where(power == 255, torch.full_like(power, 255).int(), power.int() - 126 + over)[:, :N, :K // 32]
+        return c.reshape(E * N, K // 2).contiguous(), s.to(torch.uint8).reshape(E * N, K // 32).contiguous()
+
+
+def check_rows(x: torch.Tensor, what: str) -> tuple[int, int]:
+    require(x.dim() == 2 and x.shape[1] > 0 and x.shape[1] % 32 == 0, f"{what}: rows [T, K] with K a multiple of 32, got {tuple(x.shape)}")
+    require(x.dtype in (torch.bfloat16, torch.float32), f"{what}: rows are bf16 or fp32, got {x.dtype}")
+    return x.shape[0], x.shape[1]
+
+
+def check_product(what: str, device: torch.device, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
+                  residual: Optional[torch.Tensor], epi: int, limit: float, out: Optional[torch.Tensor], dtype: torch.dtype) -> int:
+    """Checks what the two products share; returns the number of output columns."""
+    require(K == K_w, f"{what}: rows of {K} columns and weights of {K_w}")
+    require(epi in (EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_CLIP_GLU), f"{what}: unknown epilogue {epi}")
+    glu = epi in (EPI_SILU_MUL, EPI_CLIP_GLU)
+    require(not glu or N % TILE == 0, f"{what}: a gated product needs gate and up rows in groups of 64, got {N} rows")
+    require(epi != EPI_CLIP_GLU or limit > 0, f"{what}: a clipped gate needs limit > 0")
+    require(not (glu and residual is not None), f"{what}: a gated product has no residual")
+    require((epi == EPI_RESIDUAL) <= (residual is not None), f"{what}: EPI_RESIDUAL needs a residual")
+    n_out = N // 2 if glu else N
+    for t, name, shape in ((bias, "bias", (N,)), (residual, "residual", (T, n_out)), (out, "out", (T, n_out))):
+        require(t is None or (tuple(t.shape) == shape and t.dtype == dtype and t.device == device and t.stride(-1) == 1),
+                f"{what}: {name} is {dtype} {shape} on {device} with neighbouring columns")
+    return n_out
+
+
+def check_experts(what: str, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: Mx4Weight, w2: Mx4Weight,
+                  base: Optional[torch.Tensor], act_mode: int, limit: float, b1: Optional[torch.Tensor],
+                  b2: Optional[torch.Tensor]) -> None:
+    T, K = check_rows(x, what)
+    dev = x.device
+    require(ids.dim() == 2 and ids.shape[0] == T and ids.dtype == torch.int32 and ids.is_contiguous() and ids.device == dev
+            and ids.shape[1] > 0, f"{what}: ids are int32 [T, k]")
+    require(weights.shape == ids.shape and weights.dtype == torch.float32 and weights.is_contiguous() and weights.device == dev,
+            f"{what}: weights are fp32 of the shape of ids")
+    require(isinstance(w1, Mx4Weight) and isinstance(w2, Mx4Weight) and w1.experts == w2.experts and w1.device == dev
+            and w2.device == dev, f"{what}: w1 and w2 are Mx4Weights of the same experts on the rows' device")
+    require(w1.experts <= 1024, f"{what}: {w1.experts} experts, at most 1024")
+    require(w1.cols == K and w1.rows == 2 * w2.cols and w2.rows == K and w1.rows % TILE == 0,
+            f"{what}: w1 [2 I, K] and w2 [K, I] with I a multiple of 64, got [{w1.rows}, {w1.cols}] and [{w2.rows}, {w2.cols}] for rows of {K}")
+    require(act_mode in (0, 1), f"{what}: act_mode is 0 (SiLU) or 1 (clipped GLU)")
+    require(act_mode == 0 or limit > 0, f"{what}: a clipped gate needs limit > 0")
+    for t, name, n in ((b1, "b1", w1.rows), (b2, "b2", w2.rows)):
+        require(t is None or (t.numel() == n * w1.experts and t.is_contiguous() and t.dtype == x.dtype and t.device == dev),
+                f"{what}: {name} is {x.dtype} [{w1.experts} * {n}]")
+    require(base is None or (base.shape == x.shape and base.dtype == x.dtype and base.device == dev and base.is_contiguous()),
+            f"{what}: base has the rows' shape and type")

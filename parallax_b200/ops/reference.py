@@ -15,6 +15,8 @@ import math
 
 import torch
 
+from . import mx4
+
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_F32 = 0, 1, 2, 3
 EPI_CLIP_GLU = 10
 
@@ -544,6 +546,95 @@ def moe_ffn_fp8(x, ids, weights, w1q, w1s, w2q, w2s, num_experts: int, base=None
         a = linear_fp8(x[tok], w1q[e * n1:(e + 1) * n1], w1s[e * n1 // 64:(e + 1) * n1 // 64], epi=EPI_SILU_MUL)
         y = linear_fp8(a, w2q[e * n2:(e + 1) * n2], w2s[e * n2 // 64:(e + 1) * n2 // 64])
         out.index_add_(0, tok, y.float() * weights[tok, slot].float()[:, None])
+    return out.to(x.dtype)
+
+
+# ---------------------------------------------------------------------------- microscaled 4 bits
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _mx4_values(codes, scales):
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=codes.device)
+    v = table[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()].unflatten(-1, (-1, 32))
+    power = torch.ldexp(torch.ones_like(scales, dtype=torch.float32), scales.int() - 127)
+    return (v * power.masked_fill(scales == 255, float("nan")).unsqueeze(-1)).flatten(-2)
+
+
+def quant_mx4_rows(x):
+    """Rows ``[T, K]`` (bf16 or fp32, K % 32 == 0) -> microscaled ``(codes uint8 [T, K / 2], scales uint8 [T, K / 32])``: per 32 values
+    the smallest power of two that keeps the largest within 6, then the nearest e2m1 number (ties to the even code). A group with a
+    NaN or an infinity becomes NaN (scale 255)."""
+    mx4.check_rows(x, "quant_mx4_rows")
+    g = x.float().unflatten(-1, (-1, 32))
+    most = g.abs().amax(-1)
+    part, power = torch.frexp(most)
+    e = torch.where(part <= 0.75, power - 3, power - 2).clamp(-127, 127)
+    e = torch.where(most == 0, torch.full_like(e, -127), e)
+    bad = ~torch.isfinite(most)
+    q = torch.ldexp(g, -e.masked_fill(bad, 0).unsqueeze(-1))
+    a = q.abs()
+    c = sum((a > b if i % 2 == 0 else a >= b).to(torch.uint8) for i, b in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
+    c = (c + 8 * torch.signbit(q).to(torch.uint8)).masked_fill(bad.unsqueeze(-1), 0).flatten(-2)
+    return c[..., 0::2] | (c[..., 1::2] << 4), (e + 127).masked_fill(bad, 255).to(torch.uint8)
+
+
+def expand_mx4_rows(codes, scales):
+    """The values of a microscaled matrix in bf16 (exact, but for those beyond the largest bf16 number)."""
+    mx4.check_codes(codes, scales, "expand_mx4_rows")
+    return _mx4_values(codes, scales).to(torch.bfloat16)
+
+
+def _mx4_product(x, wv, bias, residual, epi, limit, out, dtype):
+    y = x @ wv.t()
+    if bias is not None:
+        y = y + bias.float()
+    if residual is not None:
+        y = y + residual.float()
+    if epi in (EPI_SILU_MUL, EPI_CLIP_GLU):
+        g, u = y.unflatten(-1, (-1, 2, 64)).unbind(-2)
+        y = act_mul(torch.cat([g.flatten(-2), u.flatten(-2)], -1), int(epi == EPI_CLIP_GLU), limit)
+    if out is not None:
+        out.copy_(y)
+        return out
+    return y.to(dtype)
+
+
+def linear_mx4(x, w, bias=None, residual=None, epi: int = EPI_NONE, limit: float = 0.0, out=None):
+    """``x [T, K] @ W^T`` with a microscaled weight (:class:`ops.Mx4Weight`, one expert): plain, with a bias, with a residual, or
+    gated (``EPI_SILU_MUL``, ``EPI_CLIP_GLU`` with ``limit``; gate / up rows in groups of 64). Rows are bf16 (on CPU fp32 too)."""
+    T, K = mx4.check_rows(x, "linear_mx4")
+    mx4.require(isinstance(w, mx4.Mx4Weight) and w.experts == 1 and w.device == x.device,
+                "linear_mx4: w is an Mx4Weight of one expert on the rows' device")
+    mx4.check_product("linear_mx4", x.device, T, w.rows, K, w.cols, bias, residual, epi, limit, out, x.dtype)
+    return _mx4_product(x.float(), _mx4_values(*w.unpack()), bias, residual, epi, limit, out, x.dtype)
+
+
+def linear_mx4_rows(codes, scales, w_codes, w_scales, bias=None, residual=None, out=None):
+    """Product of microscaled rows ``[T, K]`` and a microscaled weight ``[N, K]``, both as codes and scales, with an optional bias and
+    residual; bf16 ``[T, N]``."""
+    T, K = mx4.check_codes(codes, scales, "linear_mx4_rows: rows")
+    N, K_w = mx4.check_codes(w_codes, w_scales, "linear_mx4_rows: weights")
+    mx4.require(w_codes.device == codes.device, "linear_mx4_rows: rows and weights are on different devices")
+    mx4.check_product("linear_mx4_rows", codes.device, T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
+    return _mx4_product(_mx4_values(codes, scales), _mx4_values(w_codes, w_scales), bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
+
+
+def moe_ffn_mx4(x, ids, weights, w1, w2, base=None, act_mode: int = 0, limit: float = 7.0, b1=None, b2=None):
+    """:func:`moe_ffn` with microscaled expert matrices (:class:`ops.Mx4Weight`): ``w1`` per expert ``[2 I, K]`` with gate / up rows in
+    groups of 64 in either ``act_mode`` (0: SiLU, 1: clipped GLU with ``limit``), ``b1`` in the order of its rows, ``w2 [K, I]``. A
+    token's experts are added up in fp32. Ids outside of the experts add nothing."""
+    mx4.check_experts("moe_ffn_mx4", x, ids, weights, w1, w2, base, act_mode, limit, b1, b2)
+    E = w1.experts
+    out = torch.zeros(x.shape, dtype=torch.float32, device=x.device) if base is None else base.float().clone()
+    for e in range(E):
+        tok, slot = (ids == e).nonzero(as_tuple=True)
+        if tok.numel() == 0:
+            continue
+        a = linear_mx4(x[tok], w1.expert_slice(e, e + 1), bias=None if b1 is None else b1.view(E, -1)[e],
+                       epi=EPI_CLIP_GLU if act_mode else EPI_SILU_MUL, limit=limit)
+        y = _mx4_product(a.float(), _mx4_values(*w2.expert_slice(e, e + 1).unpack()), None if b2 is None else b2.view(E, -1)[e], None,
+                         EPI_NONE, 0.0, None, torch.float32)
+        out.index_add_(0, tok, y * weights[tok, slot][:, None])
     return out.to(x.dtype)
 
 
