@@ -8,6 +8,7 @@
 #include <cuda_fp4.h>
 
 #include "common.cuh"
+#include "mx4.cuh"
 #include "pxl_api.h"
 
 namespace {
@@ -104,85 +105,29 @@ __global__ void __launch_bounds__(256) mx4_expand_rows_kernel(const uint8_t* __r
 }
 
 // ---------------------------------------------------------------------------- products
-// Weights of pxl_gemm_mx4 are laid out once, in blocks of 128 rows x 128 columns that lie one behind the other along a row of
-// blocks: 8192 bytes of codes [column group of 32][row][16 bytes], then 512 bytes of powers [row][column group]. Rows and columns
-// are filled up to a whole block with zeros. Within a word of eight codes the bits are placed so that two numbers at a time become
-// bf16 with few instructions: the even numbers' bits are in the low half of the word, the odd ones' in the high half, and
-//
-//   number of the half   0           1           2          3
-//   sign at bit          15          12          9          14
-//   magnitude at bits    8 .. 6      5 .. 3      2 .. 0     11, 10 and 13
-//
-// A sign at bit 15 and a magnitude at 8 .. 6 is the bf16 of the number times 2^-126 (1/2 is a subnormal there), and one product
-// with a power of two makes it the value: exact. The stored power is the exponent field of 2^(scale - 1), for scales up to 128; the
-// rows' factors hold what a row with a larger scale exceeds that by, and NaN for a row with a scale of 255.
-constexpr int kTileRows = 128, kTileCols = 128;
-constexpr int kCodeBytes = kTileRows * kTileCols / 2, kBlockBytes = kCodeBytes + kTileRows * 4;
-
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// eight codes as placed above, and the power's exponent field in both halves -> eight values in bf16
-__device__ __forceinline__ void mx4_word(uint32_t w, uint32_t power2, uint32_t (&o)[4]) {
-  o[0] = mul_bf16x2(w & 0x81c081c0u, power2);
-  o[1] = mul_bf16x2((w << 3) & 0x81c081c0u, power2);
-  o[2] = mul_bf16x2((w << 6) & 0x81c081c0u, power2);
-  o[3] = mul_bf16x2(((w << 1) & 0x80008000u) | ((w >> 3) & 0x01800180u) | ((w >> 7) & 0x00400040u), power2);
-}
-__device__ __forceinline__ uint32_t mx4_power2(uint32_t field) { return field << 7 | field << 23; }
-
 struct Mx4Args {
-  const void* x;          // bf16 [*, K], or codes
-  const uint8_t* x_s;     // scales of the rows, where they are codes
-  const uint8_t* w;       // blocks as above, or codes [N, K / 2]
-  const uint8_t* w_s;     // scales of the weights, where they are plain codes
-  const float* row_scale; // [experts, N rounded up to 128]
-  void* C;
+  const uint8_t* x;       // codes and scales of the rows
+  const uint8_t* x_s;
+  const uint8_t* w;       // and of the weights
+  const uint8_t* w_s;
+  bf16* C;
   const bf16* bias;
   const bf16* residual;
-  int64_t ldx, ldc, ldr;
-  int M, N, K, epi, out_f32;
-  float limit;
-  // grouped: lists of 128-row tiles of x, each with its expert
-  const int* mt_expert;
-  const int* mt_row0;
-  const int* mt_row_end;
-  const int* num_mt;
+  int64_t ldc, ldr;
+  int M, N, K;
 };
-
-__device__ __forceinline__ float mx4_gate(float g, float u, int epi, float limit) {
-  float s = g;
-  if (epi == PXL_EPI_CLIP_GLU) {
-    g = g > limit ? limit : g;
-    u = u < -limit ? -limit : u > limit ? limit : u;
-    s = 1.702f * g;
-    u += 1.f;
-  }
-  return g * __frcp_rn(1.f + __expf(-s)) * u;
-}
 
 constexpr int kSimpleRows = 16;
 
 // A block of 128 weight rows times 16 rows of x on the FMA pipes.
-template <bool PLAIN>
 __global__ void __launch_bounds__(256) mx4_gemm_kernel(const Mx4Args g) {
   __shared__ float xs[kSimpleRows][kTileCols];
   __shared__ float part[kSimpleRows][kTileRows + 1];
   pdl_wait();
   pdl_launch_dependents();
   const int n_blk = blockIdx.x, r = threadIdx.x & 127, half = threadIdx.x >> 7;
-  int row0 = blockIdx.y * kSimpleRows, row_end = g.M, expert = 0;
-  if (g.num_mt != nullptr) {
-    const int mt = blockIdx.y / (128 / kSimpleRows);
-    if (mt >= *g.num_mt) return;
-    expert = g.mt_expert[mt];
-    row0 = g.mt_row0[mt] + blockIdx.y % (128 / kSimpleRows) * kSimpleRows;
-    row_end = min(g.mt_row_end[mt], g.mt_row0[mt] + 128);
-  }
-  if (row0 >= row_end) return;
-  const int n = n_blk * kTileRows + r, n_blocks = ceil_div(g.N, kTileRows), k_blocks = ceil_div(g.K, kTileCols);
+  const int row0 = blockIdx.y * kSimpleRows, row_end = g.M;
+  const int n = n_blk * kTileRows + r, k_blocks = ceil_div(g.K, kTileCols);
   float acc[kSimpleRows] = {};
   for (int kb = 0; kb < k_blocks; ++kb) {
     __syncthreads();
@@ -190,45 +135,22 @@ __global__ void __launch_bounds__(256) mx4_gemm_kernel(const Mx4Args g) {
       const int t = row0 + i / kTileCols, k = kb * kTileCols + i % kTileCols;
       float v = 0.f;
       if (t < row_end && k < g.K) {
-        if constexpr (PLAIN) {
-          const int64_t at = static_cast<int64_t>(t) * g.K + k;
-          const float2 f = mx4_pair(static_cast<const uint8_t*>(g.x)[at >> 1]);
-          v = (k & 1 ? f.y : f.x) * mx4_power(g.x_s[at >> 5]);
-        } else {
-          v = __bfloat162float(static_cast<const bf16*>(g.x)[t * g.ldx + k]);
-        }
+        const int64_t at = static_cast<int64_t>(t) * g.K + k;
+        const float2 f = mx4_pair(g.x[at >> 1]);
+        v = (k & 1 ? f.y : f.x) * mx4_power(g.x_s[at >> 5]);
       }
       xs[i / kTileCols][i % kTileCols] = v;
     }
     __syncthreads();
     for (int b = half * 2; b < half * 2 + 2; ++b) {
       const int k0 = kb * kTileCols + b * 32;
-      if (k0 >= g.K) break;
+      if (k0 >= g.K || n >= g.N) break;
       float wv[32];
-      if constexpr (PLAIN) {
-        if (n >= g.N) break;
-        const int64_t at = (static_cast<int64_t>(n) * g.K + k0) >> 5;
-        const float p = mx4_power(g.w_s[at]);
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = mx4_pair(g.w[at * 16 + j]);
-          wv[2 * j] = f.x * p, wv[2 * j + 1] = f.y * p;
-        }
-      } else {
-        const uint8_t* blk = g.w + (static_cast<int64_t>(expert) * n_blocks + n_blk) * k_blocks * kBlockBytes +
-                             static_cast<int64_t>(kb) * kBlockBytes;
-        const uint32_t p2 = mx4_power2(blk[kCodeBytes + r * 4 + b]);
-        const uint4 c = *reinterpret_cast<const uint4*>(blk + (b * kTileRows + r) * 16);
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t o[4];
-          mx4_word(w[j], p2, o);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack_bf16x2(o[i]);
-            wv[8 * j + 2 * i] = f.x, wv[8 * j + 2 * i + 1] = f.y;
-          }
-        }
+      const int64_t at = (static_cast<int64_t>(n) * g.K + k0) >> 5;
+      const float p = mx4_power(g.w_s[at]);
+      for (int j = 0; j < 16; ++j) {
+        const float2 f = mx4_pair(g.w[at * 16 + j]);
+        wv[2 * j] = f.x * p, wv[2 * j + 1] = f.y * p;
       }
 #pragma unroll
       for (int t = 0; t < kSimpleRows; ++t)
@@ -243,22 +165,13 @@ __global__ void __launch_bounds__(256) mx4_gemm_kernel(const Mx4Args g) {
   if (half == 1)
     for (int t = 0; t < kSimpleRows; ++t) part[t][r] += acc[t];
   __syncthreads();
-  const bool glu = g.epi == PXL_EPI_SILU_MUL || g.epi == PXL_EPI_CLIP_GLU;
-  const int cols = glu ? 64 : 128;
-  for (int i = threadIdx.x; i < kSimpleRows * cols; i += 256) {
-    const int t = row0 + i / cols, c = i % cols, n_out = n_blk * cols + c;
-    if (t >= row_end || n_out >= (glu ? g.N / 2 : g.N)) continue;
-    float f[2];
-    for (int v = 0; v < (glu ? 2 : 1); ++v) {
-      const int nn = n_blk * 128 + c + 64 * v;
-      f[v] = part[i / cols][c + 64 * v];
-      if (g.row_scale) f[v] *= g.row_scale[expert * n_blocks * 128 + nn];
-      if (g.bias) f[v] += __bfloat162float(g.bias[expert * g.N + nn]);
-    }
-    float y = glu ? mx4_gate(f[0], f[1], g.epi, g.limit) : f[0];
+  for (int i = threadIdx.x; i < kSimpleRows * 128; i += 256) {
+    const int t = row0 + i / 128, n_out = n_blk * 128 + i % 128;
+    if (t >= row_end || n_out >= g.N) continue;
+    float y = part[i / 128][i % 128];
+    if (g.bias) y += __bfloat162float(g.bias[n_out]);
     if (g.residual) y += __bfloat162float(g.residual[t * g.ldr + n_out]);
-    if (g.out_f32) static_cast<float*>(g.C)[t * g.ldc + n_out] = y;
-    else static_cast<bf16*>(g.C)[t * g.ldc + n_out] = __float2bfloat16(y);
+    g.C[t * g.ldc + n_out] = __float2bfloat16(y);
   }
 }
 
@@ -285,10 +198,6 @@ __global__ void __launch_bounds__(256) moe_combine_f32_kernel(const float* __res
     }
     *reinterpret_cast<uint2*>(out + t * H + c) = make_uint2(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]));
   }
-}
-
-bool epi_known(int epi, int N) {
-  return epi == PXL_EPI_NONE || ((epi == PXL_EPI_SILU_MUL || epi == PXL_EPI_CLIP_GLU) && N % 128 == 0);
 }
 
 }  // namespace
@@ -320,40 +229,16 @@ PXL_EXPORT int pxl_mx4_expand_rows(const void* codes, const void* scales, void* 
   return check_launch();
 }
 
-PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc,
-                            const void* bias, const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit,
-                            int* status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || K % 32 || !epi_known(epi, N)) return PXL_ERR_INVALID_ARG;
-  Mx4Args g{};
-  g.x = x, g.ldx = ldx, g.w = static_cast<const uint8_t*>(w), g.row_scale = row_scale, g.C = C, g.ldc = ldc;
-  g.bias = static_cast<const bf16*>(bias), g.residual = static_cast<const bf16*>(residual), g.ldr = ldr;
-  g.M = M, g.N = N, g.K = K, g.epi = epi, g.limit = limit;
-  pxl_host::launch(mx4_gemm_kernel<false>, dim3(pxl::ceil_div(N, 128), pxl::ceil_div(M, kSimpleRows)), 256, 0, stream, g);
-  return check_launch();
-}
-
-PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc,
-                                    int out_f32, const void* bias, int P, int E, int N, int K, const int* mt_expert,
-                                    const int* mt_row0, const int* mt_row_end, const int* num_mt, int max_m_tiles, int epi,
-                                    float limit, int* status, cudaStream_t stream) {
-  if (P <= 0 || E <= 0 || N <= 0 || K <= 0 || K % 32 || max_m_tiles <= 0 || !epi_known(epi, N)) return PXL_ERR_INVALID_ARG;
-  Mx4Args g{};
-  g.x = x, g.ldx = ldx, g.w = static_cast<const uint8_t*>(w), g.row_scale = row_scale, g.C = C, g.ldc = ldc, g.out_f32 = out_f32;
-  g.bias = static_cast<const bf16*>(bias), g.M = P, g.N = N, g.K = K, g.epi = epi, g.limit = limit;
-  g.mt_expert = mt_expert, g.mt_row0 = mt_row0, g.mt_row_end = mt_row_end, g.num_mt = num_mt;
-  pxl_host::launch(mx4_gemm_kernel<false>, dim3(pxl::ceil_div(N, 128), max_m_tiles * (128 / kSimpleRows)), 256, 0, stream, g);
-  return check_launch();
-}
-
 PXL_EXPORT int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc,
                                  const void* bias, const void* residual, int64_t ldr, int M, int N, int K, int* status,
                                  cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32) return PXL_ERR_INVALID_ARG;
   Mx4Args g{};
-  g.x = xc, g.x_s = static_cast<const uint8_t*>(xs), g.w = static_cast<const uint8_t*>(wc), g.w_s = static_cast<const uint8_t*>(ws);
-  g.C = C, g.ldc = ldc, g.bias = static_cast<const bf16*>(bias), g.residual = static_cast<const bf16*>(residual), g.ldr = ldr;
+  g.x = static_cast<const uint8_t*>(xc), g.x_s = static_cast<const uint8_t*>(xs);
+  g.w = static_cast<const uint8_t*>(wc), g.w_s = static_cast<const uint8_t*>(ws);
+  g.C = static_cast<bf16*>(C), g.ldc = ldc, g.bias = static_cast<const bf16*>(bias), g.residual = static_cast<const bf16*>(residual), g.ldr = ldr;
   g.M = M, g.N = N, g.K = K;
-  pxl_host::launch(mx4_gemm_kernel<true>, dim3(pxl::ceil_div(N, 128), pxl::ceil_div(M, kSimpleRows)), 256, 0, stream, g);
+  pxl_host::launch(mx4_gemm_kernel, dim3(pxl::ceil_div(N, 128), pxl::ceil_div(M, kSimpleRows)), 256, 0, stream, g);
   return check_launch();
 }
 

@@ -297,14 +297,16 @@ int pxl_store_rows(const void* src, int64_t ld, const int64_t* slots, void* cach
 int pxl_mx4_quant_rows(const void* x, int is_f32, int64_t ld, void* codes, void* scales, int64_t T, int K, pxl_stream_t stream);
 // ... and back: bf16 [T, K]
 int pxl_mx4_expand_rows(const void* codes, const void* scales, void* out, int64_t T, int K, pxl_stream_t stream);
-// C[M, N] = x W^T (+ bias [N]) (+ residual), or the gated forms PXL_EPI_SILU_MUL / PXL_EPI_CLIP_GLU (N / 2 columns; N % 128 == 0, W rows
-// in groups of 64 gate and 64 up). x bf16, 16-byte rows. w: laid out in blocks of 128 x 128 (see mx4.cu), row_scale fp32 [N up to 128].
+// gemm_mx4.cu: C[M, N] = x W^T (+ bias [N]) (+ residual), or the gated forms PXL_EPI_SILU_MUL / PXL_EPI_CLIP_GLU (N / 2 columns;
+// N % 128 == 0, W rows in groups of 64 gate and 64 up). x bf16, base and rows on 16 bytes. w: laid out in blocks of 128 x 128 (see
+// mx4.cuh), row_scale fp32 [N up to 128].
 int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
                  const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, int* status, pxl_stream_t stream);
-// Expert-sorted rows (lists of pxl_moe_align) times E stacked weights; fp32 results with out_f32. bias [E * N].
+// Expert-sorted rows (those of expert e are offsets[e] .. offsets[e + 1], of P at most) times E stacked weights; fp32 results with
+// out_f32. bias [E * N], E <= 1024.
 int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, int out_f32,
-                         const void* bias, int P, int E, int N, int K, const int* mt_expert, const int* mt_row0, const int* mt_row_end,
-                         const int* num_mt, int max_m_tiles, int epi, float limit, int* status, pxl_stream_t stream);
+                         const void* bias, int P, int E, int N, int K, const int* offsets, int epi, float limit, int* status,
+                         pxl_stream_t stream);
 // Both operands as codes and scales: C[M, N] bf16 = X W^T (+ bias) (+ residual).
 int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc, const void* bias,
                       const void* residual, int64_t ldr, int M, int N, int K, int* status, pxl_stream_t stream);

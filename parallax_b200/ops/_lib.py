@@ -113,8 +113,7 @@ _SIGS = {
     "pxl_mx4_quant_rows": [_P, c_int, c_int64, _P, _P, c_int64, c_int, _P],
     "pxl_mx4_expand_rows": [_P, _P, _P, c_int64, c_int, _P],
     "pxl_gemm_mx4": [_P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P],
-    "pxl_gemm_mx4_grouped": [_P, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int,
-                             c_float, _P, _P],
+    "pxl_gemm_mx4_grouped": [_P, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, _P, _P],
     "pxl_gemm_mx4_rows": [_P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, _P, _P],
     "pxl_moe_combine_f32": [_P, _P, _P, _P, _P, c_int, c_int, c_int, _P],
     "pxl_causal_conv1d_silu": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, _P],

@@ -1141,10 +1141,9 @@ def _grouped_mx4(a, w: Mx4Weight, plan: MoEPlan, epi: int, bias, limit: float, d
     n_out = w.rows // 2 if epi != EPI_NONE else w.rows
     out = torch.empty((plan.max_rows, n_out), dtype=dtype, device=a.device)
     check(_lib.lib().pxl_gemm_mx4_grouped(a.data_ptr(), a.stride(0), w.data.data_ptr(), w.row_scale.data_ptr(), out.data_ptr(), n_out,
-                                          int(dtype == torch.float32), _ptr(bias), a.shape[0], w.experts, w.rows, w.cols,
-                                          plan.mt_expert.data_ptr(), plan.mt_row0.data_ptr(), plan.mt_row_end.data_ptr(),
-                                          plan.num_mt.data_ptr(), plan.max_mt, epi, limit, status_tensor(a.device).data_ptr(),
-                                          _stream(a.device)), "pxl_gemm_mx4_grouped")
+                                          int(dtype == torch.float32), _ptr(bias), plan.max_rows, w.experts, w.rows, w.cols,
+                                          plan.offsets.data_ptr(), epi, limit, status_tensor(a.device).data_ptr(), _stream(a.device)),
+          "pxl_gemm_mx4_grouped")
     _count()
     return out
 
