@@ -8,7 +8,6 @@
 #include <cuda_fp4.h>
 
 #include "common.cuh"
-#include "mx4.cuh"
 #include "pxl_api.h"
 
 namespace {
@@ -104,77 +103,7 @@ __global__ void __launch_bounds__(256) mx4_expand_rows_kernel(const uint8_t* __r
   st_bf16x8(out + i * 8, o);
 }
 
-// ---------------------------------------------------------------------------- products
-struct Mx4Args {
-  const uint8_t* x;       // codes and scales of the rows
-  const uint8_t* x_s;
-  const uint8_t* w;       // and of the weights
-  const uint8_t* w_s;
-  bf16* C;
-  const bf16* bias;
-  const bf16* residual;
-  int64_t ldc, ldr;
-  int M, N, K;
-};
-
-constexpr int kSimpleRows = 16;
-
-// A block of 128 weight rows times 16 rows of x on the FMA pipes.
-__global__ void __launch_bounds__(256) mx4_gemm_kernel(const Mx4Args g) {
-  __shared__ float xs[kSimpleRows][kTileCols];
-  __shared__ float part[kSimpleRows][kTileRows + 1];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int n_blk = blockIdx.x, r = threadIdx.x & 127, half = threadIdx.x >> 7;
-  const int row0 = blockIdx.y * kSimpleRows, row_end = g.M;
-  const int n = n_blk * kTileRows + r, k_blocks = ceil_div(g.K, kTileCols);
-  float acc[kSimpleRows] = {};
-  for (int kb = 0; kb < k_blocks; ++kb) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSimpleRows * kTileCols; i += 256) {
-      const int t = row0 + i / kTileCols, k = kb * kTileCols + i % kTileCols;
-      float v = 0.f;
-      if (t < row_end && k < g.K) {
-        const int64_t at = static_cast<int64_t>(t) * g.K + k;
-        const float2 f = mx4_pair(g.x[at >> 1]);
-        v = (k & 1 ? f.y : f.x) * mx4_power(g.x_s[at >> 5]);
-      }
-      xs[i / kTileCols][i % kTileCols] = v;
-    }
-    __syncthreads();
-    for (int b = half * 2; b < half * 2 + 2; ++b) {
-      const int k0 = kb * kTileCols + b * 32;
-      if (k0 >= g.K || n >= g.N) break;
-      float wv[32];
-      const int64_t at = (static_cast<int64_t>(n) * g.K + k0) >> 5;
-      const float p = mx4_power(g.w_s[at]);
-      for (int j = 0; j < 16; ++j) {
-        const float2 f = mx4_pair(g.w[at * 16 + j]);
-        wv[2 * j] = f.x * p, wv[2 * j + 1] = f.y * p;
-      }
-#pragma unroll
-      for (int t = 0; t < kSimpleRows; ++t)
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[t] += wv[j] * xs[t][b * 32 + j];
-    }
-  }
-  __syncthreads();
-  if (half == 0)
-    for (int t = 0; t < kSimpleRows; ++t) part[t][r] = acc[t];
-  __syncthreads();
-  if (half == 1)
-    for (int t = 0; t < kSimpleRows; ++t) part[t][r] += acc[t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kSimpleRows * 128; i += 256) {
-    const int t = row0 + i / 128, n_out = n_blk * 128 + i % 128;
-    if (t >= row_end || n_out >= g.N) continue;
-    float y = part[i / 128][i % 128];
-    if (g.bias) y += __bfloat162float(g.bias[n_out]);
-    if (g.residual) y += __bfloat162float(g.residual[t * g.ldr + n_out]);
-    g.C[t * g.ldc + n_out] = __float2bfloat16(y);
-  }
-}
-
+// ---------------------------------------------------------------------------- experts' rows
 // out[t] = base[t] + sum_j w[t, j] y[pos_of[t, j]]: the experts' rows in fp32, so that a token's sum is rounded once.
 __global__ void __launch_bounds__(256) moe_combine_f32_kernel(const float* __restrict__ y, const int* __restrict__ pos_of,
                                                               const float* __restrict__ w, const bf16* __restrict__ base,
@@ -226,19 +155,6 @@ PXL_EXPORT int pxl_mx4_expand_rows(const void* codes, const void* scales, void* 
   if (blocks > 0x7fffffff) return PXL_ERR_TOO_LARGE;
   pxl_host::launch(mx4_expand_rows_kernel, static_cast<unsigned>(blocks), 256, 0, stream, static_cast<const uint8_t*>(codes),
                    static_cast<const uint8_t*>(scales), static_cast<bf16*>(out), words);
-  return check_launch();
-}
-
-PXL_EXPORT int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc,
-                                 const void* bias, const void* residual, int64_t ldr, int M, int N, int K, int* status,
-                                 cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || K % 32) return PXL_ERR_INVALID_ARG;
-  Mx4Args g{};
-  g.x = static_cast<const uint8_t*>(xc), g.x_s = static_cast<const uint8_t*>(xs);
-  g.w = static_cast<const uint8_t*>(wc), g.w_s = static_cast<const uint8_t*>(ws);
-  g.C = static_cast<bf16*>(C), g.ldc = ldc, g.bias = static_cast<const bf16*>(bias), g.residual = static_cast<const bf16*>(residual), g.ldr = ldr;
-  g.M = M, g.N = N, g.K = K;
-  pxl_host::launch(mx4_gemm_kernel, dim3(pxl::ceil_div(N, 128), pxl::ceil_div(M, kSimpleRows)), 256, 0, stream, g);
   return check_launch();
 }
 

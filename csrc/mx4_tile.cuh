@@ -1,0 +1,238 @@
+// Output tiles of the products with microscaled weights: 128 weight rows (lanes of the accumulator) by up to 256 rows of x, called
+// tokens here (its columns). What a launch's work items are, and how their results leave tensor memory.
+#pragma once
+
+#include "mx4.cuh"
+#include "tc_issue.cuh"
+
+namespace pxl {
+
+constexpr int kPitch = kTileRows + 4;  // floats of a token's results in shared memory
+constexpr int kChunk = 32;             // tokens whose results are staged at a time
+constexpr int kStaging = kChunk * kPitch * 4;
+
+struct TileArgs {
+  void* C;
+  const float* row_scale;  // [experts, N rounded up to 128], or none
+  const bf16* bias;
+  const bf16* residual;
+  int64_t ldc, ldr;
+  int M, N, epi, out_f32;
+  float limit;
+  int n_blocks, k_blocks, t_tiles;
+  int bt;                  // tokens of a tile, a multiple of 16
+  int stages, d_bufs, d_cols;
+  int splits, kb_per;      // SPLIT: CTAs of a cluster, one per range of K blocks
+  const int* offsets;      // grouped: first row of every expert, and the end
+  int experts;
+  int vec;                 // results and residual in whole 16-byte vectors
+  int early;               // in a launch chain: the first weights are read ahead of the wait
+};
+
+struct Item {
+  int n_blk, row0, rows, expert;
+};
+
+// Item i of the launch: a block of weight rows, and a tile of tokens. Tiles of tokens follow one another for a block of weights,
+// unless there are experts: then the blocks of an expert's weights follow for a tile.
+__device__ __forceinline__ Item item_of(int i, const TileArgs& g, const int* first_tile) {
+  Item it;
+  if (g.offsets == nullptr) {
+    it.n_blk = i / g.t_tiles;
+    it.row0 = (i % g.t_tiles) * g.bt;
+    it.rows = min(g.bt, g.M - it.row0);
+    it.expert = 0;
+    return it;
+  }
+  const int tile = i / g.n_blocks;
+  it.n_blk = i % g.n_blocks;
+  int lo = 0, hi = g.experts;  // the last expert whose first tile is not behind `tile`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first_tile[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  it.expert = lo;
+  it.row0 = g.offsets[lo] + (tile - first_tile[lo]) * g.bt;
+  it.rows = min(g.bt, g.offsets[lo + 1] - it.row0);
+  return it;
+}
+
+// Eight results of a token: columns c .. c + 7 of the block (of its 64 outputs, where it is gated).
+__device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool glu, int n_blk, int t, int c) {
+  const int n0 = n_blk * (glu ? 64 : 128) + c, n_out = glu ? g.N / 2 : g.N;
+  if (n0 >= n_out) return;
+  if (glu) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = mx4_gate(f[j], f[8 + j], g.epi, g.limit);
+  }
+  const bool whole = g.vec && n0 + 8 <= n_out;
+  if (g.residual) {
+    const bf16* r = g.residual + t * g.ldr + n0;
+    if (whole) {
+      const bf16x8 v = ld_bf16x8(r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = unpack_bf16x2(v.u[j]);
+        f[2 * j] += p.x, f[2 * j + 1] += p.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n0 + j < n_out) f[j] += __bfloat162float(r[j]);
+    }
+  }
+  if (g.out_f32) {
+    float* dst = static_cast<float*>(g.C) + t * g.ldc + n0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + j < n_out) dst[j] = f[j];
+    return;
+  }
+  bf16* dst = static_cast<bf16*>(g.C) + t * g.ldc + n0;
+  if (whole) {
+    bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.u[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+    st_bf16x8(dst, o);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + j < n_out) dst[j] = __float2bfloat16(f[j]);
+  }
+}
+
+// Four warps, one per quarter of the lanes: an accumulator's results go to shared memory as [token][weight row] (scaled, with the
+// bias) and from there to C; SPLIT: they stay there, for add_ranges. `tid`: 0 .. 127, `parts`: room for a tile's results (SPLIT).
+template <bool SPLIT>
+__device__ __forceinline__ void write_results(const TileArgs& g, const int* first_tile, int i0, int i_step, int items, bool with_bias,
+                                              uint32_t tmem, uint32_t dfull0, uint32_t dempty0, float* parts, float* staging, int q,
+                                              int lane, int tid, volatile int* abort_flag, int* status) {
+  const int r = q * 32 + lane;
+  const bool glu = g.epi != PXL_EPI_NONE;
+  int db = 0;
+  uint32_t d_phase = 0;
+  bool ok = true;
+  for (int i = i0; i < items; i += i_step) {
+    const Item it = item_of(i, g, first_tile);
+    const int n = it.n_blk * kTileRows + r;
+    const float factor = g.row_scale ? g.row_scale[it.expert * g.n_blocks * kTileRows + n] : 1.f;
+    const float add = g.bias && n < g.N && with_bias ? __bfloat162float(g.bias[it.expert * g.N + n]) : 0.f;
+    // after a wait that ran out the loop goes on without results: the warps meet at every barrier below
+    ok = ok && wait_warp(dfull0 + 8 * db, d_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
+    tc_fence_after_sync();
+    for (int c0 = 0; c0 < it.rows; c0 += kChunk) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tmem + db * g.d_cols + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
+      tmem_ld_wait();
+      if (c0 + kChunk >= it.rows) {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dempty0 + 8 * db);
+      }
+      float* part = SPLIT ? parts + c0 * kPitch : staging;
+      const int m = min(kChunk, it.rows - c0);
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < m) part[j * kPitch + r] = __uint_as_float(v[j]) * factor + add;
+      if constexpr (!SPLIT) {
+        named_bar_sync(1, 128);
+        const int per = glu ? 8 : 16;
+        for (int e = tid; e < m * per; e += 128) {
+          const int t = e / per, c = e % per * 8;
+          float f[16];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            if (h >= 2 && !glu) break;
+            const float4 x = *reinterpret_cast<const float4*>(part + t * kPitch + c + (h & 1) * 4 + (h >> 1) * 64);
+            f[4 * h] = x.x, f[4 * h + 1] = x.y, f[4 * h + 2] = x.z, f[4 * h + 3] = x.w;
+          }
+          if (ok) finish8(g, f, glu, it.n_blk, it.row0 + c0 + t, c);
+        }
+        named_bar_sync(1, 128);
+      }
+    }
+    if (++db == g.d_bufs) db = 0, d_phase ^= 1;
+  }
+}
+
+// CTA r of a cluster adds its share of the tile's tokens over the cluster, in K order, and writes it (between two cluster barriers).
+__device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t parts, int tid, int threads, volatile int* abort_flag) {
+  const Item it = item_of(i, g, nullptr);
+  const int share = ceil_div(it.rows, g.splits), r0 = static_cast<int>(cluster_cta_rank()) * share, r1 = min(r0 + share, it.rows);
+  const bool glu = g.epi != PXL_EPI_NONE;
+  const int per = glu ? 8 : 16;
+  for (int e = tid; e < (r1 - r0) * per; e += threads) {
+    const int t = r0 + e / per, c = e % per * 8;
+    float f[16] = {};
+    for (int s = 0; s < g.splits; ++s) {
+      const uint32_t src = cluster_map_shared(parts + (t * kPitch + c) * 4, s);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (h >= 2 && !glu) break;
+        const float4 x = ld_shared_cluster_f32x4(src + (h & 1) * 16 + (h >> 1) * 256);
+        f[4 * h] += x.x, f[4 * h + 1] += x.y, f[4 * h + 2] += x.z, f[4 * h + 3] += x.w;
+      }
+    }
+    if (!*abort_flag) finish8(g, f, glu, it.n_blk, it.row0 + t, c);
+  }
+}
+
+}  // namespace pxl
+
+namespace pxl_host {
+
+// Ranges of K blocks for a launch of `items` tiles on `slots` places, at least `least` blocks each, none of them empty.
+inline void split_k(pxl::TileArgs& g, int items, int slots, int least) {
+  g.splits = 1, g.kb_per = g.k_blocks;
+  if (g.offsets) return;
+  int s = slots / items;
+  s = s > 8 ? 8 : s;
+  while (s > 1 && g.k_blocks / s < least) --s;
+  if (s > 1) {
+    g.kb_per = pxl::ceil_div(g.k_blocks, s);
+    g.splits = pxl::ceil_div(g.k_blocks, g.kb_per);
+  }
+}
+
+inline bool on16(const void* p, int64_t row_bytes) { return !((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row_bytes)) & 15); }
+
+// one[i] / split[i]: the forms without and with a cluster
+template <typename Kernel, typename... Args>
+inline int launch_tiles(Kernel one, Kernel split, bool (&configured)[64], pxl::TileArgs& g, int items, int slots, int threads, int smem,
+                        cudaStream_t stream, int max_smem, Args... args) {
+  const int dev = current_device_slot();
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem) != cudaSuccess ||
+        cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem) != cudaSuccess)
+      return PXL_ERR_CUDA;
+    configured[dev] = true;
+  }
+  const bool is_split = g.splits > 1;
+  const int64_t grid = is_split ? static_cast<int64_t>(items) * g.splits : items < slots ? items : slots;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (is_split) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(g.splits);
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  const bool in_chain = chained();
+  g.early = in_chain && !g.offsets;
+  if (in_chain) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, is_split ? split : one, args..., g) == cudaSuccess ? PXL_OK : PXL_ERR_CUDA;
+}
+
+}  // namespace pxl_host

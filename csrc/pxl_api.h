@@ -307,7 +307,7 @@ int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_sca
 int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, int out_f32,
                          const void* bias, int P, int E, int N, int K, const int* offsets, int epi, float limit, int* status,
                          pxl_stream_t stream);
-// Both operands as codes and scales: C[M, N] bf16 = X W^T (+ bias) (+ residual).
+// gemm_mx4_rows.cu: both operands as codes and scales: C[M, N] bf16 = X W^T (+ bias) (+ residual).
 int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc, const void* bias,
                       const void* residual, int64_t ldr, int M, int N, int K, int* status, pxl_stream_t stream);
 // pxl_moe_combine of fp32 rows
