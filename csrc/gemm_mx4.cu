@@ -14,32 +14,33 @@
 namespace {
 using namespace pxl;
 
-constexpr int kWarps = 14, kThreads = kWarps * 32;
+constexpr int kSets = 2, kThreads = (6 + 4 * kSets) * 32;  // (a set may be a stage or a buffer ahead of another: at least as many of each)
+constexpr int kMaxBufs = 4;
 constexpr int kWeightBytes = 9216;  // a block of weights in a stage, filled up to 1024 bytes
 constexpr int kMaxStages = 8;
 constexpr int kMaxExperts = 1024;
 
 template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmap, const uint8_t* __restrict__ w, int box,
-                                                                int a_bufs, int* status, const TileArgs g) {
+                                                                int a_bufs, const Mx4Shift shift, int* status, const TileArgs g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stage_bytes = kWeightBytes + g.bt * 256;
   float* staging = reinterpret_cast<float*>(smem + g.stages * stage_bytes);
   int* first_tile = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(staging) + (SPLIT ? 0 : kStaging));
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * 4 + 2 * 2];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBufs + 2 * 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, afull0 = empty0 + 8 * kMaxStages, aempty0 = afull0 + 32,
-                 dfull0 = aempty0 + 32, dempty0 = dfull0 + 16;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, afull0 = empty0 + 8 * kMaxStages, aempty0 = afull0 + 8 * kMaxBufs,
+                 dfull0 = aempty0 + 8 * kMaxBufs, dempty0 = dfull0 + 16;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int tmem_cols = g.d_bufs * g.d_cols + a_bufs * 64 > 256 ? 512 : 256;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int s = 0; s < g.stages; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
-    for (int b = 0; b < a_bufs; ++b) mbar_init(afull0 + 8 * b, 8), mbar_init(aempty0 + 8 * b, 1);
+    for (int b = 0; b < a_bufs; ++b) mbar_init(afull0 + 8 * b, 4), mbar_init(aempty0 + 8 * b, 1);
     for (int b = 0; b < g.d_bufs; ++b) mbar_init(dfull0 + 8 * b, 1), mbar_init(dempty0 + 8 * b, 4);
     mbar_fence_init();
     fence_proxy_async_smem();
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
       for (int kb = kb0; kb < kb1; ++kb, ++done) {
         const uint32_t fb = full0 + 8 * stage, at = s0 + stage * stage_bytes;
         if (!early || done >= g.stages) {
-          ok = wait_warp(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
+          ok = wait_parked(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
           expect_tx(fb, stage_tx(it), leader);
           if (leader) bulk_load_g2s(at, weights(it, kb), kBlockBytes, fb);
@@ -126,10 +127,10 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
     for (int i = i0; ok && i < items; i += i_step) {
       const Item it = item_of(i, g, first_tile);
       const uint32_t idesc = umma_idesc(kTileRows, ceil_div(it.rows, 16) * 16, 1, 1);
-      ok = wait_warp(dempty0 + 8 * db, d_phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY);
+      ok = wait_parked(dempty0 + 8 * db, d_phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY);
       for (int kb = kb0; ok && kb < kb1; ++kb) {
-        ok = wait_warp(full0 + 8 * stage, phase, abort_flag, status, PXL_DEV_TIMEOUT_FULL) &&
-             wait_warp(afull0 + 8 * ab, a_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
+        // (the warps that filled the buffer have waited for the stage, rows of x and all)
+        ok = wait_parked(afull0 + 8 * ab, a_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after_sync();
         const uint64_t desc = umma_desc_k_sw128(smem_u32(smem) + stage * stage_bytes + kWeightBytes);
@@ -147,51 +148,47 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
       if (++db == g.d_bufs) db = 0, d_phase ^= 1;
     }
   } else if (warp < 6) {
-    write_results<SPLIT>(g, first_tile, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem), staging, warp & 3,
+    write_results<SPLIT>(g, first_tile, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem), staging, 0, 1, warp & 3,
                          lane, static_cast<int>(threadIdx.x) - 64, abort_flag, status);
   } else {
-    // ---- codes -> bf16 in tensor memory
-    const int q = warp & 3, half = (warp - 6) >> 2, r = q * 32 + lane;
-    const uint32_t row_at = smem_u32(smem) + half * 2 * (kTileRows * 16) + r * 16, pow_at = smem_u32(smem) + kCodeBytes + r * 4;
-    const uint32_t dst0 = tmem_a + half * 32 + (static_cast<uint32_t>(q * 32) << 16);
-    int stage = 0, ab = 0;
-    uint32_t phase = 0, a_phase = 0;
-    bool ok = true;
-    for (int i = i0; ok && i < items; i += i_step) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = wait_warp(full0 + 8 * stage, phase, abort_flag, status, PXL_DEV_TIMEOUT_FULL);
-        if (!ok) break;
-        uint32_t code[2][4], p;
+    // ---- codes -> bf16 in tensor memory: sets of four warps take the blocks in turn, a set a whole block
+    const int q = warp & 3, set = (warp - 6) >> 2, r = q * 32 + lane;
+    const uint32_t dst0 = tmem_a + (static_cast<uint32_t>(q * 32) << 16);
+    // every block of the CTA's items in turn
+    const int blocks = (kb1 - kb0) * (i0 < items ? (items - i0 + i_step - 1) / i_step : 0);
+    int stage = set % g.stages, ab = set % a_bufs;
+    uint32_t phase = (set / g.stages) & 1, a_phase = 1 ^ ((set / a_bufs) & 1);
+    for (int n = set; n < blocks; n += kSets) {
+      const uint32_t at = smem_u32(smem) + stage * stage_bytes;
+      if (!wait_parked(full0 + 8 * stage, phase, abort_flag, status, PXL_DEV_TIMEOUT_FULL)) break;
+      uint32_t code[4][4], p;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(code[h][0]), "=r"(code[h][1]), "=r"(code[h][2]), "=r"(code[h][3])
-                       : "r"(row_at + stage * stage_bytes + h * (kTileRows * 16)));
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p) : "r"(pow_at + stage * stage_bytes));
-        p >>= half * 16;
-        ok = wait_warp(aempty0 + 8 * ab, a_phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY);
-        if (!ok) break;
-        tc_fence_after_sync();
+      for (int h = 0; h < 4; ++h)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(code[h][0]), "=r"(code[h][1]), "=r"(code[h][2]), "=r"(code[h][3])
+                     : "r"(at + r * 16 + h * (kTileRows * 16)));
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p) : "r"(at + kCodeBytes + r * 4));
+      if (!wait_parked(aempty0 + 8 * ab, a_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY)) break;
+      tc_fence_after_sync();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t p2 = mx4_power2((p >> (8 * h)) & 255u);
-          uint32_t o[16];
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t p2 = mx4_power2(p, h);
+        uint32_t o[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t y[4];
-            mx4_word(code[h][j], p2, y);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t y[4];
+          mx4_word(code[h][j], p2, shift, y);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) o[4 * j + v] = y[v];
-          }
-          tmem_st_32x32b_x16(dst0 + ab * 64 + h * 16, o);
+          for (int v = 0; v < 4; ++v) o[4 * j + v] = y[v];
         }
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(afull0 + 8 * ab);
-        if (++stage == g.stages) stage = 0, phase ^= 1;
-        if (++ab == a_bufs) ab = 0, a_phase ^= 1;
+        tmem_st_32x32b_x16(dst0 + ab * 64 + h * 16, o);
       }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(afull0 + 8 * ab);
+      for (ab += kSets; ab >= a_bufs; ab -= a_bufs) a_phase ^= 1;
+      for (stage += kSets; stage >= g.stages; stage -= g.stages) phase ^= 1;
     }
   }
 
@@ -213,25 +210,28 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
 
 int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w, int box, TileArgs g, int64_t items, int* status,
                    cudaStream_t stream) {
-  const int sms = pxl_host::num_sms();
+  static bool configured[64] = {};
+  if (!pxl_host::allow_smem(configured, gemm_mx4_kernel<false>, gemm_mx4_kernel<true>)) return PXL_ERR_CUDA;
   if (items > 0x7fffffff) items = 0x7fffffff;
+  const int sms = pxl_host::num_sms();
   // two CTAs per SM where their tiles are narrow: 256 columns of tensor memory and half of the shared memory each
-  const bool two = g.bt <= 128;
-  const int a_bufs = two ? 2 : 4, slots = two ? 2 * sms : sms;
-  g.d_bufs = 1;
+  const bool two = g.bt <= 64;
+  const int slots = two ? 2 * sms : sms;
   g.d_cols = pxl::ceil_div(g.bt, 32) * 32;
-  pxl_host::split_k(g, static_cast<int>(items), slots, 2);
+  g.d_bufs = !two && g.d_cols <= 192 ? 2 : 1;
+  int a_bufs = ((two ? 256 : 512) - g.d_bufs * g.d_cols) / 64;
+  if (a_bufs > kMaxBufs) a_bufs = kMaxBufs;
+  pxl_host::split_k(g, items, slots, 12, gemm_mx4_kernel<true>, kThreads);
   const int stage_bytes = kWeightBytes + g.bt * 256, rest = 1024 + (g.offsets ? (g.experts + 1) * 4 : 0) + (g.splits > 1 ? 0 : kStaging);
-  g.stages = ((two ? 113 : 226) * 1024 - 512 - rest) / stage_bytes;
+  g.stages = ((two ? 113 * 1024 : pxl_host::kTileSmem) - 512 - rest) / stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
-  if (g.stages < 1) return PXL_ERR_TOO_LARGE;
+  if (g.stages < kSets) return PXL_ERR_TOO_LARGE;
   int smem = rest + g.stages * stage_bytes;
   if (g.splits > 1 && smem < 1024 + g.bt * kPitch * 4) smem = 1024 + g.bt * kPitch * 4;
   CUtensorMap tmap;
   if (!pxl_host::make_tmap_2d(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_rows, K, ldx, box, 64)) return PXL_ERR_TENSORMAP;
-  static bool configured[64] = {false};
-  return pxl_host::launch_tiles(gemm_mx4_kernel<false>, gemm_mx4_kernel<true>, configured, g, static_cast<int>(items), slots, kThreads, smem,
-                                stream, 226 * 1024, tmap, static_cast<const uint8_t*>(w), box, a_bufs, status);
+  return pxl_host::launch_tiles(gemm_mx4_kernel<false>, gemm_mx4_kernel<true>, g, static_cast<int>(items), slots, kThreads, smem, stream,
+                                tmap, static_cast<const uint8_t*>(w), box, a_bufs, kMx4Shift, status);
 }
 
 bool epi_known(int epi, int N) {
@@ -244,11 +244,13 @@ PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const flo
                             const void* bias, const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit,
                             int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32 || !epi_known(epi, N) || !pxl_host::on16(x, 2 * ldx)) return PXL_ERR_INVALID_ARG;
+  if (pxl_gemv_mx4_takes(M, N, K))
+    return pxl_gemv_mx4(x, ldx, w, row_scale, C, ldc, bias, residual, ldr, M, N, K, epi, limit, stream);
   TileArgs g{};
   g.C = C, g.row_scale = row_scale, g.ldc = ldc, g.bias = static_cast<const bf16*>(bias);
   g.residual = static_cast<const bf16*>(residual), g.ldr = ldr, g.M = M, g.N = N, g.epi = epi, g.limit = limit;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kTileCols);
-  g.t_tiles = pxl::ceil_div(M, 256);
+  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, pxl_host::tile_tokens(M, g.n_blocks, 160, 48));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   g.vec = pxl_host::on16(C, 2 * ldc) && (!residual || pxl_host::on16(residual, 2 * ldr));
   return launch_product(x, ldx, M, K, w, g.bt, g, static_cast<int64_t>(g.n_blocks) * g.t_tiles, status, stream);
@@ -264,8 +266,9 @@ PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, c
   g.M = P, g.N = N, g.epi = epi, g.limit = limit;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kTileCols);
   g.offsets = offsets, g.experts = E;
-  const int mean = pxl::ceil_div(P, E);
-  g.bt = mean <= 16 ? 32 : mean <= 64 ? 64 : mean <= 256 ? 128 : 256;
+  // an expert with n rows has about n / bt + 1 / 2 tiles, each as long as bt + 48 rows: least at bt^2 = 96 n
+  g.bt = 32;
+  while (g.bt < 160 && static_cast<int64_t>(g.bt + 8) * (g.bt + 8) * E < 96ll * P) g.bt += 16;
   g.vec = !out_f32 && pxl_host::on16(C, 2 * ldc);
   const int64_t items = static_cast<int64_t>(g.n_blocks) * (pxl::ceil_div(P, g.bt) + (P < E ? P : E));  // at most
   return launch_product(x, ldx, P, K, w, 32, g, items, status, stream);

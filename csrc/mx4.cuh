@@ -26,14 +26,21 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// Factors of the shifts to the left, as arguments of the kernel: multiplications of unknown factors run on the FMA pipe, where the
+// compiler would put shifts on the ALU, whose rate bounds the expansion.
+struct Mx4Shift {
+  uint32_t by1, by3, by6;  // 2, 8, 64
+};
+constexpr Mx4Shift kMx4Shift{2u, 8u, 64u};
 // eight codes as placed above, and the power's exponent field in both halves -> eight values in bf16
-__device__ __forceinline__ void mx4_word(uint32_t w, uint32_t power2, uint32_t (&o)[4]) {
+__device__ __forceinline__ void mx4_word(uint32_t w, uint32_t power2, const Mx4Shift& s, uint32_t (&o)[4]) {
   o[0] = mul_bf16x2(w & 0x81c081c0u, power2);
-  o[1] = mul_bf16x2((w << 3) & 0x81c081c0u, power2);
-  o[2] = mul_bf16x2((w << 6) & 0x81c081c0u, power2);
-  o[3] = mul_bf16x2(((w << 1) & 0x80008000u) | ((w >> 3) & 0x01800180u) | ((w >> 7) & 0x00400040u), power2);
+  o[1] = mul_bf16x2((w * s.by3) & 0x81c081c0u, power2);
+  o[2] = mul_bf16x2((w * s.by6) & 0x81c081c0u, power2);
+  o[3] = mul_bf16x2(((w * s.by1) & 0x80008000u) | ((w >> 3) & 0x01800180u) | ((w >> 7) & 0x00400040u), power2);
 }
-__device__ __forceinline__ uint32_t mx4_power2(uint32_t field) { return field << 7 | field << 23; }
+// byte h of four powers in the exponent fields of both halves
+__device__ __forceinline__ uint32_t mx4_power2(uint32_t four, int h) { return __byte_perm(four, 0, 0x4040 | h | h << 8) << 7; }
 
 __device__ __forceinline__ float mx4_gate(float g, float u, int epi, float limit) {
   float s = g;

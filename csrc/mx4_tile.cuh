@@ -11,6 +11,38 @@ constexpr int kPitch = kTileRows + 4;  // floats of a token's results in shared 
 constexpr int kChunk = 32;             // tokens whose results are staged at a time
 constexpr int kStaging = kChunk * kPitch * 4;
 
+// Warp-collective wait, the same result in every lane. The hardware parks the warp for up to the hint's time, so that a wait costs
+// three instructions: expanding 4-bit weights is bound by the instructions that a SM issues.
+__device__ __forceinline__ uint32_t wait_hinted(uint32_t bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(ns)
+      : "memory");
+  return ok;
+}
+static __device__ __noinline__ bool wait_again(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    if (wait_hinted(bar, parity, 100000u)) return true;
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      if (status) atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait_parked(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, wait_hinted(bar, parity, 100000u))) return true;
+  return __all_sync(0xffffffffu, wait_again(bar, parity, abort_flag, status, code)) != 0;
+}
+
 struct TileArgs {
   void* C;
   const float* row_scale;  // [experts, N rounded up to 128], or none
@@ -102,12 +134,12 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
   }
 }
 
-// Four warps, one per quarter of the lanes: an accumulator's results go to shared memory as [token][weight row] (scaled, with the
+// Groups of four warps, one per quarter of the lanes, that take an accumulator's chunks of tokens in turn. The results go to shared memory as [token][weight row] (scaled, with the
 // bias) and from there to C; SPLIT: they stay there, for add_ranges. `tid`: 0 .. 127, `parts`: room for a tile's results (SPLIT).
 template <bool SPLIT>
 __device__ __forceinline__ void write_results(const TileArgs& g, const int* first_tile, int i0, int i_step, int items, bool with_bias,
-                                              uint32_t tmem, uint32_t dfull0, uint32_t dempty0, float* parts, float* staging, int q,
-                                              int lane, int tid, volatile int* abort_flag, int* status) {
+                                              uint32_t tmem, uint32_t dfull0, uint32_t dempty0, float* parts, float* staging, int group,
+                                              int groups, int q, int lane, int tid, volatile int* abort_flag, int* status) {
   const int r = q * 32 + lane;
   const bool glu = g.epi != PXL_EPI_NONE;
   int db = 0;
@@ -119,24 +151,19 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
     const float factor = g.row_scale ? g.row_scale[it.expert * g.n_blocks * kTileRows + n] : 1.f;
     const float add = g.bias && n < g.N && with_bias ? __bfloat162float(g.bias[it.expert * g.N + n]) : 0.f;
     // after a wait that ran out the loop goes on without results: the warps meet at every barrier below
-    ok = ok && wait_warp(dfull0 + 8 * db, d_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
+    ok = ok && wait_parked(dfull0 + 8 * db, d_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
     tc_fence_after_sync();
-    for (int c0 = 0; c0 < it.rows; c0 += kChunk) {
+    for (int c0 = group * kChunk; c0 < it.rows; c0 += groups * kChunk) {
       uint32_t v[32];
       tmem_ld_32x32b_x32(tmem + db * g.d_cols + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
       tmem_ld_wait();
-      if (c0 + kChunk >= it.rows) {
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dempty0 + 8 * db);
-      }
       float* part = SPLIT ? parts + c0 * kPitch : staging;
       const int m = min(kChunk, it.rows - c0);
 #pragma unroll
       for (int j = 0; j < 32; ++j)
         if (j < m) part[j * kPitch + r] = __uint_as_float(v[j]) * factor + add;
       if constexpr (!SPLIT) {
-        named_bar_sync(1, 128);
+        named_bar_sync(1 + group, 128);
         const int per = glu ? 8 : 16;
         for (int e = tid; e < m * per; e += 128) {
           const int t = e / per, c = e % per * 8;
@@ -149,9 +176,12 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
           }
           if (ok) finish8(g, f, glu, it.n_blk, it.row0 + c0 + t, c);
         }
-        named_bar_sync(1, 128);
+        named_bar_sync(1 + group, 128);
       }
     }
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(dempty0 + 8 * db);
     if (++db == g.d_bufs) db = 0, d_phase ^= 1;
   }
 }
@@ -182,32 +212,73 @@ __device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t pa
 
 namespace pxl_host {
 
-// Ranges of K blocks for a launch of `items` tiles on `slots` places, at least `least` blocks each, none of them empty.
-inline void split_k(pxl::TileArgs& g, int items, int slots, int least) {
+// Width of the token tiles for more than 256 tokens: whole rounds of the SMs times a tile's time, which is that of `fixed` tokens
+// more than it has.
+inline int tile_tokens(int M, int n_blocks, int widest, int fixed) {
+  const int sms = num_sms();
+  int best = widest;
+  int64_t least = INT64_MAX;
+  for (int bt = 96; bt <= widest; bt += 16) {
+    const int64_t rounds = (static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks + sms - 1) / sms, cost = rounds * (bt + fixed);
+    if (cost <= least) least = cost, best = bt;
+  }
+  return best;
+}
+
+// Clusters of `size` CTAs that run at a time; of kernels that leave room for one CTA per SM. (A GPU processing cluster's SMs that are
+// no multiple of the size stay empty.)
+template <typename Kernel>
+inline int max_clusters(Kernel kernel, int size, int threads, int smem) {
+  static int cached[64][9] = {};
+  int& n = cached[current_device_slot()][size];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size * 64);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = num_sms() / size;
+    }
+  }
+  return n;
+}
+
+// Ranges of K blocks for a launch of `items` tiles, none of them empty and of two blocks at least: the number of rounds times a
+// range's blocks and what a round costs besides, in blocks. `slots`: CTAs at a time without clusters.
+template <typename Kernel>
+inline void split_k(pxl::TileArgs& g, int64_t items, int slots, int besides, Kernel split, int threads) {
   g.splits = 1, g.kb_per = g.k_blocks;
-  if (g.offsets) return;
-  int s = slots / items;
-  s = s > 8 ? 8 : s;
-  while (s > 1 && g.k_blocks / s < least) --s;
-  if (s > 1) {
-    g.kb_per = pxl::ceil_div(g.k_blocks, s);
-    g.splits = pxl::ceil_div(g.k_blocks, g.kb_per);
+  if (g.offsets || items >= slots) return;
+  int64_t least = g.k_blocks + besides;
+  for (int s = 2; s <= 8 && g.k_blocks >= 2 * s; ++s) {
+    const int per = pxl::ceil_div(g.k_blocks, s), used = pxl::ceil_div(g.k_blocks, per);
+    const int n = max_clusters(split, used, threads, 200 * 1024);
+    const int64_t cost = (items + n - 1) / n * (per + besides + 2);
+    if (cost < least) least = cost, g.splits = used, g.kb_per = per;
   }
 }
 
 inline bool on16(const void* p, int64_t row_bytes) { return !((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(row_bytes)) & 15); }
 
-// one[i] / split[i]: the forms without and with a cluster
+constexpr int kTileSmem = 226 * 1024;
+template <typename... Kernels>
+inline bool allow_smem(bool (&configured)[64], Kernels... kernels) {
+  bool& done = configured[current_device_slot()];
+  if (!done) done = ((cudaFuncSetAttribute(kernels, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem) == cudaSuccess) && ...);
+  return done;
+}
+
+// one / split: the kernel without and with a cluster
 template <typename Kernel, typename... Args>
-inline int launch_tiles(Kernel one, Kernel split, bool (&configured)[64], pxl::TileArgs& g, int items, int slots, int threads, int smem,
-                        cudaStream_t stream, int max_smem, Args... args) {
-  const int dev = current_device_slot();
-  if (!configured[dev]) {
-    if (cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem) != cudaSuccess ||
-        cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem) != cudaSuccess)
-      return PXL_ERR_CUDA;
-    configured[dev] = true;
-  }
+inline int launch_tiles(Kernel one, Kernel split, pxl::TileArgs& g, int items, int slots, int threads, int smem, cudaStream_t stream,
+                        Args... args) {
   const bool is_split = g.splits > 1;
   const int64_t grid = is_split ? static_cast<int64_t>(items) * g.splits : items < slots ? items : slots;
   cudaLaunchConfig_t cfg{};

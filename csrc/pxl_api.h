@@ -302,14 +302,28 @@ int pxl_mx4_expand_rows(const void* codes, const void* scales, void* out, int64_
 // mx4.cuh), row_scale fp32 [N up to 128].
 int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
                  const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, int* status, pxl_stream_t stream);
+// gemv_mx4.cu: the same for up to eight rows; pxl_gemm_mx4 takes it by itself where it is the faster way
+#define PXL_GEMV_MX4_MAX_M 8
+int pxl_gemv_mx4_takes(int M, int N, int K);
+int pxl_gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
+                 const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, pxl_stream_t stream);
+// Routed gated experts of a few tokens, every pair of a token and an expert on its own: h [T * top, I] (scratch, 16-byte aligned) and
+// out [T, K] = base (optional) + sum_j weights[t, j] FFN_{ids[t, j]}(x[t]); w1 [E * 2 I, K] with gate / up rows in groups of 64, w2
+// [E * K, I]. epi PXL_EPI_SILU_MUL or PXL_EPI_CLIP_GLU; ids outside of [0, E) add nothing.
+int pxl_moe_mx4_few(const void* x, int64_t ldx, const int* ids, const float* weights, const void* w1, const float* row_scale1,
+                    const void* b1, const void* w2, const float* row_scale2, const void* b2, const void* base, void* h, void* out, int T,
+                    int top, int E, int K, int I, int epi, float limit, pxl_stream_t stream);
 // Expert-sorted rows (those of expert e are offsets[e] .. offsets[e + 1], of P at most) times E stacked weights; fp32 results with
 // out_f32. bias [E * N], E <= 1024.
 int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, int out_f32,
                          const void* bias, int P, int E, int N, int K, const int* offsets, int epi, float limit, int* status,
                          pxl_stream_t stream);
 // gemm_mx4_rows.cu: both operands as codes and scales: C[M, N] bf16 = X W^T (+ bias) (+ residual).
+// workspace: scratch of pxl_gemm_mx4_rows_workspace bytes (16-byte aligned; may be null where that is 0).
+int64_t pxl_gemm_mx4_rows_workspace(int M, int N, int K);
 int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc, const void* bias,
-                      const void* residual, int64_t ldr, int M, int N, int K, int* status, pxl_stream_t stream);
+                      const void* residual, int64_t ldr, int M, int N, int K, void* workspace, int64_t workspace_bytes, int* status,
+                      pxl_stream_t stream);
 // pxl_moe_combine of fp32 rows
 int pxl_moe_combine_f32(const float* y, const int* pos_of, const float* w, const void* base, void* out, int T, int k, int H,
                         pxl_stream_t stream);

@@ -37,7 +37,7 @@ NVCC_FLAGS = [
 
 # Sources whose elementary functions must be accurate in fp32 (arithmetic of a recurrence, tanh norms, fp32 attention) or whose
 # subnormals count (powers of two of 4-bit numbers)
-ACCURATE = ("attention_any", "delta_rule", "gated_delta", "gemm_mx4", "gemm_mx4_rows", "matrix_memory", "mx4",
+ACCURATE = ("attention_any", "delta_rule", "gated_delta", "gemm_mx4", "gemm_mx4_rows", "gemv_mx4", "matrix_memory", "mx4",
             "tanh_norm")
 
 

@@ -114,7 +114,9 @@ _SIGS = {
     "pxl_mx4_expand_rows": [_P, _P, _P, c_int64, c_int, _P],
     "pxl_gemm_mx4": [_P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P],
     "pxl_gemm_mx4_grouped": [_P, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, _P, _P],
-    "pxl_gemm_mx4_rows": [_P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, _P, _P],
+    "pxl_moe_mx4_few": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
+    "pxl_gemm_mx4_rows": [_P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, _P, c_int64, _P, _P],
+    "pxl_gemm_mx4_rows_workspace": [c_int] * 3,
     "pxl_moe_combine_f32": [_P, _P, _P, _P, _P, c_int, c_int, c_int, _P],
     "pxl_causal_conv1d_silu": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, _P],
     "pxl_gated_delta_rule": [_P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, c_int64,
@@ -181,7 +183,7 @@ _SIGS = {
 }
 
 
-_SIZES = {"pxl_delta_rule_workspace", "pxl_gated_delta_workspace"}      # functions that return a number of bytes
+_SIZES = {"pxl_delta_rule_workspace", "pxl_gated_delta_workspace", "pxl_gemm_mx4_rows_workspace"}      # functions that return a number of bytes
 
 
 @lru_cache(maxsize=1)

@@ -1053,17 +1053,20 @@ def moe_ffn_fp8(x, ids, weights, w1q, w1s, w2q, w2s, num_experts: int, base=None
 
 
 # ---------------------------------------------------------------------------- microscaled 4 bits
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The device of the tensors as the current one, for kernels that ask the runtime about it."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _bf16_rows(x: torch.Tensor, what: str) -> torch.Tensor:
     """Rows as TMA reads them: a copy where their base or stride is not a multiple of 16 bytes."""
-    mx4.require(x.dtype == torch.bfloat16, f"{what}: the kernels take bf16 rows, got {x.dtype}")
-    return x if x.stride(1) == 1 and not x.stride(0) & 7 and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
+    if x.dtype is not torch.bfloat16:
+        mx4.refuse(what, f"the kernels take bf16 rows, got {x.dtype}")
+    s0, s1 = x.stride()
+    return x if s1 == 1 and not s0 & 7 and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1075,11 +1078,12 @@ def _codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, tor
 def quant_mx4_rows(x: torch.Tensor):
     T, K = mx4.check_rows(x, "quant_mx4_rows")
     x = x if x.stride(1) == 1 else x.contiguous()
-    codes = torch.empty((T, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((T, K // 32), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        check(_lib.lib().pxl_mx4_quant_rows(x.data_ptr(), int(x.dtype == torch.float32), x.stride(0), codes.data_ptr(),
-                                            scales.data_ptr(), T, K, _stream(x.device)), "pxl_mx4_quant_rows")
+    dev = x.device
+    codes = torch.empty((T, K // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((T, K // 32), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(_lib.lib().pxl_mx4_quant_rows(x.data_ptr(), int(x.dtype is torch.float32), x.stride(0), codes.data_ptr(),
+                                            scales.data_ptr(), T, K, _stream(dev)), "pxl_mx4_quant_rows")
     _count()
     return codes, scales
 
@@ -1087,9 +1091,10 @@ def quant_mx4_rows(x: torch.Tensor):
 def expand_mx4_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     T, K = mx4.check_codes(codes, scales, "expand_mx4_rows")
     codes, scales = _codes(codes, scales)
-    out = torch.empty((T, K), dtype=torch.bfloat16, device=codes.device)
-    with _on(codes.device):
-        check(_lib.lib().pxl_mx4_expand_rows(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), T, K, _stream(codes.device)),
+    dev = codes.device
+    out = torch.empty((T, K), dtype=torch.bfloat16, device=dev)
+    with _on(dev):
+        check(_lib.lib().pxl_mx4_expand_rows(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), T, K, _stream(dev)),
               "pxl_mx4_expand_rows")
     _count()
     return out
@@ -1098,19 +1103,19 @@ def expand_mx4_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 def linear_mx4(x: torch.Tensor, w: Mx4Weight, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                epi: int = EPI_NONE, limit: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     T, K = mx4.check_rows(x, "linear_mx4")
-    mx4.require(isinstance(w, Mx4Weight) and w.experts == 1 and w.device == x.device,
-                "linear_mx4: w is an Mx4Weight of one expert on the rows' device")
-    n_out = mx4.check_product("linear_mx4", x.device, T, w.rows, K, w.cols, bias, residual, epi, limit, out, torch.bfloat16)
+    dev, N = x.device, w.rows if isinstance(w, Mx4Weight) else 0
+    mx4.check_weight(w, dev, "linear_mx4")
+    n_out = mx4.check_product("linear_mx4", dev, T, N, K, w.cols, bias, residual, epi, limit, out, torch.bfloat16)
     x = _bf16_rows(x, "linear_mx4")
     if out is None:
-        out = torch.empty((T, n_out), dtype=torch.bfloat16, device=x.device)
+        out = torch.empty((T, n_out), dtype=torch.bfloat16, device=dev)
     if T == 0:
         return out
-    epi = EPI_NONE if epi == EPI_RESIDUAL else epi
-    with _on(x.device):
+    r, ldr = (None, 0) if residual is None else (residual.data_ptr(), residual.stride(0))
+    with _on(dev):
         check(_lib.lib().pxl_gemm_mx4(x.data_ptr(), x.stride(0), w.data.data_ptr(), w.row_scale.data_ptr(), out.data_ptr(),
-                                      out.stride(0), _ptr(bias), _ptr(residual), 0 if residual is None else residual.stride(0), T,
-                                      w.rows, K, epi, limit, status_tensor(x.device).data_ptr(), _stream(x.device)), "pxl_gemm_mx4")
+                                      out.stride(0), _ptr(bias), r, ldr, T, N, K, EPI_NONE if epi == EPI_RESIDUAL else epi, limit,
+                                      status_tensor(dev).data_ptr(), _stream(dev)), "pxl_gemm_mx4")
     _count()
     return out
 
@@ -1121,18 +1126,22 @@ def linear_mx4_rows(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Te
     T, K = mx4.check_codes(codes, scales, "linear_mx4_rows: rows")
     N, K_w = mx4.check_codes(w_codes, w_scales, "linear_mx4_rows: weights")
     dev = codes.device
-    mx4.require(w_codes.device == dev, "linear_mx4_rows: rows and weights are on different devices")
+    if w_codes.device != dev:
+        mx4.refuse("linear_mx4_rows", "rows and weights are on different devices")
     mx4.check_product("linear_mx4_rows", dev, T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
     if out is None:
         out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0:
         return out
     (codes, scales), (w_codes, w_scales) = _codes(codes, scales), _codes(w_codes, w_scales)
+    r, ldr = (None, 0) if residual is None else (residual.data_ptr(), residual.stride(0))
     with _on(dev):
+        need = _lib.lib().pxl_gemm_mx4_rows_workspace(T, N, K)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         check(_lib.lib().pxl_gemm_mx4_rows(codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), out.data_ptr(),
-                                           out.stride(0), _ptr(bias), _ptr(residual), 0 if residual is None else residual.stride(0),
-                                           T, N, K, status_tensor(dev).data_ptr(), _stream(dev)), "pxl_gemm_mx4_rows")
-    _count()
+                                           out.stride(0), _ptr(bias), r, ldr, T, N, K, _ptr(ws), need, status_tensor(dev).data_ptr(),
+                                           _stream(dev)), "pxl_gemm_mx4_rows")
+    _count(2 if need else 1)
     return out
 
 
@@ -1148,6 +1157,9 @@ def _grouped_mx4(a, w: Mx4Weight, plan: MoEPlan, epi: int, bias, limit: float, d
     return out
 
 
+_FEW_PAIRS = 8
+
+
 def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: Mx4Weight, w2: Mx4Weight,
                 base: Optional[torch.Tensor] = None, act_mode: int = 0, limit: float = 7.0, b1: Optional[torch.Tensor] = None,
                 b2: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1157,9 +1169,19 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
     out = torch.empty((T, K), dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return out
+    epi = EPI_CLIP_GLU if act_mode else EPI_SILU_MUL
+    if T * k <= _FEW_PAIRS:
+        h = torch.empty((T * k, w2.cols), dtype=torch.bfloat16, device=x.device)
+        with _on(x.device):
+            check(_lib.lib().pxl_moe_mx4_few(x.data_ptr(), x.stride(0), ids.data_ptr(), weights.data_ptr(), w1.data.data_ptr(),
+                                             w1.row_scale.data_ptr(), _ptr(b1), w2.data.data_ptr(), w2.row_scale.data_ptr(), _ptr(b2),
+                                             _ptr(base), h.data_ptr(), out.data_ptr(), T, k, w1.experts, K, w2.cols, epi, limit,
+                                             _stream(x.device)), "pxl_moe_mx4_few")
+        _count(2)
+        return out
     with _on(x.device):
         plan = moe_align(ids, w1.experts)
-        act = _grouped_mx4(moe_gather(x, plan), w1, plan, EPI_CLIP_GLU if act_mode else EPI_SILU_MUL, b1, limit, torch.bfloat16)
+        act = _grouped_mx4(moe_gather(x, plan), w1, plan, epi, b1, limit, torch.bfloat16)
         y = _grouped_mx4(act, w2, plan, EPI_NONE, b2, 0.0, torch.float32)
         check(_lib.lib().pxl_moe_combine_f32(y.data_ptr(), plan.pos_of.data_ptr(), weights.data_ptr(), _ptr(base), out.data_ptr(), T, k,
                                              K, _stream(x.device)), "pxl_moe_combine_f32")

@@ -21,19 +21,20 @@ _SLOTS = ((15, 8, 7, 6), (12, 5, 4, 3), (9, 2, 1, 0), (14, 11, 10, 13))     # bi
 _CHUNK = 1 << 24                 # values that are laid out at a time
 
 
-def require(ok: bool, what: str) -> None:
-    if not ok:
-        raise KernelError(what)
+def refuse(what: str, why: str):
+    raise KernelError(f"{what}: {why}")
 
 
 def check_codes(codes: torch.Tensor, scales: torch.Tensor, what: str) -> tuple[int, int]:
     """Rows and columns of a microscaled matrix."""
-    require(isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype == torch.uint8
-            and scales.dtype == torch.uint8, f"{what}: codes and scales are uint8 tensors")
-    require(codes.dim() == 2 and scales.dim() == 2 and codes.shape[0] == scales.shape[0] and codes.shape[1] == 16 * scales.shape[1]
-            and scales.shape[1] > 0, f"{what}: codes [rows, K / 2] {tuple(codes.shape)} need scales [rows, K / 32] {tuple(scales.shape)}")
-    require(codes.device == scales.device, f"{what}: codes and scales are on different devices")
-    return codes.shape[0], 2 * codes.shape[1]
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+        refuse(what, "codes and scales are uint8 tensors")
+    c, s = codes.shape, scales.shape
+    if len(c) != 2 or len(s) != 2 or c[0] != s[0] or c[1] != 16 * s[1] or s[1] <= 0:
+        refuse(what, f"codes [rows, K / 2] {tuple(c)} need scales [rows, K / 32] {tuple(s)}")
+    if codes.device != scales.device:
+        refuse(what, "codes and scales are on different devices")
+    return c[0], 2 * c[1]
 
 
 class Mx4Weight:
@@ -70,7 +71,8 @@ class Mx4Weight:
         """``codes [experts * rows, K / 2]``, ``scales [experts * rows, K / 32]`` -> laid out. Gate and up rows of a gated weight come
         in alternating groups of 64 per expert (:func:`ops.interleave_gate_up`)."""
         total, K = check_codes(codes, scales, "Mx4Weight.pack")
-        require(experts > 0 and total > 0 and total % experts == 0, f"Mx4Weight.pack: {total} rows do not divide by {experts} experts")
+        if experts <= 0 or total <= 0 or total % experts:
+            refuse("Mx4Weight.pack", f"{total} rows do not divide by {experts} experts")
         N = total // experts
         dev, nt, kt = codes.device, -(-N // TILE), -(-K // TILE)
         data = torch.empty(experts * nt * kt * BLOCK_BYTES, dtype=torch.uint8, device=dev)
@@ -121,25 +123,49 @@ class Mx4Weight:
 
 
 def check_rows(x: torch.Tensor, what: str) -> tuple[int, int]:
-    require(x.dim() == 2 and x.shape[1] > 0 and x.shape[1] % 32 == 0, f"{what}: rows [T, K] with K a multiple of 32, got {tuple(x.shape)}")
-    require(x.dtype in (torch.bfloat16, torch.float32), f"{what}: rows are bf16 or fp32, got {x.dtype}")
-    return x.shape[0], x.shape[1]
+    shape = x.shape
+    if len(shape) != 2 or shape[1] <= 0 or shape[1] % 32:
+        refuse(what, f"rows [T, K] with K a multiple of 32, got {tuple(shape)}")
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float32:
+        refuse(what, f"rows are bf16 or fp32, got {x.dtype}")
+    return shape[0], shape[1]
+
+
+def check_weight(w, device: torch.device, what: str) -> None:
+    if not isinstance(w, Mx4Weight) or w.experts != 1 or w.data.device != device:
+        refuse(what, "w is an Mx4Weight of one expert on the rows' device")
+
+
+def _check_operand(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> None:
+    if t.shape != shape or t.dtype is not dtype or t.device != device or t.stride(-1) != 1:
+        refuse(what, f"{name} is {dtype} {shape} on {device} with neighbouring columns, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def check_product(what: str, device: torch.device, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
                   residual: Optional[torch.Tensor], epi: int, limit: float, out: Optional[torch.Tensor], dtype: torch.dtype) -> int:
     """Checks what the two products share; returns the number of output columns."""
-    require(K == K_w, f"{what}: rows of {K} columns and weights of {K_w}")
-    require(epi in (EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_CLIP_GLU), f"{what}: unknown epilogue {epi}")
-    glu = epi in (EPI_SILU_MUL, EPI_CLIP_GLU)
-    require(not glu or N % TILE == 0, f"{what}: a gated product needs gate and up rows in groups of 64, got {N} rows")
-    require(epi != EPI_CLIP_GLU or limit > 0, f"{what}: a clipped gate needs limit > 0")
-    require(not (glu and residual is not None), f"{what}: a gated product has no residual")
-    require((epi == EPI_RESIDUAL) <= (residual is not None), f"{what}: EPI_RESIDUAL needs a residual")
-    n_out = N // 2 if glu else N
-    for t, name, shape in ((bias, "bias", (N,)), (residual, "residual", (T, n_out)), (out, "out", (T, n_out))):
-        require(t is None or (tuple(t.shape) == shape and t.dtype == dtype and t.device == device and t.stride(-1) == 1),
-                f"{what}: {name} is {dtype} {shape} on {device} with neighbouring columns")
+    if K != K_w:
+        refuse(what, f"rows of {K} columns and weights of {K_w}")
+    n_out = N
+    if epi == EPI_SILU_MUL or epi == EPI_CLIP_GLU:
+        n_out = N // 2
+        if N % TILE:
+            refuse(what, f"a gated product needs gate and up rows in groups of 64, got {N} rows")
+        if epi == EPI_CLIP_GLU and not limit > 0:
+            refuse(what, "a clipped gate needs limit > 0")
+        if residual is not None:
+            refuse(what, "a gated product has no residual")
+    elif epi == EPI_RESIDUAL:
+        if residual is None:
+            refuse(what, "EPI_RESIDUAL needs a residual")
+    elif epi != EPI_NONE:
+        refuse(what, f"unknown epilogue {epi}")
+    if bias is not None:
+        _check_operand(bias, "bias", (N,), dtype, device, what)
+    if residual is not None:
+        _check_operand(residual, "residual", (T, n_out), dtype, device, what)
+    if out is not None:
+        _check_operand(out, "out", (T, n_out), dtype, device, what)
     return n_out
 
 
@@ -148,19 +174,25 @@ def check_experts(what: str, x: torch.Tensor, ids: torch.Tensor, weights: torch.
                   b2: Optional[torch.Tensor]) -> None:
     T, K = check_rows(x, what)
     dev = x.device
-    require(ids.dim() == 2 and ids.shape[0] == T and ids.dtype == torch.int32 and ids.is_contiguous() and ids.device == dev
-            and ids.shape[1] > 0, f"{what}: ids are int32 [T, k]")
-    require(weights.shape == ids.shape and weights.dtype == torch.float32 and weights.is_contiguous() and weights.device == dev,
-            f"{what}: weights are fp32 of the shape of ids")
-    require(isinstance(w1, Mx4Weight) and isinstance(w2, Mx4Weight) and w1.experts == w2.experts and w1.device == dev
-            and w2.device == dev, f"{what}: w1 and w2 are Mx4Weights of the same experts on the rows' device")
-    require(w1.experts <= 1024, f"{what}: {w1.experts} experts, at most 1024")
-    require(w1.cols == K and w1.rows == 2 * w2.cols and w2.rows == K and w1.rows % TILE == 0,
-            f"{what}: w1 [2 I, K] and w2 [K, I] with I a multiple of 64, got [{w1.rows}, {w1.cols}] and [{w2.rows}, {w2.cols}] for rows of {K}")
-    require(act_mode in (0, 1), f"{what}: act_mode is 0 (SiLU) or 1 (clipped GLU)")
-    require(act_mode == 0 or limit > 0, f"{what}: a clipped gate needs limit > 0")
+    shape = ids.shape
+    if len(shape) != 2 or shape[0] != T or shape[1] <= 0 or ids.dtype is not torch.int32 or not ids.is_contiguous() or ids.device != dev:
+        refuse(what, "ids are int32 [T, k]")
+    if weights.shape != shape or weights.dtype is not torch.float32 or not weights.is_contiguous() or weights.device != dev:
+        refuse(what, "weights are fp32 of the shape of ids")
+    if not isinstance(w1, Mx4Weight) or not isinstance(w2, Mx4Weight) or w1.experts != w2.experts or w1.data.device != dev \
+            or w2.data.device != dev:
+        refuse(what, "w1 and w2 are Mx4Weights of the same experts on the rows' device")
+    if w1.experts > 1024:
+        refuse(what, f"{w1.experts} experts, at most 1024")
+    if w1.cols != K or w1.rows != 2 * w2.cols or w2.rows != K or w1.rows % TILE:
+        refuse(what, f"w1 [2 I, K] and w2 [K, I] with I a multiple of 64, got [{w1.rows}, {w1.cols}] and [{w2.rows}, {w2.cols}] for "
+               f"rows of {K}")
+    if act_mode != 0 and act_mode != 1:
+        refuse(what, "act_mode is 0 (SiLU) or 1 (clipped GLU)")
+    if act_mode == 1 and not limit > 0:
+        refuse(what, "a clipped gate needs limit > 0")
     for t, name, n in ((b1, "b1", w1.rows), (b2, "b2", w2.rows)):
-        require(t is None or (t.numel() == n * w1.experts and t.is_contiguous() and t.dtype == x.dtype and t.device == dev),
-                f"{what}: {name} is {x.dtype} [{w1.experts} * {n}]")
-    require(base is None or (base.shape == x.shape and base.dtype == x.dtype and base.device == dev and base.is_contiguous()),
-            f"{what}: base has the rows' shape and type")
+        if t is not None and (t.numel() != n * w1.experts or not t.is_contiguous() or t.dtype is not x.dtype or t.device != dev):
+            refuse(what, f"{name} is {x.dtype} [{w1.experts} * {n}]")
+    if base is not None and (base.shape != x.shape or base.dtype is not x.dtype or base.device != dev or not base.is_contiguous()):
+        refuse(what, "base has the rows' shape and type")

@@ -603,8 +603,7 @@ def linear_mx4(x, w, bias=None, residual=None, epi: int = EPI_NONE, limit: float
     """``x [T, K] @ W^T`` with a microscaled weight (:class:`ops.Mx4Weight`, one expert): plain, with a bias, with a residual, or
     gated (``EPI_SILU_MUL``, ``EPI_CLIP_GLU`` with ``limit``; gate / up rows in groups of 64). Rows are bf16 (on CPU fp32 too)."""
     T, K = mx4.check_rows(x, "linear_mx4")
-    mx4.require(isinstance(w, mx4.Mx4Weight) and w.experts == 1 and w.device == x.device,
-                "linear_mx4: w is an Mx4Weight of one expert on the rows' device")
+    mx4.check_weight(w, x.device, "linear_mx4")
     mx4.check_product("linear_mx4", x.device, T, w.rows, K, w.cols, bias, residual, epi, limit, out, x.dtype)
     return _mx4_product(x.float(), _mx4_values(*w.unpack()), bias, residual, epi, limit, out, x.dtype)
 
@@ -614,7 +613,8 @@ def linear_mx4_rows(codes, scales, w_codes, w_scales, bias=None, residual=None, 
     residual; bf16 ``[T, N]``."""
     T, K = mx4.check_codes(codes, scales, "linear_mx4_rows: rows")
     N, K_w = mx4.check_codes(w_codes, w_scales, "linear_mx4_rows: weights")
-    mx4.require(w_codes.device == codes.device, "linear_mx4_rows: rows and weights are on different devices")
+    if w_codes.device != codes.device:
+        mx4.refuse("linear_mx4_rows", "rows and weights are on different devices")
     mx4.check_product("linear_mx4_rows", codes.device, T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
     return _mx4_product(_mx4_values(codes, scales), _mx4_values(w_codes, w_scales), bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
 
