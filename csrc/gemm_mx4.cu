@@ -269,7 +269,7 @@ PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, c
   // an expert with n rows has about n / bt + 1 / 2 tiles, each as long as bt + 48 rows: least at bt^2 = 96 n
   g.bt = 32;
   while (g.bt < 160 && static_cast<int64_t>(g.bt + 8) * (g.bt + 8) * E < 96ll * P) g.bt += 16;
-  g.vec = !out_f32 && pxl_host::on16(C, 2 * ldc);
+  g.vec = pxl_host::on16(C, (out_f32 ? 4 : 2) * ldc);
   const int64_t items = static_cast<int64_t>(g.n_blocks) * (pxl::ceil_div(P, g.bt) + (P < E ? P : E));  // at most
   return launch_product(x, ldx, P, K, w, 32, g, items, status, stream);
 }

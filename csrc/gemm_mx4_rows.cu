@@ -258,20 +258,22 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_rows_kernel(const __grid
   if (warp == 1) tmem_dealloc(tmem, tmem_cols);
 }
 
+constexpr int kLaySteps = 4;
 // Scales [R, row_bytes] -> the stages' order: for every tile of `per` rows and step of K, 1 or 2 times 128 rows' eight bytes as they
-// go to tensor memory; zeros (a finite power, for codes of 0) where there are no rows or groups. A block: 128 rows, eight steps.
+// go to tensor memory; zeros (a finite power, for codes of 0) where there are no rows or groups. A block: 128 rows, four steps.
 __global__ void __launch_bounds__(256) mx4_lay_powers_kernel(const uint8_t* __restrict__ ws, int w_rows, const uint8_t* __restrict__ xs,
                                                              int x_rows, int x_per, int x_halves, int row_bytes, int steps, int w_tiles,
                                                              uint8_t* __restrict__ laid_w, uint8_t* __restrict__ laid_x) {
-  __shared__ __align__(16) uint32_t out[8 * 256];
+  __shared__ __align__(16) uint32_t out[kLaySteps * 256];
   pdl_wait();
   pdl_launch_dependents();
   const bool is_x = static_cast<int>(blockIdx.x) >= w_tiles;
   const int t = is_x ? blockIdx.x - w_tiles : blockIdx.x, halves = is_x ? x_halves : 1, half = t % halves, tile = t / halves;
-  const int per = is_x ? x_per : kTileRows, step0 = blockIdx.y * 8;
+  const int per = is_x ? x_per : kTileRows, step0 = blockIdx.y * kLaySteps;
   const uint8_t* s = is_x ? xs : ws;
-  for (int i = threadIdx.x; i < 128 * 16; i += 256) {
-    const int r = i >> 4, w = i & 15, row = tile * per + half * 128 + r, at = step0 * 8 + w * 4;
+#pragma unroll
+  for (int i = threadIdx.x; i < 128 * 2 * kLaySteps; i += 256) {
+    const int r = i / (2 * kLaySteps), w = i % (2 * kLaySteps), row = tile * per + half * 128 + r, at = step0 * 8 + w * 4;
     uint32_t v = 0;
     if (half * 128 + r < per && row < (is_x ? x_rows : w_rows) && at < row_bytes) {
       const uint8_t* p = s + static_cast<int64_t>(row) * row_bytes + at;
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(256) mx4_lay_powers_kernel(const uint8_t* __re
     out[(w >> 1) * 256 + (w & 1) * 128 + (r & 31) * 4 + (r >> 5)] = v;
   }
   __syncthreads();
-  const int count = min(8, steps - step0);
+  const int count = min(kLaySteps, steps - step0);
   uint8_t* dst = (is_x ? laid_x : laid_w) + ((static_cast<int64_t>(tile) * steps + step0) * halves + half) * (2 * kAtom);
   for (int i = threadIdx.x; i < count * 64; i += 256)
     *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(i >> 6) * halves * (2 * kAtom) + (i & 63) * 16) = reinterpret_cast<const uint4*>(out)[i];
@@ -356,7 +358,7 @@ PXL_EXPORT int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc,
     uint8_t* const laid_w = static_cast<uint8_t*>(workspace);
     uint8_t* const laid_x = laid_w + static_cast<int64_t>(g.n_blocks) * g.k_blocks * (2 * kAtom);
     sc.laid_w = laid_w, sc.laid_x = laid_x;
-    pxl_host::launch(mx4_lay_powers_kernel, dim3(g.n_blocks + g.t_tiles * halves, pxl::ceil_div(g.k_blocks, 8)), 256, 0, stream, sc.ws, N,
+    pxl_host::launch(mx4_lay_powers_kernel, dim3(g.n_blocks + g.t_tiles * halves, pxl::ceil_div(g.k_blocks, kLaySteps)), 256, 0, stream, sc.ws, N,
                      sc.xs, M, g.bt, halves, sc.row_bytes, g.k_blocks, g.n_blocks, laid_w, laid_x);
     return pxl_host::launch_tiles(gemm_mx4_rows_kernel<false, true>, gemm_mx4_rows_kernel<true, false>, g, static_cast<int>(p.items), p.slots,
                                   kThreads, smem, stream, tx, tw, sc, status);

@@ -8,6 +8,7 @@
 #include <cuda_fp4.h>
 
 #include "common.cuh"
+#include "mx4.cuh"
 #include "pxl_api.h"
 
 namespace {
@@ -103,6 +104,82 @@ __global__ void __launch_bounds__(256) mx4_expand_rows_kernel(const uint8_t* __r
   st_bf16x8(out + i * 8, o);
 }
 
+// ---------------------------------------------------------------------------- weights laid out once (see mx4.cuh)
+// A warp per row: the factor that its largest scale exceeds 128 by, NaN where it has a scale of 255.
+__global__ void __launch_bounds__(256) mx4_row_scale_kernel(const uint8_t* __restrict__ scales, float* __restrict__ row_scale, int N,
+                                                            int padded, int64_t rows, int groups) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 31, n = static_cast<int>(r % padded);
+  int most = 0, nan = 0;
+  if (n < N) {
+    const uint8_t* s = scales + (r / padded * N + n) * groups;
+    for (int g = lane; g < groups; g += 32) {
+      const int v = s[g];
+      if (v == 255) nan = 1;
+      else most = max(most, v);
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  nan = __any_sync(0xffffffffu, nan);
+  if (lane == 0) row_scale[r] = nan ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(127 + max(0, most - 128)) << 23);
+}
+
+__device__ __forceinline__ uint32_t mx4_place(uint32_t half) {  // four codes of a half word, where mx4_word takes them from
+  const uint32_t a = half & 15u, b = half >> 4 & 15u, c = half >> 8 & 15u, d = half >> 12 & 15u;
+  return (a >> 3) << 15 | (a & 7u) << 6 | (b >> 3) << 12 | (b & 7u) << 3 | (c >> 3) << 9 | (c & 7u) | (d >> 3) << 14 | (d & 6u) << 9 |
+         (d & 1u) << 13;
+}
+// A thread per row of a block. (The powers of a row with a NaN scale are relative to the largest of its others too, which its factor
+// does not say.)
+__global__ void __launch_bounds__(256) mx4_pack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                       const float* __restrict__ row_scale, uint8_t* __restrict__ data, int N, int groups,
+                                                       int n_blocks, int k_blocks) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int r = threadIdx.x & 127, kb = blockIdx.x * 2 + (threadIdx.x >> 7), n_blk = blockIdx.y % n_blocks, n = n_blk * kTileRows + r;
+  if (kb >= k_blocks) return;
+  const int64_t expert = blockIdx.y / n_blocks, row = expert * N + n;
+  uint8_t* const blk = data + ((expert * n_blocks + n_blk) * k_blocks + kb) * kBlockBytes;
+  const float factor = row_scale[(expert * n_blocks + n_blk) * kTileRows + r];
+  int over = static_cast<int>(__float_as_uint(factor) >> 23) - 127;
+  if (isnan(factor)) {
+    over = 0;
+    for (int g = 0; g < groups; ++g) {
+      const int v = scales[row * groups + g];
+      if (v != 255) over = max(over, v - 128);
+    }
+  }
+  uint32_t powers = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int g = kb * 4 + b;
+    const bool in = n < N && g < groups;
+    const int s = in ? scales[row * groups + g] : 0;
+    const bool nan = s == 255;
+    powers |= static_cast<uint32_t>(nan ? 255 : max(s - over, 0) + 126) << (8 * b);
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (in && (nan || s >= over)) {
+      const uint4 c = *reinterpret_cast<const uint4*>(codes + (row * groups + g) * 16);
+      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // codes 0 .. 7 of a word: the even ones into the low half, the odd ones into the high half
+        uint32_t even = 0, odd = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) even |= (w[j] >> (8 * i) & 15u) << (4 * i), odd |= (w[j] >> (8 * i + 4) & 15u) << (4 * i);
+        o[j] = mx4_place(even) | mx4_place(odd) << 16;
+      }
+      out = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    *reinterpret_cast<uint4*>(blk + (b * kTileRows + r) * 16) = out;
+  }
+  *reinterpret_cast<uint32_t*>(blk + kCodeBytes + r * 4) = powers;
+}
+
 // ---------------------------------------------------------------------------- experts' rows
 // out[t] = base[t] + sum_j w[t, j] y[pos_of[t, j]]: the experts' rows in fp32, so that a token's sum is rounded once.
 __global__ void __launch_bounds__(256) moe_combine_f32_kernel(const float* __restrict__ y, const int* __restrict__ pos_of,
@@ -118,12 +195,20 @@ __global__ void __launch_bounds__(256) moe_combine_f32_kernel(const float* __res
       const float2 f0 = unpack_bf16x2(b.x), f1 = unpack_bf16x2(b.y);
       a[0] = f0.x, a[1] = f0.y, a[2] = f1.x, a[3] = f1.y;
     }
-    for (int j = 0; j < k; ++j) {
-      const int p = pos_of[t * k + j];
-      if (p < 0) continue;
-      const float f = w[t * k + j];
-      const float4 v = *reinterpret_cast<const float4*>(y + static_cast<int64_t>(p) * H + c);
-      a[0] += f * v.x, a[1] += f * v.y, a[2] += f * v.z, a[3] += f * v.w;
+    for (int j0 = 0; j0 < k; j0 += 4) {  // four rows in flight
+      int p[4];
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = j0 + j < k ? pos_of[t * k + j0 + j] : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p[j] >= 0) v[j] = __ldcs(reinterpret_cast<const float4*>(y + static_cast<int64_t>(p[j]) * H + c));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (p[j] < 0) continue;
+        const float f = w[t * k + j0 + j];
+        a[0] += f * v[j].x, a[1] += f * v[j].y, a[2] += f * v[j].z, a[3] += f * v[j].w;
+      }
     }
     *reinterpret_cast<uint2*>(out + t * H + c) = make_uint2(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]));
   }
@@ -164,5 +249,24 @@ PXL_EXPORT int pxl_moe_combine_f32(const float* y, const int* pos_of, const floa
   if (T == 0) return PXL_OK;
   pxl_host::launch(moe_combine_f32_kernel, T, 256, 0, stream, y, pos_of, w, static_cast<const bf16*>(base), static_cast<bf16*>(out),
                    k, H);
+  return check_launch();
+}
+
+PXL_EXPORT int pxl_mx4_pack(const void* codes, const void* scales, void* data, float* row_scale, int E, int N, int K, cudaStream_t stream) {
+  if (E <= 0 || N <= 0 || K <= 0 || K % 32 || (reinterpret_cast<uintptr_t>(codes) & 15)) return PXL_ERR_INVALID_ARG;
+  const int n_blocks = pxl::ceil_div(N, kTileRows), k_blocks = pxl::ceil_div(K, kTileCols), groups = K / 32;
+  const int64_t rows = static_cast<int64_t>(E) * n_blocks * kTileRows;
+  if (rows / 8 > 0x7fffffff) return PXL_ERR_TOO_LARGE;
+  pxl_host::launch(mx4_row_scale_kernel, static_cast<unsigned>(rows / 8), 256, 0, stream, static_cast<const uint8_t*>(scales), row_scale, N,
+                   n_blocks * kTileRows, rows, groups);
+  // (the grid's second dimension ends at 65535: parts of whole experts' blocks of rows)
+  const int per = 65535 / n_blocks;
+  if (per < 1) return PXL_ERR_TOO_LARGE;
+  for (int64_t e = 0; e < E; e += per) {
+    const int n = static_cast<int>(E - e < per ? E - e : per);
+    pxl_host::launch(mx4_pack_kernel, dim3(pxl::ceil_div(k_blocks, 2), n * n_blocks), 256, 0, stream,
+                     static_cast<const uint8_t*>(codes) + e * N * groups * 16, static_cast<const uint8_t*>(scales) + e * N * groups,
+                     row_scale + e * n_blocks * kTileRows, static_cast<uint8_t*>(data) + e * n_blocks * k_blocks * kBlockBytes, N, groups, n_blocks, k_blocks);
+  }
   return check_launch();
 }

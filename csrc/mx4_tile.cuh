@@ -116,6 +116,11 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
   }
   if (g.out_f32) {
     float* dst = static_cast<float*>(g.C) + t * g.ldc + n0;
+    if (whole) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (n0 + j < n_out) dst[j] = f[j];

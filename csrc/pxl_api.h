@@ -297,6 +297,9 @@ int pxl_store_rows(const void* src, int64_t ld, const int64_t* slots, void* cach
 int pxl_mx4_quant_rows(const void* x, int is_f32, int64_t ld, void* codes, void* scales, int64_t T, int K, pxl_stream_t stream);
 // ... and back: bf16 [T, K]
 int pxl_mx4_expand_rows(const void* codes, const void* scales, void* out, int64_t T, int K, pxl_stream_t stream);
+// Codes and scales of E stacked [N, K] weights -> the layout of pxl_gemm_mx4: data (E * ceil(N / 128) * ceil(K / 128) * 8704 bytes, 16-byte
+// aligned) and row_scale [E, N up to 128].
+int pxl_mx4_pack(const void* codes, const void* scales, void* data, float* row_scale, int E, int N, int K, pxl_stream_t stream);
 // gemm_mx4.cu: C[M, N] = x W^T (+ bias [N]) (+ residual), or the gated forms PXL_EPI_SILU_MUL / PXL_EPI_CLIP_GLU (N / 2 columns;
 // N % 128 == 0, W rows in groups of 64 gate and 64 up). x bf16, base and rows on 16 bytes. w: laid out in blocks of 128 x 128 (see
 // mx4.cuh), row_scale fp32 [N up to 128].

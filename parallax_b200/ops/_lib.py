@@ -112,6 +112,7 @@ _SIGS = {
     "pxl_quant_fp8_rows": [_P, c_int64, _P, _P, c_int, c_int, _P],
     "pxl_mx4_quant_rows": [_P, c_int, c_int64, _P, _P, c_int64, c_int, _P],
     "pxl_mx4_expand_rows": [_P, _P, _P, c_int64, c_int, _P],
+    "pxl_mx4_pack": [_P, _P, _P, _P, c_int, c_int, c_int, _P],
     "pxl_gemm_mx4": [_P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P],
     "pxl_gemm_mx4_grouped": [_P, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, _P, _P],
     "pxl_moe_mx4_few": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],

@@ -1100,6 +1100,15 @@ def expand_mx4_rows(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def pack_mx4(codes: torch.Tensor, scales: torch.Tensor, data: torch.Tensor, row_scale: torch.Tensor, experts: int, N: int, K: int) -> None:
+    """Fills the tensors of an :class:`Mx4Weight`."""
+    codes, scales = _codes(codes, scales)
+    with _on(codes.device):
+        check(_lib.lib().pxl_mx4_pack(codes.data_ptr(), scales.data_ptr(), data.data_ptr(), row_scale.data_ptr(), experts, N, K,
+                                      _stream(codes.device)), "pxl_mx4_pack")
+    _count(2)
+
+
 def linear_mx4(x: torch.Tensor, w: Mx4Weight, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                epi: int = EPI_NONE, limit: float = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     T, K = mx4.check_rows(x, "linear_mx4")

@@ -76,9 +76,14 @@ class Mx4Weight:
         N = total // experts
         dev, nt, kt = codes.device, -(-N // TILE), -(-K // TILE)
         data = torch.empty(experts * nt * kt * BLOCK_BYTES, dtype=torch.uint8, device=dev)
-        blocks = data.view(experts, nt, kt, BLOCK_BYTES)
         row_scale = torch.ones((experts, nt * TILE), dtype=torch.float32, device=dev)
-        codes, scales = codes.view(experts, N, K // 2), scales.view(experts, N, K // 32)
+        if codes.is_cuda:
+            from . import cuda
+
+            cuda.pack_mx4(codes, scales, data, row_scale, experts, N, K)
+            return cls(data, row_scale, N, K, experts)
+        blocks = data.view(experts, nt, kt, BLOCK_BYTES)
+        codes, scales = codes.reshape(experts, N, K // 2), scales.reshape(experts, N, K // 32)
         step = max(1, _CHUNK // (kt * TILE * TILE))
         for e in range(experts):
             for t0 in range(0, nt, step):

@@ -95,6 +95,21 @@ def test_no_rows():
     assert ops.linear_mx4_rows(codes, scales, *w).shape == (0, 64)
 
 
+@pytest.mark.parametrize("experts,N,K", [(1, 1, 32), (1, 130, 160), (3, 128, 128), (2, 300, 96), (5, 257, 1056)])
+def test_layout(experts, N, K):
+    codes, scales = _matrix(experts * N, K, N, 0, 129)
+    for _ in range(2):
+        want = ops.Mx4Weight.pack(codes, scales, experts=experts)
+        got = ops.Mx4Weight.pack(*_dev(codes, scales), experts=experts)
+        assert torch.equal(got.data.cpu(), want.data)
+        assert torch.equal(torch.nan_to_num(got.row_scale.cpu(), nan=-1.0), torch.nan_to_num(want.row_scale, nan=-1.0))
+        g = torch.Generator().manual_seed(N)                # and scales of all sizes, NaN among them
+        scales = torch.randint(0, 256, scales.shape, generator=g, dtype=torch.uint8)
+    view = torch.zeros(codes.shape[0], codes.shape[1] + 3, dtype=torch.uint8, device=DEV)
+    view[:, 3:] = codes.to(DEV)
+    assert torch.equal(ops.Mx4Weight.pack(view[:, 3:], scales.to(DEV), experts=experts).data.cpu(), want.data)
+
+
 # ------------------------------------------------------------------------------------------------ products
 def _product_case(T, N, K, bias=False, residual=False, act="", seed=0, lo=117, hi=126):
     x, (codes, scales) = _normal(T, K, seed=seed), _matrix(N, K, seed + 1, lo, hi)
