@@ -42,6 +42,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--kv-block-size", type=int, default=16, help="Block size for KV cache management")
     p.add_argument("--kv-cache-dtype", type=str, default="auto", choices=["auto", "bf16", "fp8_e4m3"],
                    help="Storage type of the K / V pages of softmax-attention layers (auto: the model's dtype)")
+    p.add_argument("--expert-format", type=str, default="bf16", choices=["bf16", "mxfp4"],
+                   help="Storage of the routed experts' matrices: the model's type, or microscaled 4-bit numbers (single-process engine)")
     p.add_argument("--disable-prefix-cache", dest="enable_prefix_cache", action="store_false", default=True,
                    help="Disable the radix prefix cache")
     p.add_argument("--chunked-prefill-size", type=int, default=1024, help="Max prompt tokens per prefill chunk (0: off)")

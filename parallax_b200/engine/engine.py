@@ -35,7 +35,7 @@ from parallax_b200.engine.batch import BatchBuilder
 from parallax_b200.engine.request import PENDING_TOKEN, Request, RequestStatus, SamplingParams
 from parallax_b200.engine.scheduler import BatchScheduler, ScheduledSeq
 from parallax_b200.engine.worker import StageWorker
-from parallax_b200.models.config import ModelConfig
+from parallax_b200.models.config import ModelConfig, with_expert_format
 
 logger = logging.getLogger(__name__)
 
@@ -212,11 +212,14 @@ class Engine:
         tokenizer=None,
         return_routed_experts: bool = False,
         max_requests: Optional[int] = None,
+        expert_format: Optional[str] = None,
     ):
-        """``max_requests``: rows (block tables, state slots) for requests that are live at the same time; by
+        """``expert_format="mxfp4"`` keeps the routed experts' matrices as microscaled 4-bit numbers: those of a checkpoint that has
+        them, else quantised when they are loaded (None or "bf16": in the model's type). ``max_requests``: rows (block tables, state slots) for requests that are live at the same time; by
         default twice the batch size. ``tokenizer`` (anything with ``token_text(id)`` and ``eos_token_ids``) is only needed for requests
         with a ``json_schema``: constrained decoding checks candidate tokens by their text."""
         self.tokenizer = tokenizer
+        cfg = with_expert_format(cfg, expert_format)
         self.cfg = cfg
         self.device = torch.device(device)
         self.page_size = page_size

@@ -73,7 +73,7 @@ def build_engine(args, cfg, loader, start: int, end: int, shared_state=None):
                   max_total_length=args.max_sequence_length, request_timeout_s=args.request_timeout_s,
                   weights=weights, shared_state=shared_state,
                   num_blocks=None if device != "cpu" else 1024, lora=_lora_spec(args),
-                  kv_cache_dtype=getattr(args, "kv_cache_dtype", None),
+                  kv_cache_dtype=getattr(args, "kv_cache_dtype", None), expert_format=getattr(args, "expert_format", None),
                   return_routed_experts=bool(getattr(args, "enable_return_routed_experts", False)))
 
 
@@ -110,6 +110,9 @@ def run_standalone(args) -> None:
     start = 0 if args.start_layer is None else args.start_layer
     end = cfg.num_hidden_layers if args.end_layer is None else args.end_layer
     state.set_layer_allocation(name, start, end, args.tp_size, changed=False)
+    if getattr(args, "expert_format", "bf16") != "bf16" and ((start, end) != (0, cfg.num_hidden_layers)
+                                                             or args.pp_size * args.tp_size * args.ep_size > 1):
+        raise ValueError("--expert-format mxfp4 is available in the single-process engine only")
     if (start, end) != (0, cfg.num_hidden_layers):
         run_static_peer(args, state, name, start, end)     # one peer of a pipeline (tensor-parallel with --tp-size)
         return
@@ -181,6 +184,8 @@ def wait_for_allocation(state: SharedState, timeout_s: float = 300.0, poll_s: fl
 
 def run_scheduler_mode(args) -> None:
     """Join a cluster and serve whatever layer range the scheduler assigns (reloading on change)."""
+    if getattr(args, "expert_format", "bf16") != "bf16":
+        raise ValueError("--expert-format mxfp4 is available in the single-process engine only")
     from parallax_b200.p2p.node_runtime import NodeRuntime
     from parallax_b200.p2p.server import NodeAgent, SchedulerClient
 

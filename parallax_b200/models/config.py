@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import json
 import os
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Optional
 
 # layer kinds (same vocabulary as the reference's ``utils/layer_types.py:5-20``)
@@ -82,6 +82,7 @@ class ModelConfig:
     # quantisation
     quant_method: str = ""
     weight_block_size: Optional[list] = None
+    expert_format: str = ""             # "mxfp4": expert matrices as microscaled 4-bit numbers (set by the engine)
     dtype: str = "bfloat16"
     # models whose config lists every layer with its own mixer / feed-forward sizes (models/layer_spec.py)
     layer_specs: list = field(default_factory=list)
@@ -369,6 +370,19 @@ def config_from_hf(cfg: dict) -> ModelConfig:
         mc.layer_types = ["sliding_attention" if i % 2 == 0 else "full_attention"
                           for i in range(mc.num_hidden_layers)]
     return mc
+
+
+def with_expert_format(cfg: ModelConfig, expert_format: Optional[str]) -> ModelConfig:
+    """``cfg`` with the storage of the routed experts' matrices: None or "bf16" (the model's type), or "mxfp4" (microscaled 4-bit
+    numbers, on stages that hold all experts)."""
+    if expert_format in (None, "bf16"):
+        return cfg
+    if expert_format != "mxfp4":
+        raise ValueError(f"unknown expert format {expert_format!r}: bf16 or mxfp4")
+    if not cfg.is_moe or cfg.layer_specs or cfg.quant_method == "fp8":
+        raise ValueError(f"expert_format mxfp4 needs a model with routed experts in bf16 or MXFP4, which {cfg.architecture} as configured "
+                         "is not")
+    return replace(cfg, expert_format=expert_format)
 
 
 def load_config(model_path: str) -> ModelConfig:

@@ -48,6 +48,14 @@ class ExpertParallelMixin:
                 lw.moe.idle(self.device, self.dtype)
 
 
+def _grouped_rows(I: int, device, halves: bool) -> torch.Tensor:
+    """Order of ``2 I`` gate and up rows, given as ``[gate | up]`` halves or alternating, that puts them into groups of 64 gate rows
+    and the 64 up rows of the same outputs."""
+    i = torch.arange(I, device=device).view(-1, 1, 64)
+    gate_up = (i, i + I) if halves else (2 * i, 2 * i + 1)
+    return torch.cat(gate_up, 1).flatten()
+
+
 class MoEWeights:
     def __init__(self, cfg: ModelConfig):
         self.cfg = cfg
@@ -59,6 +67,7 @@ class MoEWeights:
         self.shared_down: Optional[torch.Tensor] = None  # [H, Is]
         self.shared_gate: Optional[torch.Tensor] = None  # [1, H] sigmoid gate on the shared expert (Qwen2-MoE style)
         self.fp8: Optional[dict] = None                 # block-scaled e4m3 copies: name -> (q, scales per 64 rows)
+        self.mx4: Optional[dict] = None                 # microscaled 4-bit expert matrices: "w1" / "w2" -> ops.Mx4Weight
         self.router_bias: Optional[torch.Tensor] = None  # [E] (GPT-OSS)
         self.b1: Optional[torch.Tensor] = None          # [E*2I] expert biases of the first projection
         self.b2: Optional[torch.Tensor] = None          # [E*H]
@@ -79,6 +88,8 @@ class MoEWeights:
                           self.shared_gate, self.router_bias, self.b1, self.b2) if t is not None]
         for q, s in (self.fp8 or {}).values():
             ts += [q, s]
+        for w in (self.mx4 or {}).values():
+            ts += w.tensors()
         return ts
 
     def shard_experts(self, rank: int, ep: int) -> int:
@@ -90,6 +101,8 @@ class MoEWeights:
         epr = E // ep
         if self.experts_per_rank == epr:      # already built with this rank's experts only
             return epr
+        if self.mx4 is not None:
+            raise ValueError("microscaled experts are not sharded: use bf16 experts with expert or tensor parallelism")
 
         def rows(t):
             n = t.shape[0] // E
@@ -127,6 +140,26 @@ class MoEWeights:
                 self.fp8[name] = quantize_fp8_block(w, (64, 128))
                 setattr(self, name, None)
 
+    def _install_mx4(self, c1: torch.Tensor, s1: torch.Tensor, c2: torch.Tensor, s2: torch.Tensor) -> None:
+        """Codes and scales of the expert matrices: of ``w1`` with gate / up rows in groups of 64 per expert."""
+        E = self.experts_per_rank
+        self.mx4 = {"w1": ops.Mx4Weight.pack(c1, s1, experts=E), "w2": ops.Mx4Weight.pack(c2, s2, experts=E)}
+        self.w1 = self.w2 = None
+
+    def quantize_mx4(self) -> None:
+        """Replace the expert matrices by microscaled 4-bit ones (a shared expert stays as it is). The clipped gate's rows, gate
+        rows then up rows, go into the groups of 64 that the kernels take; so do its biases."""
+        E = self.experts_per_rank
+        I = self.w1.shape[0] // (2 * E)
+        if I % 64 or self.cfg.hidden_size % 32:
+            raise ValueError(f"microscaled experts need an inner size in 64s and a hidden size in 32s, got {I} and {self.cfg.hidden_size}")
+        if self.act_mode:
+            order = _grouped_rows(I, self.w1.device, halves=True)
+            self.w1 = self.w1.view(E, 2 * I, -1)[:, order].reshape(E * 2 * I, -1)
+            if self.b1 is not None:
+                self.b1 = self.b1.view(E, 2 * I)[:, order].reshape(-1).contiguous()
+        self._install_mx4(*ops.quant_mx4_rows(self.w1), *ops.quant_mx4_rows(self.w2))
+
     # ------------------------------------------------------------------ construction
     @classmethod
     def random(cls, cfg: ModelConfig, device, dtype, rnd: Callable, expert_shard=None) -> "MoEWeights":
@@ -157,10 +190,19 @@ class MoEWeights:
         if Is:
             m.shared_gu = ops.interleave_gate_up(shared_rnd(Is, H, k=4), shared_rnd(Is, H, k=5))
             m.shared_down = shared_rnd(H, Is, k=6)
+        if cfg.expert_format == "mxfp4":
+            m.quantize_mx4()
         return m
 
     @classmethod
     def from_hf(cls, cfg: ModelConfig, tensors: dict, prefix: str, device, dtype) -> "MoEWeights":
+        m = cls._from_hf(cfg, tensors, prefix, device, dtype)
+        if cfg.expert_format == "mxfp4" and m.mx4 is None:
+            m.quantize_mx4()
+        return m
+
+    @classmethod
+    def _from_hf(cls, cfg: ModelConfig, tensors: dict, prefix: str, device, dtype) -> "MoEWeights":
         m = cls(cfg)
         E = cfg.num_experts
 
@@ -173,9 +215,12 @@ class MoEWeights:
             return t.to(device=device, dtype=dt)
 
         if prefix + "experts.gate_up_proj_blocks" in tensors:
-            # GPT-OSS as published: MXFP4 expert matrices, expanded to bf16 here. The rows of gate_up
-            # alternate gate / up; [E, rows, K] is already the [N, K] layout of the grouped GEMM.
+            # GPT-OSS as published: MXFP4 expert matrices, kept as they are (expert_format "mxfp4") or expanded to bf16 here. The
+            # rows of gate_up alternate gate / up; [E, rows, K] is already the [N, K] layout of the grouped GEMM.
             from parallax_b200.loader.quant import dequant_mxfp4
+
+            if cfg.expert_format == "mxfp4":
+                return m._from_blocks(tensors, prefix, get, device)
 
             def expand(name):
                 return dequant_mxfp4(tensors[prefix + name + "_blocks"], tensors[prefix + name + "_scales"],
@@ -230,6 +275,24 @@ class MoEWeights:
         m.shared_gate = get("shared_expert_gate.weight", required=False)
         return m
 
+    def _from_blocks(self, tensors: dict, prefix: str, get: Callable, device) -> "MoEWeights":
+        def codes(name):
+            t, s = tensors[prefix + name + "_blocks"].to(device), tensors[prefix + name + "_scales"].to(device)
+            return t.flatten(-2), s                                               # [E, rows, K / 2], [E, rows, K / 32]
+
+        self.router = get("router.weight").contiguous()
+        self.router_bias = get("router.bias", required=False)
+        (c1, s1), (c2, s2) = codes("experts.gate_up_proj"), codes("experts.down_proj")
+        if c1.shape[1] % 128:
+            raise ValueError(f"microscaled experts need an inner size in 64s, got {c1.shape[1] // 2}")
+        order = _grouped_rows(c1.shape[1] // 2, device, halves=False)
+        self._install_mx4(c1[:, order].flatten(0, 1), s1[:, order].flatten(0, 1), c2.flatten(0, 1), s2.flatten(0, 1))
+        b1, b2 = get("experts.gate_up_proj_bias", required=False), get("experts.down_proj_bias", required=False)
+        self.b1 = None if b1 is None else b1[:, order].reshape(-1).contiguous()
+        self.b2 = None if b2 is None else b2.reshape(-1).contiguous()
+        self.act_mode = 1
+        return self
+
     # ------------------------------------------------------------------ forward
     def idle(self, device, dtype) -> None:
         H, k = self.cfg.hidden_size, self.top_k
@@ -269,6 +332,9 @@ class MoEWeights:
                 base = ops.gate_mul_grouped(y, ops.row_dot(xn, self.shared_gate), y.shape[1], residual=h)
         if self.ep is not None:
             return self.ep.moe_ffn(self, xn, ids, w, base=base)
+        if self.mx4 is not None:
+            return ops.moe_ffn_mx4(xn, ids, w, self.mx4["w1"], self.mx4["w2"], base=base, act_mode=self.act_mode, limit=self.limit,
+                                   b1=self.b1, b2=self.b2)
         if self.act_mode:
             return ops.moe_ffn(xn, ids, w, self.w1, self.w2, self.num_experts, base=base, act_mode=self.act_mode,
                                limit=self.limit, b1=self.b1, b2=self.b2)

@@ -192,3 +192,113 @@ def test_refusals():
         with pytest.raises(ops.KernelError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+# ------------------------------------------------------------------------------------------------ engine
+def _gpt_oss(hidden=128, inner=64):
+    from parallax_b200.models.config import config_from_hf
+
+    return config_from_hf(dict(
+        architectures=["GptOssForCausalLM"], model_type="gpt_oss", hidden_size=hidden, num_hidden_layers=2, num_attention_heads=4,
+        num_key_value_heads=2, head_dim=32, intermediate_size=inner, moe_intermediate_size=inner, num_local_experts=4, num_experts_per_tok=2, sliding_window=16,
+        layer_types=["sliding_attention", "full_attention"], vocab_size=256, max_position_embeddings=512, rope_theta=10000.0,
+        attention_bias=True, tie_word_embeddings=False))
+
+
+def _checkpoint(cfg, seed=0):
+    """Random weights of a small GPT-OSS under their published names, experts as MXFP4 blocks."""
+    g = torch.Generator().manual_seed(seed)
+    H, D, I, E = cfg.hidden_size, cfg.head_dim, cfg.moe_intermediate_size, cfg.num_experts
+    rnd = lambda *sh: torch.randn(*sh, generator=g) * 0.1  # noqa: E731
+    sd = {"model.embed_tokens.weight": rnd(cfg.vocab_size, H), "model.norm.weight": torch.ones(H), "lm_head.weight": rnd(cfg.vocab_size, H)}
+    for i in range(cfg.num_hidden_layers):
+        p, m = f"model.layers.{i}.", f"model.layers.{i}.mlp."
+        for n in ("input_layernorm", "post_attention_layernorm"):
+            sd[p + n + ".weight"] = torch.ones(H)
+        for n, rows in (("q", 4 * D), ("k", 2 * D), ("v", 2 * D)):
+            sd[p + f"self_attn.{n}_proj.weight"], sd[p + f"self_attn.{n}_proj.bias"] = rnd(rows, H), rnd(rows)
+        sd[p + "self_attn.o_proj.weight"], sd[p + "self_attn.o_proj.bias"], sd[p + "self_attn.sinks"] = rnd(H, 4 * D), rnd(H), rnd(4)
+        sd[m + "router.weight"], sd[m + "router.bias"] = rnd(E, H), rnd(E)
+        for n, rows, cols in (("gate_up_proj", 2 * I, H), ("down_proj", H, I)):
+            c, s = ops.quant_mx4_rows(rnd(E * rows, cols) * 3)
+            sd[m + f"experts.{n}_blocks"], sd[m + f"experts.{n}_scales"] = c.view(E, rows, cols // 32, 16), s.view(E, rows, cols // 32)
+            sd[m + f"experts.{n}_bias"] = rnd(E, rows)
+    return sd
+
+
+def _logits(cfg, weights, **kw):
+    from parallax_b200.engine.engine import Engine
+    from parallax_b200.engine.request import Request, SamplingParams
+
+    eng = Engine(cfg, device="cpu", num_blocks=64, page_size=16, max_batch_size=4, weights=weights, **kw)
+    eng.keep_logits = True
+    req = Request(input_ids=list(range(3, 40)), sampling_params=SamplingParams(max_new_tokens=3, temperature=0.0, ignore_eos=True))
+    eng.add_request(req)
+    out = []
+    while eng.has_work():
+        eng.step()
+        if eng.last_logits is not None and eng.last_logits.shape[0] > 0:
+            out.append(eng.last_logits[0].clone())
+        eng.last_logits = None
+    return eng, torch.stack(out), req.output_ids
+
+
+def test_engine_keeps_packed_experts():
+    """The same model with its experts expanded and kept in 4 bits."""
+    cfg = _gpt_oss()
+    sd = _checkpoint(cfg)
+    _eng, a, ta = _logits(cfg, sd)
+    eng, b, tb = _logits(cfg, sd, expert_format="mxfp4")
+    assert ta == tb and torch.allclose(a, b, rtol=1e-4, atol=1e-5)
+    moe = eng.stages[0].model.layers[0].moe
+    assert moe.w1 is None and moe.w2 is None and set(moe.mx4) == {"w1", "w2"}
+    before = moe.mx4["w1"].data.data_ptr()
+    other = _checkpoint(cfg, seed=1)
+    eng.stages[0].model.reload_layers(other)                       # online refit moves new blocks into the same storage
+    assert eng.stages[0].model.layers[0].moe.mx4["w1"].data.data_ptr() == before
+    _e, c, tc = _logits(cfg, other)
+    got = [lw.moe.mx4["w2"].unpack()[0] for lw in eng.stages[0].model.layers]
+    for i, w in enumerate(got):
+        assert torch.equal(w.view(-1), other[f"model.layers.{i}.mlp.experts.down_proj_blocks"].reshape(-1))
+
+
+@pytest.mark.parametrize("clipped", [False, True])
+def test_engine_quantises_experts_when_it_loads(clipped):
+    """Random weights: the engine with 4-bit experts is the one whose experts hold the quantised values."""
+    from parallax_b200.engine.engine import Engine
+    from parallax_b200.models.config import config_from_hf
+
+    cfg = _gpt_oss() if clipped else config_from_hf(dict(
+        architectures=["Qwen3MoeForCausalLM"], model_type="qwen3_moe", hidden_size=128, num_hidden_layers=2, num_attention_heads=4,
+        num_key_value_heads=2, head_dim=32, intermediate_size=128, moe_intermediate_size=64, num_experts=4, num_experts_per_tok=2,
+        vocab_size=256, norm_topk_prob=True, rope_theta=1e4))
+    plain = Engine(cfg, device="cpu", num_blocks=32, page_size=16, max_batch_size=2)
+    packed = Engine(cfg, device="cpu", num_blocks=32, page_size=16, max_batch_size=2, expert_format="mxfp4")
+    x = torch.randn(5, cfg.hidden_size)
+    for lp, lq in zip(plain.stages[0].model.layers, packed.stages[0].model.layers):
+        for name in ("w1", "w2"):
+            w = getattr(lp.moe, name)
+            w.copy_(ops.expand_mx4_rows(*ops.quant_mx4_rows(w)))
+        assert torch.allclose(lp.moe.forward(x, x), lq.moe.forward(x, x), rtol=1e-4, atol=1e-5)
+
+
+def test_engine_refuses():
+    from parallax_b200.engine.engine import Engine
+    from parallax_b200.models.config import named_config
+
+    for cfg, fmt in ((named_config("tiny"), "mxfp4"), (_gpt_oss(), "int4"), (_gpt_oss(inner=96), "mxfp4")):
+        with pytest.raises(ValueError):
+            Engine(cfg, device="cpu", num_blocks=16, expert_format=fmt)
+    moe = Engine(_gpt_oss(), device="cpu", num_blocks=16, expert_format="mxfp4").stages[0].model.layers[0].moe
+    with pytest.raises(ValueError):
+        moe.shard_experts(0, 2)
+
+
+def test_launcher_refuses_several_processes():
+    from parallax_b200.args import parse_args
+    from parallax_b200.launch import run_scheduler_mode, run_standalone
+
+    args = parse_args(["--model-path", "tiny-moe", "--random-init", "--expert-format", "mxfp4", "--pp-size", "2"])
+    for run in (run_standalone, run_scheduler_mode):
+        with pytest.raises(ValueError):
+            run(args)

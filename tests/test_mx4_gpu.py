@@ -312,3 +312,37 @@ def test_refusals():
                  lambda: ops.linear_mx4(x.bfloat16(), ops.Mx4Weight.pack(*_matrix(64, 64, 0)))):
         with pytest.raises(ops.KernelError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------ engine
+@pytest.mark.parametrize("clipped", [False, True])
+def test_engine_with_packed_experts(clipped):
+    """Requests through the serving engine, and its experts' layers against the definition."""
+    from parallax_b200.engine.engine import Engine
+    from parallax_b200.engine.request import SamplingParams
+    from parallax_b200.models.config import config_from_hf
+
+    sizes = dict(hidden_size=512, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, head_dim=64, vocab_size=1024,
+                 num_experts_per_tok=4, max_position_embeddings=2048, rope_theta=10000.0)
+    if clipped:
+        cfg = config_from_hf(dict(architectures=["GptOssForCausalLM"], model_type="gpt_oss", intermediate_size=320, moe_intermediate_size=320,
+                                  num_local_experts=8, sliding_window=32, attention_bias=True,
+                                  layer_types=["sliding_attention", "full_attention"], **sizes))
+    else:
+        cfg = config_from_hf(dict(architectures=["Qwen3MoeForCausalLM"], model_type="qwen3_moe", intermediate_size=512,
+                                  moe_intermediate_size=192, num_experts=16, norm_topk_prob=True, **sizes))
+    plain = Engine(cfg, device=DEV + ":0", num_blocks=64, max_batch_size=4)
+    eng = Engine(cfg, device=DEV + ":0", num_blocks=64, max_batch_size=4, expert_format="mxfp4")
+    outs = eng.generate([list(range(5, 60)), [7, 8, 9]], SamplingParams(max_new_tokens=6, temperature=0.0, ignore_eos=True))
+    assert all(len(o) == 6 for o in outs)
+    assert eng.stages[0].model.weight_bytes() < plain.stages[0].model.weight_bytes()
+    for T in (1, 3, 50):
+        x = _normal(T, cfg.hidden_size, seed=T)
+        for lw in eng.stages[0].model.layers:
+            moe = lw.moe
+            ids, wts = moe.route(x.to(DEV))
+            E, w1, w2 = cfg.num_experts, moe.mx4["w1"], moe.mx4["w2"]
+            wide = [oracle.values(*(t.cpu() for t in w.unpack())).view(E, w.rows, w.cols) for w in (w1, w2)]
+            b = [None if t is None else t.cpu().view(E, -1) for t in (moe.b1, moe.b2)]
+            want = oracle.experts(x, ids.cpu(), wts.cpu(), *wide, x, clipped, moe.limit, *b)
+            oracle.within(moe.forward(x.to(DEV), x.to(DEV)), *want, T)
