@@ -14,7 +14,7 @@
 namespace {
 using namespace pxl;
 
-constexpr int kSets = 2, kThreads = (6 + 4 * kSets) * 32;  // (a set may be a stage or a buffer ahead of another: at least as many of each)
+constexpr int kSets = 2, kThreads = (6 + 4 * kSets) * 32;
 constexpr int kMaxBufs = 4;
 constexpr int kWeightBytes = 9216;  // a block of weights in a stage, filled up to 1024 bytes
 constexpr int kMaxStages = 8;
@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stage_bytes = kWeightBytes + g.bt * 256;
   float* staging = reinterpret_cast<float*>(smem + g.stages * stage_bytes);
-  int* first_tile = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(staging) + (SPLIT ? 0 : kStaging));
+  int* first_tile = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(staging) + (!SPLIT && g.epi != PXL_EPI_NONE ? kStaging : 0));
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBufs + 2 * 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
       if (++db == g.d_bufs) db = 0, d_phase ^= 1;
     }
   } else if (warp < 6) {
-    write_results<SPLIT>(g, first_tile, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem), staging, 0, 1, warp & 3,
-                         lane, static_cast<int>(threadIdx.x) - 64, abort_flag, status);
+    write_results<SPLIT, false>(g, first_tile, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem), staging, 0, 1, warp & 3,
+                         lane, abort_flag, status);
   } else {
     // ---- codes -> bf16 in tensor memory: sets of four warps take the blocks in turn, a set a whole block
     const int q = warp & 3, set = (warp - 6) >> 2, r = q * 32 + lane;
@@ -160,6 +160,11 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
     uint32_t phase = (set / g.stages) & 1, a_phase = 1 ^ ((set / a_bufs) & 1);
     for (int n = set; n < blocks; n += kSets) {
       const uint32_t at = smem_u32(smem) + stage * stage_bytes;
+      // First the buffer: that the product of a_bufs blocks ago is done says that every block up to it has been loaded, and with at
+      // least as many stages as buffers so has the one that the stage held before. Loads end in any order, and the other set's may be
+      // the later one: a wait for a phase whose predecessor is still open would return at once, with the stage half full.
+      if (!wait_parked(aempty0 + 8 * ab, a_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY)) break;
+      tc_fence_after_sync();
       if (!wait_parked(full0 + 8 * stage, phase, abort_flag, status, PXL_DEV_TIMEOUT_FULL)) break;
       uint32_t code[4][4], p;
 #pragma unroll
@@ -168,8 +173,6 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
                      : "=r"(code[h][0]), "=r"(code[h][1]), "=r"(code[h][2]), "=r"(code[h][3])
                      : "r"(at + r * 16 + h * (kTileRows * 16)));
       asm volatile("ld.shared.u32 %0, [%1];" : "=r"(p) : "r"(at + kCodeBytes + r * 4));
-      if (!wait_parked(aempty0 + 8 * ab, a_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_EMPTY)) break;
-      tc_fence_after_sync();
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const uint32_t p2 = mx4_power2(p, h);
@@ -222,10 +225,11 @@ int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w,
   int a_bufs = ((two ? 256 : 512) - g.d_bufs * g.d_cols) / 64;
   if (a_bufs > kMaxBufs) a_bufs = kMaxBufs;
   pxl_host::split_k(g, items, slots, 12, gemm_mx4_kernel<true>, kThreads);
-  const int stage_bytes = kWeightBytes + g.bt * 256, rest = 1024 + (g.offsets ? (g.experts + 1) * 4 : 0) + (g.splits > 1 ? 0 : kStaging);
+  const int stage_bytes = kWeightBytes + g.bt * 256, rest = 1024 + (g.offsets ? (g.experts + 1) * 4 : 0) + (g.splits == 1 && g.epi != PXL_EPI_NONE ? kStaging : 0);
   g.stages = ((two ? 113 * 1024 : pxl_host::kTileSmem) - 512 - rest) / stage_bytes;
   if (g.stages > kMaxStages) g.stages = kMaxStages;
-  if (g.stages < kSets) return PXL_ERR_TOO_LARGE;
+  if (a_bufs > g.stages) a_bufs = g.stages;  // (see the warps that expand)
+  if (a_bufs < kSets) return PXL_ERR_TOO_LARGE;
   int smem = rest + g.stages * stage_bytes;
   if (g.splits > 1 && smem < 1024 + g.bt * kPitch * 4) smem = 1024 + g.bt * kPitch * 4;
   CUtensorMap tmap;
@@ -269,7 +273,6 @@ PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, c
   // an expert with n rows has about n / bt + 1 / 2 tiles, each as long as bt + 48 rows: least at bt^2 = 96 n
   g.bt = 32;
   while (g.bt < 160 && static_cast<int64_t>(g.bt + 8) * (g.bt + 8) * E < 96ll * P) g.bt += 16;
-  g.vec = pxl_host::on16(C, (out_f32 ? 4 : 2) * ldc);
   const int64_t items = static_cast<int64_t>(g.n_blocks) * (pxl::ceil_div(P, g.bt) + (P < E ? P : E));  // at most
   return launch_product(x, ldx, P, K, w, 32, g, items, status, stream);
 }

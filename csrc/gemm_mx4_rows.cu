@@ -236,10 +236,9 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_rows_kernel(const __grid
     cp_async_wait<0>();
   } else {
     // (with the powers laid out ahead, both fours of warps write results)
-    const int group = LAID ? (warp - 2) >> 2 : 0, tid = (static_cast<int>(threadIdx.x) - 64) & 127;
-    float* const own = staging + group * (kStaging / 4);
-    write_results<SPLIT>(g, nullptr, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem), own, group,
-                         LAID ? 2 : 1, warp & 3, lane, tid, abort_flag, status);
+    const int group = LAID ? (warp - 2) >> 2 : 0;
+    write_results<SPLIT, true>(g, nullptr, i0, i_step, items, kb0 == 0, tmem, dfull0, dempty0, reinterpret_cast<float*>(smem),
+                               staging + group * (kStaging / 4), group, LAID ? 2 : 1, warp & 3, lane, abort_flag, status);
   }
 
   if constexpr (SPLIT) {

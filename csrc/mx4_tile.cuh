@@ -8,8 +8,13 @@
 namespace pxl {
 
 constexpr int kPitch = kTileRows + 4;  // floats of a token's results in shared memory
-constexpr int kChunk = 32;             // tokens whose results are staged at a time
-constexpr int kStaging = kChunk * kPitch * 4;
+constexpr int kChunk = 32;             // tokens whose results are written at a time
+constexpr int kStaging = kChunk * kPitch * 4;  // of the four warps that write (also: two chunks' halves of 64 rows)
+
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 
 // Warp-collective wait, the same result in every lane. The hardware parks the warp for up to the hint's time, so that a wait costs
 // three instructions: expanding 4-bit weights is bound by the instructions that a SM issues.
@@ -57,7 +62,7 @@ struct TileArgs {
   int splits, kb_per;      // SPLIT: CTAs of a cluster, one per range of K blocks
   const int* offsets;      // grouped: first row of every expert, and the end
   int experts;
-  int vec;                 // results and residual in whole 16-byte vectors
+  int vec;                 // SPLIT, STAGED: results and residual in whole 16-byte vectors
   int early;               // in a launch chain: the first weights are read ahead of the wait
 };
 
@@ -90,7 +95,7 @@ __device__ __forceinline__ Item item_of(int i, const TileArgs& g, const int* fir
   return it;
 }
 
-// Eight results of a token: columns c .. c + 7 of the block (of its 64 outputs, where it is gated).
+// SPLIT, STAGED: eight results of a token, columns c .. c + 7 of the block (of its 64 outputs, where it is gated), in bf16.
 __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool glu, int n_blk, int t, int c) {
   const int n0 = n_blk * (glu ? 64 : 128) + c, n_out = glu ? g.N / 2 : g.N;
   if (n0 >= n_out) return;
@@ -114,18 +119,6 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
         if (n0 + j < n_out) f[j] += __bfloat162float(r[j]);
     }
   }
-  if (g.out_f32) {
-    float* dst = static_cast<float*>(g.C) + t * g.ldc + n0;
-    if (whole) {
-      reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n0 + j < n_out) dst[j] = f[j];
-    return;
-  }
   bf16* dst = static_cast<bf16*>(g.C) + t * g.ldc + n0;
   if (whole) {
     bf16x8 o;
@@ -139,15 +132,19 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
   }
 }
 
-// Groups of four warps, one per quarter of the lanes, that take an accumulator's chunks of tokens in turn. The results go to shared memory as [token][weight row] (scaled, with the
-// bias) and from there to C; SPLIT: they stay there, for add_ranges. `tid`: 0 .. 127, `parts`: room for a tile's results (SPLIT).
-template <bool SPLIT>
+// Groups of four warps, one per quarter of the lanes, that take an accumulator's chunks of tokens in turn. A lane has a weight row.
+// A warp writes 32 neighbours of a token at a time; or (STAGED) a chunk goes through shared memory to be written in vectors of eight:
+// which pays where the products are quick (8111 x 12288 x 4096 in 4 bits on both sides 208 us, 222 without) and costs where they are
+// not (24008 rows of 128 experts in fp32, six blocks of K each: 427 us for the whole, 400 without; 8192 x 24576 x 4096 1.50 and 1.48
+// ms). Gate and up rows are 64 lanes apart: their warps hand each other half of a chunk's tokens. SPLIT: results stay in shared memory
+// as [token][weight row], for add_ranges. `parts`: room for a tile's results (SPLIT), `staging`: kStaging bytes (STAGED, gated).
+template <bool SPLIT, bool STAGED>
 __device__ __forceinline__ void write_results(const TileArgs& g, const int* first_tile, int i0, int i_step, int items, bool with_bias,
                                               uint32_t tmem, uint32_t dfull0, uint32_t dempty0, float* parts, float* staging, int group,
-                                              int groups, int q, int lane, int tid, volatile int* abort_flag, int* status) {
+                                              int groups, int q, int lane, volatile int* abort_flag, int* status) {
   const int r = q * 32 + lane;
   const bool glu = g.epi != PXL_EPI_NONE;
-  int db = 0;
+  int db = 0, buf = 0;
   uint32_t d_phase = 0;
   bool ok = true;
   for (int i = i0; i < items; i += i_step) {
@@ -162,26 +159,83 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
       uint32_t v[32];
       tmem_ld_32x32b_x32(tmem + db * g.d_cols + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
       tmem_ld_wait();
-      float* part = SPLIT ? parts + c0 * kPitch : staging;
       const int m = min(kChunk, it.rows - c0);
+      const int64_t t0 = it.row0 + c0;
+      if constexpr (SPLIT) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < m) part[j * kPitch + r] = __uint_as_float(v[j]) * factor + add;
-      if constexpr (!SPLIT) {
+        for (int j = 0; j < 32; ++j)
+          if (j < m) parts[(c0 + j) * kPitch + r] = __uint_as_float(v[j]) * factor + add;
+      } else if constexpr (STAGED) {
+        named_bar_sync(1 + group, 128);  // (the last chunk has been read)
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < m) staging[j * kPitch + r] = __uint_as_float(v[j]) * factor + add;
         named_bar_sync(1 + group, 128);
-        const int per = glu ? 8 : 16;
-        for (int e = tid; e < m * per; e += 128) {
-          const int t = e / per, c = e % per * 8;
+        for (int e = r; ok && e < m * 16; e += 128) {
+          const int t = e / 16, c = e % 16 * 8;
           float f[16];
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            if (h >= 2 && !glu) break;
-            const float4 x = *reinterpret_cast<const float4*>(part + t * kPitch + c + (h & 1) * 4 + (h >> 1) * 64);
+          for (int h = 0; h < 2; ++h) {
+            const float4 x = *reinterpret_cast<const float4*>(staging + t * kPitch + c + h * 4);
             f[4 * h] = x.x, f[4 * h + 1] = x.y, f[4 * h + 2] = x.z, f[4 * h + 3] = x.w;
           }
-          if (ok) finish8(g, f, glu, it.n_blk, it.row0 + c0 + t, c);
+          finish8(g, f, false, it.n_blk, it.row0 + c0 + t, c);
         }
-        named_bar_sync(1 + group, 128);
+      } else if (!glu) {
+        if (!ok || n >= g.N) continue;
+        // (one kind of loop each: a choice per result, or its address from scratch, doubles the whole kernel's time)
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) * factor + add;
+        if (g.residual) {
+          const bf16* res = g.residual + t0 * g.ldr + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j >= m) break;
+            y[j] += __bfloat162float(res[j * g.ldr]);
+          }
+        }
+        if (g.out_f32) {
+          float* dst = static_cast<float*>(g.C) + t0 * g.ldc + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j >= m) break;
+            dst[j * g.ldc] = y[j];
+          }
+        } else {
+          bf16* dst = static_cast<bf16*>(g.C) + t0 * g.ldc + n;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j >= m) break;
+            dst[j * g.ldc] = __float2bfloat16(y[j]);
+          }
+        }
+      } else {
+        float* const mine = staging + buf * (kChunk * 64) + (r & 63);
+        const int col = it.n_blk * 64 + (r & 63);
+        auto half = [&](auto up) {  // gate rows give away tokens 16 .. 31 of the chunk, up rows 0 .. 15
+          constexpr bool kUp = decltype(up)::value;
+          constexpr int kGive = kUp ? 0 : 16, kKeep = kUp ? 16 : 0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) mine[(kGive + j) * 64] = __uint_as_float(v[kGive + j]) * factor + add;
+          named_bar_sync(1 + group, 128);  // (the buffer's readers of two chunks ago have met at the one before)
+          if (!ok) return;
+          float y[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float own = __uint_as_float(v[kKeep + j]) * factor + add, other = mine[(kKeep + j) * 64];
+            y[j] = kUp ? mx4_gate(other, own, g.epi, g.limit) : mx4_gate(own, other, g.epi, g.limit);
+          }
+          bf16* dst = static_cast<bf16*>(g.C) + (t0 + kKeep) * g.ldc + col;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (kKeep + j >= m) break;
+            dst[j * g.ldc] = __float2bfloat16(y[j]);
+          }
+        };
+        if (q >= 2) half(Bool<true>());
+        else half(Bool<false>());
+        buf ^= 1;
       }
     }
     tc_fence_before_sync();

@@ -190,6 +190,25 @@ def test_strides_and_unaligned_operands(T):
     oracle.within(ops.linear_mx4(x.to(DEV), w, b.to(DEV), acc, out=acc), *want, "in place")
 
 
+@pytest.mark.parametrize("T,N,K,act", [(203, 5120, 25600, ""), (256, 5120, 8192, ""), (230, 2560, 12800, "silu"), (13, 25600, 5120, "silu"),
+                                       (60, 25600, 5120, ""), (90, 12800, 5120, ""), (1000, 5120, 5120, ""), (8192, 12288, 4096, "silu")])
+def test_large_products_again_and_again(T, N, K, act):
+    """Every SM loads at full rate, so that loads end in any order: the same bits every time, and samples against 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device=DEV)
+    scales = torch.randint(112, 120, (N, K // 32), generator=g, dtype=torch.uint8, device=DEV)
+    x = torch.randn(T, K, generator=g, device=DEV).bfloat16()
+    w = ops.Mx4Weight.pack(codes, scales)
+    first = ops.linear_mx4(x, w, epi=EPIS[act])
+    for _ in range(10):
+        assert torch.equal(ops.linear_mx4(x, w, epi=EPIS[act]), first)
+    tokens = torch.randperm(T)[:32]
+    rows = torch.arange(N).view(-1, 128)[torch.randperm(N // 128)[:2]].flatten()       # two blocks of weight rows
+    want = oracle.linear(x.cpu()[tokens].double(), oracle.values(codes.cpu()[rows], scales.cpu()[rows]), act=act)
+    cols = rows if not act else (rows.view(-1, 128)[:, :1] // 2 + torch.arange(64)).flatten()
+    oracle.within(first.cpu()[tokens][:, cols], *want)
+
+
 # ------------------------------------------------------------------------------------------------ both operands in 4 bits
 @pytest.mark.parametrize("T,N,K", SIZES)
 def test_product_of_codes(T, N, K):
