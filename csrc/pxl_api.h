@@ -313,6 +313,7 @@ int pxl_gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_sca
 // Routed gated experts of a few tokens, every pair of a token and an expert on its own: h [T * top, I] (scratch, 16-byte aligned) and
 // out [T, K] = base (optional) + sum_j weights[t, j] FFN_{ids[t, j]}(x[t]); w1 [E * 2 I, K] with gate / up rows in groups of 64, w2
 // [E * K, I]. epi PXL_EPI_SILU_MUL or PXL_EPI_CLIP_GLU; ids outside of [0, E) add nothing.
+int pxl_moe_mx4_few_takes(int T, int top, int K, int I);  // whether it is the faster way
 int pxl_moe_mx4_few(const void* x, int64_t ldx, const int* ids, const float* weights, const void* w1, const float* row_scale1,
                     const void* b1, const void* w2, const float* row_scale2, const void* b2, const void* base, void* h, void* out, int T,
                     int top, int E, int K, int I, int epi, float limit, pxl_stream_t stream);

@@ -115,6 +115,7 @@ _SIGS = {
     "pxl_mx4_pack": [_P, _P, _P, _P, c_int, c_int, c_int, _P],
     "pxl_gemm_mx4": [_P, c_int64, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_float, _P, _P],
     "pxl_gemm_mx4_grouped": [_P, c_int64, _P, _P, _P, c_int64, c_int, _P, c_int, c_int, c_int, c_int, _P, c_int, c_float, _P, _P],
+    "pxl_moe_mx4_few_takes": [c_int] * 4,
     "pxl_moe_mx4_few": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P],
     "pxl_gemm_mx4_rows": [_P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, _P, c_int64, _P, _P],
     "pxl_gemm_mx4_rows_workspace": [c_int] * 3,

@@ -1062,11 +1062,11 @@ def _on(device: torch.device):
 
 
 def _bf16_rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """Rows as TMA reads them: a copy where their base or stride is not a multiple of 16 bytes."""
+    """Rows as TMA reads them: a copy where they overlap, or their base or stride is not a multiple of 16 bytes."""
     if x.dtype is not torch.bfloat16:
         mx4.refuse(what, f"the kernels take bf16 rows, got {x.dtype}")
     s0, s1 = x.stride()
-    return x if s1 == 1 and not s0 & 7 and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
+    return x if s1 == 1 and not s0 & 7 and s0 >= x.shape[1] and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -1166,9 +1166,6 @@ def _grouped_mx4(a, w: Mx4Weight, plan: MoEPlan, epi: int, bias, limit: float, d
     return out
 
 
-_FEW_PAIRS = 8
-
-
 def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: Mx4Weight, w2: Mx4Weight,
                 base: Optional[torch.Tensor] = None, act_mode: int = 0, limit: float = 7.0, b1: Optional[torch.Tensor] = None,
                 b2: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1179,7 +1176,7 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
     if T == 0:
         return out
     epi = EPI_CLIP_GLU if act_mode else EPI_SILU_MUL
-    if T * k <= _FEW_PAIRS:
+    if _lib.lib().pxl_moe_mx4_few_takes(T, k, K, w2.cols):
         h = torch.empty((T * k, w2.cols), dtype=torch.bfloat16, device=x.device)
         with _on(x.device):
             check(_lib.lib().pxl_moe_mx4_few(x.data_ptr(), x.stride(0), ids.data_ptr(), weights.data_ptr(), w1.data.data_ptr(),

@@ -171,6 +171,8 @@ def check_product(what: str, device: torch.device, T: int, N: int, K: int, K_w: 
         _check_operand(residual, "residual", (T, n_out), dtype, device, what)
     if out is not None:
         _check_operand(out, "out", (T, n_out), dtype, device, what)
+        if T > 1 and out.stride(0) < n_out:
+            refuse(what, "rows of out overlap")
     return n_out
 
 

@@ -68,7 +68,7 @@ def test_quantisation_on_borders_and_extremes():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantisation_of_strided_and_unaligned_rows(dtype):
     base = _normal(9, 300, dtype=dtype).to(DEV)
-    for x in (base[:, 8:104], base[:, 1:97], base[1:, 3:35], base[:, :96].t().contiguous().t(), base[:, ::2][:, :96]):
+    for x in (base[:1, 5:37].expand(7, 32), base[:, 8:104], base[:, 1:97], base[1:, 3:35], base[:, :96].t().contiguous().t(), base[:, ::2][:, :96]):
         want = ops.reference.quant_mx4_rows(x.cpu())
         got = ops.quant_mx4_rows(x)
         assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
@@ -186,6 +186,12 @@ def test_strides_and_unaligned_operands(T):
         assert ops.linear_mx4(x.to(DEV), w, bias, res[:, at + 1:at + 1 + N], out=out) is out
         oracle.within(out, *want, at)
         assert bool((dst[:, :at] == 7).all()) and bool((dst[:, at + N:] == 7).all())
+    one = x[:1].expand(T, K)                            # rows that are one and the same, and a residual that is
+    want = oracle.linear(one.double(), oracle.values(codes, scales), b, r[:1].expand(T, N))
+    oracle.within(ops.linear_mx4(x[:1].to(DEV).expand(T, K), w, b.to(DEV), r[:1].to(DEV).expand(T, N)), *want, "expanded")
+    with pytest.raises(ops.KernelError):
+        ops.linear_mx4(x.to(DEV), w, out=torch.zeros(1, N, dtype=torch.bfloat16, device=DEV).expand(T, N))
+    want = oracle.linear(x.double(), oracle.values(codes, scales), b, r)
     acc = r.to(DEV)                                     # the residual is written in place
     oracle.within(ops.linear_mx4(x.to(DEV), w, b.to(DEV), acc, out=acc), *want, "in place")
 
@@ -269,6 +275,37 @@ def test_experts(T, E, k, K, I, clip):
         got = ops.moe_ffn_mx4(*_dev(x, ids, wts), w1, w2, base=None if bs is None else bs.to(DEV), act_mode=int(clip), limit=1.5,
                               b1=None if b1 is None else b1.to(DEV), b2=None if b2 is None else b2.to(DEV))
         oracle.within(got, *want, (T, E, bs is None))
+
+
+@pytest.mark.parametrize("T,E,k,K,I", [(1, 5, 1, 32, 64), (2, 8, 4, 2880, 192), (3, 4, 5, 352, 320), (8, 6, 2, 4096, 64), (1, 3, 16, 160, 1024)])
+def test_experts_of_a_few_pairs(T, E, k, K, I):
+    """Every pair on its own: experts twice in a row, none, and NaN weights and scales of experts that are not asked."""
+    x, base, c1, s1, c2, s2, b1, b2, _ids, wts = _experts_case(T, E, min(k, E), K, I, seed=T + 50)
+    g = torch.Generator().manual_seed(k)
+    ids, wts = torch.randint(0, E - 1, (T, k), generator=g).int(), torch.rand(T, k, generator=g)
+    ids[0, 0], wts[0, 0] = (E if k > 1 else 0), (float("nan") if k > 1 else 0.5)
+    ids[-1, -1] = -1 if k > 1 or T > 1 else 0
+    s1.view(E, -1)[E - 1], s2.view(E, -1)[E - 1] = 255, 255
+    w1, w2 = ops.Mx4Weight.pack(*_dev(c1, s1), experts=E), ops.Mx4Weight.pack(*_dev(c2, s2), experts=E)
+    want = oracle.experts(x, ids, wts, oracle.values(c1, s1).view(E, 2 * I, K), oracle.values(c2, s2).view(E, K, I), base, True, 1.5,
+                          b1.view(E, -1), b2.view(E, -1))
+    from parallax_b200.ops import _lib
+
+    assert _lib.lib().pxl_moe_mx4_few_takes(T, k, K, I) == 1
+    got = ops.moe_ffn_mx4(*_dev(x, ids, wts), w1, w2, base=base.to(DEV), act_mode=1, limit=1.5, b1=b1.to(DEV), b2=b2.to(DEV))
+    oracle.within(got, *want)
+
+
+def test_experts_too_wide_for_shared_memory():
+    """Few pairs, but more columns of the inner rows than the direct form holds: the sorted form takes them."""
+    from parallax_b200.ops import _lib
+
+    T, E, k, K, I = 1, 2, 2, 32, 401408
+    assert _lib.lib().pxl_moe_mx4_few_takes(T, k, K, I) == 0
+    x, base, c1, s1, c2, s2, _b1, _b2, ids, wts = _experts_case(T, E, k, K, I, seed=3, biases=False)
+    w1, w2 = ops.Mx4Weight.pack(*_dev(c1, s1), experts=E), ops.Mx4Weight.pack(*_dev(c2, s2), experts=E)
+    want = oracle.experts(x, ids, wts, oracle.values(c1, s1).view(E, 2 * I, K), oracle.values(c2, s2).view(E, K, I), base, False, 1.5, None, None)
+    oracle.within(ops.moe_ffn_mx4(*_dev(x, ids, wts), w1, w2, base=base.to(DEV)), *want)
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, repeats
