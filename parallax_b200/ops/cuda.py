@@ -1154,15 +1154,13 @@ def linear_mx4_rows(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Te
     return out
 
 
-def _grouped_mx4(a, w: Mx4Weight, plan: MoEPlan, epi: int, bias, limit: float, dtype) -> torch.Tensor:
-    """Expert-sorted rows ``a [P, K]`` times stacked microscaled expert weights."""
+def _grouped_mx4(a: torch.Tensor, w: Mx4Weight, offsets: int, P: int, epi: int, bias, limit: float, dtype, status: int, stream: int):
+    """Expert-sorted rows ``a [P, K]`` times stacked microscaled expert weights (``offsets``: address of the experts' first rows)."""
     n_out = w.rows // 2 if epi != EPI_NONE else w.rows
-    out = torch.empty((plan.max_rows, n_out), dtype=dtype, device=a.device)
-    check(_lib.lib().pxl_gemm_mx4_grouped(a.data_ptr(), a.stride(0), w.data.data_ptr(), w.row_scale.data_ptr(), out.data_ptr(), n_out,
-                                          int(dtype == torch.float32), _ptr(bias), plan.max_rows, w.experts, w.rows, w.cols,
-                                          plan.offsets.data_ptr(), epi, limit, status_tensor(a.device).data_ptr(), _stream(a.device)),
-          "pxl_gemm_mx4_grouped")
-    _count()
+    out = torch.empty((P, n_out), dtype=dtype, device=a.device)
+    check(_lib.lib().pxl_gemm_mx4_grouped(a.data_ptr(), w.cols, w.data.data_ptr(), w.row_scale.data_ptr(), out.data_ptr(), n_out,
+                                          int(dtype is torch.float32), _ptr(bias), P, w.experts, w.rows, w.cols, offsets, epi, limit,
+                                          status, stream), "pxl_gemm_mx4_grouped")
     return out
 
 
@@ -1185,13 +1183,26 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
                                              _stream(x.device)), "pxl_moe_mx4_few")
         _count(2)
         return out
-    with _on(x.device):
-        plan = moe_align(ids, w1.experts)
-        act = _grouped_mx4(moe_gather(x, plan), w1, plan, epi, b1, limit, torch.bfloat16)
-        y = _grouped_mx4(act, w2, plan, EPI_NONE, b2, 0.0, torch.float32)
-        check(_lib.lib().pxl_moe_combine_f32(y.data_ptr(), plan.pos_of.data_ptr(), weights.data_ptr(), _ptr(base), out.data_ptr(), T, k,
-                                             K, _stream(x.device)), "pxl_moe_combine_f32")
-    _count()
+    # (the lists of pxl_moe_align in one buffer, by their addresses: a tensor for each costs as much host time as the launches)
+    dev, E, P, L = x.device, w1.experts, T * k, _lib.lib()
+    tiles = (P + 127) // 128 + E
+    alone = L.pxl_moe_align_alone(T, k)
+    lists = (torch.empty if alone else torch.zeros)(3 * E + 2 + 3 * tiles + 2 * P, dtype=torch.int32, device=dev)
+    at = lists.data_ptr()
+    counts, cursor, offsets, mt = at, at + 4 * E, at + 8 * E, at + 4 * (3 * E + 1)
+    num_mt = mt + 12 * tiles
+    pos_of, src_tok = num_mt + 4, num_mt + 4 + 4 * P
+    with _on(dev):
+        stream, status = _stream(dev), status_tensor(dev).data_ptr()
+        check(L.pxl_moe_align(ids.data_ptr(), T, k, E, 0, E, counts, offsets, cursor, mt, mt + 4 * tiles, mt + 8 * tiles, num_mt, tiles,
+                              pos_of, src_tok, stream), "pxl_moe_align")
+        xp = torch.empty((P, K), dtype=torch.bfloat16, device=dev)
+        check(L.pxl_moe_gather(x.data_ptr(), src_tok, offsets + 4 * E, xp.data_ptr(), P, K, stream), "pxl_moe_gather")
+        act = _grouped_mx4(xp, w1, offsets, P, epi, b1, limit, torch.bfloat16, status, stream)
+        y = _grouped_mx4(act, w2, offsets, P, EPI_NONE, b2, 0.0, torch.float32, status, stream)
+        check(L.pxl_moe_combine_f32(y.data_ptr(), pos_of, weights.data_ptr(), _ptr(base), out.data_ptr(), T, k, K, stream),
+              "pxl_moe_combine_f32")
+    _count(5 if alone else 7)
     return out
 
 
