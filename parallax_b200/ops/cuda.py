@@ -1079,8 +1079,8 @@ def quant_mx4_rows(x: torch.Tensor):
     T, K = mx4.check_rows(x, "quant_mx4_rows")
     x = x if x.stride(1) == 1 else x.contiguous()
     dev = x.device
-    codes = torch.empty((T, K // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty((T, K // 32), dtype=torch.uint8, device=dev)
+    codes = x.new_empty((T, K // 2), dtype=torch.uint8)
+    scales = x.new_empty((T, K // 32), dtype=torch.uint8)
     with _on(dev):
         check(_lib.lib().pxl_mx4_quant_rows(x.data_ptr(), int(x.dtype is torch.float32), x.stride(0), codes.data_ptr(),
                                             scales.data_ptr(), T, K, _stream(dev)), "pxl_mx4_quant_rows")
