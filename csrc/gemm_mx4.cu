@@ -84,10 +84,11 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
   };
   auto stage_tx = [&](const Item& it) { return static_cast<uint32_t>(kBlockBytes + ceil_div(it.rows, box) * box * 256); };
 
-  const bool early = g.early && i0 < items;  // (never with experts, whose lists are written in the chain)
-  if (warp == 0 && lane == 0 && early) {
+  // blocks whose weights are read ahead: of the first tile (never with experts, whose lists are written in the chain)
+  const int ahead = g.early && i0 < items ? min(g.stages, kb1 - kb0) : 0;
+  if (warp == 0 && lane == 0 && ahead > 0) {
     const Item it = item_of(i0, g, first_tile);
-    for (int s = 0; s < g.stages && kb0 + s < kb1; ++s) {
+    for (int s = 0; s < ahead; ++s) {
       mbar_arrive_expect_tx(full0 + 8 * s, stage_tx(it));
       bulk_load_g2s(smem_u32(smem + s * stage_bytes), weights(it, kb0 + s), kBlockBytes, full0 + 8 * s);
     }
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
       const int boxes = ceil_div(it.rows, box);
       for (int kb = kb0; kb < kb1; ++kb, ++done) {
         const uint32_t fb = full0 + 8 * stage, at = s0 + stage * stage_bytes;
-        if (!early || done >= g.stages) {
+        if (done >= ahead) {
           ok = wait_parked(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
           expect_tx(fb, stage_tx(it), leader);

@@ -111,31 +111,22 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_rows_kernel(const __grid
   const int kb1 = SPLIT ? min(kb0 + g.kb_per, g.k_blocks) : g.k_blocks;
 
   const uint32_t stage_tx = stage_bytes + (LAID ? power_bytes : 0);
-  if (warp == 0 && lane == 0 && g.early) {
-    const Item it = item_of(i0, g, nullptr);
-    for (int s = 0; s < g.stages && kb0 + s < kb1; ++s) {
-      mbar_arrive_expect_tx(full0 + 8 * s, stage_tx);
-      tma_load_2d(smem_u32(smem) + s * stage_bytes, &tmap_w, full0 + 8 * s, (kb0 + s) * (kStep / 2), it.n_blk * kTileRows);
-    }
-  }
-  pdl_wait();
+  pdl_wait();  // (either operand may be of rows that the kernel before quantises)
   pdl_launch_dependents();
 
   if (warp == 0) {
     const uint32_t leader = elect_leader(), s0 = smem_u32(smem);
-    int stage = 0, done = 0;
+    int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int i = i0; ok && i < items; i += i_step) {
       const Item it = item_of(i, g, nullptr);
-      for (int kb = kb0; kb < kb1; ++kb, ++done) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         const uint32_t fb = full0 + 8 * stage, at = s0 + stage * stage_bytes;
-        if (!g.early || done >= g.stages) {
-          ok = wait_parked(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
-          if (!ok) break;
-          expect_tx(fb, stage_tx, leader);
-          tma_box(at, &tmap_w, fb, kb * (kStep / 2), it.n_blk * kTileRows, leader);
-        }
+        ok = wait_parked(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
+        if (!ok) break;
+        expect_tx(fb, stage_tx, leader);
+        tma_box(at, &tmap_w, fb, kb * (kStep / 2), it.n_blk * kTileRows, leader);
         tma_box(at + kCodes, &tmap_x, fb, kb * (kStep / 2), it.row0, leader);
         if (LAID && leader) {
           const uint32_t to = smem_u32(powers) + stage * power_bytes;

@@ -63,7 +63,7 @@ struct TileArgs {
   const int* offsets;      // grouped: first row of every expert, and the end
   int experts;
   int vec;                 // SPLIT, STAGED: results and residual in whole 16-byte vectors
-  int early;               // in a launch chain: the first weights are read ahead of the wait
+  int early;               // in a launch chain: weights of the first tile may be read ahead of the wait
 };
 
 struct Item {

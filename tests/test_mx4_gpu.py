@@ -360,6 +360,23 @@ def test_layer_on_another_stream_in_a_chain_and_in_graphs(T):
     assert torch.equal(graphs[0][1], want_a) and torch.equal(graphs[1][1], want_b)
 
 
+@pytest.mark.parametrize("T,N,K", [(300, 40000, 64), (1000, 20000, 32), (20, 60000, 96), (60, 40000, 224), (2, 60000, 64)])
+def test_many_short_tiles_in_a_chain(T, N, K):
+    """Weights are read ahead of a kernel's turn, here more blocks of them than its first tile has."""
+    from parallax_b200.ops import cuda as cu
+
+    x, r = _normal(T, K, seed=1).to(DEV), _normal(T, N, seed=2).to(DEV)
+    codes, scales = _dev(*_matrix(N, K, 3))
+    w, xq = ops.Mx4Weight.pack(codes, scales), ops.quant_mx4_rows(x)
+    want, want44 = ops.linear_mx4(x, w, residual=r), ops.linear_mx4_rows(*xq, codes, scales, residual=r)
+    torch.cuda.synchronize()
+    with cu.launch_chain():
+        got = [ops.linear_mx4(x, w, residual=r) for _ in range(3)]
+        got44 = [ops.linear_mx4_rows(*xq, codes, scales, residual=r) for _ in range(3)]
+    assert all(torch.equal(y, want) for y in got) and all(torch.equal(y, want44) for y in got44)
+    oracle.within(want, *oracle.linear(x.cpu().double(), oracle.values(codes.cpu(), scales.cpu()), residual=r.cpu()))
+
+
 def test_refusals():
     x = torch.zeros(2, 64, device=DEV)
     w = ops.Mx4Weight.pack(*_dev(*_matrix(64, 64, 0)))
