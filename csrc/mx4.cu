@@ -240,6 +240,7 @@ PXL_EXPORT int pxl_mx4_expand_rows(const void* codes, const void* scales, void* 
   if (blocks > 0x7fffffff) return PXL_ERR_TOO_LARGE;
   pxl_host::launch(mx4_expand_rows_kernel, static_cast<unsigned>(blocks), 256, 0, stream, static_cast<const uint8_t*>(codes),
                    static_cast<const uint8_t*>(scales), static_cast<bf16*>(out), words);
+  pxl_host::next_launch_follows_whole();  // (the rows may be weights)
   return check_launch();
 }
 
@@ -268,5 +269,6 @@ PXL_EXPORT int pxl_mx4_pack(const void* codes, const void* scales, void* data, f
                      static_cast<const uint8_t*>(codes) + e * N * groups * 16, static_cast<const uint8_t*>(scales) + e * N * groups,
                      row_scale + e * n_blocks * kTileRows, static_cast<uint8_t*>(data) + e * n_blocks * k_blocks * kBlockBytes, N, groups, n_blocks, k_blocks);
   }
+  pxl_host::next_launch_follows_whole();
   return check_launch();
 }

@@ -377,6 +377,26 @@ def test_many_short_tiles_in_a_chain(T, N, K):
     oracle.within(want, *oracle.linear(x.cpu().double(), oracle.values(codes.cpu(), scales.cpu()), residual=r.cpu()))
 
 
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_weights_made_inside_a_chain(T):
+    from parallax_b200.ops import cuda as cu
+
+    x, weight = _normal(T, 512, seed=1).to(DEV), _normal(640, 512, seed=2).to(DEV)
+    q = ops.quant_mx4_rows(weight)
+    want = ops.linear_mx4(x, ops.Mx4Weight.pack(*q)), ops.linear_mx4_rows(*ops.quant_mx4_rows(x), *q), ops.linear(x, ops.expand_mx4_rows(*q))
+    torch.cuda.synchronize()
+    with cu.launch_chain():
+        rows = ops.quant_mx4_rows(x)
+        got = ops.linear_mx4_rows(*rows, *ops.quant_mx4_rows(weight))
+        assert torch.equal(got, want[1])
+    for _ in range(3):
+        with cu.launch_chain():
+            q = ops.quant_mx4_rows(weight)
+            a = ops.linear_mx4(x, ops.Mx4Weight.pack(*q))
+            c = ops.linear(x, ops.expand_mx4_rows(*q))
+        assert torch.equal(a, want[0]) and torch.equal(c, want[2])
+
+
 def test_refusals():
     x = torch.zeros(2, 64, device=DEV)
     w = ops.Mx4Weight.pack(*_dev(*_matrix(64, 64, 0)))
