@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
 
 int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w, int box, TileArgs g, int64_t items, int* status,
                    cudaStream_t stream) {
+  if (g.bt % box) return PXL_ERR_INVALID_ARG;  // (whole boxes fill a stage's rows of x, and nothing behind them)
   static bool configured[64] = {};
   if (!pxl_host::allow_smem(configured, gemm_mx4_kernel<false>, gemm_mx4_kernel<true>)) return PXL_ERR_CUDA;
   if (items > 0x7fffffff) items = 0x7fffffff;
@@ -275,5 +276,5 @@ PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, c
   g.bt = 32;
   while (g.bt < 160 && static_cast<int64_t>(g.bt + 8) * (g.bt + 8) * E < 96ll * P) g.bt += 16;
   const int64_t items = static_cast<int64_t>(g.n_blocks) * (pxl::ceil_div(P, g.bt) + (P < E ? P : E));  // at most
-  return launch_product(x, ldx, P, K, w, 32, g, items, status, stream);
+  return launch_product(x, ldx, P, K, w, g.bt % 32 ? 16 : 32, g, items, status, stream);
 }

@@ -296,6 +296,21 @@ def test_experts_of_a_few_pairs(T, E, k, K, I):
     oracle.within(got, *want)
 
 
+@pytest.mark.parametrize("T", [35, 60, 80, 111, 144, 201, 260, 330, 440, 700])
+def test_experts_of_every_tile_height(T):
+    """Rows per expert from a few to two tiles' worth, evenly over the experts and nearly all on one."""
+    E, k, K, I = 4, 2, 1056, 192
+    x, base, c1, s1, c2, s2, _b1, _b2, ids, wts = _experts_case(T, E, k, K, I, seed=T, biases=False)
+    w1, w2 = ops.Mx4Weight.pack(*_dev(c1, s1), experts=E), ops.Mx4Weight.pack(*_dev(c2, s2), experts=E)
+    v1, v2 = oracle.values(c1, s1).view(E, 2 * I, K), oracle.values(c2, s2).view(E, K, I)
+    skewed = ids.clone()
+    skewed[3:, 0], skewed[3:, 1] = 2, 2
+    for which in (ids, skewed):
+        want = oracle.experts(x, which, wts, v1, v2, base, False, 1.5, None, None)
+        for _ in range(3):
+            oracle.within(ops.moe_ffn_mx4(*_dev(x, which, wts), w1, w2, base=base.to(DEV)), *want)
+
+
 def test_experts_too_wide_for_shared_memory():
     """Few pairs, but more columns of the inner rows than the direct form holds: the sorted form takes them."""
     from parallax_b200.ops import _lib
