@@ -21,7 +21,7 @@ constexpr int kMaxStages = 8;
 constexpr int kMaxExperts = 1024;
 
 template <bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmap, const uint8_t* __restrict__ w, int box,
+__global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_constant__ CUtensorMap tmap, const uint8_t* __restrict__ w,
                                                                 int a_bufs, const Mx4Shift shift, int* status, const TileArgs g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -82,14 +82,14 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
   auto weights = [&](const Item& it, int kb) {
     return w + ((static_cast<int64_t>(it.expert) * g.n_blocks + it.n_blk) * g.k_blocks + kb) * kBlockBytes;
   };
-  auto stage_tx = [&](const Item& it) { return static_cast<uint32_t>(kBlockBytes + ceil_div(it.rows, box) * box * 256); };
+  const uint32_t stage_tx = kBlockBytes + g.bt * 256;
 
   // blocks whose weights are read ahead: of the first tile (never with experts, whose lists are written in the chain)
   const int ahead = g.early && i0 < items ? min(g.stages, kb1 - kb0) : 0;
   if (warp == 0 && lane == 0 && ahead > 0) {
     const Item it = item_of(i0, g, first_tile);
     for (int s = 0; s < ahead; ++s) {
-      mbar_arrive_expect_tx(full0 + 8 * s, stage_tx(it));
+      mbar_arrive_expect_tx(full0 + 8 * s, stage_tx);
       bulk_load_g2s(smem_u32(smem + s * stage_bytes), weights(it, kb0 + s), kBlockBytes, full0 + 8 * s);
     }
   }
@@ -103,20 +103,17 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
     bool ok = true;
     for (int i = i0; ok && i < items; i += i_step) {
       const Item it = item_of(i, g, first_tile);
-      const int boxes = ceil_div(it.rows, box);
       for (int kb = kb0; kb < kb1; ++kb, ++done) {
         const uint32_t fb = full0 + 8 * stage, at = s0 + stage * stage_bytes;
         if (done >= ahead) {
           ok = wait_parked(empty0 + 8 * stage, phase ^ 1, abort_flag, status, PXL_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
-          expect_tx(fb, stage_tx(it), leader);
+          expect_tx(fb, stage_tx, leader);
           if (leader) bulk_load_g2s(at, weights(it, kb), kBlockBytes, fb);
         }
-        for (int b = 0; b < boxes; ++b) {
-          const uint32_t dst = at + kWeightBytes + b * box * 128;
-          tma_box(dst, &tmap, fb, kb * kTileCols, it.row0 + b * box, leader);
-          tma_box(dst + g.bt * 128, &tmap, fb, kb * kTileCols + 64, it.row0 + b * box, leader);
-        }
+        // (rows behind an expert's last one come along: less costly than more and smaller boxes)
+        tma_box(at + kWeightBytes, &tmap, fb, kb * kTileCols, it.row0, leader);
+        tma_box(at + kWeightBytes + g.bt * 128, &tmap, fb, kb * kTileCols + 64, it.row0, leader);
         if (++stage == g.stages) stage = 0, phase ^= 1;
       }
     }
@@ -212,9 +209,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_mx4_kernel(const __grid_cons
   if (warp == 1) tmem_dealloc(tmem, tmem_cols);
 }
 
-int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w, int box, TileArgs g, int64_t items, int* status,
+int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w, TileArgs g, int64_t items, int* status,
                    cudaStream_t stream) {
-  if (g.bt % box) return PXL_ERR_INVALID_ARG;  // (whole boxes fill a stage's rows of x, and nothing behind them)
   static bool configured[64] = {};
   if (!pxl_host::allow_smem(configured, gemm_mx4_kernel<false>, gemm_mx4_kernel<true>)) return PXL_ERR_CUDA;
   if (items > 0x7fffffff) items = 0x7fffffff;
@@ -235,9 +231,9 @@ int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w,
   int smem = rest + g.stages * stage_bytes;
   if (g.splits > 1 && smem < 1024 + g.bt * kPitch * 4) smem = 1024 + g.bt * kPitch * 4;
   CUtensorMap tmap;
-  if (!pxl_host::make_tmap_2d(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_rows, K, ldx, box, 64)) return PXL_ERR_TENSORMAP;
+  if (!pxl_host::make_tmap_2d(&tmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_rows, K, ldx, g.bt, 64)) return PXL_ERR_TENSORMAP;
   return pxl_host::launch_tiles(gemm_mx4_kernel<false>, gemm_mx4_kernel<true>, g, static_cast<int>(items), slots, kThreads, smem, stream,
-                                tmap, static_cast<const uint8_t*>(w), box, a_bufs, kMx4Shift, status);
+                                tmap, static_cast<const uint8_t*>(w), a_bufs, kMx4Shift, status);
 }
 
 bool epi_known(int epi, int N) {
@@ -259,7 +255,7 @@ PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const flo
   g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, pxl_host::tile_tokens(M, g.n_blocks, 160, 48));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   g.vec = pxl_host::on16(C, 2 * ldc) && (!residual || pxl_host::on16(residual, 2 * ldr));
-  return launch_product(x, ldx, M, K, w, g.bt, g, static_cast<int64_t>(g.n_blocks) * g.t_tiles, status, stream);
+  return launch_product(x, ldx, M, K, w, g, static_cast<int64_t>(g.n_blocks) * g.t_tiles, status, stream);
 }
 
 PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc,
@@ -272,9 +268,11 @@ PXL_EXPORT int pxl_gemm_mx4_grouped(const void* x, int64_t ldx, const void* w, c
   g.M = P, g.N = N, g.epi = epi, g.limit = limit;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kTileCols);
   g.offsets = offsets, g.experts = E;
-  // an expert with n rows has about n / bt + 1 / 2 tiles, each as long as bt + 48 rows: least at bt^2 = 96 n
+  // One tile for an expert of an eighth more rows than the mean, up to 160. Lower tiles expand the weights of more experts twice (32
+  // experts of 112 rows, 2880 x 2880, layer in us: 96 rows 347, 112 302, 128 252, 160 255), higher ones load rows that are not theirs
+  // and have fewer stages (of 30 rows: 48 157, 64 157, 80 169, 128 175; of 512: 128 929, 160 877, 192 916).
   g.bt = 32;
-  while (g.bt < 160 && static_cast<int64_t>(g.bt + 8) * (g.bt + 8) * E < 96ll * P) g.bt += 16;
+  while (g.bt < 160 && 8ll * g.bt * E < 9ll * P) g.bt += 16;
   const int64_t items = static_cast<int64_t>(g.n_blocks) * (pxl::ceil_div(P, g.bt) + (P < E ? P : E));  // at most
-  return launch_product(x, ldx, P, K, w, g.bt % 32 ? 16 : 32, g, items, status, stream);
+  return launch_product(x, ldx, P, K, w, g, items, status, stream);
 }
