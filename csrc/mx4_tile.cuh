@@ -150,8 +150,8 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
   for (int i = i0; i < items; i += i_step) {
     const Item it = item_of(i, g, first_tile);
     const int n = it.n_blk * kTileRows + r;
-    const float factor = g.row_scale ? g.row_scale[it.expert * g.n_blocks * kTileRows + n] : 1.f;
-    const float add = g.bias && n < g.N && with_bias ? __bfloat162float(g.bias[it.expert * g.N + n]) : 0.f;
+    const float factor = g.row_scale ? g.row_scale[static_cast<int64_t>(it.expert) * g.n_blocks * kTileRows + n] : 1.f;
+    const float add = g.bias && n < g.N && with_bias ? __bfloat162float(g.bias[static_cast<int64_t>(it.expert) * g.N + n]) : 0.f;
     // after a wait that ran out the loop goes on without results: the warps meet at every barrier below
     ok = ok && wait_parked(dfull0 + 8 * db, d_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
     tc_fence_after_sync();
