@@ -298,6 +298,7 @@ bool plan_rows(RowsPlan& p, int M, int N, int K) {
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kStep);
   g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, pxl_host::tile_tokens(M, g.n_blocks, 192, 24));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
+  g.t_group = g.t_tiles;
   p.items = static_cast<int64_t>(g.n_blocks) * g.t_tiles;
   const int sms = pxl_host::num_sms();
   const bool two = g.bt <= 64;  // CTAs per SM, as in gemm_mx4.cu

@@ -57,6 +57,7 @@ struct TileArgs {
   int M, N, epi, out_f32;
   float limit;
   int n_blocks, k_blocks, t_tiles;
+  int t_group;             // tiles of tokens that go through all weights together
   int bt;                  // tokens of a tile, a multiple of 16
   int stages, d_bufs, d_cols;
   int splits, kb_per;      // SPLIT: CTAs of a cluster, one per range of K blocks
@@ -70,13 +71,14 @@ struct Item {
   int n_blk, row0, rows, expert;
 };
 
-// Item i of the launch: a block of weight rows, and a tile of tokens. Tiles of tokens follow one another for a block of weights,
-// unless there are experts: then the blocks of an expert's weights follow for a tile.
+// Item i of the launch: a block of weight rows, and a tile of tokens. Tiles of tokens of a group follow one another for a block of
+// weights, unless there are experts: then the blocks of an expert's weights follow for a tile.
 __device__ __forceinline__ Item item_of(int i, const TileArgs& g, const int* first_tile) {
   Item it;
   if (g.offsets == nullptr) {
-    it.n_blk = i / g.t_tiles;
-    it.row0 = (i % g.t_tiles) * g.bt;
+    const int per = g.t_group * g.n_blocks, first = i / per * g.t_group, wide = min(g.t_group, g.t_tiles - first), at = i % per;
+    it.n_blk = at / wide;
+    it.row0 = (first + at % wide) * g.bt;
     it.rows = min(g.bt, g.M - it.row0);
     it.expert = 0;
     return it;
