@@ -146,9 +146,20 @@ def _check_operand(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype,
         refuse(what, f"{name} is {dtype} {shape} on {device} with neighbouring columns, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def check_product(what: str, device: torch.device, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices with neighbouring columns have a byte in common (for rows of unlike strides: may have one)."""
+    a0, b0, wa, wb = a.data_ptr(), b.data_ptr(), a.shape[1] * a.element_size(), b.shape[1] * b.element_size()
+    sa, sb = a.stride(0) * a.element_size(), b.stride(0) * b.element_size()
+    if a0 >= b0 + (b.shape[0] - 1) * sb + wb or b0 >= a0 + (a.shape[0] - 1) * sa + wa:
+        return False
+    apart = (b0 - a0) % sa if sa == sb and sa > 0 else 0       # columns of one buffer: b's behind a's, and before a's of the next row
+    return not (apart >= wa and apart + wb <= sa)
+
+
+def check_product(what: str, x: torch.Tensor, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
                   residual: Optional[torch.Tensor], epi: int, limit: float, out: Optional[torch.Tensor], dtype: torch.dtype) -> int:
     """Checks what the two products share; returns the number of output columns."""
+    device = x.device
     if K != K_w:
         refuse(what, f"rows of {K} columns and weights of {K_w}")
     n_out = N
@@ -173,6 +184,10 @@ def check_product(what: str, device: torch.device, T: int, N: int, K: int, K_w: 
         _check_operand(out, "out", (T, n_out), dtype, device, what)
         if T > 1 and out.stride(0) < n_out:
             refuse(what, "rows of out overlap")
+        # (the residual may be out itself: a result is written by the thread that has read its place)
+        if T > 0 and n_out > 0 and (_share_memory(x, out) or residual is not None and _share_memory(residual, out) and (
+                residual.data_ptr() != out.data_ptr() or residual.stride(0) != out.stride(0))):
+            refuse(what, "out overlaps the rows, or the residual in other places than its own")
     return n_out
 
 

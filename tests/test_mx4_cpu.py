@@ -166,6 +166,27 @@ def test_experts_refuse(kw):
         _expert_call(**kw)
 
 
+def test_results_that_share_memory():
+    """Refused, but for a residual's own place and other columns of the rows' buffer."""
+    codes, scales = _matrix(128, 128, 0)
+    w = ops.Mx4Weight.pack(codes, scales)
+    buf = torch.randn(6, 384, generator=torch.Generator().manual_seed(0)).bfloat16()
+    x, y = buf[:, :128], buf[:, 128:256]
+    want = ops.linear_mx4(x, w)
+    assert torch.equal(ops.linear_mx4(x, w, out=y), want) and torch.equal(y, want)
+    assert torch.equal(ops.linear_mx4(x[1:], w, out=buf[:5, 256:]), want[1:])
+    r = torch.randn(6, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    want = ops.linear_mx4(x, w, residual=r)
+    assert torch.equal(ops.linear_mx4(x, w, residual=r, out=r), want) and torch.equal(r, want)
+    flat = torch.zeros(2000, dtype=torch.bfloat16)
+    for call in (lambda: ops.linear_mx4(x, w, out=x), lambda: ops.linear_mx4(x, w, out=buf[:, 64:192]),
+                 lambda: ops.linear_mx4(buf[:, 256:], w, out=buf[:, 192:320]), lambda: ops.linear_mx4(x[:3], w, out=x[2:5]),
+                 lambda: ops.linear_mx4(x, w, residual=flat[:768].view(6, 128), out=flat[128:896].view(6, 128)),
+                 lambda: ops.linear_mx4(x, w, residual=flat[:768].view(6, 128), out=flat[:1536].view(6, 256)[:, :128])):
+        with pytest.raises(ops.KernelError):
+            call()
+
+
 def test_refusals():
     codes, scales = _matrix(128, 64, 0)
     w, x = ops.Mx4Weight.pack(codes, scales), torch.zeros(2, 64, dtype=torch.bfloat16)
