@@ -68,7 +68,7 @@ __device__ __forceinline__ void copy_word(uint32_t dst, const uint8_t* src, int 
 }
 
 template <bool SPLIT, bool LAID>
-__global__ void __launch_bounds__(kThreads, 2) gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmap_x,
+__global__ void __launch_bounds__(kThreads, LAID ? 1 : 2) gemm_mx4_rows_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                                                     const __grid_constant__ CUtensorMap tmap_w, const ScaleArgs sc,
                                                                     int* status, const TileArgs g) {
   extern __shared__ uint8_t smem_raw[];

@@ -63,7 +63,7 @@ struct TileArgs {
   int splits, kb_per;      // SPLIT: CTAs of a cluster, one per range of K blocks
   const int* offsets;      // grouped: first row of every expert, and the end
   int experts;
-  int vec;                 // SPLIT, STAGED: results and residual in whole 16-byte vectors
+  int vec;                 // SPLIT, STAGED: results and residual may be taken in whole 16-byte vectors
   int early;               // in a launch chain: weights of the first tile may be read ahead of the wait
 };
 
@@ -97,8 +97,16 @@ __device__ __forceinline__ Item item_of(int i, const TileArgs& g, const int* fir
   return it;
 }
 
-// SPLIT, STAGED: eight results of a token, columns c .. c + 7 of the block (of its 64 outputs, where it is gated), in bf16.
-__device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool glu, int n_blk, int t, int c) {
+// SPLIT, STAGED: the residual of eight results in one vector, where there is one; asked for ahead of the results, because its way from
+// memory takes as long as a chunk of them.
+__device__ __forceinline__ bf16x8 residual8(const TileArgs& g, bool glu, int n_blk, int t, int c) {
+  const int n0 = n_blk * (glu ? 64 : 128) + c;
+  bf16x8 v = {};
+  if (g.residual && g.vec && n0 + 8 <= (glu ? g.N / 2 : g.N)) v = ld_bf16x8(g.residual + t * g.ldr + n0);
+  return v;
+}
+// Eight results of a token, columns c .. c + 7 of the block (of its 64 outputs, where it is gated), in bf16.
+__device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool glu, int n_blk, int t, int c, const bf16x8& v) {
   const int n0 = n_blk * (glu ? 64 : 128) + c, n_out = glu ? g.N / 2 : g.N;
   if (n0 >= n_out) return;
   if (glu) {
@@ -109,7 +117,6 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
   if (g.residual) {
     const bf16* r = g.residual + t * g.ldr + n0;
     if (whole) {
-      const bf16x8 v = ld_bf16x8(r);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 p = unpack_bf16x2(v.u[j]);
@@ -138,8 +145,10 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
 // A warp writes 32 neighbours of a token at a time; or (STAGED) a chunk goes through shared memory to be written in vectors of eight:
 // which pays where the products are quick (8111 x 12288 x 4096 in 4 bits on both sides 208 us, 222 without) and costs where they are
 // not (24008 rows of 128 experts in fp32, six blocks of K each: 427 us for the whole, 400 without; 8192 x 24576 x 4096 1.50 and 1.48
-// ms). Gate and up rows are 64 lanes apart: their warps hand each other half of a chunk's tokens. SPLIT: results stay in shared memory
-// as [token][weight row], for add_ranges. `parts`: room for a tile's results (SPLIT), `staging`: kStaging bytes (STAGED, gated).
+// ms) or where rows start on no 16 bytes (3484 x 28286 x 768 in 4 bits on both sides: 305 us, 86 without). A chunk's residual is asked
+// for as a whole: one value after the other, 4718 x 6656 x 8544 takes 863 us, 465 so. Gate and up rows are 64 lanes apart: their warps
+// hand each other half of a chunk's tokens. SPLIT: results stay in shared memory as [token][weight row], for add_ranges. `parts`: room
+// for a tile's results (SPLIT), `staging`: kStaging bytes (STAGED, gated).
 template <bool SPLIT, bool STAGED>
 __device__ __forceinline__ void write_results(const TileArgs& g, const int* first_tile, int i0, int i_step, int items, bool with_bias,
                                               uint32_t tmem, uint32_t dfull0, uint32_t dempty0, float* parts, float* staging, int group,
@@ -158,6 +167,14 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
     ok = ok && wait_parked(dfull0 + 8 * db, d_phase, abort_flag, status, PXL_DEV_TIMEOUT_TMEM_FULL);
     tc_fence_after_sync();
     for (int c0 = group * kChunk; c0 < it.rows; c0 += groups * kChunk) {
+      bf16x8 res[4];
+      if constexpr (STAGED && !SPLIT) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int e = r + 128 * u, t = min(c0 + e / 16, it.rows - 1);
+          res[u] = residual8(g, false, it.n_blk, it.row0 + t, e % 16 * 8);
+        }
+      }
       uint32_t v[32];
       tmem_ld_32x32b_x32(tmem + db * g.d_cols + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
       tmem_ld_wait();
@@ -167,35 +184,38 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (j < m) parts[(c0 + j) * kPitch + r] = __uint_as_float(v[j]) * factor + add;
-      } else if constexpr (STAGED) {
+      } else if (STAGED && g.vec) {
         named_bar_sync(1 + group, 128);  // (the last chunk has been read)
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (j < m) staging[j * kPitch + r] = __uint_as_float(v[j]) * factor + add;
         named_bar_sync(1 + group, 128);
-        for (int e = r; ok && e < m * 16; e += 128) {
-          const int t = e / 16, c = e % 16 * 8;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int e = r + 128 * u, t = e / 16, c = e % 16 * 8;
+          if (!ok || t >= m) break;
           float f[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 x = *reinterpret_cast<const float4*>(staging + t * kPitch + c + h * 4);
             f[4 * h] = x.x, f[4 * h + 1] = x.y, f[4 * h + 2] = x.z, f[4 * h + 3] = x.w;
           }
-          finish8(g, f, false, it.n_blk, it.row0 + c0 + t, c);
+          finish8(g, f, false, it.n_blk, it.row0 + c0 + t, c, res[u]);
         }
-      } else if (!glu) {
+      } else if (STAGED || !glu) {
         if (!ok || n >= g.N) continue;
         // (one kind of loop each: a choice per result, or its address from scratch, doubles the whole kernel's time)
         float y[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) * factor + add;
         if (g.residual) {
-          const bf16* res = g.residual + t0 * g.ldr + n;
+          // (all asked for at once: behind the last token, the last one's again)
+          const bf16* from = g.residual + t0 * g.ldr + n;
+          bf16 z[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= m) break;
-            y[j] += __bfloat162float(res[j * g.ldr]);
-          }
+          for (int j = 0; j < 32; ++j) z[j] = from[min(j, m - 1) * g.ldr];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] += __bfloat162float(z[j]);
         }
         if (g.out_f32) {
           float* dst = static_cast<float*>(g.C) + t0 * g.ldc + n;
@@ -255,6 +275,7 @@ __device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t pa
   const int per = glu ? 8 : 16;
   for (int e = tid; e < (r1 - r0) * per; e += threads) {
     const int t = r0 + e / per, c = e % per * 8;
+    const bf16x8 res = residual8(g, glu, it.n_blk, it.row0 + t, c);
     float f[16] = {};
     for (int s = 0; s < g.splits; ++s) {
       const uint32_t src = cluster_map_shared(parts + (t * kPitch + c) * 4, s);
@@ -265,7 +286,7 @@ __device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t pa
         f[4 * h] += x.x, f[4 * h + 1] += x.y, f[4 * h + 2] += x.z, f[4 * h + 3] += x.w;
       }
     }
-    if (!*abort_flag) finish8(g, f, glu, it.n_blk, it.row0 + t, c);
+    if (!*abort_flag) finish8(g, f, glu, it.n_blk, it.row0 + t, c, res);
   }
 }
 
@@ -275,7 +296,7 @@ namespace pxl_host {
 
 // Width of the token tiles for more than 256 tokens: whole rounds of the SMs times a tile's time, which is that of `fixed` tokens more
 // than it has. Tiles wider than 192 have one accumulator, which is as good in a single round only; beyond `good` a tile's time grows by
-// a twentieth (8192 x 12288 x 4096 in 160-wide tiles 706 us, 740 in 192-wide ones; 512 x 5120 x 5120 in two rounds of the former 36.5
+// a twentieth (4096 x 24576 x 4096 in 160-wide tiles 656 us, 677 in 192-wide ones; 512 x 5120 x 5120 in two rounds of the former 36.5
 // us, one of the latter 28.5).
 inline int tile_tokens(int M, int n_blocks, int good, int fixed) {
   const int sms = num_sms();
