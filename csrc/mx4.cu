@@ -29,8 +29,12 @@ __global__ void __launch_bounds__(256) mx4_quant_rows_kernel(const void* __restr
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x >> 2);
   const int l = threadIdx.x & 3;
   const bool in = i < total;  // (whole fours of lanes; the others take part in the shuffles)
-  const int64_t row = in ? i / groups : 0;
-  const int64_t at = row * ld + (in ? i - row * groups : 0) * 32 + l * 8;
+  int64_t at = in ? i * 32 : 0;
+  if (ld != groups * 32 && in) {  // (a division of 64 bits takes as long as the rest)
+    const int64_t row = i >> 32 ? i / groups : static_cast<uint32_t>(i) / static_cast<uint32_t>(groups);
+    at = row * ld + (i - row * groups) * 32;
+  }
+  at += l * 8;
   float v[8];
   if constexpr (F32) {
     const float* src = static_cast<const float*>(x) + at;

@@ -71,8 +71,8 @@ def dequant_if_needed(tensors: dict, name: str, cfg=None, dtype: Optional[torch.
 # dimension share one power-of-two scale (e8m0, bias 127) and each value is a 4-bit e2m1 float,
 # two per byte with the low nibble first (``<name>_blocks`` uint8 [..., rows, K/32, 16] and
 # ``<name>_scales`` uint8 [..., rows, K/32]). The reference passes these checkpoints to its
-# backends untouched (``src/parallax/sglang/model_runner.py:358-366``); here they are expanded
-# to bf16 when the shard is loaded.
+# backends untouched (``src/parallax/sglang/model_runner.py:358-366``); here they are kept as they
+# are (``expert_format="mxfp4"``, see ``models/moe.py``) or expanded to bf16 when the shard is loaded.
 _FP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
 
 

@@ -9,6 +9,8 @@ the weighted combine are the kernels of ``csrc/moe.cu`` / ``csrc/gemm_tcgen05.cu
 
 Expert weights are stacked: ``w1 [E*2I, H]`` (gate/up rows interleaved in groups of 64 per
 expert) and ``w2 [E*H, I]``. With expert parallelism a rank holds experts ``[e_lo, e_hi)``.
+With ``expert_format="mxfp4"`` both are microscaled 4-bit numbers (``ops.Mx4Weight``, ``ops.moe_ffn_mx4``):
+those of a checkpoint that has them, others quantised when they are loaded.
 """
 
 from __future__ import annotations
