@@ -240,6 +240,24 @@ int launch_product(const void* x, int64_t ldx, int x_rows, int K, const void* w,
                                 tmap, static_cast<const uint8_t*>(w), a_bufs, kMx4Shift, status);
 }
 
+// Width of the token tiles for more than 256 tokens. A tile's time is bound by the expansion up to 160 tokens (128, 144, 160: 0.89, 0.95,
+// 1), and grows faster than its tokens beyond, where accumulators or buffers are fewer (176, 192, 224, 256: 1.15, 1.25, 1.48, 1.62), in
+// the last case by results that no products hide. A last round that is not full takes about the mean of a round and of its part of one.
+// 8192 x 4096 x 12288 in tiles of 160 tokens 660 us, 192 691, 256 621; 1000 x 8192 x 12288 185, 180, 159; 8192 x 24576 x 4096 1287,
+// 1311, 1310.
+int tile_tokens(int M, int n_blocks, int k_blocks) {
+  const int sms = pxl_host::num_sms();
+  int best = 160;
+  int64_t least = INT64_MAX;
+  for (int bt = 96; bt <= 256; bt += 16) {
+    const int64_t tiles = static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks, rounds = (tiles + sms - 1) / sms;
+    const int64_t time = bt <= 160 ? 8 * (bt + 126) : bt < 256 ? 15 * bt : 3670 + 3300 / k_blocks;
+    const int64_t cost = (rounds * sms + tiles) * time;
+    if (cost <= least) least = cost, best = bt;
+  }
+  return best;
+}
+
 bool epi_known(int epi, int N) {
   return epi == PXL_EPI_NONE || ((epi == PXL_EPI_SILU_MUL || epi == PXL_EPI_CLIP_GLU) && N % 128 == 0);
 }
@@ -256,7 +274,7 @@ PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const flo
   g.C = C, g.row_scale = row_scale, g.ldc = ldc, g.bias = static_cast<const bf16*>(bias);
   g.residual = static_cast<const bf16*>(residual), g.ldr = ldr, g.M = M, g.N = N, g.epi = epi, g.limit = limit;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kTileCols);
-  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, pxl_host::tile_tokens(M, g.n_blocks, 160, 48));
+  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks, g.k_blocks));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   // The SMs at work on 8 tiles of tokens share those and some 18 blocks of weights, from L2; with all tiles in one group x comes from
   // memory again for every few blocks (8192 rows of 24576 x 4096 1.45 -> 1.30 ms, of 4096 x 12288 0.90 -> 0.69; groups of 4 and 16: within

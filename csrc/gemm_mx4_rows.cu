@@ -284,6 +284,21 @@ __global__ void __launch_bounds__(256) mx4_lay_powers_kernel(const uint8_t* __re
     *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(i >> 6) * halves * (2 * kAtom) + (i & 63) * 16) = reinterpret_cast<const uint4*>(out)[i];
 }
 
+// Width of the token tiles for more than 256 tokens: whole rounds of the SMs times a tile's time, which is that of 24 tokens more than it
+// has. Tiles wider than 192 have one accumulator, which is as good in a single round only.
+int tile_tokens(int M, int n_blocks) {
+  const int sms = pxl_host::num_sms();
+  int best = 192;
+  int64_t least = INT64_MAX;
+  for (int bt = 96; bt <= 256; bt += 16) {
+    const int64_t rounds = (static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks + sms - 1) / sms;
+    if (rounds > 1 && bt > 192) break;
+    const int64_t cost = rounds * (bt + 24);
+    if (cost <= least) least = cost, best = bt;
+  }
+  return best;
+}
+
 struct RowsPlan {
   TileArgs g;
   int64_t items;
@@ -299,7 +314,7 @@ bool plan_rows(RowsPlan& p, int M, int N, int K) {
   TileArgs& g = p.g;
   g.M = M, g.N = N;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kStep);
-  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, pxl_host::tile_tokens(M, g.n_blocks, 192, 24));
+  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   g.t_group = g.t_tiles;
   p.items = static_cast<int64_t>(g.n_blocks) * g.t_tiles;

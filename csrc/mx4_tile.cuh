@@ -294,23 +294,6 @@ __device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t pa
 
 namespace pxl_host {
 
-// Width of the token tiles for more than 256 tokens: whole rounds of the SMs times a tile's time, which is that of `fixed` tokens more
-// than it has. Tiles wider than 192 have one accumulator, which is as good in a single round only; beyond `good` a tile's time grows by
-// a twentieth (4096 x 24576 x 4096 in 160-wide tiles 656 us, 677 in 192-wide ones; 512 x 5120 x 5120 in two rounds of the former 36.5
-// us, one of the latter 28.5).
-inline int tile_tokens(int M, int n_blocks, int good, int fixed) {
-  const int sms = num_sms();
-  int best = good;
-  int64_t least = INT64_MAX;
-  for (int bt = 96; bt <= 256; bt += 16) {
-    const int64_t rounds = (static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks + sms - 1) / sms;
-    if (rounds > 1 && bt > 192) break;
-    const int64_t cost = rounds * (bt + fixed) * (rounds > 1 && bt > good ? 21 : 20);
-    if (cost <= least) least = cost, best = bt;
-  }
-  return best;
-}
-
 // Clusters of `size` CTAs that run at a time; of kernels that leave room for one CTA per SM. (A GPU processing cluster's SMs that are
 // no multiple of the size stay empty.)
 template <typename Kernel>
