@@ -284,16 +284,18 @@ __global__ void __launch_bounds__(256) mx4_lay_powers_kernel(const uint8_t* __re
     *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(i >> 6) * halves * (2 * kAtom) + (i & 63) * 16) = reinterpret_cast<const uint4*>(out)[i];
 }
 
-// Width of the token tiles for more than 256 tokens: whole rounds of the SMs times a tile's time, which is that of 24 tokens more than it
-// has. Tiles wider than 192 have one accumulator, which is as good in a single round only.
-int tile_tokens(int M, int n_blocks) {
+// Width of the token tiles for more than 256 tokens. A tile's time is that of 92 tokens more than it has (128, 160, 192: 0.77, 0.88, 1);
+// beyond 192 there is one accumulator, and no products hide its results (224, 256: 1.35, 1.54 for 16 steps of K, 1.25, 1.44 for 48). A
+// last round that is not full takes about the mean of a round and of its part of one. 8192 x 12288 x 4096 in tiles of 160 tokens 230 us,
+// 192 211, 256 246; 1000 x 8192 x 12288 66, 62, 60; 1500 x 5120 x 25600 114, 115, 111, and 98 in tiles of 224.
+int tile_tokens(int M, int n_blocks, int steps) {
   const int sms = pxl_host::num_sms();
   int best = 192;
   int64_t least = INT64_MAX;
   for (int bt = 96; bt <= 256; bt += 16) {
-    const int64_t rounds = (static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks + sms - 1) / sms;
-    if (rounds > 1 && bt > 192) break;
-    const int64_t cost = rounds * (bt + 24);
+    const int64_t tiles = static_cast<int64_t>(pxl::ceil_div(M, bt)) * n_blocks, rounds = (tiles + sms - 1) / sms;
+    const int64_t time = bt <= 192 ? 20 * (bt + 92) : 31 * bt + 13200 / steps;
+    const int64_t cost = (rounds * sms + tiles) * time;
     if (cost <= least) least = cost, best = bt;
   }
   return best;
@@ -314,7 +316,7 @@ bool plan_rows(RowsPlan& p, int M, int N, int K) {
   TileArgs& g = p.g;
   g.M = M, g.N = N;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kStep);
-  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks));
+  g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks, g.k_blocks));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   g.t_group = g.t_tiles;
   p.items = static_cast<int64_t>(g.n_blocks) * g.t_tiles;
