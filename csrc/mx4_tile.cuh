@@ -144,9 +144,9 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
 // Groups of four warps, one per quarter of the lanes, that take an accumulator's chunks of tokens in turn. A lane has a weight row.
 // A warp writes 32 neighbours of a token at a time; or (STAGED) a chunk goes through shared memory to be written in vectors of eight:
 // which pays where the products are quick (8111 x 12288 x 4096 in 4 bits on both sides 208 us, 222 without) and costs where they are
-// not (24008 rows of 128 experts in fp32, six blocks of K each: 427 us for the whole, 400 without; 8192 x 24576 x 4096 1.50 and 1.48
-// ms) or where rows start on no 16 bytes (3484 x 28286 x 768 in 4 bits on both sides: 305 us, 86 without). A chunk's residual is asked
-// for as a whole: one value after the other, 4718 x 6656 x 8544 takes 863 us, 465 so. Gate and up rows are 64 lanes apart: their warps
+// not (the experts of 24008 rows with fp32 results 7 %, 8192 x 24576 x 4096 1 %) or where rows start on no 16 bytes (3484 x 28286 x 768
+// in 4 bits on both sides: 305 us, 86 without). A chunk's residual is asked for as a whole: one value after the other, 4718 x 6656 x
+// 8544 takes 863 us, 465 so. Gate and up rows are 64 lanes apart: their warps
 // hand each other half of a chunk's tokens. SPLIT: results stay in shared memory as [token][weight row], for add_ranges. `parts`: room
 // for a tile's results (SPLIT), `staging`: kStaging bytes (STAGED, gated).
 template <bool SPLIT, bool STAGED>
