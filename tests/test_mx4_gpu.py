@@ -323,6 +323,21 @@ def test_experts_too_wide_for_shared_memory():
     oracle.within(ops.moe_ffn_mx4(*_dev(x, ids, wts), w1, w2, base=base.to(DEV)), *want)
 
 
+@pytest.mark.parametrize("T,N,K", [(700, 5120, 12288), (1500, 5120, 12800), (2048, 20480, 6144), (4000, 2047, 8192)])
+def test_wide_tiles_of_deep_products(T, N, K):
+    """Tiles of more than 192 rows, one and several per CTA, with a residual; samples against 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device=DEV)
+    scales = torch.randint(112, 120, (N, K // 32), generator=g, dtype=torch.uint8, device=DEV)
+    x, r = torch.randn(T, K, generator=g, device=DEV).bfloat16(), torch.randn(T, N, generator=g, device=DEV).bfloat16()
+    xc, xs = ops.quant_mx4_rows(x)
+    got, got44 = ops.linear_mx4(x, ops.Mx4Weight.pack(codes, scales), residual=r), ops.linear_mx4_rows(xc, xs, codes, scales, residual=r)
+    tokens, rows = torch.cat([torch.randperm(T)[:32], torch.tensor([0, 255, 256, T - 1])]), torch.randperm(N)[:300]
+    w, res = oracle.values(codes.cpu()[rows], scales.cpu()[rows]), r.cpu()[tokens][:, rows]
+    oracle.within(got.cpu()[tokens][:, rows], *oracle.linear(x.cpu()[tokens].double(), w, residual=res))
+    oracle.within(got44.cpu()[tokens][:, rows], *oracle.linear(oracle.values(xc.cpu()[tokens], xs.cpu()[tokens]), w, residual=res))
+
+
 # ------------------------------------------------------------------------------------------------ streams, graphs, repeats
 def _layer(x, w_in, w_out, wr, ids, wts, w1, w2):
     """The operators one behind the other, as a layer uses them."""
