@@ -274,6 +274,9 @@ PXL_EXPORT int pxl_mx4_expand_rows(const void* codes, const void* scales, void* 
 PXL_EXPORT int pxl_moe_combine_f32(const float* y, const int* pos_of, const float* w, const void* base, void* out, int T, int k,
                                    int H, cudaStream_t stream) {
   if (T < 0 || k <= 0 || H <= 0 || H % 8) return PXL_ERR_INVALID_ARG;
+  // (rows are read and written in vectors of four)
+  if ((reinterpret_cast<uintptr_t>(y) & 15) || ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(out)) & 7))
+    return PXL_ERR_INVALID_ARG;
   if (T == 0) return PXL_OK;
   pxl_host::launch(moe_combine_f32_kernel, T, 256, 0, stream, y, pos_of, w, static_cast<const bf16*>(base), static_cast<bf16*>(out),
                    k, H);

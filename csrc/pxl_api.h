@@ -328,7 +328,7 @@ int64_t pxl_gemm_mx4_rows_workspace(int M, int N, int K);
 int pxl_gemm_mx4_rows(const void* xc, const void* xs, const void* wc, const void* ws, void* C, int64_t ldc, const void* bias,
                       const void* residual, int64_t ldr, int M, int N, int K, void* workspace, int64_t workspace_bytes, int* status,
                       pxl_stream_t stream);
-// pxl_moe_combine of fp32 rows
+// pxl_moe_combine of fp32 rows; y on 16 bytes, base and out on 8
 int pxl_moe_combine_f32(const float* y, const int* pos_of, const float* w, const void* base, void* out, int T, int k, int H,
                         pxl_stream_t stream);
 

@@ -1069,10 +1069,14 @@ def _bf16_rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return x if s1 == 1 and not s0 & 7 and s0 >= x.shape[1] and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
 
 
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """A tensor as kernels read it that take its rows one behind the other in vectors: a copy where they lie apart or start on no 16 bytes."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Contiguous codes on a 16-byte boundary, contiguous scales."""
-    codes = codes.contiguous()
-    return codes.clone() if codes.data_ptr() & 15 else codes, scales.contiguous()
+    return _vectors(codes), scales.contiguous()
 
 
 def quant_mx4_rows(x: torch.Tensor):
@@ -1170,6 +1174,7 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
     mx4.check_experts("moe_ffn_mx4", x, ids, weights, w1, w2, base, act_mode, limit, b1, b2)
     (T, K), k = x.shape, ids.shape[1]
     x = _bf16_rows(x, "moe_ffn_mx4").contiguous()
+    base = None if base is None else _vectors(base)
     out = torch.empty((T, K), dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return out

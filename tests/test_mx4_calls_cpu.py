@@ -1,0 +1,76 @@
+"""What the wrappers of the microscaled 4-bit kernels hand to the library, and what the library refuses: no GPU is needed for either."""
+
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+from parallax_b200 import ops
+from parallax_b200.ops import _lib, cuda as cu
+
+INVALID_ARG = 1
+
+
+class Recorder:
+    """Stands in for the kernel library: remembers every call, launches nothing. `answers`: what a function returns, or calls."""
+
+    def __init__(self, **answers):
+        self.answers, self.calls = answers, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            answer = self.answers.get(name, 0)
+            return answer(*args) if callable(answer) else answer
+
+        return call
+
+
+@pytest.fixture
+def record(monkeypatch):
+    def start(**answers):
+        lib = Recorder(**answers)
+        monkeypatch.setattr(_lib, "lib", lambda: lib)
+        monkeypatch.setattr(cu, "_on", lambda device: contextlib.nullcontext())
+        monkeypatch.setattr(cu, "_stream", lambda device: 0)
+        monkeypatch.setattr(cu, "status_tensor", lambda device: torch.zeros(1, dtype=torch.int32))
+        return lib
+
+    return start
+
+
+def _bytes(address, n):
+    return torch.frombuffer(bytearray(ctypes.string_at(address, n)), dtype=torch.uint8)
+
+
+def _weight(rows, K, experts=1):
+    g = torch.Generator().manual_seed(rows)
+    return ops.Mx4Weight.pack(torch.randint(0, 256, (experts * rows, K // 2), generator=g, dtype=torch.uint8),
+                              torch.randint(117, 126, (experts * rows, K // 32), generator=g, dtype=torch.uint8), experts)
+
+
+@pytest.mark.parametrize("few", [0, 1])
+@pytest.mark.parametrize("at", [0, 1, 4, 8])
+def test_base_of_experts_on_any_address(record, few, at):
+    """The kernel that adds the experts' rows up reads `base` in vectors: it gets one that starts on 16 bytes, with the same values."""
+    T, K, I, E = 5, 64, 64, 2
+    x, ids, wts = torch.randn(T, K).bfloat16(), torch.zeros(T, 2, dtype=torch.int32), torch.ones(T, 2)
+    base = torch.randn(T * K + 8).bfloat16()[at:at + T * K].view(T, K)
+    seen = []
+
+    def took(position):
+        return lambda *args: seen.append((args[position] % 16, _bytes(args[position], 2 * T * K))) or 0
+
+    record(pxl_moe_mx4_few_takes=few, pxl_moe_align_alone=1, pxl_moe_combine_f32=took(3), pxl_moe_mx4_few=took(10))
+    cu.moe_ffn_mx4(x, ids, wts, _weight(2 * I, K, E), _weight(K, I, E), base=base)
+    (off, values), = seen
+    assert off == 0 and torch.equal(values.view(torch.bfloat16).view(T, K), base)
+
+
+@pytest.mark.parametrize("which", [0, 3, 4])
+def test_sum_of_experts_refuses_odd_addresses(which):
+    """Refused by the entry point itself, before any launch."""
+    args = [0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 1, 1, 64, 0]
+    args[which] += 2
+    assert _lib.lib().pxl_moe_combine_f32(*args) == INVALID_ARG
