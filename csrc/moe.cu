@@ -504,6 +504,9 @@ PXL_EXPORT int pxl_moe_combine(const void* y_perm, const int* pos_of, const floa
                                pxl_stream_t stream) {
   if (T <= 0) return PXL_OK;
   if (H % 8) return PXL_ERR_INVALID_ARG;
+  // (rows are read and written in vectors of eight)
+  if ((reinterpret_cast<uintptr_t>(y_perm) | reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(out)) & 15)
+    return PXL_ERR_INVALID_ARG;
   auto go = [&](auto kern) {
     pxl_host::launch(kern, T, 256, 0, stream, static_cast<const bf16*>(y_perm), pos_of, w, static_cast<const bf16*>(base),
                      static_cast<bf16*>(out), k, H);

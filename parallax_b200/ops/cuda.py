@@ -44,6 +44,11 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """A tensor as kernels read it that take its rows one behind the other in vectors: a copy where they lie apart or start on no 16 bytes."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _stream(device: torch.device) -> int:
     # (a Stream object costs 6 of the 16 us that an op takes on the host)
     idx = device.index
@@ -715,6 +720,7 @@ def grouped_linear(a: torch.Tensor, w: torch.Tensor, plan: MoEPlan, num_local_ex
 def moe_combine(y_perm: torch.Tensor, plan: MoEPlan, weights: torch.Tensor, base: Optional[torch.Tensor],
                 T: int) -> torch.Tensor:
     k, H = weights.shape[1], y_perm.shape[1]
+    base = None if base is None else _vectors(base)
     out = torch.empty((T, H), dtype=y_perm.dtype, device=y_perm.device)
     check(_lib.lib().pxl_moe_combine(y_perm.data_ptr(), plan.pos_of.data_ptr(), weights.data_ptr(), _ptr(base),
                                      out.data_ptr(), T, k, H, _stream(y_perm.device)), "pxl_moe_combine")
@@ -1067,11 +1073,6 @@ def _bf16_rows(x: torch.Tensor, what: str) -> torch.Tensor:
         mx4.refuse(what, f"the kernels take bf16 rows, got {x.dtype}")
     s0, s1 = x.stride()
     return x if s1 == 1 and not s0 & 7 and s0 >= x.shape[1] and not x.data_ptr() & 15 else x.clone(memory_format=torch.contiguous_format)
-
-
-def _vectors(t: torch.Tensor) -> torch.Tensor:
-    """A tensor as kernels read it that take its rows one behind the other in vectors: a copy where they lie apart or start on no 16 bytes."""
-    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _codes(codes: torch.Tensor, scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

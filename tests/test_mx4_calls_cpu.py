@@ -74,3 +74,27 @@ def test_sum_of_experts_refuses_odd_addresses(which):
     args = [0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 1, 1, 64, 0]
     args[which] += 2
     assert _lib.lib().pxl_moe_combine_f32(*args) == INVALID_ARG
+
+
+def test_base_of_bf16_experts_on_any_address(record):
+    """So it is for the experts in bf16: their sum is read in vectors of eight values."""
+    T, K, I, E = 5, 64, 64, 2
+    base = torch.randn(T * K + 8).bfloat16()[1:1 + T * K].view(T, K)
+    seen = []
+
+    def took(*args):
+        seen.append((args[3] % 16, _bytes(args[3], 2 * T * K)))
+        return 0
+
+    record(pxl_moe_align_alone=1, pxl_moe_combine=took)
+    cu.moe_ffn(torch.randn(T, K).bfloat16(), torch.zeros(T, 2, dtype=torch.int32), torch.ones(T, 2), torch.zeros(E * 2 * I, K).bfloat16(),
+               torch.zeros(E * K, I).bfloat16(), E, base=base)
+    (off, values), = seen
+    assert off == 0 and torch.equal(values.view(torch.bfloat16).view(T, K), base)
+
+
+@pytest.mark.parametrize("which", [0, 3, 4])
+def test_sum_of_bf16_experts_refuses_odd_addresses(which):
+    args = [0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 1, 1, 64, 0]
+    args[which] += 2
+    assert _lib.lib().pxl_moe_combine(*args) == INVALID_ARG
