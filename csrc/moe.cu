@@ -468,7 +468,7 @@ PXL_EXPORT int pxl_moe_align(const int* ids, int T, int k, int E, int e_lo, int 
 PXL_EXPORT int pxl_moe_gather(const void* x, const int* src_tok, const int* n_rows, void* x_perm,
                               int max_rows, int H, pxl_stream_t stream) {
   if (max_rows <= 0) return PXL_OK;
-  if (H % 8) return PXL_ERR_INVALID_ARG;
+  if (H % 8 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_perm)) & 15)) return PXL_ERR_INVALID_ARG;
   const int nvec = H >> 3;
   auto go = [&](auto kern, int u) {
     const int per_row = pxl::ceil_div(nvec, 32 * u);

@@ -691,7 +691,7 @@ def moe_align(ids: torch.Tensor, num_experts: int, e_lo: int = 0, e_hi: Optional
 
 
 def moe_gather(x: torch.Tensor, plan: MoEPlan) -> torch.Tensor:
-    H = x.shape[1]
+    H, x = x.shape[1], _vectors(x)
     # one padding tile so that the last m-tile's TMA box stays inside the allocation
     xp = torch.empty((plan.max_rows + 128, H), dtype=x.dtype, device=x.device)
     check(_lib.lib().pxl_moe_gather(x.data_ptr(), plan.src_tok.data_ptr(), plan.offsets[plan.n_local:].data_ptr(),

@@ -98,3 +98,28 @@ def test_sum_of_bf16_experts_refuses_odd_addresses(which):
     args = [0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 1, 1, 64, 0]
     args[which] += 2
     assert _lib.lib().pxl_moe_combine(*args) == INVALID_ARG
+
+
+@pytest.mark.parametrize("view", ["odd", "wide", "columns"])
+def test_rows_of_bf16_experts_on_any_address(record, view):
+    """The experts' rows are gathered in vectors, one row of the tokens behind the other."""
+    T, K, I, E = 5, 64, 64, 2
+    x = {"odd": torch.randn(T * K + 8).bfloat16()[1:1 + T * K].view(T, K), "wide": torch.randn(T, 3 * K).bfloat16()[:, K:2 * K],
+         "columns": torch.randn(K, T).bfloat16().t()}[view]
+    seen = []
+
+    def took(*args):
+        seen.append((args[0] % 16, _bytes(args[0], 2 * T * K)))
+        return 0
+
+    record(pxl_moe_align_alone=1, pxl_moe_gather=took)
+    cu.moe_ffn(x, torch.zeros(T, 2, dtype=torch.int32), torch.ones(T, 2), torch.zeros(E * 2 * I, K).bfloat16(), torch.zeros(E * K, I).bfloat16(), E)
+    (off, values), = seen
+    assert off == 0 and torch.equal(values.view(torch.bfloat16).view(T, K), x)
+
+
+@pytest.mark.parametrize("which", [0, 3])
+def test_gathered_rows_refuse_odd_addresses(which):
+    args = [0x10000, 0x20000, 0x30000, 0x40000, 1, 64, 0]
+    args[which] += 2
+    assert _lib.lib().pxl_moe_gather(*args) == INVALID_ARG
