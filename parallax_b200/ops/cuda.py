@@ -1119,7 +1119,7 @@ def linear_mx4(x: torch.Tensor, w: Mx4Weight, bias: Optional[torch.Tensor] = Non
     T, K = mx4.check_rows(x, "linear_mx4")
     dev, N = x.device, w.rows if isinstance(w, Mx4Weight) else 0
     mx4.check_weight(w, dev, "linear_mx4")
-    n_out = mx4.check_product("linear_mx4", x, T, N, K, w.cols, bias, residual, epi, limit, out, torch.bfloat16)
+    n_out = mx4.check_product("linear_mx4", (x, w.data, w.row_scale), T, N, K, w.cols, bias, residual, epi, limit, out, torch.bfloat16)
     x = _bf16_rows(x, "linear_mx4")
     if out is None:
         out = torch.empty((T, n_out), dtype=torch.bfloat16, device=dev)
@@ -1142,7 +1142,7 @@ def linear_mx4_rows(codes: torch.Tensor, scales: torch.Tensor, w_codes: torch.Te
     dev = codes.device
     if w_codes.device != dev:
         mx4.refuse("linear_mx4_rows", "rows and weights are on different devices")
-    mx4.check_product("linear_mx4_rows", codes, T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
+    mx4.check_product("linear_mx4_rows", (codes, scales, w_codes, w_scales), T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
     if out is None:
         out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
     if T == 0 or N == 0:

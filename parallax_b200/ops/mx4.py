@@ -156,10 +156,10 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return not (apart >= wa and apart + wb <= sa)
 
 
-def check_product(what: str, x: torch.Tensor, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
+def check_product(what: str, operands: tuple, T: int, N: int, K: int, K_w: int, bias: Optional[torch.Tensor],
                   residual: Optional[torch.Tensor], epi: int, limit: float, out: Optional[torch.Tensor], dtype: torch.dtype) -> int:
-    """Checks what the two products share; returns the number of output columns."""
-    device = x.device
+    """Checks what the two products share; returns the number of output columns. ``operands``: what is multiplied, the rows first."""
+    device = operands[0].device
     if K != K_w:
         refuse(what, f"rows of {K} columns and weights of {K_w}")
     n_out = N
@@ -184,10 +184,15 @@ def check_product(what: str, x: torch.Tensor, T: int, N: int, K: int, K_w: int, 
         _check_operand(out, "out", (T, n_out), dtype, device, what)
         if T > 1 and out.stride(0) < n_out:
             refuse(what, "rows of out overlap")
-        # (the residual may be out itself: a result is written by the thread that has read its place)
-        if T > 0 and n_out > 0 and (_share_memory(x, out) or residual is not None and _share_memory(residual, out) and (
-                residual.data_ptr() != out.data_ptr() or residual.stride(0) != out.stride(0))):
-            refuse(what, "out overlaps the rows, or the residual in other places than its own")
+        if T > 0 and n_out > 0:
+            for t in operands if bias is None else operands + (bias,):
+                # (a matrix whose columns lie apart is copied before the kernel runs)
+                if (t.stride(-1) == 1 or t.shape[-1] == 1) and _share_memory(t if t.dim() == 2 else t.unsqueeze(0), out):
+                    refuse(what, "out overlaps the rows, the weights or the bias")
+            # (the residual may be out itself: a result is written by the thread that has read its place)
+            if residual is not None and _share_memory(residual, out) and (
+                    residual.data_ptr() != out.data_ptr() or residual.stride(0) != out.stride(0)):
+                refuse(what, "out overlaps the residual in other places than its own")
     return n_out
 
 

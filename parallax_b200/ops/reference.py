@@ -602,10 +602,11 @@ def _mx4_product(x, wv, bias, residual, epi, limit, out, dtype):
 def linear_mx4(x, w, bias=None, residual=None, epi: int = EPI_NONE, limit: float = 0.0, out=None):
     """``x [T, K] @ W^T`` with a microscaled weight (:class:`ops.Mx4Weight`, one expert): plain, with a bias, with a residual, or
     gated (``EPI_SILU_MUL``, ``EPI_CLIP_GLU`` with ``limit``; gate / up rows in groups of 64). Rows are bf16 (on CPU fp32 too).
-    ``out`` may be the residual or other columns of the rows' buffer; where it shares memory with the rows it is refused."""
+    ``out`` may be the residual or other columns of the rows' buffer; over the rows, the weight, the bias or other places of the
+    residual it is refused."""
     T, K = mx4.check_rows(x, "linear_mx4")
     mx4.check_weight(w, x.device, "linear_mx4")
-    mx4.check_product("linear_mx4", x, T, w.rows, K, w.cols, bias, residual, epi, limit, out, x.dtype)
+    mx4.check_product("linear_mx4", (x, w.data, w.row_scale), T, w.rows, K, w.cols, bias, residual, epi, limit, out, x.dtype)
     return _mx4_product(x.float(), _mx4_values(*w.unpack()), bias, residual, epi, limit, out, x.dtype)
 
 
@@ -616,7 +617,7 @@ def linear_mx4_rows(codes, scales, w_codes, w_scales, bias=None, residual=None, 
     N, K_w = mx4.check_codes(w_codes, w_scales, "linear_mx4_rows: weights")
     if w_codes.device != codes.device:
         mx4.refuse("linear_mx4_rows", "rows and weights are on different devices")
-    mx4.check_product("linear_mx4_rows", codes, T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
+    mx4.check_product("linear_mx4_rows", (codes, scales, w_codes, w_scales), T, N, K, K_w, bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
     return _mx4_product(_mx4_values(codes, scales), _mx4_values(w_codes, w_scales), bias, residual, EPI_NONE, 0.0, out, torch.bfloat16)
 
 

@@ -123,3 +123,49 @@ def test_gathered_rows_refuse_odd_addresses(which):
     args = [0x10000, 0x20000, 0x30000, 0x40000, 1, 64, 0]
     args[which] += 2
     assert _lib.lib().pxl_moe_gather(*args) == INVALID_ARG
+
+
+def _spoil(t):
+    """A bf16 tensor [2, 64] over the first bytes of `t`."""
+    return t.flatten().view(torch.uint8)[:256].view(torch.bfloat16).view(2, 64)
+
+
+@pytest.mark.parametrize("operand", ["codes", "factors", "bias", "rows"])
+def test_results_over_an_operand_of_linear_mx4(operand):
+    """A result is written while other blocks still read: over weights, their factors, a bias or the rows it is refused."""
+    w, x = _weight(64, 64), torch.randn(2, 64).bfloat16()
+    bias = torch.zeros(128).bfloat16()[:64]
+    out = {"codes": _spoil(w.data), "factors": _spoil(w.row_scale), "bias": torch.zeros(0), "rows": x}[operand]
+    if operand == "bias":
+        buf = torch.zeros(2, 64).bfloat16()
+        bias, out = buf[1], buf
+    kept = w.data.clone(), w.row_scale.clone()
+    with pytest.raises(ops.KernelError):
+        ops.linear_mx4(x, w, bias, out=out)
+    assert torch.equal(w.data, kept[0]) and torch.equal(w.row_scale, kept[1])
+    assert ops.linear_mx4(x, w, bias, out=torch.empty(2, 64).bfloat16()).shape == (2, 64)
+
+
+@pytest.mark.parametrize("operand", ["codes", "scales", "w_codes", "w_scales", "bias"])
+def test_results_over_an_operand_of_linear_mx4_rows(operand):
+    K = 4096
+    g = torch.Generator().manual_seed(0)
+    t = {n: torch.randint(100, 120, (r, c), generator=g, dtype=torch.uint8)
+         for n, r, c in (("codes", 2, K // 2), ("scales", 2, K // 32), ("w_codes", 64, K // 2), ("w_scales", 64, K // 32))}
+    buf = torch.zeros(2, 64).bfloat16()
+    bias, out = (buf[1], buf) if operand == "bias" else (None, _spoil(t[operand]))
+    kept = {n: v.clone() for n, v in t.items()}
+    with pytest.raises(ops.KernelError):
+        ops.linear_mx4_rows(*t.values(), bias=bias, out=out)
+    assert all(torch.equal(v, kept[n]) for n, v in t.items())
+    assert ops.linear_mx4_rows(*t.values(), bias=bias, out=torch.empty(2, 64).bfloat16()).shape == (2, 64)
+
+
+def test_results_over_rows_whose_columns_lie_apart():
+    """Rows of a transposed view are copied for the kernels, so that a result may lie anywhere in what they span."""
+    w, buf = _weight(64, 64), torch.randn(64, 200).bfloat16()
+    x = buf[:, :2].t()
+    want = ops.linear_mx4(x.clone(), w)
+    for at in (lambda b: b[40:42, 100:164], lambda b: b[:2, :64]):
+        b = buf.clone()
+        assert torch.equal(ops.linear_mx4(b[:, :2].t(), w, out=at(b)), want)
