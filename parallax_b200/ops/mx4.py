@@ -191,7 +191,7 @@ def check_product(what: str, operands: tuple, T: int, N: int, K: int, K_w: int, 
                     refuse(what, "out overlaps the rows, the weights or the bias")
             # (the residual may be out itself: a result is written by the thread that has read its place)
             if residual is not None and _share_memory(residual, out) and (
-                    residual.data_ptr() != out.data_ptr() or residual.stride(0) != out.stride(0)):
+                    residual.data_ptr() != out.data_ptr() or T > 1 and residual.stride(0) != out.stride(0)):
                 refuse(what, "out overlaps the residual in other places than its own")
     return n_out
 

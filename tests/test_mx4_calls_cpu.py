@@ -169,3 +169,19 @@ def test_results_over_rows_whose_columns_lie_apart():
     for at in (lambda b: b[40:42, 100:164], lambda b: b[:2, :64]):
         b = buf.clone()
         assert torch.equal(ops.linear_mx4(b[:, :2].t(), w, out=at(b)), want)
+
+
+def test_a_single_row_in_the_place_of_its_residual():
+    """The strides of a single row say nothing: the residual may be out, as it may with many."""
+    w, x = _weight(64, 64), torch.randn(1, 64).bfloat16()
+    buf = torch.randn(1, 128).bfloat16()
+    want = ops.linear_mx4(x, w, residual=buf[:, :64].clone())
+    for residual, out in ((buf[:1, :64], buf.view(-1)[:64].view(1, 64)), (buf.view(-1)[:64].view(1, 64), buf[:1, :64])):
+        kept = buf.clone()
+        assert torch.equal(ops.linear_mx4(x, w, residual=residual, out=out), want)
+        assert torch.equal(buf[:, :64], want) and torch.equal(buf[:, 64:], kept[:, 64:])
+        buf.copy_(kept)
+    with pytest.raises(ops.KernelError):
+        ops.linear_mx4(x, w, residual=buf[:, 1:65], out=buf[:, :64])
+    r = torch.randn(1, 1).bfloat16()
+    assert ops.linear_mx4(x, _weight(1, 64), residual=r, out=r) is r
