@@ -52,6 +52,16 @@ class Mx4Weight:
     __slots__ = ("data", "row_scale", "rows", "cols", "experts")
 
     def __init__(self, data: torch.Tensor, row_scale: torch.Tensor, rows: int, cols: int, experts: int = 1):
+        # (the kernels take addresses from these sizes)
+        nt, kt = -(-rows // TILE), -(-cols // TILE)
+        if rows <= 0 or cols <= 0 or cols % 32 or experts <= 0:
+            refuse("Mx4Weight", f"{experts} x [{rows}, {cols}]: at least one expert and row, columns in 32s")
+        if data.dtype is not torch.uint8 or data.shape != (experts * nt * kt * BLOCK_BYTES,) or not data.is_contiguous() or data.data_ptr() & 15:
+            refuse("Mx4Weight", f"data is uint8 [{experts * nt * kt * BLOCK_BYTES}] on 16 bytes, got {data.dtype} {tuple(data.shape)}")
+        if row_scale.dtype is not torch.float32 or row_scale.shape != (experts, nt * TILE) or not row_scale.is_contiguous():
+            refuse("Mx4Weight", f"row_scale is fp32 [{experts}, {nt * TILE}], got {row_scale.dtype} {tuple(row_scale.shape)}")
+        if data.device != row_scale.device:
+            refuse("Mx4Weight", "data and row_scale are on different devices")
         self.data, self.row_scale, self.rows, self.cols, self.experts = data, row_scale, rows, cols, experts
 
     @property
@@ -63,6 +73,8 @@ class Mx4Weight:
 
     def expert_slice(self, lo: int, hi: int) -> "Mx4Weight":
         """Experts ``[lo, hi)``, as views of this weight."""
+        if not 0 <= lo < hi <= self.experts:
+            refuse("expert_slice", f"experts [{lo}, {hi}) of {self.experts}")
         n = self.data.numel() // self.experts
         return Mx4Weight(self.data[lo * n:hi * n], self.row_scale[lo:hi], self.rows, self.cols, hi - lo)
 

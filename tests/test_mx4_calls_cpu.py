@@ -185,3 +185,27 @@ def test_a_single_row_in_the_place_of_its_residual():
         ops.linear_mx4(x, w, residual=buf[:, 1:65], out=buf[:, :64])
     r = torch.randn(1, 1).bfloat16()
     assert ops.linear_mx4(x, _weight(1, 64), residual=r, out=r) is r
+
+
+@pytest.mark.parametrize("lo,hi", [(-1, 1), (1, 1), (2, 1), (0, 4), (3, 4), (-2, -1)])
+def test_experts_that_a_weight_does_not_have(lo, hi):
+    """A slice past the last expert would say that it has experts whose bytes are not its own."""
+    w = _weight(64, 64, 3)
+    with pytest.raises(ops.KernelError):
+        w.expert_slice(lo, hi)
+    assert w.expert_slice(1, 3).experts == 2 and w.expert_slice(0, 3).data.numel() == w.data.numel()
+
+
+def test_weights_of_other_sizes_than_they_say():
+    """The kernels take addresses from a weight's sizes: its tensors have to hold that many bytes."""
+    w = _weight(130, 160, 2)
+    new = ops.Mx4Weight
+    assert new(w.data, w.row_scale, 130, 160, 2).cols == 160 and new(w.data, w.row_scale, 256, 256, 2).rows == 256
+    odd = torch.zeros(w.data.numel() + 1, dtype=torch.uint8)[1:]
+    for args in ((w.data[:-1], w.row_scale, 130, 160, 2), (w.data, w.row_scale, 130, 160, 3), (w.data, w.row_scale, 257, 160, 2),
+                 (w.data, w.row_scale, 130, 288, 2), (w.data, w.row_scale, 130, 170, 2), (w.data, w.row_scale[:1], 130, 160, 2),
+                 (w.data, w.row_scale.double(), 130, 160, 2), (w.data.int(), w.row_scale, 130, 160, 2), (odd, w.row_scale, 130, 160, 2),
+                 (w.data, w.row_scale.t().contiguous().t(), 130, 160, 2), (w.data, w.row_scale, 0, 160, 2), (w.data, w.row_scale, 130, 0, 2),
+                 (w.data[:0], w.row_scale[:0], 130, 160, 0), (w.data.to("meta"), w.row_scale, 130, 160, 2)):
+        with pytest.raises(ops.KernelError):
+            new(*args)
