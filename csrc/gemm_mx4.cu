@@ -268,8 +268,8 @@ PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const flo
                             const void* bias, const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit,
                             int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || K % 32 || !epi_known(epi, N) || !pxl_host::on16(x, 2 * ldx)) return PXL_ERR_INVALID_ARG;
-  if (pxl_gemv_mx4_takes(M, N, K))
-    return pxl_gemv_mx4(x, ldx, w, row_scale, C, ldc, bias, residual, ldr, M, N, K, epi, limit, stream);
+  if (pxl_host::gemv_mx4_takes(M, N, K))
+    return pxl_host::gemv_mx4(x, ldx, w, row_scale, C, ldc, bias, residual, ldr, M, N, K, epi, limit, stream);
   TileArgs g{};
   g.C = C, g.row_scale = row_scale, g.ldc = ldc, g.bias = static_cast<const bf16*>(bias);
   g.residual = static_cast<const bf16*>(residual), g.ldr = ldr, g.M = M, g.N = N, g.epi = epi, g.limit = limit;

@@ -1,10 +1,10 @@
-// Products of up to eight rows with microscaled 4-bit weights, and a few tokens' routed experts, straight from global memory.
+// Products of up to four rows with microscaled 4-bit weights, and a few tokens' routed experts, straight from global memory.
 //
 // Bound by the bytes of the weights and, with few of them, by latency: no tensor memory, no stages, no barriers on the way. A warp
 // takes 16 weight rows and every so many blocks of 128 columns; lane (g, t) = (lane / 4, lane % 4) reads the 32 codes of column
 // group t for two of the rows (16 bytes each, four blocks ahead), makes them bf16 and feeds mma.sync, whose K order is free: the
 // lane's own 32 columns take the places of its quarter of K, and it reads x there (32 values of row g) in the same order. The
-// warps that share rows add their sums in shared memory, and over a cluster where K is split further.
+// warps that share rows add their sums in shared memory, and over a cluster where an expert's K is split further.
 //
 // The two rows of a lane are 8 apart, or a gate row and its up row (64 apart), so that a lane has both.
 #include "mx4.cuh"
@@ -29,7 +29,7 @@ struct FewArgs {
   float limit;
   int n_blocks, k_blocks;
   int share;             // warps of a CTA that share rows (a power of two)
-  int splits;            // CTAs of a cluster, each with a part of K
+  int splits;            // CTAs of a cluster, each with a part of K; 1 for kDense
   // experts: item = a pair of a token and one of its experts (kExpertsIn), or a token (kExpertsOut)
   const int* ids;
   const float* weights;
@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(kThreads, MODE == kDense ? 3 : 2) gemv_mx4_ker
   extern __shared__ __align__(16) uint8_t x_smem[];  // [row of x][block][column group][16 bytes, in another order per group]
   __shared__ float4 red[kThreads];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, row = lane >> 2, t4 = lane & 3;
-  const int rank = g.splits > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
-  const int cta = g.splits > 1 ? blockIdx.x / g.splits : blockIdx.x;
+  const int splits = MODE == kDense ? 1 : g.splits;
+  const int rank = splits > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
+  const int cta = splits > 1 ? blockIdx.x / splits : blockIdx.x;
   const int n_blk = cta / g.share, group = cta % g.share * (8 / g.share) + warp / g.share;  // 16 rows: group of the block
   const int r_lo = GLU ? 8 * group + row : 16 * group + row;
   constexpr int kApart = GLU ? 64 : 8;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kDense ? 3 : 2) gemv_mx4_ker
   auto expert_of = [&](int slot) { return MODE == kDense ? 0 : s_expert[slot]; };
 
   // ---- blocks of columns (kExpertsOut: those of a token's experts one behind the other): the CTA's [b0, b1), every share-th a warp's
-  const int total = g.k_blocks * slots, per = ceil_div(total, g.splits);
+  const int total = g.k_blocks * slots, per = ceil_div(total, splits);
   const int b0 = rank * per, b1 = min(b0 + per, total), first = b0 + warp % g.share;
   const int count = first < b1 ? (b1 - first + g.share - 1) / g.share : 0;
   const uint8_t* const row_of_blocks = g.w + static_cast<int64_t>(n_blk) * g.k_blocks * kBlockBytes;
@@ -202,13 +203,13 @@ __global__ void __launch_bounds__(kThreads, MODE == kDense ? 3 : 2) gemv_mx4_ker
       v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
     }
     acc[0] = v.x, acc[1] = v.y, acc[2] = v.z, acc[3] = v.w;
-    if (g.splits > 1) red[threadIdx.x] = v;
+    if (splits > 1) red[threadIdx.x] = v;
   }
-  if (g.splits > 1) {
+  if (splits > 1) {
     __syncwarp();
     cluster_sync_all();
     if (rank == 0 && warp % g.share == 0) {
-      for (int s = 1; s < g.splits; ++s) {
+      for (int s = 1; s < splits; ++s) {
         const float4 o = ld_shared_cluster_f32x4(cluster_map_shared(smem_u32(&red[threadIdx.x]), s));
         acc[0] += o.x, acc[1] += o.y, acc[2] += o.z, acc[3] += o.w;
       }
@@ -281,7 +282,7 @@ int launch_few(FewArgs g, int items, cudaStream_t stream) {
   g.shift = kMx4Shift;
   const int total = g.k_blocks * (MODE == kExpertsOut ? g.top : 1), T = MODE == kDense ? g.T : 1;
   g.splits = few_splits(8 * g.n_blocks * items, total, T, &g.share);
-  if (g.splits == 0) return PXL_ERR_TOO_LARGE;
+  if (g.splits == 0 || (MODE == kDense && g.splits > 1)) return PXL_ERR_TOO_LARGE;
   static bool configured[64] = {false};
   const int dev = pxl_host::current_device_slot();
   if (!configured[dev]) {
@@ -314,25 +315,26 @@ int launch_few(FewArgs g, int items, cudaStream_t stream) {
 
 }  // namespace
 
+namespace pxl_host {
+
 // Up to four rows where two warps at least share rows, else the tensor-memory kernel is as fast (4 rows: 12288 x 4096 15.0 us here
 // and 17.2 there, 51200 x 5120 46 and 40; 8 rows of 4096 x 4096 11.0 and 9.9).
-PXL_EXPORT int pxl_gemv_mx4_takes(int M, int N, int K) {
+bool gemv_mx4_takes(int M, int N, int K) {
   int share;
   const int groups = 8 * pxl::ceil_div(N, kTileRows), total = pxl::ceil_div(K, kTileCols);
-  return M <= 4 && groups * 2 <= pxl_host::num_sms() * 40 && few_splits(groups, total, M, &share) == 1;
+  return M <= 4 && groups * 2 <= num_sms() * 40 && few_splits(groups, total, M, &share) == 1;
 }
 
-PXL_EXPORT int pxl_gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
-                            const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, cudaStream_t stream) {
-  if (M <= 0 || M > PXL_GEMV_MX4_MAX_M || N <= 0 || K <= 0 || K % 32) return PXL_ERR_INVALID_ARG;
-  if ((reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(ldx * 2)) & 15) return PXL_ERR_INVALID_ARG;
-  if (epi != PXL_EPI_NONE && ((epi != PXL_EPI_SILU_MUL && epi != PXL_EPI_CLIP_GLU) || N % 128)) return PXL_ERR_INVALID_ARG;
+int gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
+             const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, cudaStream_t stream) {
   FewArgs g{};
   g.x = static_cast<const bf16*>(x), g.ldx = ldx, g.w = static_cast<const uint8_t*>(w), g.row_scale = row_scale, g.C = C, g.ldc = ldc;
   g.bias = static_cast<const bf16*>(bias), g.residual = static_cast<const bf16*>(residual), g.ldr = ldr;
   g.T = M, g.N = N, g.K = K, g.epi = epi, g.limit = limit;
   return epi == PXL_EPI_NONE ? launch_few<kDense, false>(g, 1, stream) : launch_few<kDense, true>(g, 1, stream);
 }
+
+}  // namespace pxl_host
 
 // Up to sixteen pairs whose experts' matrices (read for every pair) are 64 MB together, and whose columns of x fit shared memory. Device
 // time here and by way of sorted rows and grouped products: one token through 4 of 32 experts of 2880 x 2880 37 and 45 us, two tokens

@@ -54,3 +54,10 @@ __device__ __forceinline__ float mx4_gate(float g, float u, int epi, float limit
 }
 
 }  // namespace pxl
+
+namespace pxl_host {
+// gemv_mx4.cu: what pxl_gemm_mx4 does, for up to four rows; whether that is the faster way for them
+bool gemv_mx4_takes(int M, int N, int K);
+int gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
+             const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, cudaStream_t stream);
+}  // namespace pxl_host

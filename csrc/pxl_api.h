@@ -305,12 +305,7 @@ int pxl_mx4_pack(const void* codes, const void* scales, void* data, float* row_s
 // mx4.cuh), row_scale fp32 [N up to 128].
 int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
                  const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, int* status, pxl_stream_t stream);
-// gemv_mx4.cu: the same for up to eight rows; pxl_gemm_mx4 takes it by itself where it is the faster way
-#define PXL_GEMV_MX4_MAX_M 8
-int pxl_gemv_mx4_takes(int M, int N, int K);
-int pxl_gemv_mx4(const void* x, int64_t ldx, const void* w, const float* row_scale, void* C, int64_t ldc, const void* bias,
-                 const void* residual, int64_t ldr, int M, int N, int K, int epi, float limit, pxl_stream_t stream);
-// Routed gated experts of a few tokens, every pair of a token and an expert on its own: h [T * top, I] (scratch, 16-byte aligned) and
+// gemv_mx4.cu: routed gated experts of a few tokens, every pair of a token and an expert on its own: h [T * top, I] (scratch, 16-byte aligned) and
 // out [T, K] = base (optional) + sum_j weights[t, j] FFN_{ids[t, j]}(x[t]); w1 [E * 2 I, K] with gate / up rows in groups of 64, w2
 // [E * K, I]. epi PXL_EPI_SILU_MUL or PXL_EPI_CLIP_GLU; ids outside of [0, E) add nothing.
 int pxl_moe_mx4_few_takes(int T, int top, int K, int I);  // whether it is the faster way

@@ -2,6 +2,8 @@
 
 import contextlib
 import ctypes
+import pathlib
+import re
 
 import pytest
 import torch
@@ -209,3 +211,12 @@ def test_weights_of_other_sizes_than_they_say():
                  (w.data[:0], w.row_scale[:0], 130, 160, 0), (w.data.to("meta"), w.row_scale, 130, 160, 2)):
         with pytest.raises(ops.KernelError):
             new(*args)
+
+
+def test_every_entry_point_is_called():
+    """What the library exports for microscaled numbers is what the wrappers call."""
+    header = (pathlib.Path(_lib.__file__).parents[2] / "csrc" / "pxl_api.h").read_text()
+    names = set(re.findall(r"\b(pxl_\w*mx4\w*)\(", header))
+    wrappers = pathlib.Path(cu.__file__).read_text()
+    assert {"pxl_gemm_mx4", "pxl_moe_mx4_few", "pxl_mx4_pack"} <= names <= set(_lib._SIGS)
+    assert all(f".{n}(" in wrappers for n in names)
