@@ -44,7 +44,7 @@ class Mx4Weight:
     ``data``: per expert, blocks of 128 rows x 128 columns, those of a row of blocks one behind the other. A block holds its codes
     ``[column group of 32][row][16 bytes]`` and then a byte of power per ``[row][column group]``; rows and columns are filled up to
     a whole block with zeros. Eight neighbouring codes share a 32-bit word, the even ones in its low half, the odd ones in its high
-    half, with their bits where two at a time become bf16 with few instructions (see ``csrc/mx4.cu``).
+    half, with their bits where two at a time become bf16 with few instructions (see ``csrc/mx4.cuh``).
     ``row_scale`` fp32 ``[experts, rows filled up]``: factors of the rows, powers of two (1 where no scale of the row exceeds 128; a
     row with a larger one is stored relative to it, and values 2^128 times smaller than the row's largest scale become 0), NaN where
     the row has a scale of 255."""
@@ -124,7 +124,9 @@ class Mx4Weight:
         return cls(data, row_scale, N, K, experts)
 
     def unpack(self) -> tuple[torch.Tensor, torch.Tensor]:
-        """The codes and scales that :meth:`pack` was given (``[experts * rows, ...]``)."""
+        """Codes and scales ``[experts * rows, ...]`` of the values that products see: those that :meth:`pack` was given, but for groups more
+        than 2^128 below the largest scale of their row, which come back as zeros with the smallest power that the row holds, and rows with a scale
+        of 255, whose other scales come back relative to the largest of them where that exceeds 128 (every result of such a row is NaN)."""
         E, N, K = self.experts, self.rows, self.cols
         nt, kt = -(-N // TILE), -(-K // TILE)
         blocks = self.data.view(E, nt, kt, BLOCK_BYTES)

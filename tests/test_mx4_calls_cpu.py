@@ -220,3 +220,17 @@ def test_every_entry_point_is_called():
     wrappers = pathlib.Path(cu.__file__).read_text()
     assert {"pxl_gemm_mx4", "pxl_moe_mx4_few", "pxl_mx4_pack"} <= names <= set(_lib._SIGS)
     assert all(f".{n}(" in wrappers for n in names)
+
+
+def test_what_a_laid_out_weight_gives_back():
+    """All of a row whose scales are powers within 2^128 of its largest; elsewhere the values that products see, as the docstring says."""
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randint(0, 256, (4, 48), generator=g, dtype=torch.uint8)
+    scales = torch.tensor([[130, 200, 254], [10, 200, 72], [255, 200, 130], [255, 1, 128]], dtype=torch.uint8)
+    w = ops.Mx4Weight.pack(codes, scales)
+    c, s = w.unpack()
+    assert torch.equal(c[0], codes[0]) and torch.equal(s[0], scales[0])
+    assert s[1].tolist() == [72, 200, 72] and int(c[1, :16].max()) == 0 and torch.equal(c[1, 16:], codes[1, 16:])   # 10 is below 200 - 128
+    assert s[2].tolist() == [255, 128, 58] and torch.isnan(w.row_scale[0, 2])                 # relative to 200, which the factor does not say
+    assert torch.equal(s[3], scales[3]) and torch.equal(c[2:], codes[2:])
+    assert "NaN" in ops.Mx4Weight.unpack.__doc__ and "mx4.cuh" in ops.Mx4Weight.__doc__
