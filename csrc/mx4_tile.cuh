@@ -142,11 +142,12 @@ __device__ __forceinline__ void finish8(const TileArgs& g, float (&f)[16], bool 
 }
 
 // Groups of four warps, one per quarter of the lanes, that take an accumulator's chunks of tokens in turn. A lane has a weight row.
-// A warp writes 32 neighbours of a token at a time; or (STAGED) a chunk goes through shared memory to be written in vectors of eight:
-// which pays where the products are quick (8111 x 12288 x 4096 in 4 bits on both sides 208 us, 222 without) and costs where they are
-// not (the experts of 24008 rows with fp32 results 7 %, 8192 x 24576 x 4096 1 %) or where rows start on no 16 bytes (3484 x 28286 x 768
-// in 4 bits on both sides: 305 us, 86 without). A chunk's residual is asked for as a whole: one value after the other, 4718 x 6656 x
-// 8544 takes 863 us, 465 so. Gate and up rows are 64 lanes apart: their warps
+// A warp writes 32 neighbours of a token at a time; or (STAGED, with a residual) a chunk goes through shared memory to be read and written
+// in vectors of eight: which pays for products of two 4-bit matrices with a residual (100 x 16384 x 512 7.6 us, 8.2 without; 8192 x 4096 x
+// 12288 234 and 241; 4718 x 6656 x 8544 204 and 205), and costs without one (4096 x 12288 x 1024 55.1 us, 50.6 without; 4096 x 4096 x 4096
+// 41.6 and 39.6; 8111 x 12288 x 4096 216 and 213), with bf16 rows (8192 x 24576 x 4096 1 %; 24008 experts' rows in fp32 7 %) and where rows
+// start on no 16 bytes (3484 x 28286 x 768 305 us, 86 without). A chunk's residual is asked for as a whole: one value after the other,
+// 4718 x 6656 x 8544 with bf16 rows takes 863 us, 465 so. Gate and up rows are 64 lanes apart: their warps
 // hand each other half of a chunk's tokens. SPLIT: results stay in shared memory as [token][weight row], for add_ranges. `parts`: room
 // for a tile's results (SPLIT), `staging`: kStaging bytes (STAGED, gated).
 template <bool SPLIT, bool STAGED>
@@ -184,7 +185,7 @@ __device__ __forceinline__ void write_results(const TileArgs& g, const int* firs
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (j < m) parts[(c0 + j) * kPitch + r] = __uint_as_float(v[j]) * factor + add;
-      } else if (STAGED && g.vec) {
+      } else if (STAGED && g.vec && g.residual) {
         named_bar_sync(1 + group, 128);  // (the last chunk has been read)
 #pragma unroll
         for (int j = 0; j < 32; ++j)

@@ -110,3 +110,14 @@ def test_a_result_in_the_place_of_its_residual(T):
     out = buf.view(-1)[:192].view(1, 192) if T == 1 else buf[:, :192]          # (of one row the strides may differ)
     oracle.within(ops.linear_mx4(x, w, residual=buf[:, :192], out=out), *want)
     assert torch.equal(buf[:, 192:], kept[:, 192:])
+
+
+@pytest.mark.parametrize("T,N,K", [(5, 640, 4096), (60, 40000, 224), (130, 2800, 768), (300, 512, 1024), (1500, 1536, 512)])
+def test_results_with_and_without_a_residual_of_zeros(T, N, K):
+    """Results leave the kernel in another way beside a residual: the same bits."""
+    (xc, xs), (wc, ws) = (tuple(t.to(DEV) for t in _matrix(r, K, r)) for r in (T, N))
+    b = _normal(N, seed=1).to(DEV)
+    want = ops.linear_mx4_rows(xc, xs, wc, ws, b)
+    assert torch.equal(ops.linear_mx4_rows(xc, xs, wc, ws, b, residual=torch.zeros_like(want)), want)
+    wide = torch.zeros(T, N + 3, dtype=torch.bfloat16, device=DEV)             # and to rows that start on no 16 bytes
+    assert torch.equal(ops.linear_mx4_rows(xc, xs, wc, ws, b, out=wide[:, 3:]), want)
