@@ -274,6 +274,8 @@ PXL_EXPORT int pxl_gemm_mx4(const void* x, int64_t ldx, const void* w, const flo
   g.C = C, g.row_scale = row_scale, g.ldc = ldc, g.bias = static_cast<const bf16*>(bias);
   g.residual = static_cast<const bf16*>(residual), g.ldr = ldr, g.M = M, g.N = N, g.epi = epi, g.limit = limit;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kTileCols);
+  // One tile for up to 256 tokens; in two, which expand all weights twice (us, one and two): 96 x 5120 x 25600 38 and 47, 203 60 and 75, 256
+  // 66 and 86; 128 x 25600 x 5120 42 and 47, 203 64 and 64, 256 71 and 66; 128 x 12288 x 4096 19 and 25; 203 x 4096 x 4096 20.5 and 16.5.
   g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks, g.k_blocks));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   // The SMs at work on 8 tiles of tokens share those and some 18 blocks of weights, from L2; with all tiles in one group x comes from

@@ -11,8 +11,8 @@
 // lanes x 16 bytes, repeated for the four quarters) takes them: four groups of row r at (r % 32) * 16 + (r / 32) * 4. Where rows
 // start on four bytes they come by cp.async, else through registers, a step ahead.
 //
-// 48 x 4096 x 12288 takes 14 us, by the latency of launch, loads and exchange (25 MB of weights); 8111 x 12288 x 4096 168 us and 5 for the
-// powers, 4.9 PFLOP/s, by the results: a tile has 16 steps of K.
+// 48 x 4096 x 12288 takes 13 us, by the latency of launch, loads and exchange (25 MB of weights); 8111 x 12288 x 4096 212 us under the power
+// cap, powers laid out and all, 3.9 PFLOP/s, by the results: a tile has 16 steps of K.
 #include "mx4_tile.cuh"
 
 namespace {
@@ -308,7 +308,7 @@ struct RowsPlan {
 };
 // Tiles of tokens and how their powers are brought in; the same for the workspace's size and the launch. Rows of x that share their
 // powers' copies with few others take them from where they are (one launch less); with more than 128 the copies, of four bytes here
-// and there, would be what bounds the kernel (8111 x 12288 x 4096: 357 us, 182 with the powers laid out ahead, 4 us of them for that).
+// and there, would be what bounds the kernel (8111 x 12288 x 4096: 336 us, 212 with the powers laid out ahead; 3484 x 28286 x 768 126, 87).
 bool plan_rows(RowsPlan& p, int M, int N, int K) {
   static bool configured[64] = {};
   if (!pxl_host::allow_smem(configured, gemm_mx4_rows_kernel<false, false>, gemm_mx4_rows_kernel<true, false>, gemm_mx4_rows_kernel<false, true>))
@@ -316,6 +316,8 @@ bool plan_rows(RowsPlan& p, int M, int N, int K) {
   TileArgs& g = p.g;
   g.M = M, g.N = N;
   g.n_blocks = pxl::ceil_div(N, kTileRows), g.k_blocks = pxl::ceil_div(K, kStep);
+  // One tile for up to 256 tokens (us, one and two): 96 x 5120 x 25600 26 and 32, 203 29 and 50, 256 39 and 53; 128 x 25600 x 5120 27 and 25,
+  // 256 34 and 31; 128 x 12288 x 4096 15 and 19, 256 18 and 19; 203 x 4096 x 4096 15.7 and 13.3.
   g.t_tiles = M <= 256 ? 1 : pxl::ceil_div(M, tile_tokens(M, g.n_blocks, g.k_blocks));
   g.bt = pxl::ceil_div(pxl::ceil_div(M, g.t_tiles), 16) * 16;
   g.t_group = g.t_tiles;

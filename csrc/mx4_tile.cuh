@@ -295,8 +295,8 @@ __device__ __forceinline__ void add_ranges(const TileArgs& g, int i, uint32_t pa
 
 namespace pxl_host {
 
-// Clusters of `size` CTAs that run at a time; of kernels that leave room for one CTA per SM. (A GPU processing cluster's SMs that are
-// no multiple of the size stay empty.)
+// Clusters of `size` CTAs that run at a time, counted as if there were room for one CTA per SM, also where tiles of up to 64 rows leave
+// room for two. (A GPU processing cluster's SMs that are no multiple of the size stay empty.)
 template <typename Kernel>
 inline int max_clusters(Kernel kernel, int size, int threads, int smem) {
   static int cached[64][9] = {};
@@ -320,8 +320,8 @@ inline int max_clusters(Kernel kernel, int size, int threads, int smem) {
   return n;
 }
 
-// Ranges of K blocks for a launch of `items` tiles, none of them empty and of two blocks at least: the number of rounds times a
-// range's blocks and what a round costs besides, in blocks. `slots`: CTAs at a time without clusters.
+// Ranges of K blocks for a launch of `items` tiles, none of them empty and all but the last of two blocks at least: the number of rounds
+// times a range's blocks and what a round costs besides, in blocks. `slots`: CTAs at a time without clusters.
 template <typename Kernel>
 inline void split_k(pxl::TileArgs& g, int64_t items, int slots, int besides, Kernel split, int threads) {
   g.splits = 1, g.kb_per = g.k_blocks;

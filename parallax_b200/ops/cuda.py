@@ -1204,6 +1204,7 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
                               pos_of, src_tok, stream), "pxl_moe_align")
         xp = torch.empty((P, K), dtype=torch.bfloat16, device=dev)
         check(L.pxl_moe_gather(x.data_ptr(), src_tok, offsets + 4 * E, xp.data_ptr(), P, K, stream), "pxl_moe_gather")
+        # (the rows between the products are bf16, the tensor cores' operand; those behind them stay fp32 until a token's sum is rounded)
         act = _grouped_mx4(xp, w1, offsets, P, epi, b1, limit, torch.bfloat16, status, stream)
         y = _grouped_mx4(act, w2, offsets, P, EPI_NONE, b2, 0.0, torch.float32, status, stream)
         check(L.pxl_moe_combine_f32(y.data_ptr(), pos_of, weights.data_ptr(), _ptr(base), out.data_ptr(), T, k, K, stream),
