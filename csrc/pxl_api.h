@@ -568,6 +568,32 @@ int pxl_tanh_norm(const float* x, const float* w, const float* b, float alpha, c
 int pxl_act_rows(const void* x, int64_t ldx, int x_f32, int act, const void* table, int64_t ldt, int col, const int* ids,
                  int64_t num_ids, void* out, int64_t ldo, int out_f32, int T, int N, int* status, pxl_stream_t stream);
 
+// ---- kv_i8.cu, attn_i8.cu: keys and values in 8 bits ---------------------------------------------
+// k_cache, v_cache: int8 codes [num_blocks, Hkv, page, D], D 64 or 128, page 16, 32 or 64; kv_max [num_blocks, Hkv, 2]: the largest
+// magnitude of a page's keys and of its values. A code stands for code * (kv_max / 127). Block tables [B, max_blocks].
+// New tokens into the cache: rows cu_q[b] .. cu_q[b + 1] of k and v [T, Hkv, D] (heads side by side, strides in elements) are the last
+// of the ctx_lens[b] tokens of sequence b, at most max_q_len of each.
+int pxl_kv_i8_store(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int* block_tables, const int* cu_q,
+                    const int* ctx_lens, void* k_cache, void* v_cache, float* kv_max, int T, int B, int max_q_len, int Hkv, int D, int page,
+                    int max_blocks, int64_t num_blocks, int* status, pxl_stream_t stream);
+// The first cu_k[b + 1] - cu_k[b] tokens of sequence b from row cu_k[b] of k and v [rows, Hkv, D] bf16 on; other rows become zeros.
+int pxl_kv_i8_load(const void* k_cache, const void* v_cache, const float* kv_max, const int* block_tables, const int* cu_k, void* k, void* v,
+                   int rows, int B, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, int* status, pxl_stream_t stream);
+// Of every sequence the first, the recent and the heaviest tokens, keep of them, into the pages of new_tables [B, max_new]. weights
+// [slots, Hkv, W], a sequence's in slot seq_slots[b] (null: b). kept [B, Hkv, keep] (-1 behind the last), new_lens [B].
+int pxl_kv_i8_evict(void* k_cache, void* v_cache, float* kv_max, float* weights, int64_t W, int slots, const int* seq_slots,
+                    const int* block_tables, const int* ctx_lens, const int* new_tables, int* kept, int* new_lens, int B, int Hkv, int D,
+                    int page, int max_blocks, int max_new, int64_t num_blocks, int keep, int recent, int first, int* status,
+                    pxl_stream_t stream);
+// Attention of the queries q [T, Hq, D] (heads side by side) over the cache. cu_q null: one query per sequence. weights (null: none): what
+// a token got, summed over the queries of the call and over the query heads of its key head, is added to weights[slot, head, token].
+// workspace: pxl_attn_i8_workspace bytes.
+int64_t pxl_attn_i8_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights, int decode);
+int pxl_attn_i8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max, const int* block_tables,
+                const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks, float* weights, int64_t W, int slots,
+                const int* seq_slots, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page,
+                int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
+
 // ---- stage_exec.cu: all layers of a dense GQA stage for one step behind one call --------------
 // The descriptor structs are defined in stage_exec.cu (mirrored by parallax_b200/engine/native_stage.py).
 struct PxlStageDesc;

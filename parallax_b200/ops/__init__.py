@@ -19,7 +19,8 @@ _NAMES = [
     "add_inplace", "patch_ids", "attn_decode", "attn_prefill", "argmax", "apply_penalties", "sample", "moe_route", "moe_ffn",
     "mla_kv_prep", "mla_q_absorb", "mla_attn", "mla_unabsorb", "mla_prefill", "store_rows", "dsa_index_prep", "dsa_index_scores", "topk_select",
     "quant_fp8_rows", "linear_fp8", "moe_ffn_fp8",
-    "quant_mx4_rows", "expand_mx4_rows", "linear_mx4", "linear_mx4_rows", "moe_ffn_mx4", "causal_conv1d_silu", "gated_delta_rule", "sigmoid_gate_mul", "gate_mul_grouped", "row_dot", "msa_block_scores", "msa_select",
+    "quant_mx4_rows", "expand_mx4_rows", "linear_mx4", "linear_mx4_rows", "moe_ffn_mx4",
+    "store_kv_i8", "load_kv_i8", "attn_decode_i8", "attn_prefill_i8", "evict_kv_i8", "causal_conv1d_silu", "gated_delta_rule", "sigmoid_gate_mul", "gate_mul_grouped", "row_dot", "msa_block_scores", "msa_select",
     "embed_rows", "to_low", "residual_norm", "row_norm", "latent_prep", "head_linear", "latent_attn",
     "glu_linear", "routed_ffn", "residual_add", "conv_qkv_prep", "gated_rows", "lightning_attn",
     "latent_rows", "latent_queries", "act_linear", "tanh_norm", "residual_step", "matrix_memory",

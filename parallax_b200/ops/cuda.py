@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib, mx4
+from . import _lib, kv_i8, mx4
 from ._lib import EPI_CLIP_GLU, EPI_F32, EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, check
 from .mx4 import Mx4Weight
 
@@ -1211,6 +1211,103 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
               "pxl_moe_combine_f32")
     _count(5 if alone else 7)
     return out
+
+
+# ------------------------------------------------------------------- keys and values in 8 bits
+def _head_rows(x: torch.Tensor) -> torch.Tensor:
+    """Rows whose heads lie side by side and start on 16 bytes: a copy of others."""
+    ok = x.stride(2) == 1 and (x.stride(1) == x.shape[2] or x.shape[1] == 1) and not x.stride(0) & 7 and not x.data_ptr() & 15
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def store_kv_i8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor,
+                block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_lens: torch.Tensor, max_q_len: int) -> None:
+    N, Hkv, page, D, B, MB = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
+    k, v, dev = _head_rows(k), _head_rows(v), k_cache.device
+    if B == 0 or k.shape[0] == 0 or max_q_len == 0:
+        return
+    with _on(dev):
+        check(_lib.lib().pxl_kv_i8_store(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), block_tables.data_ptr(), cu_q.data_ptr(),
+                                         ctx_lens.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), k.shape[0], B,
+                                         min(max_q_len, k.shape[0]), Hkv, D, page, MB, N, status_tensor(dev).data_ptr(), _stream(dev)),
+              "pxl_kv_i8_store")
+    _count()
+
+
+def load_kv_i8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor, block_tables: torch.Tensor, cu_k: torch.Tensor,
+               rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    N, Hkv, page, D, B, MB = kv_i8.check_load("load_kv_i8", (k_cache, v_cache, kv_max), block_tables, cu_k, rows)
+    dev = k_cache.device
+    k = torch.empty((rows, Hkv, D), dtype=torch.bfloat16, device=dev)
+    v = torch.empty((rows, Hkv, D), dtype=torch.bfloat16, device=dev)
+    if rows == 0:
+        return k, v
+    with _on(dev):
+        check(_lib.lib().pxl_kv_i8_load(k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(), cu_k.data_ptr(),
+                                        k.data_ptr(), v.data_ptr(), rows, B, Hkv, D, page, MB, N, status_tensor(dev).data_ptr(),
+                                        _stream(dev)), "pxl_kv_i8_load")
+    _count()
+    return k, v
+
+
+def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, window, sinks, max_ctx, out, weights, seq_slots):
+    N, Hkv, page, D, B, MB, max_ctx = kv_i8.check_attention(what, q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks, out, weights,
+                                                            seq_slots, max_ctx)
+    q, dev = _head_rows(q), q.device
+    T, Hq, _ = q.shape
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    if T == 0 or B == 0 or max_q_len == 0:
+        return out
+    k_cache, v_cache, kv_max = cache
+    W, slots = (weights.shape[2], weights.shape[0]) if weights is not None else (0, 0)
+    with _on(dev):
+        lib = _lib.lib()
+        need = lib.pxl_attn_i8_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, int(weights is not None), int(cu_q is None))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None      # of this call: calls on other streams have their own
+        check(lib.pxl_attn_i8(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(),
+                              _ptr(cu_q), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks), _ptr(weights), W, slots,
+                              _ptr(seq_slots), _ptr(ws), need, T, B, max_q_len, Hq, Hkv, D, page, MB, N, float(scale), window, max_ctx,
+                              status_tensor(dev).data_ptr(), _stream(dev)), "pxl_attn_i8")
+    _count(1 if weights is None else 2)
+    return out
+
+
+def attn_decode_i8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor, block_tables: torch.Tensor,
+                   ctx_lens: torch.Tensor, scale: float, window: int = 0, sinks: Optional[torch.Tensor] = None, max_ctx: int = 0,
+                   out: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                   seq_slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return _attn_i8("attn_decode_i8", q, (k_cache, v_cache, kv_max), block_tables, None, ctx_lens, 1, scale, window, sinks, max_ctx, out,
+                    weights, seq_slots)
+
+
+def attn_prefill_i8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor, block_tables: torch.Tensor,
+                    cu_q: torch.Tensor, ctx_lens: torch.Tensor, max_q_len: int, scale: float, window: int = 0,
+                    sinks: Optional[torch.Tensor] = None, max_ctx: int = 0, out: Optional[torch.Tensor] = None,
+                    weights: Optional[torch.Tensor] = None, seq_slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if cu_q is None:
+        kv_i8.refuse("attn_prefill_i8", "cu_q is int32 [sequences + 1]")
+    return _attn_i8("attn_prefill_i8", q, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len, scale, window, sinks, max_ctx,
+                    out, weights, seq_slots)
+
+
+def evict_kv_i8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
+                ctx_lens: torch.Tensor, new_tables: torch.Tensor, keep: int, recent: int, first: int = 0,
+                seq_slots: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    N, Hkv, page, D, B, MB, MN = kv_i8.check_evict("evict_kv_i8", (k_cache, v_cache, kv_max), weights, block_tables, ctx_lens, new_tables, keep,
+                                                   recent, first, seq_slots)
+    dev = k_cache.device
+    kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return kept, lens
+    with _on(dev):
+        check(_lib.lib().pxl_kv_i8_evict(k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), weights.data_ptr(), weights.shape[2],
+                                         weights.shape[0], _ptr(seq_slots), block_tables.data_ptr(), ctx_lens.data_ptr(),
+                                         new_tables.data_ptr(), kept.data_ptr(), lens.data_ptr(), B, Hkv, D, page, MB, MN, N, keep, recent,
+                                         first, status_tensor(dev).data_ptr(), _stream(dev)), "pxl_kv_i8_evict")
+    _count(2)
+    return kept, lens
 
 
 # ---------------------------------------------------------------------------- gated delta net

@@ -15,7 +15,7 @@ import math
 
 import torch
 
-from . import mx4
+from . import kv_i8, mx4
 
 EPI_NONE, EPI_RESIDUAL, EPI_SILU_MUL, EPI_F32 = 0, 1, 2, 3
 EPI_CLIP_GLU = 10
@@ -638,6 +638,145 @@ def moe_ffn_mx4(x, ids, weights, w1, w2, base=None, act_mode: int = 0, limit: fl
                          EPI_NONE, 0.0, None, torch.float32)
         out.index_add_(0, tok, y * weights[tok, slot][:, None])
     return out.to(x.dtype)
+
+
+# ------------------------------------------------------------------------ keys and values in 8 bits
+def _kv_i8_codes(x, most):
+    """Codes of values for magnitudes: round(127 x / most), 0 where that is none. fp64 holds 127 x, so that a tie is one."""
+    c = torch.round(x.double() * 127 / torch.where(most > 0, most, torch.ones_like(most)).double())
+    return torch.where(most.isnan(), torch.zeros_like(c), c).to(torch.int8)
+
+
+def _kv_i8_again(codes, old, new):
+    """Codes for another magnitude: round(code * old / new); as they are where that is none."""
+    c = torch.round(codes.double() * old.double() / torch.where(new > 0, new, torch.ones_like(new)).double())
+    return torch.where(new.isnan(), codes.double(), c).to(torch.int8)
+
+
+def _kv_i8_sequence(k_cache, v_cache, kv_max, table, n):
+    """Keys and values ``[heads, n, D]`` of a sequence's first n tokens, fp32."""
+    page = k_cache.shape[2]
+    blocks = table[:-(-n // page)].long()
+    scale = kv_max[blocks] / 127
+    return [(c[blocks].float() * scale[..., j, None, None]).transpose(0, 1).flatten(1, 2)[:, :n] for j, c in enumerate((k_cache, v_cache))]
+
+
+def store_kv_i8(k, v, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, max_q_len):
+    """Writes the new tokens' keys and values ``[T, heads, D]`` into an 8-bit cache (see :mod:`.kv_i8`): rows ``cu_q[b]`` to ``cu_q[b + 1]``
+    are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each. The pages that are written belong to one
+    sequence each; what a page holds behind the last token stays."""
+    _, Hkv, page, D, B, _ = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
+    for b in range(B):
+        row, n, t = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b]), int(ctx_lens[b])
+        for p in range((t - n) // page, (t - 1) // page + 1) if n > 0 else ():
+            lo, hi = max(0, t - n - p * page), min(page, t - p * page)
+            blk, r = int(block_tables[b, p]), row + p * page + lo - (t - n)
+            for j, (x, cache) in enumerate(((k, k_cache), (v, v_cache))):
+                x = x[r:r + hi - lo].float().transpose(0, 1)                                  # [heads, tokens, D]
+                top = torch.where(torch.isfinite(x), x.abs(), torch.full_like(x, float("nan"))).amax((1, 2))
+                if lo > 0:
+                    old = kv_max[blk, :, j].clone()
+                    top = torch.maximum(top, old)
+                    cache[blk, :, :lo] = _kv_i8_again(cache[blk, :, :lo], old[:, None, None], top[:, None, None])
+                cache[blk, :, lo:hi] = _kv_i8_codes(x, top[:, None, None])
+                kv_max[blk, :, j] = top
+
+
+def load_kv_i8(k_cache, v_cache, kv_max, block_tables, cu_k, rows):
+    """Keys and values of an 8-bit cache as bf16 ``[rows, heads, D]``: the first ``cu_k[b + 1] - cu_k[b]`` tokens of sequence b from row
+    ``cu_k[b]`` on. Rows behind the last sequence are zero."""
+    _, Hkv, page, D, B, _ = kv_i8.check_load("load_kv_i8", (k_cache, v_cache, kv_max), block_tables, cu_k, rows)
+    out = [torch.zeros((rows, Hkv, D), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2)]
+    for b in range(B):
+        lo, hi = int(cu_k[b]), int(cu_k[b + 1])
+        for o, x in zip(out, _kv_i8_sequence(k_cache, v_cache, kv_max, block_tables[b], hi - lo) if hi > lo else ()):
+            o[lo:hi] = x.transpose(0, 1).bfloat16()
+    return out[0], out[1]
+
+
+def _attend_i8(q, cache, table, n, t, scale, window, sinks, weights):
+    """Output of the last n of t tokens' queries ``[n, Hq, D]``; weights: ``[heads, tokens]`` to add to."""
+    k, v = _kv_i8_sequence(*cache, table, t)
+    G = q.shape[1] // k.shape[0]
+    s = torch.einsum("qhgd,hkd->hgqk", q.float().unflatten(1, (-1, G)), k) * scale
+    pos, key = torch.arange(t - n, t)[:, None], torch.arange(t)[None]
+    seen = (key <= pos) & (key > pos - window) if window else key <= pos
+    s = s.masked_fill(~seen, float("-inf"))
+    if sinks is not None:
+        s = torch.cat([s, sinks.view(-1, G, 1, 1).expand(-1, -1, n, 1)], -1)
+    p = torch.softmax(s, -1)[..., :t].masked_fill(~seen, 0.0)
+    if weights is not None:
+        weights[:, :t] += p.double().sum((1, 2)).float()
+    none = v.isnan().any(-1)                     # tokens whose values are no numbers: for those who see them
+    o = torch.einsum("hgqk,hkd->qhgd", p, v.masked_fill(none[..., None], 0.0))
+    o[(none[:, None] & seen).any(-1).T] = float("nan")
+    return o.flatten(1, 2).to(q.dtype)
+
+
+def attn_decode_i8(q, k_cache, v_cache, kv_max, block_tables, ctx_lens, scale, window=0, sinks=None, max_ctx=0, out=None, weights=None,
+                   seq_slots=None):
+    """One query per sequence, ``q [B, Hq, D]``, over an 8-bit cache (see :mod:`.kv_i8`): ``window`` keys per query (0: all), ``sinks [Hq]``
+    beside them. ``max_ctx``: no sequence is longer (0: as long as the tables reach). ``weights [slots, heads, tokens]``: what the query
+    gave to each token, summed over the query heads of a key head, is added there, sequence b in slot ``seq_slots[b]`` (None: b)."""
+    cache = (k_cache, v_cache, kv_max)
+    kv_i8.check_attention("attn_decode_i8", q, cache, block_tables, None, ctx_lens, scale, window, sinks, out, weights, seq_slots, max_ctx)
+    res = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    for b in range(q.shape[0]):
+        t, slot = int(ctx_lens[b]), b if seq_slots is None else int(seq_slots[b])
+        res[b] = 0
+        if t > 0:
+            res[b:b + 1] = _attend_i8(q[b:b + 1], cache, block_tables[b], 1, t, scale, window, sinks, None if weights is None else weights[slot])
+    return res
+
+
+def attn_prefill_i8(q, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, max_q_len, scale, window=0, sinks=None, max_ctx=0, out=None,
+                    weights=None, seq_slots=None):
+    """The queries of new tokens, ``q [T, Hq, D]``, over an 8-bit cache that holds their keys and values already: rows ``cu_q[b]`` to
+    ``cu_q[b + 1]`` are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each, and see the tokens up to their
+    own. The other arguments are those of ``attn_decode_i8``; rows behind the last sequence stay as they are."""
+    cache = (k_cache, v_cache, kv_max)
+    kv_i8.check_attention("attn_prefill_i8", q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks, out, weights, seq_slots, max_ctx)
+    res = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    for b in range(ctx_lens.shape[0]):
+        lo, hi, t = int(cu_q[b]), int(cu_q[b + 1]), int(ctx_lens[b])
+        if hi > lo and t > 0:
+            slot = b if seq_slots is None else int(seq_slots[b])
+            res[lo:hi] = _attend_i8(q[lo:hi], cache, block_tables[b], hi - lo, t, scale, window, sinks, None if weights is None else weights[slot])
+    return res
+
+
+def evict_kv_i8(k_cache, v_cache, kv_max, weights, block_tables, ctx_lens, new_tables, keep, recent, first=0, seq_slots=None):
+    """Thins the sequences of an 8-bit cache out to ``keep`` tokens per key head: the ``first`` first, the ``recent`` last and, of those
+    between, the ones with the largest ``weights`` (of equal ones the earliest; NaN counts as the largest). They move, in their order, into
+    the pages of ``new_tables``, which no sequence of ``block_tables`` reads; shorter sequences move whole. A new page has the largest of the
+    magnitudes that its tokens had. ``weights`` move along, and are zero behind what stayed. Returns the tokens that stayed, int32
+    ``[B, heads, keep]`` (-1 behind the last), and the new lengths, int32 ``[B]``."""
+    cache = (k_cache, v_cache, kv_max)
+    _, Hkv, page, D, B, _, _ = kv_i8.check_evict("evict_kv_i8", cache, weights, block_tables, ctx_lens, new_tables, keep, recent, first, seq_slots)
+    kept = torch.full((B, Hkv, keep), -1, dtype=torch.int32, device=k_cache.device)
+    head = torch.arange(Hkv)[:, None]
+    for b in range(B):
+        t, row = int(ctx_lens[b]), weights[b if seq_slots is None else int(seq_slots[b])]
+        n = min(t, keep)
+        if n <= 0:
+            continue
+        idx = torch.arange(n).expand(Hkv, -1)
+        if t > keep:
+            best = torch.sort(row[:, first:t - recent], dim=-1, descending=True, stable=True).indices[:, :keep - first - recent] + first
+            ends = torch.cat([torch.arange(first), torch.arange(t - recent, t)]).expand(Hkv, -1)
+            idx = torch.cat([best, ends], 1).sort(-1).values
+        kept[b, :, :n] = idx.int()
+        row[:, :t] = torch.cat([row.gather(1, idx), row.new_zeros(Hkv, t - n)], 1)
+        src = block_tables[b].long()[idx // page]
+        moved = [(c[src, head, idx % page], kv_max[src, head, j]) for j, c in enumerate((k_cache, v_cache))]
+        for p in range(-(-n // page)):
+            blk, hi = int(new_tables[b, p]), min(page, n - p * page)
+            for j, (c, dst) in enumerate(zip(moved, (k_cache, v_cache))):
+                codes, most = (x[:, p * page:p * page + hi] for x in c)
+                top = most.amax(1)
+                dst[blk, :, :hi] = _kv_i8_again(codes, most[..., None], top[:, None, None])
+                kv_max[blk, :, j] = top
+    return kept, ctx_lens.clamp(min=0, max=keep)
 
 
 # ---------------------------------------------------------------------------- gated delta net
