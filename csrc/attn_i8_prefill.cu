@@ -147,11 +147,11 @@ attn_i8_weights_kernel(const bf16* __restrict__ q, int64_t q_stride, const Cache
 
 }  // namespace
 
-PXL_EXPORT int64_t pxl_attn_i8_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights, int decode) {
+PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights) {
   return with_weights ? static_cast<int64_t>(T) * Hq * 4 : 0;
 }
 
-PXL_EXPORT int pxl_attn_i8(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max,
+PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max,
                            const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks,
                            float* weights, int64_t W, int slots, const int* seq_slots, void* workspace, int64_t workspace_bytes, int T, int B,
                            int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, float scale, int window,
@@ -160,7 +160,7 @@ PXL_EXPORT int pxl_attn_i8(const void* q, int64_t q_stride, const void* k_cache,
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv > kMaxGroup || !(scale > 0.f) ||
       (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
       ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) || max_blocks <= 0 || num_blocks <= 0 ||
-      num_blocks * Hkv * page >= (1ll << 31) || workspace_bytes < pxl_attn_i8_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, weights != nullptr, !cu_q))
+      num_blocks * Hkv * page >= (1ll << 31) || workspace_bytes < pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, weights != nullptr))
     return PXL_ERR_INVALID_ARG;
   if (Hkv > 65535 || B > 65535) return PXL_ERR_TOO_LARGE;
   const Cache cache{static_cast<const int8_t*>(k_cache), static_cast<const int8_t*>(v_cache), kv_max, block_tables, Hkv, page, max_blocks,

@@ -1261,14 +1261,22 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
         return out
     k_cache, v_cache, kv_max = cache
     W, slots = (weights.shape[2], weights.shape[0]) if weights is not None else (0, 0)
+    w = (_ptr(weights), W, slots, _ptr(seq_slots))
+    where = (Hq, Hkv, D, page, MB, N, float(scale), window, max_ctx, status_tensor(dev).data_ptr(), _stream(dev))
     with _on(dev):
         lib = _lib.lib()
-        need = lib.pxl_attn_i8_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, int(weights is not None), int(cu_q is None))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None      # of this call: calls on other streams have their own
-        check(lib.pxl_attn_i8(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(),
-                              _ptr(cu_q), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks), _ptr(weights), W, slots,
-                              _ptr(seq_slots), _ptr(ws), need, T, B, max_q_len, Hq, Hkv, D, page, MB, N, float(scale), window, max_ctx,
-                              status_tensor(dev).data_ptr(), _stream(dev)), "pxl_attn_i8")
+        if cu_q is None:
+            need = lib.pxl_attn_i8_decode_workspace(B, Hq, Hkv, D, max_ctx, int(weights is not None))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)      # of this call: calls on other streams and graphs have their own
+            check(lib.pxl_attn_i8_decode(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
+                                         block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks), *w,
+                                         ws.data_ptr(), need, B, *where), "pxl_attn_i8_decode")
+        else:
+            need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, int(weights is not None))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            check(lib.pxl_attn_i8_prefill(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
+                                          block_tables.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0),
+                                          _ptr(sinks), *w, _ptr(ws), need, T, B, max_q_len, *where), "pxl_attn_i8_prefill")
     _count(1 if weights is None else 2)
     return out
 
