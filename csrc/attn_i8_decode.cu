@@ -140,7 +140,7 @@ struct Rows {
     // (of pages that have a token which is seen; a NaN is passed over)
     const float r_new = fmaxf(r_run, fmaxf(tok_base + 16 > lo ? near.y : 0.f, tok_base + 16 < hi ? far.y : 0.f));
     const float share[2] = {page_share(near.y, r_new), page_share(far.y, r_new)};
-    const float r_corr = r_new > r_run ? __fdividef(r_run, r_new) : 1.f;
+    const float r_corr = r_new > r_run ? page_share(r_run, r_new) : 1.f;
     r_run = r_new;
 #pragma unroll
     for (int h = 0; h < kRows; ++h) {

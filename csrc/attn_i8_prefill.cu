@@ -1,27 +1,571 @@
-// Attention over keys and values in 8 bits (layout: kv_i8.cu): one CTA per (query row, key head), a thread per key for the scores and per
-// column for the output.
+// Attention of new tokens over keys and values in 8 bits (layout: kv_i8.cu) on the 5th-generation tensor cores.
+//
+// A CTA takes 128 / G tokens of a sequence twice (G query heads of a key head: G rows per token, two units of 128 rows) and a range of
+// its keys in tiles of 128:
+//   warp 8      : TMA producer. The queries once (a box of tokens x heads x 64 columns per unit and half), then the codes of K and V of a
+//                 tile, page by page, into a ring of staging tiles; and what the softmax needs to know of the tile's pages.
+//   warps 12-15 : convert the codes to f16 tiles, K-major for K, MN-major for V, in a ring that the tensor cores read: once for the 256
+//                 rows of both units.
+//   warp 9      : MMA issuer. P_u V, then S_u = Q_u K^T of the next tile, u = 0, 1 in turn: the products of one unit run under the softmax
+//                 of the other.
+//   warps 0-7   : softmax, a row of 128 scores per thread. First they scale their rows of Q by powers of two into f16. P replaces S in
+//                 tensor memory as f16, the A operand of the second product.
+// A score is multiplied by its page's key magnitude with the softmax scale. Values are held relative to R, at least the largest value
+// magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R, so
+// that what is rounded to f16 is the probability times the share (2^-11 of it, down to 2^-21 of the row's largest; 2^-32 below), and the
+// sum of a page's 16 columns is divided by the share again. Both the reference maximum (by 2^8) and R are let run ahead before O in tensor
+// memory is rescaled.
+// Few rows: the keys are split over several CTAs, whose results a second kernel adds up.
+// Every wait is bounded; on expiry the kernel records a status code, all roles unwind, tensor memory is freed.
+#include <atomic>
+
+#include "attention_rows.cuh"
+#include "attention_walk.cuh"
 #include "common.cuh"
+#include "kv_i8.cuh"
 #include "pxl_api.h"
+#include "tc_issue.cuh"
 
 namespace {
 using namespace pxl;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxGroup = 16, kKeys = 128;
+constexpr int kT = 128;  // keys per tile
+constexpr int kRowsQ = 128;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kConvertWarp = 12, kThreads = 512;
+constexpr int kHalf = 128 * 128;  // bytes of 64 columns of 128 rows
+constexpr float kUp = 7.f;        // log2 of the factor on probabilities; 2^8 of a stale maximum on top stays below 2^16
+constexpr int kRing = 8;          // tiles whose pages' numbers are kept: the producer is at most three ahead of a softmax, five at D = 64
 
+template <int D>
+struct Shape {
+  static constexpr int kTile = D / 64 * kHalf;         // a f16 tile of 128 rows
+  static constexpr int kCodes = 128 * D;               // codes of a tile
+  static constexpr int kStages = D == 128 ? 2 : 4;     // staging tiles
+  static constexpr int kSlots = D == 128 ? 4 : 6;      // f16 tiles
+  static constexpr int kOffKV = 2 * kTile;             // behind the two units of Q
+  static constexpr int kOffCodes = kOffKV + kSlots * kTile;
+  static constexpr int kOffPages = kOffCodes + kStages * kCodes;  // [kRing][8] float4
+  static constexpr int kOffBars = kOffPages + kRing * 8 * 16;
+  static constexpr int kSmem = 1024 + kOffBars + 256;
+  static constexpr uint32_t kIdescS = umma_idesc(kRowsQ, kT, 0, 0);
+  static constexpr uint32_t kIdescPV = umma_idesc(kRowsQ, D, 0, 0) | (1u << 16);  // B (V) is MN-major
+};
+static_assert(Shape<128>::kSmem <= 232448);
+
+struct Args {
+  const float2* kv_max;
+  const int *block_tables, *cu_q, *ctx_lens;
+  bf16* out;
+  int64_t out_stride;
+  const float* sinks;
+  float *lse, *parts;  // log2 of the sums [T, Hq] (null: not wanted); partial results [splits][T * Hq][D + 4]
+  int T, Hq, Hkv, page, max_blocks;
+  int64_t num_blocks;
+  float scale_log2;
+  int window, splits;
+  int* status;
+};
+
+// What a row's keys gave: maximum (log2), sum, output in units of R times 2^kUp.
+constexpr int kPartTail = 4;
+
+// V tile as B operand of all its columns: 64-column chunks kHalf apart
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
+  return (umma_desc_k_sw128(addr) & ~(0x3fffull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
+}
+
+// One tile of 128 codes x D into f16. Eight neighbouring lanes take four chunks of 16 codes of rows r and r ^ 5: both the chunk that is
+// read and the two that are written fall on all banks.
+template <int D>
+__device__ __forceinline__ void convert_tile(uint32_t codes, uint32_t tile, int warp, int lane) {
+  constexpr int kSteps = D / 16;  // 8 rows x 4 chunks at a time, 16 * D / 64 of them for four warps
+  const int c4 = lane & 3, r8 = (lane >> 3) ^ ((lane & 4) ? 5 : 0);
+#pragma unroll
+  for (int s0 = 0; s0 < kSteps; s0 += 4) {
+    uint32_t w[4][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int i = (s0 + s) * 4 + warp, half = D == 128 ? i & 1 : 0, row = (D == 128 ? i >> 1 : i) * 8 + r8, c = half * 4 + c4;
+      const uint32_t at = D == 128 ? row * 128 + ((c ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[s][0]), "=r"(w[s][1]), "=r"(w[s][2]), "=r"(w[s][3])
+                   : "r"(codes + at));
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int i = (s0 + s) * 4 + warp, half = D == 128 ? i & 1 : 0, row = (D == 128 ? i >> 1 : i) * 8 + r8;
+      const uint32_t at = tile + half * kHalf + row * 128;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t a = flip_codes(w[s][2 * p]), b = flip_codes(w[s][2 * p + 1]);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((c4 * 2 + p) ^ (row & 7)) << 4)), "r"(codes_f16x2<0x4140>(a)),
+                     "r"(codes_f16x2<0x4342>(a)), "r"(codes_f16x2<0x4140>(b)), "r"(codes_f16x2<0x4342>(b))
+                     : "memory");
+      }
+    }
+  }
+}
+
+// This thread's row of Q in f16, in place, scaled by a power of two; returns the inverse of that. 0 for a row that is nobody's.
+template <int D>
+__device__ __forceinline__ float convert_row(uint32_t row_addr, int r, bool valid) {
+  float most = 0.f;
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    uint32_t x[4];
+    const uint32_t at = row_addr + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(x[j]);
+      most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
+  }
+  float down;
+  const float up = row_up(most, down);
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    uint32_t x[4];
+    const uint32_t at = row_addr + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(x[j]);
+      x[j] = valid ? pack_f16x2(f.x * up, f.y * up) : 0u;
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+  }
+  return down;
+}
+
+// One tile of a row: S from tensor memory, P back to its place. pages: 16 bytes for each page of the tile (key magnitude / 127, log2 of its
+// share of R plus kUp, the inverse of that power, R); shift: log2 of the 16-column groups in a page.
+template <int D, bool INTERIOR, typename Masked>
+__device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool first, Masked masked, float row_scale, const float4* pages,
+                                           int shift, float& m_run, float& r_run, float& l_run, uint32_t p_ready) {
+  uint32_t sc[kT];
+#pragma unroll
+  for (int c = 0; c < kT; c += 32) tmem_ld_32x32b_x32(my_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sc[c]));
+  const float r_new = pages[0].w;
+  tmem_ld_wait();
+  if constexpr (!INTERIOR) {
+#pragma unroll
+    for (int j = 0; j < kT; ++j)
+      if (masked(j)) sc[j] = 0xff800000u;  // -inf
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    float m2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        m2[k] = fmaxf(fmaxf(m2[k], __uint_as_float(sc[g * 16 + j + k])), __uint_as_float(sc[g * 16 + j + 2 + k]));
+    }
+    mx = fmaxf(mx, fmaxf(m2[0], m2[1]) * (pages[g >> shift].x * row_scale));  // (a NaN is passed over, also -inf times 0)
+  }
+  const float m_new = fmaxf(m_run, mx);
+  if (first) {
+    m_run = m_new;
+    r_run = r_new;
+  } else if (__any_sync(0xffffffffu, m_new > m_run + 8.f || r_new != r_run)) {
+    const float grown = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new)), corr = grown * page_share(r_run, r_new);
+    m_run = m_new;
+    r_run = r_new;
+    l_run *= grown;
+#pragma unroll
+    for (int c = 0; c < D; c += 16) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(my_o + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
+      tmem_st_32x32b_x16(my_o + c, v);
+    }
+  }
+  const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int c = h * 64; c < h * 64 + 64; c += 32) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float4 page = pages[((c >> 4) + g) >> shift];
+        const float scale = page.x * row_scale, off = page.y - m_use;
+        const uint64_t scale2 = pair2(scale, scale), off2 = pair2(off, off);
+        uint64_t sum = 0ull;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float s0 = __uint_as_float(sc[c + g * 16 + j]), s1 = __uint_as_float(sc[c + g * 16 + j + 1]);
+          const float2 x = unpair2(fma2(pair2(s0, s1), scale2, off2));
+          float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+          if constexpr (!INTERIOR) {  // (a magnitude of zero, or none, of a key that is not seen)
+            p0 = s0 == -INFINITY ? 0.f : p0;
+            p1 = s1 == -INFINITY ? 0.f : p1;
+          }
+          sum = add2(sum, pair2(p0, p1));
+          pk[g * 8 + (j >> 1)] = pack_f16x2(p0, p1);
+        }
+        const float2 two = unpair2(sum);
+        const float both = two.x + two.y;
+        l_run += INTERIOR || both != 0.f ? both * page.z : 0.f;
+      }
+      tmem_st_32x32b_x16(my_s + c / 2, pk);
+    }
+    tmem_st_wait();
+    tc_fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(p_ready + 8 * h);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sm0 = smem_u32(smem);
+  float4* pages_sm = reinterpret_cast<float4*>(smem + S::kOffPages);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
+  // q_full, q_ready | codes_full, codes_empty [kStages] | kv_full, kv_empty [kSlots] | s_full, o_full [2] | p_ready [2][2]
+  const uint32_t q_full = smem_u32(bars), q_ready = q_full + 8, codes_full = q_full + 16, codes_empty = codes_full + 8 * S::kStages,
+                 kv_full = codes_empty + 8 * S::kStages, kv_empty = kv_full + 8 * S::kSlots, s_full = kv_empty + 8 * S::kSlots,
+                 o_full = s_full + 16, p_ready = o_full + 16;
+  static_assert((2 + 2 * S::kStages + 2 * S::kSlots + 8) * 8 + 8 <= 256);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 + 2 * S::kStages + 2 * S::kSlots + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  pdl_wait();
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int b = blockIdx.z, kvh = blockIdx.y % a.Hkv, split = blockIdx.y / a.Hkv, G = a.Hq / a.Hkv;
+  const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin, ctx = a.ctx_lens[b];
+  const int per_unit = kRowsQ / G;  // tokens
+  // heavy blocks (late queries see the most keys) are scheduled first
+  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * per_unit;
+  if (q0 >= L || q_begin < 0 || q_begin + L > a.T) return;  // uniform for the CTA, before any barrier or allocation
+  const int units = L - q0 > per_unit ? 2 : 1, tokens = min(L - q0, 2 * per_unit);
+  const int pos0 = ctx - L + q0;      // position of the first token
+  const int hi = pos0 + tokens;       // keys [lo, hi) are seen by some row
+  const int lo = (a.window > 0 && pos0 - a.window + 1 > 0) ? pos0 - a.window + 1 : 0;
+  const int t_first = lo / kT, t_all = hi > lo ? ceil_div(hi, kT) - t_first : 0, t_each = ceil_div(t_all, a.splits);
+  const int t_begin = t_first + min(split * t_each, t_all);
+  const int n_tiles = __shfl_sync(0xffffffffu, min(t_each, t_first + t_all - t_begin), 0);
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    const int ppt = kT / a.page;
+    mbar_init(q_full, 1);
+    mbar_init(q_ready, 4 * units);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(codes_full + 8 * s, 1 + ppt);  // the bytes, and each page's numbers
+      mbar_init(codes_empty + 8 * s, 4);
+    }
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(kv_full + 8 * s, 4);
+      mbar_init(kv_empty + 8 * s, 1);
+    }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(s_full + 8 * u, 1);
+      mbar_init(o_full + 8 * u, 1);
+      for (int h = 0; h < 2; ++h) mbar_init(p_ready + 16 * u + 8 * h, 4);  // one arrival per softmax warp of the unit
+    }
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), 512);  // S_0 | S_1 | O_0 | O_1
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  pdl_launch_dependents();
+  const uint32_t tm_s = *tmem_slot, tm_o = tm_s + 2 * kT;
+
+  // 512 threads x 128 registers at launch cover 256 x 200 + 256 x 56
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kProducerWarp && n_tiles > 0) {
+      // ------------------------------------------------------------------ TMA producer: lane p has page p of a tile
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, units * (D / 64) * per_unit * G * 128);
+        for (int u = 0; u < units; ++u)
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_3d(sm0 + u * S::kTile + h * kHalf, &tm_q, q_full, h * 64, kvh * G, q_begin + q0 + u * per_unit);
+      }
+      const int ppt = kT / a.page;
+      const int* bt = a.block_tables + static_cast<size_t>(b) * a.max_blocks;
+      auto block_of = [&](int it) {
+        if (lane >= ppt || it >= n_tiles) return -1;
+        int bi = (t_begin + it) * ppt + lane;
+        if (bi * a.page >= ctx) bi = (ctx - 1) / a.page;  // beyond the context: the last page again (masked)
+        return bi < a.max_blocks ? bt[bi] : -1;
+      };
+      auto head_of = [&](int blk, int it) {
+        if (lane < ppt && it < n_tiles && (blk < 0 || blk >= a.num_blocks)) {
+          if (a.status) atomicCAS(a.status, 0, PXL_DEV_BAD_BLOCK_PREFILL);
+          blk = 0;
+        }
+        return (lane < ppt && it < n_tiles ? blk : 0) * a.Hkv + kvh;
+      };
+      int head = head_of(block_of(0), 0), blk = block_of(1);
+      float2 most = a.kv_max[head];
+      float r_all = 0.f;
+      bool ok = true;
+      int item = 0;
+      for (int it = 0; ok && it < n_tiles; ++it) {
+        const int next_head = head_of(blk, it + 1);
+        const float2 next = a.kv_max[next_head];  // on its way while this tile is issued
+        blk = block_of(it + 2);
+        // R and the tile's pages
+        const int tok = (t_begin + it) * kT + lane * a.page;
+        float m = lane < ppt && tok < hi && tok + a.page > lo ? most.y : 0.f;
+        m = m == m ? m : 0.f;
+        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+        if (m > r_all) r_all = fminf(2.f * m, 3.3e38f);
+        for (int kv = 0; ok && kv < 2; ++kv, ++item) {
+          const int stage = item % S::kStages;
+          if (item >= S::kStages)
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(codes_empty + 8 * stage, (item / S::kStages - 1) & 1, abort_flag, a.status,
+                                                           PXL_DEV_TIMEOUT_EMPTY));
+          if (!ok) break;
+          const uint32_t bar = codes_full + 8 * stage, dst = sm0 + S::kOffCodes + stage * S::kCodes + lane * a.page * D;
+          if (lane == 0) mbar_arrive_expect_tx(bar, S::kCodes);
+          __syncwarp();
+          if (lane < ppt) {
+            tma_load_2d(dst, kv ? &tm_v : &tm_k, bar, 0, head * a.page);
+            if (kv == 0) {
+              const float share = most.y == most.y ? fmaxf(page_share(most.y, r_all), 0x1p-40f) : most.y;
+              pages_sm[(it % kRing) * 8 + lane] = make_float4(most.x * kInv127, __log2f(share) + kUp, __fdividef(0x1p-7f, share), r_all);
+            }
+            mbar_arrive(bar);
+          }
+        }
+        head = next_head;
+        most = next;
+      }
+    } else if (warp == kMmaWarp && n_tiles > 0) {
+      // ------------------------------------------------------------------ MMA issuer
+      const uint32_t leader = elect_leader();
+      auto wait = [&](uint32_t bar, int parity, int code) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.status, code));
+        tc_fence_after_sync();
+        return ok;
+      };
+      auto slot_of = [](int item) { return item % S::kSlots; };  // item 2 i: K of tile i, 2 i + 1: V
+      auto full = [&](int item) { return wait(kv_full + 8 * slot_of(item), (item / S::kSlots) & 1, PXL_DEV_TIMEOUT_FULL); };
+      auto issue_s = [&](int u, int it) {
+        const uint32_t q = sm0 + u * S::kTile, k = sm0 + S::kOffKV + slot_of(2 * it) * S::kTile;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          mma_ss(tm_s + u * kT, umma_desc_k_sw128(q + off), umma_desc_k_sw128(k + off), S::kIdescS, ks > 0 ? 1u : 0u, leader);
+        }
+        commit(s_full + 8 * u, leader);
+      };
+      bool ok = wait(q_ready, 0, PXL_DEV_TIMEOUT_FULL) && full(0);
+      if (ok) {
+        for (int u = 0; u < units; ++u) issue_s(u, 0);
+        commit(kv_empty + 8 * slot_of(0), leader);
+      }
+      for (int it = 0; ok && it < n_tiles; ++it) {
+        const bool more = it + 1 < n_tiles;
+        ok = full(2 * it + 1);
+        const uint64_t dv = desc_v(sm0 + S::kOffKV + slot_of(2 * it + 1) * S::kTile);
+        for (int u = 0; ok && u < units; ++u) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && wait(p_ready + 16 * u + 8 * h, it & 1, PXL_DEV_TIMEOUT_TMEM_EMPTY);
+            if (!ok) break;
+#pragma unroll
+            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)  // 16 keys: 8 columns of P, 16 rows of V
+              mma_ts(tm_o + u * D, tm_s + u * kT + ks * 8, dv + 128 * ks, S::kIdescPV, (it > 0 || ks > 0) ? 1u : 0u, leader);
+          }
+          if (!ok) break;
+          if (u == units - 1) commit(kv_empty + 8 * slot_of(2 * it + 1), leader);
+          if (!more) commit(o_full + 8 * u, leader);
+          if (more) {
+            if (u == 0) ok = full(2 * it + 2);
+            if (!ok) break;
+            issue_s(u, it + 1);
+            if (u == units - 1) commit(kv_empty + 8 * slot_of(2 * it + 2), leader);
+          }
+        }
+      }
+    } else if (warp >= kConvertWarp) {
+      // ------------------------------------------------------------------ codes -> f16 tiles
+      for (int item = 0; item < 2 * n_tiles; ++item) {
+        const int stage = item % S::kStages, slot = item % S::kSlots;
+        bool ok = mbar_wait_bounded(codes_full + 8 * stage, (item / S::kStages) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_FULL);
+        if (ok && item >= S::kSlots)
+          ok = mbar_wait_bounded(kv_empty + 8 * slot, (item / S::kSlots - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_EMPTY);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        convert_tile<D>(sm0 + S::kOffCodes + stage * S::kCodes, sm0 + S::kOffKV + slot * S::kTile, warp - kConvertWarp, lane);
+        fence_proxy_async_smem();  // written through the generic proxy, read by the tensor cores through the async one
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(kv_full + 8 * slot);
+          mbar_arrive(codes_empty + 8 * stage);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax warps
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int u = warp >> 2, q4 = warp & 3;
+    if (u < units) {
+      const int r = q4 * 32 + lane, tok = u * per_unit + r / G, head = kvh * G + r % G;  // query row = TMEM lane
+      const bool valid = r < per_unit * G && tok < tokens;
+      const int q_pos = pos0 + tok, last = pos0 + min((u + 1) * per_unit, tokens) - 1;  // the unit's last position
+      const int key_lo = (a.window > 0 && q_pos - a.window + 1 > 0) ? q_pos - a.window + 1 : 0;
+      const uint32_t lane_sel = static_cast<uint32_t>(q4 * 32) << 16;
+      const uint32_t my_s = tm_s + u * kT + lane_sel, my_o = tm_o + u * D + lane_sel;
+      const int shift = a.page == 16 ? 0 : a.page == 32 ? 1 : 2;
+      float m_run = -INFINITY, r_run = 0.f, l_run = 0.f, row_scale = 0.f;
+      int failed = 0;
+      if (n_tiles > 0) {
+        failed = mbar_wait_bounded(q_full, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_FULL) ? 0 : 1;
+        if (!failed) row_scale = convert_row<D>(sm0 + u * S::kTile + r * 128, r, valid) * a.scale_log2;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_ready);
+      }
+      for (int it = 0; it < n_tiles; ++it) {
+        failed = mbar_wait_bounded(s_full + 8 * u, it & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
+        failed = __any_sync(0xffffffffu, failed);  // warp-uniform: the TMEM accesses below are warp-wide
+        if (failed) break;
+        tc_fence_after_sync();
+        const int key0 = (t_begin + it) * kT;
+        const float4* pages = pages_sm + (it % kRing) * 8;
+        // every key is seen by every row of the unit
+        const bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
+        if (interior) {
+          softmax_i8<D, true>(my_s, my_o, it == 0, [](int) { return false; }, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+        } else {
+          const int from = key_lo - key0, to = (valid ? q_pos + 1 : 0) - key0;  // columns that this row sees
+          softmax_i8<D, false>(my_s, my_o, it == 0, [&](int j) { return j < from || j >= to; }, row_scale, pages, shift, m_run, r_run, l_run,
+                               p_ready + 16 * u);
+        }
+      }
+      if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
+      failed = __any_sync(0xffffffffu, failed);
+      const int64_t row = static_cast<int64_t>(q_begin + q0 + tok) * a.Hq + head;
+      if (!failed && a.splits == 1) {
+        const float sink = a.sinks && valid ? a.sinks[head] * kLog2e : -INFINITY;
+        const float M = fmaxf(m_run, sink), Mu = M == -INFINITY ? 0.f : M, f = fast_exp2(m_run - Mu);
+        const float denom = l_run * f + fast_exp2(sink - Mu);
+        if (a.lse && valid) a.lse[row] = denom == 0.f ? INFINITY : Mu + log2f(denom);
+        const float inv = denom == 0.f ? 0.f : f / denom * (r_run * (kInv127 * 0x1p-7f));
+        bf16* dst = a.out + static_cast<int64_t>(q_begin + q0 + tok) * a.out_stride + head * D;
+        if (n_tiles > 0) tc_fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          if (n_tiles > 0) {
+            tmem_ld_32x32b_x32(my_o + c, v);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          }
+#pragma unroll
+          for (int c8 = 0; c8 < 32; c8 += 8) {
+            bf16x8 ov;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              ov.u[j] = denom == 0.f ? 0u
+                                     : pack_bf16x2(__uint_as_float(v[c8 + 2 * j]) * inv, __uint_as_float(v[c8 + 2 * j + 1]) * inv);
+            if (valid) st_bf16x8(dst + c + c8, ov);
+          }
+        }
+      } else if (!failed) {
+        float* po = a.parts + (split * static_cast<int64_t>(a.T) * a.Hq + row) * (D + kPartTail);
+        if (valid) *reinterpret_cast<float4*>(po + D) = make_float4(m_run, l_run, r_run, 0.f);
+        if (n_tiles > 0) {
+          tc_fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(my_o + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (valid) *reinterpret_cast<uint4*>(po + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          }
+        }
+      }
+      tc_fence_before_sync();
+    }
+  }
+
+  // ---------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (*abort_flag) __nanosleep(200000);  // loads that are still in flight must land before smem is released
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == kMmaWarp) tmem_dealloc(tm_s, 512);
+}
+
+// Adds up the parts of a row of a split call: a warp per (token, query head).
+template <int D>
+__global__ void __launch_bounds__(128)
+attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), rows = static_cast<int64_t>(a.T) * a.Hq;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int token = static_cast<int>(row / a.Hq), head = static_cast<int>(row % a.Hq);
+  if (row >= rows || token < a.cu_q[0] || token >= a.cu_q[B]) return;
+  const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
+  float M = -INFINITY, R = 0.f;
+  const float* p = a.parts + row * (D + kPartTail);
+  const int64_t next = rows * (D + kPartTail);
+  for (int s = lane; s < a.splits; s += 32) {
+    const float4 t = *reinterpret_cast<const float4*>(p + s * next + D);
+    M = fmaxf(M, t.x);
+    R = fmaxf(R, t.z);
+  }
+  M = warp_reduce_max(M);
+  R = warp_reduce_max(R);
+  const float top = fmaxf(M, sink), Mu = top == -INFINITY ? 0.f : top;
+  float l = fast_exp2(sink - Mu), acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 t = *reinterpret_cast<const float4*>(p + s * next + D);
+    if (t.y == 0.f) continue;  // none of its keys is seen (and its output was not written)
+    const float f = fast_exp2(t.x - Mu), fr = f * page_share(t.z, R);
+    l += t.y * f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] += p[s * next + i * 32 + lane] * fr;
+  }
+  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? INFINITY : Mu + log2f(l);
+  const float inv = l == 0.f ? 0.f : R * (kInv127 * 0x1p-7f) / l;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) a.out[token * a.out_stride + head * D + i * 32 + lane] = __float2bfloat16(acc[i] * inv);
+}
+
+// What each token got: a thread per key goes through the queries that see it.
 struct Cache {
-  const int8_t *k, *v;
-  const float* kv_max;
+  const int8_t* k;
+  const float2* kv_max;
   const int* block_tables;
   int Hkv, page, max_blocks;
   int64_t num_blocks;
   int* status;
-
-  // row of token t of sequence b (whose codes and magnitude are found by it); -1 off the cache
   __device__ __forceinline__ int64_t row(int b, int t, int h) const {
     const int p = t / page, blk = p < max_blocks ? block_tables[static_cast<size_t>(b) * max_blocks + p] : -1;
     if (blk < 0 || blk >= num_blocks) {
-      if (status) atomicCAS(status, 0, PXL_DEV_BAD_BLOCK_DECODE);
+      if (status) atomicCAS(status, 0, PXL_DEV_BAD_BLOCK_PREFILL);
       return -1;
     }
     return (static_cast<int64_t>(blk) * Hkv + h) * page + t % page;
@@ -42,99 +586,26 @@ __device__ __forceinline__ float dot(const int8_t* k, const float* q) {
 
 template <int D>
 __global__ void __launch_bounds__(128)
-attn_i8_kernel(const bf16* __restrict__ q, int64_t q_stride, const Cache cache, const int* __restrict__ cu_q, const int* __restrict__ ctx_lens,
-               bf16* __restrict__ out, int64_t out_stride, const float* __restrict__ sinks, float* __restrict__ lse, int B, int Hq,
-               float scale_log2, int window) {
-  __shared__ float q_sm[kMaxGroup][D], p_sm[kMaxGroup][kKeys], m_sm[4], l_sm[4];
-  __shared__ int64_t row_sm[kKeys];
-  __shared__ float M[kMaxGroup], L[kMaxGroup];
-  const int row = blockIdx.x, h = blockIdx.y, G = Hq / cache.Hkv, tid = threadIdx.x, warp = tid >> 5;
-  pdl_wait();
-  pdl_launch_dependents();
-  int b = row, pos = ctx_lens[cu_q ? 0 : row] - 1;
-  if (cu_q) {
-    if (row < cu_q[0] || row >= cu_q[B]) return;
-    b = 0;
-    while (cu_q[b + 1] <= row) ++b;
-    pos = ctx_lens[b] - cu_q[b + 1] + row;
-  }
-  const int hi = pos + 1, lo = window > 0 && hi > window ? hi - window : 0;
-  for (int i = tid; i < G * D; i += 128)
-    q_sm[i / D][i % D] = __bfloat162float(q[row * q_stride + (h * G + i / D) * D + i % D]) * scale_log2;
-  __syncthreads();
-  auto score = [&](int64_t at, int g) {
-    return dot<D>(cache.k + at * D, q_sm[g]) * (cache.kv_max[at / cache.page * 2] * (1.f / 127.f));
-  };
-  for (int g = 0; g < G; ++g) {
-    float m = -INFINITY, l = 0.f;
-    for (int t = lo + tid; t < hi; t += kKeys) {
-      const int64_t at = cache.row(b, t, h);
-      if (at < 0) continue;
-      const float s = score(at, g), mn = fmaxf(m, s);
-      l = l * exp2f(m - mn) + exp2f(s - mn);
-      m = mn;
-    }
-    const float wm = warp_reduce_max(m);
-    l = warp_reduce_sum(m == -INFINITY ? 0.f : l * exp2f(m - wm));
-    if ((tid & 31) == 0) m_sm[warp] = wm, l_sm[warp] = l;
-    __syncthreads();
-    if (tid == 0) {
-      float top = sinks ? sinks[h * G + g] * kLog2e : -INFINITY;
-      const float sink = top;
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, m_sm[i]);
-      float sum = sinks ? exp2f(sink - top) : 0.f;
-      for (int i = 0; i < 4; ++i) sum += m_sm[i] == -INFINITY ? 0.f : l_sm[i] * exp2f(m_sm[i] - top);
-      M[g] = top;
-      L[g] = sum;
-      if (lse) lse[static_cast<size_t>(row) * Hq + h * G + g] = sum > 0.f || !(sum == sum) ? top + log2f(sum) : INFINITY;
-    }
-    __syncthreads();
-  }
-  float acc[kMaxGroup];
-  for (int g = 0; g < G; ++g) acc[g] = 0.f;
-  for (int t0 = lo; t0 < hi; t0 += kKeys) {
-    const int64_t at = t0 + tid < hi ? cache.row(b, t0 + tid, h) : -1;
-    __syncthreads();
-    row_sm[tid] = at;
-    const float vs = at < 0 ? 0.f : cache.kv_max[at / cache.page * 2 + 1] * (1.f / 127.f);
-    for (int g = 0; g < G; ++g) p_sm[g][tid] = at < 0 ? 0.f : exp2f(score(at, g) - M[g]) * vs;
-    __syncthreads();
-    if (tid < D) {
-      for (int j = 0; j < kKeys; ++j) {
-        if (row_sm[j] < 0) continue;
-        const float x = cache.v[row_sm[j] * D + tid];
-        for (int g = 0; g < G; ++g) acc[g] = fmaf(p_sm[g][j], x, acc[g]);
-      }
-    }
-  }
-  if (tid < D)
-    for (int g = 0; g < G; ++g)
-      out[row * out_stride + (h * G + g) * D + tid] = __float2bfloat16(L[g] > 0.f || !(L[g] == L[g]) ? acc[g] / L[g] : 0.f);
-}
-
-// What each token got: a thread per key goes through the queries that see it.
-template <int D>
-__global__ void __launch_bounds__(128)
 attn_i8_weights_kernel(const bf16* __restrict__ q, int64_t q_stride, const Cache cache, const int* __restrict__ cu_q,
                        const int* __restrict__ ctx_lens, const float* __restrict__ lse, float* __restrict__ weights, int64_t W, int slots,
                        const int* __restrict__ seq_slots, int Hq, float scale_log2, int window) {
-  __shared__ float q_sm[kMaxGroup][D];
-  const int b = blockIdx.z, h = blockIdx.y, G = Hq / cache.Hkv, t = blockIdx.x * kKeys + threadIdx.x;
+  __shared__ float q_sm[16][D];
+  const int b = blockIdx.z, h = blockIdx.y, G = Hq / cache.Hkv, t = blockIdx.x * kT + threadIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  const int row0 = cu_q ? cu_q[b] : b, n = cu_q ? cu_q[b + 1] - row0 : 1, ctx = ctx_lens[b];
+  const int row0 = cu_q[b], n = cu_q[b + 1] - row0, ctx = ctx_lens[b];
   const int slot = seq_slots ? seq_slots[b] : b;
-  if (n <= 0 || static_cast<int>(blockIdx.x) * kKeys >= ctx) return;
+  if (n <= 0 || static_cast<int>(blockIdx.x) * kT >= ctx) return;
   if (slot < 0 || slot >= slots || ctx > W) {
     if (threadIdx.x == 0 && cache.status) atomicCAS(cache.status, 0, slot < 0 || slot >= slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
     return;
   }
   const int64_t at = t < ctx ? cache.row(b, t, h) : -1;
-  const float ks = at < 0 ? 0.f : cache.kv_max[at / cache.page * 2] * (1.f / 127.f);
+  const float ks = at < 0 ? 0.f : cache.kv_max[at / cache.page].x * kInv127;
   float sum = 0.f;
   for (int r = 0; r < n; ++r) {
     const int pos = ctx - n + r;
-    if (pos < static_cast<int>(blockIdx.x) * kKeys) continue;
+    if (pos < static_cast<int>(blockIdx.x) * kT) continue;
     __syncthreads();
     for (int i = threadIdx.x; i < G * D; i += 128)
       q_sm[i / D][i % D] = __bfloat162float(q[(row0 + r) * q_stride + (h * G + i / D) * D + i % D]) * scale_log2;
@@ -145,34 +616,93 @@ attn_i8_weights_kernel(const bf16* __restrict__ q, int64_t q_stride, const Cache
   if (at >= 0) weights[(static_cast<int64_t>(slot) * cache.Hkv + h) * W + t] += sum;
 }
 
+// Queries [T, Hq, D] as boxes of tokens x heads of a key head x 64 columns.
+bool make_tmap_q(CUtensorMap* out, const void* q, int64_t q_stride, int T, int Hq, int D, int G) {
+  pxl_host::EncodeTiledFn fn = pxl_host::encode_tiled_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(T > 1 ? q_stride : static_cast<int64_t>(Hq) * D) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRowsQ / G)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// CTAs that share a block of queries' keys: as many as fill the chip, each with at least four tiles.
+int splits_of(int B, int max_q_len, int Hq, int Hkv, int max_ctx) {
+  const int64_t blocks = static_cast<int64_t>(ceil_div(max_q_len, 2 * (kRowsQ / (Hq / Hkv)))) * Hkv * B;
+  const int64_t fill = pxl_host::num_sms() / (blocks > 0 ? blocks : 1), most = max_ctx / (4 * kT);
+  const int64_t s = fill < most ? fill : most;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+struct Layout {  // floats of the workspace
+  int splits;
+  int64_t parts, total;
+  Layout(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, bool weights) {
+    splits = splits_of(B, max_q_len, Hq, Hkv, max_ctx);
+    const int64_t rows = static_cast<int64_t>(T) * Hq;
+    parts = weights ? ceil_div64(rows, 4) * 4 : 0;
+    total = parts + (splits > 1 ? splits * rows * (D + kPartTail) : 0);
+  }
+};
+
+template <int D>
+int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int B, int max_q_len, cudaStream_t stream) {
+  static std::atomic<bool> configured[64];  // function attributes are per device
+  std::atomic<bool>& done = configured[pxl_host::current_device_slot()];
+  if (!done.load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(attn_i8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem) != cudaSuccess)
+      return PXL_ERR_CUDA;
+    done.store(true, std::memory_order_relaxed);
+  }
+  const int per = 2 * (kRowsQ / (a.Hq / a.Hkv));
+  pxl_host::launch(attn_i8_prefill_kernel<D>, dim3(ceil_div(max_q_len, per), a.Hkv * a.splits, B), dim3(kThreads), Shape<D>::kSmem, stream, tq,
+                   tk, tv, a);
+  if (a.splits > 1)
+    pxl_host::launch_behind(attn_i8_prefill_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div64(static_cast<int64_t>(a.T) * a.Hq, 4))), dim3(128),
+                            0, stream, a, B);
+  return cudaGetLastError() == cudaSuccess ? PXL_OK : PXL_ERR_CUDA;
+}
+
 }  // namespace
 
 PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights) {
-  return with_weights ? static_cast<int64_t>(T) * Hq * 4 : 0;
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len <= 0) return 0;
+  return Layout(T, B, max_q_len, Hq, Hkv, D, max_ctx, with_weights != 0).total * 4;
 }
 
 PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max,
-                           const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks,
-                           float* weights, int64_t W, int slots, const int* seq_slots, void* workspace, int64_t workspace_bytes, int T, int B,
-                           int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, float scale, int window,
-                           int max_ctx, int* status, cudaStream_t stream) {
-  if (T <= 0 || B <= 0) return PXL_OK;
-  if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv > kMaxGroup || !(scale > 0.f) ||
-      (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
-      ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) || max_blocks <= 0 || num_blocks <= 0 ||
-      num_blocks * Hkv * page >= (1ll << 31) || workspace_bytes < pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, weights != nullptr))
+                                   const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride,
+                                   const float* sinks, float* weights, int64_t W, int slots, const int* seq_slots, void* workspace,
+                                   int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
+                                   int64_t num_blocks, float scale, int window, int max_ctx, int* status, cudaStream_t stream) {
+  if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
+  if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
+      !(scale > 0.f) || (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+      ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || num_blocks <= 0 ||
+      num_blocks * Hkv * page >= (1ll << 31))
     return PXL_ERR_INVALID_ARG;
-  if (Hkv > 65535 || B > 65535) return PXL_ERR_TOO_LARGE;
-  const Cache cache{static_cast<const int8_t*>(k_cache), static_cast<const int8_t*>(v_cache), kv_max, block_tables, Hkv, page, max_blocks,
-                    num_blocks, status};
-  float* lse = weights ? static_cast<float*>(workspace) : nullptr;
-  auto go = [&](auto attend, auto weigh) {
-    pxl_host::launch(attend, dim3(T, Hkv), dim3(128), 0, stream, static_cast<const bf16*>(q), q_stride, cache, cu_q, ctx_lens,
-                     static_cast<bf16*>(out), out_stride, sinks, lse, B, Hq, scale * kLog2e, window);
-    if (weights)
-      pxl_host::launch(weigh, dim3(ceil_div(max_ctx, kKeys), Hkv, B), dim3(128), 0, stream, static_cast<const bf16*>(q), q_stride, cache, cu_q,
-                       ctx_lens, lse, weights, W, slots, seq_slots, Hq, scale * kLog2e, window);
+  const Layout at(T, B, max_q_len, Hq, Hkv, D, max_ctx, weights != nullptr);
+  if (workspace_bytes < at.total * 4 || (at.total > 0 && !workspace)) return PXL_ERR_INVALID_ARG;
+  if (static_cast<int64_t>(Hkv) * at.splits > 65535 || B > 65535) return PXL_ERR_TOO_LARGE;
+  CUtensorMap tq, tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * page;
+  if (!make_tmap_q(&tq, q, q_stride, T, Hq, D, Hq / Hkv) || !pxl_host::make_tmap_codes(&tk, k_cache, rows, D, page) ||
+      !pxl_host::make_tmap_codes(&tv, v_cache, rows, D, page))
+    return PXL_ERR_TENSORMAP;
+  float* ws = static_cast<float*>(workspace);
+  const Args a{reinterpret_cast<const float2*>(kv_max), block_tables, cu_q, ctx_lens, static_cast<bf16*>(out), out_stride, sinks,
+               weights ? ws : nullptr, at.splits > 1 ? ws + at.parts : nullptr, T, Hq, Hkv, page, max_blocks, num_blocks, scale * kLog2e, window,
+               at.splits, status};
+  const int rc = D == 64 ? launch_prefill<64>(tq, tk, tv, a, B, max_q_len, stream) : launch_prefill<128>(tq, tk, tv, a, B, max_q_len, stream);
+  if (rc || !weights) return rc;
+  const Cache cache{static_cast<const int8_t*>(k_cache), a.kv_max, block_tables, Hkv, page, max_blocks, num_blocks, status};
+  auto weigh = [&](auto kernel) {
+    pxl_host::launch_behind(kernel, dim3(ceil_div(max_ctx, kT), Hkv, B), dim3(128), 0, stream, static_cast<const bf16*>(q), q_stride, cache, cu_q,
+                            ctx_lens, a.lse, weights, W, slots, seq_slots, Hq, a.scale_log2, window);
     return cudaGetLastError() == cudaSuccess ? PXL_OK : PXL_ERR_CUDA;
   };
-  return D == 64 ? go(attn_i8_kernel<64>, attn_i8_weights_kernel<64>) : go(attn_i8_kernel<128>, attn_i8_weights_kernel<128>);
+  return D == 64 ? weigh(attn_i8_weights_kernel<64>) : weigh(attn_i8_weights_kernel<128>);
 }

@@ -38,7 +38,7 @@ constexpr float kInv127 = 1.f / 127.f;
 constexpr float kPUp = 15.f;  // log2 of the factor on probabilities in f16
 
 // share of a page's magnitude in the largest so far; 0 for a page of zeros, NaN for one without a magnitude
-__device__ __forceinline__ float page_share(float m, float most) { return m == 0.f ? 0.f : __fdividef(m, most); }
+__device__ __forceinline__ float page_share(float m, float most) { return m == 0.f ? 0.f : __fdiv_rn(m, most); }
 
 }  // namespace pxl
 

@@ -1215,8 +1215,10 @@ def moe_ffn_mx4(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w1: M
 
 # ------------------------------------------------------------------- keys and values in 8 bits
 def _head_rows(x: torch.Tensor) -> torch.Tensor:
-    """Rows whose heads lie side by side and start on 16 bytes: a copy of others."""
-    ok = x.stride(2) == 1 and (x.stride(1) == x.shape[2] or x.shape[1] == 1) and not x.stride(0) & 7 and not x.data_ptr() & 15
+    """Rows whose heads lie side by side, that do not overlap and start on 16 bytes: a copy of others."""
+    T, H, D = x.shape
+    s0, s1, s2 = x.stride()
+    ok = s2 == 1 and (s1 == D or H == 1) and not s0 & 7 and (s0 >= H * D or T < 2) and not x.data_ptr() & 15
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
