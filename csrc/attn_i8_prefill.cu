@@ -554,80 +554,6 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   for (int i = 0; i < D / 32; ++i) a.out[token * a.out_stride + head * D + i * 32 + lane] = __float2bfloat16(acc[i] * inv);
 }
 
-// What each token got: a thread per key goes through the queries that see it.
-struct Cache {
-  const int8_t* k;
-  const float2* kv_max;
-  const int* block_tables;
-  int Hkv, page, max_blocks;
-  int64_t num_blocks;
-  int* status;
-  __device__ __forceinline__ int64_t row(int b, int t, int h) const {
-    const int p = t / page, blk = p < max_blocks ? block_tables[static_cast<size_t>(b) * max_blocks + p] : -1;
-    if (blk < 0 || blk >= num_blocks) {
-      if (status) atomicCAS(status, 0, PXL_DEV_BAD_BLOCK_PREFILL);
-      return -1;
-    }
-    return (static_cast<int64_t>(blk) * Hkv + h) * page + t % page;
-  }
-};
-
-template <int D>
-__device__ __forceinline__ float dot(const int8_t* k, const float* q) {
-  float s = 0.f;
-  for (int c = 0; c < D; c += 16) {
-    const int4 x = *reinterpret_cast<const int4*>(k + c);
-    const int w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s = fmaf(static_cast<int8_t>(w[j >> 2] >> (8 * (j & 3))), q[c + j], s);
-  }
-  return s;
-}
-
-template <int D>
-__global__ void __launch_bounds__(128)
-attn_i8_weights_kernel(const bf16* __restrict__ q, int64_t q_stride, const Cache cache, const int* __restrict__ cu_q,
-                       const int* __restrict__ ctx_lens, const float* __restrict__ lse, float* __restrict__ weights, int64_t W, int slots,
-                       const int* __restrict__ seq_slots, int Hq, float scale_log2, int window) {
-  __shared__ float q_sm[16][D];
-  const int b = blockIdx.z, h = blockIdx.y, G = Hq / cache.Hkv, t = blockIdx.x * kT + threadIdx.x;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int row0 = cu_q[b], n = cu_q[b + 1] - row0, ctx = ctx_lens[b];
-  const int slot = seq_slots ? seq_slots[b] : b;
-  if (n <= 0 || static_cast<int>(blockIdx.x) * kT >= ctx) return;
-  if (slot < 0 || slot >= slots || ctx > W) {
-    if (threadIdx.x == 0 && cache.status) atomicCAS(cache.status, 0, slot < 0 || slot >= slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
-    return;
-  }
-  const int64_t at = t < ctx ? cache.row(b, t, h) : -1;
-  const float ks = at < 0 ? 0.f : cache.kv_max[at / cache.page].x * kInv127;
-  float sum = 0.f;
-  for (int r = 0; r < n; ++r) {
-    const int pos = ctx - n + r;
-    if (pos < static_cast<int>(blockIdx.x) * kT) continue;
-    __syncthreads();
-    for (int i = threadIdx.x; i < G * D; i += 128)
-      q_sm[i / D][i % D] = __bfloat162float(q[(row0 + r) * q_stride + (h * G + i / D) * D + i % D]) * scale_log2;
-    __syncthreads();
-    if (at >= 0 && t <= pos && (window <= 0 || t > pos - window))
-      for (int g = 0; g < G; ++g) sum += exp2f(dot<D>(cache.k + at * D, q_sm[g]) * ks - lse[static_cast<size_t>(row0 + r) * Hq + h * G + g]);
-  }
-  if (at >= 0) weights[(static_cast<int64_t>(slot) * cache.Hkv + h) * W + t] += sum;
-}
-
-// Queries [T, Hq, D] as boxes of tokens x heads of a key head x 64 columns.
-bool make_tmap_q(CUtensorMap* out, const void* q, int64_t q_stride, int T, int Hq, int D, int G) {
-  pxl_host::EncodeTiledFn fn = pxl_host::encode_tiled_fn();
-  if (!fn) return false;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D) * 2, static_cast<cuuint64_t>(T > 1 ? q_stride : static_cast<int64_t>(Hq) * D) * 2};
-  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRowsQ / G)};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // CTAs that share a block of queries' keys: as many as fill the chip, each with at least four tiles.
 int splits_of(int B, int max_q_len, int Hq, int Hkv, int max_ctx) {
   const int64_t blocks = static_cast<int64_t>(ceil_div(max_q_len, 2 * (kRowsQ / (Hq / Hkv)))) * Hkv * B;
@@ -638,12 +564,11 @@ int splits_of(int B, int max_q_len, int Hq, int Hkv, int max_ctx) {
 
 struct Layout {  // floats of the workspace
   int splits;
-  int64_t parts, total;
-  Layout(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, bool weights) {
+  int64_t total;
+  Layout(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx) {
     splits = splits_of(B, max_q_len, Hq, Hkv, max_ctx);
     const int64_t rows = static_cast<int64_t>(T) * Hq;
-    parts = weights ? ceil_div64(rows, 4) * 4 : 0;
-    total = parts + (splits > 1 ? splits * rows * (D + kPartTail) : 0);
+    total = splits > 1 ? splits * rows * (D + kPartTail) : 0;
   }
 };
 
@@ -667,15 +592,14 @@ int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 
 }  // namespace
 
-PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights) {
+PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx) {
   if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len <= 0) return 0;
-  return Layout(T, B, max_q_len, Hq, Hkv, D, max_ctx, with_weights != 0).total * 4;
+  return Layout(T, B, max_q_len, Hq, Hkv, D, max_ctx).total * 4;
 }
 
 PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max,
                                    const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride,
-                                   const float* sinks, float* weights, int64_t W, int slots, const int* seq_slots, void* workspace,
-                                   int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
+                                   const float* sinks, float* lse, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
                                    int64_t num_blocks, float scale, int window, int max_ctx, int* status, cudaStream_t stream) {
   if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
@@ -684,25 +608,15 @@ PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* 
       (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || num_blocks <= 0 ||
       num_blocks * Hkv * page >= (1ll << 31))
     return PXL_ERR_INVALID_ARG;
-  const Layout at(T, B, max_q_len, Hq, Hkv, D, max_ctx, weights != nullptr);
+  const Layout at(T, B, max_q_len, Hq, Hkv, D, max_ctx);
   if (workspace_bytes < at.total * 4 || (at.total > 0 && !workspace)) return PXL_ERR_INVALID_ARG;
   if (static_cast<int64_t>(Hkv) * at.splits > 65535 || B > 65535) return PXL_ERR_TOO_LARGE;
   CUtensorMap tq, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * page;
-  if (!make_tmap_q(&tq, q, q_stride, T, Hq, D, Hq / Hkv) || !pxl_host::make_tmap_codes(&tk, k_cache, rows, D, page) ||
+  if (!pxl_host::make_tmap_queries(&tq, q, q_stride, T, Hq, D, Hq / Hkv) || !pxl_host::make_tmap_codes(&tk, k_cache, rows, D, page) ||
       !pxl_host::make_tmap_codes(&tv, v_cache, rows, D, page))
     return PXL_ERR_TENSORMAP;
-  float* ws = static_cast<float*>(workspace);
-  const Args a{reinterpret_cast<const float2*>(kv_max), block_tables, cu_q, ctx_lens, static_cast<bf16*>(out), out_stride, sinks,
-               weights ? ws : nullptr, at.splits > 1 ? ws + at.parts : nullptr, T, Hq, Hkv, page, max_blocks, num_blocks, scale * kLog2e, window,
-               at.splits, status};
-  const int rc = D == 64 ? launch_prefill<64>(tq, tk, tv, a, B, max_q_len, stream) : launch_prefill<128>(tq, tk, tv, a, B, max_q_len, stream);
-  if (rc || !weights) return rc;
-  const Cache cache{static_cast<const int8_t*>(k_cache), a.kv_max, block_tables, Hkv, page, max_blocks, num_blocks, status};
-  auto weigh = [&](auto kernel) {
-    pxl_host::launch_behind(kernel, dim3(ceil_div(max_ctx, kT), Hkv, B), dim3(128), 0, stream, static_cast<const bf16*>(q), q_stride, cache, cu_q,
-                            ctx_lens, a.lse, weights, W, slots, seq_slots, Hq, a.scale_log2, window);
-    return cudaGetLastError() == cudaSuccess ? PXL_OK : PXL_ERR_CUDA;
-  };
-  return D == 64 ? weigh(attn_i8_weights_kernel<64>) : weigh(attn_i8_weights_kernel<128>);
+  const Args a{reinterpret_cast<const float2*>(kv_max), block_tables, cu_q, ctx_lens, static_cast<bf16*>(out), out_stride, sinks, lse,
+               static_cast<float*>(workspace), T, Hq, Hkv, page, max_blocks, num_blocks, scale * kLog2e, window, at.splits, status};
+  return D == 64 ? launch_prefill<64>(tq, tk, tv, a, B, max_q_len, stream) : launch_prefill<128>(tq, tk, tv, a, B, max_q_len, stream);
 }

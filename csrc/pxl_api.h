@@ -568,7 +568,7 @@ int pxl_tanh_norm(const float* x, const float* w, const float* b, float alpha, c
 int pxl_act_rows(const void* x, int64_t ldx, int x_f32, int act, const void* table, int64_t ldt, int col, const int* ids,
                  int64_t num_ids, void* out, int64_t ldo, int out_f32, int T, int N, int* status, pxl_stream_t stream);
 
-// ---- kv_i8.cu, attn_i8_decode.cu, attn_i8_prefill.cu: keys and values in 8 bits ---------------------------------------------
+// ---- kv_i8.cu, attn_i8_decode.cu, attn_i8_prefill.cu, attn_i8_weigh.cu: keys and values in 8 bits ---------------------------------------------
 // k_cache, v_cache: int8 codes [num_blocks, Hkv, page, D], D 64 or 128, page 16, 32 or 64; kv_max [num_blocks, Hkv, 2]: the largest
 // magnitude of a page's keys and of its values. A code stands for code * (kv_max / 127). Block tables [B, max_blocks].
 // New tokens into the cache: rows cu_q[b] .. cu_q[b + 1] of k and v [T, Hkv, D] (heads side by side, strides in elements) are the last
@@ -594,13 +594,18 @@ int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k_cache, con
                        const int* seq_slots, void* workspace, int64_t workspace_bytes, int B, int Hq, int Hkv, int D, int page, int max_blocks,
                        int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
 // The same of the queries of new tokens, rows cu_q[b] .. cu_q[b + 1] of q [T, Hq, D], the last of the ctx_lens[b] tokens of sequence b, at
-// most max_q_len of each; weights are summed over the queries too.
-int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx, int with_weights);
+// most max_q_len of each. lse (null: not wanted) [T, Hq]: log2 of the sums of exponentials.
+int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx);
 int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max, const int* block_tables,
-                        const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks, float* weights, int64_t W,
-                        int slots, const int* seq_slots, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv,
-                        int D, int page, int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx, int* status,
-                        pxl_stream_t stream);
+                        const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks, float* lse, void* workspace,
+                        int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
+                        int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
+// What these queries gave to each token, from their sums: added to weights [slots, Hkv, W].
+int64_t pxl_attn_i8_weigh_workspace(int B, int max_q_len, int Hq, int Hkv, int max_ctx);
+int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_cache, const float* kv_max, const int* block_tables, const int* cu_q,
+                      const int* ctx_lens, const float* lse, float* weights, int64_t W, int slots, const int* seq_slots, void* workspace,
+                      int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
+                      int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
 
 // ---- stage_exec.cu: all layers of a dense GQA stage for one step behind one call --------------
 // The descriptor structs are defined in stage_exec.cu (mirrored by parallax_b200/engine/native_stage.py).

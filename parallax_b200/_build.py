@@ -37,7 +37,7 @@ NVCC_FLAGS = [
 
 # Sources whose elementary functions must be accurate in fp32 (arithmetic of a recurrence, tanh norms, fp32 attention), whose
 # subnormals count (powers of two of 4-bit numbers) or whose quotients are rounded again (8-bit codes)
-ACCURATE = ("attention_any", "attn_i8_decode", "attn_i8_prefill", "delta_rule", "gated_delta", "gemm_mx4", "gemm_mx4_rows", "gemv_mx4", "kv_i8", "matrix_memory",
+ACCURATE = ("attention_any", "attn_i8_decode", "attn_i8_prefill", "attn_i8_weigh", "delta_rule", "gated_delta", "gemm_mx4", "gemm_mx4_rows", "gemv_mx4", "kv_i8", "matrix_memory",
             "mx4", "tanh_norm")
 
 

@@ -126,9 +126,10 @@ _SIGS = {
     "pxl_attn_i8_decode_workspace": [c_int] * 6,
     "pxl_attn_i8_decode": [_P, c_int64] + [_P] * 6 + [c_int64, _P, _P, c_int64, c_int, _P, _P, c_int64] + [c_int] * 6 + [c_int64, c_float, c_int,
                            c_int, _P, _P],
-    "pxl_attn_i8_prefill_workspace": [c_int] * 8,
-    "pxl_attn_i8_prefill": [_P, c_int64] + [_P] * 7 + [c_int64, _P, _P, c_int64, c_int, _P, _P, c_int64] + [c_int] * 8 + [c_int64, c_float, c_int,
-                            c_int, _P, _P],
+    "pxl_attn_i8_prefill_workspace": [c_int] * 7,
+    "pxl_attn_i8_prefill": [_P, c_int64] + [_P] * 7 + [c_int64, _P, _P, _P, c_int64] + [c_int] * 8 + [c_int64, c_float, c_int, c_int, _P, _P],
+    "pxl_attn_i8_weigh_workspace": [c_int] * 5,
+    "pxl_attn_i8_weigh": [_P, c_int64] + [_P] * 7 + [c_int64, c_int, _P, _P, c_int64] + [c_int] * 8 + [c_int64, c_float, c_int, c_int, _P, _P],
     "pxl_causal_conv1d_silu": [_P, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, _P],
     "pxl_gated_delta_rule": [_P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, _P, _P, _P, c_int64,
                              c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P, c_int64, _P],
@@ -194,7 +195,7 @@ _SIGS = {
 }
 
 
-_SIZES = {"pxl_attn_i8_decode_workspace", "pxl_attn_i8_prefill_workspace", "pxl_delta_rule_workspace", "pxl_gated_delta_workspace", "pxl_gemm_mx4_rows_workspace"}      # functions that return a number of bytes
+_SIZES = {"pxl_attn_i8_decode_workspace", "pxl_attn_i8_prefill_workspace", "pxl_attn_i8_weigh_workspace", "pxl_delta_rule_workspace", "pxl_gated_delta_workspace", "pxl_gemm_mx4_rows_workspace"}      # functions that return a number of bytes
 
 
 @lru_cache(maxsize=1)

@@ -1274,11 +1274,18 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
                                          block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks), *w,
                                          ws.data_ptr(), need, B, *where), "pxl_attn_i8_decode")
         else:
-            need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx, int(weights is not None))
+            need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            lse = None if weights is None else torch.empty((T, Hq), dtype=torch.float32, device=dev)
             check(lib.pxl_attn_i8_prefill(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
                                           block_tables.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0),
-                                          _ptr(sinks), *w, _ptr(ws), need, T, B, max_q_len, *where), "pxl_attn_i8_prefill")
+                                          _ptr(sinks), _ptr(lse), _ptr(ws), need, T, B, max_q_len, *where), "pxl_attn_i8_prefill")
+            if weights is not None:
+                need = lib.pxl_attn_i8_weigh_workspace(B, max_q_len, Hq, Hkv, max_ctx)
+                ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+                check(lib.pxl_attn_i8_weigh(q.data_ptr(), q.stride(0), k_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(),
+                                            cu_q.data_ptr(), ctx_lens.data_ptr(), lse.data_ptr(), *w, _ptr(ws), need, T, B, max_q_len, *where),
+                      "pxl_attn_i8_weigh")
     _count(1 if weights is None else 2)
     return out
 
