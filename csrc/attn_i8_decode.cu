@@ -2,10 +2,12 @@
 //
 // Every CTA gets the same number of tiles of 64 keys of the row of all (sequence, key head) pairs (attention_walk.cuh). A producer warp
 // brings the codes by TMA, page by page, and the pages' magnitudes by 8-byte cp.async into the same stage; four consumer warps, two per
-// tile, convert the codes where they multiply them (mma.sync, f16) and keep a running maximum, sum and output of the 16 rows of a warp's
-// products (the query heads of a key head; rows 8 to 15 are left out where there are at most 8). A score is multiplied by its page's key
-// magnitude in fp32. The output is held relative to the largest value magnitude R so far, beside the running maximum: probabilities times
-// a page's share of R are what is rounded to f16 (2^-11), with a factor of 2^15 so that they keep their bits down to 2^-29.
+// tile, convert the codes where they multiply them (mma.sync, f16). Keys, and columns of the values, are the 16 rows of the products, the
+// query heads of a key head their 8 columns (twice where there are more): S^T = K q^T, O^T = V^T P^T, a transposition of 8 x 8 between them.
+// A score is multiplied by its page's key magnitude with the softmax scale. Values are held relative to R, at least the largest value
+// magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R,
+// so that what is rounded to f16 (2^-11) is the probability times the share; a factor of 2^11 keeps its bits down to 2^-25 of the row's
+// largest, and it is rounded in steps of 2^-35 below. The reference maximum may lag by 2^4 before anything is rescaled.
 // A pair that lies in several CTAs is added up by a second kernel. Where the weights are wanted, the scores go to the workspace (4 bytes
 // per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are known.
 #include <atomic>
@@ -22,17 +24,23 @@ using namespace pxl;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 160;  // four consumer warps and the producer
 
-template <int D, bool HIGH>
+constexpr float kUp = 11.f;    // log2 of the factor on probabilities in f16
+constexpr float kLag = 4.f;    // log2 of how far the reference maximum may lag
+
+// NH: tiles of 8 query heads
+template <int D, int NH>
 struct Shape {
+  static constexpr int kCtas = NH == 1 ? 3 : 2;                  // on an SM
   static constexpr int kTileBytes = kKeyTile * D;                // of K, or of V
-  static constexpr int kStages = D == 64 ? 8 : HIGH ? 4 : 6;     // even: a stage belongs to one pair of warps
-  static constexpr int kTiles = D / 8;                           // of 8 columns of the output
-  static constexpr int kVecs = kTiles * (HIGH ? 4 : 2) / 4;      // 16-byte vectors of a lane's output
-  static constexpr int kOffParts = kStages * 2 * kTileBytes;     // [3][kVecs][32] float4
-  static constexpr int kOffStats = kOffParts + 3 * kVecs * 512;  // [3][5][32] floats: maxima, sums, R
-  static constexpr int kOffMax = kOffStats + 3 * 5 * 128;        // [stages][4] magnitudes of a stage's pages
+  static constexpr int kStages = D == 64 ? 8 : 4;                // even: a stage belongs to one pair of warps
+  static constexpr int kVecs = NH * D / 16;                      // 16-byte vectors of a lane's output
+  static constexpr int kStats = 4 * NH + 1;                      // maxima and sums of a lane's heads, R
+  static constexpr int kOffParts = kStages * 2 * kTileBytes;     // [2][kVecs][32] float4
+  static constexpr int kOffStats = kOffParts + 2 * kVecs * 512;  // [2][kStats][32] floats
+  static constexpr int kOffMax = kOffStats + 2 * kStats * 128;   // [stages][4] magnitudes of a stage's pages
   static constexpr int kOffBars = kOffMax + kStages * 32;
   static constexpr int kSmem = 1024 + kOffBars + kStages * 16 + 16;
+  static_assert(kCtas * (kSmem + 1024) <= 233472);
 };
 
 struct Args {
@@ -60,11 +68,29 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-template <int D, bool HIGH>
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// largest of, and sum over, the lanes that have the same heads
+__device__ __forceinline__ float keys_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float keys_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Lane 4 g + t has keys g and g + 8 of a product, heads 2 t and 2 t + 1 of a tile of heads, columns 16 c + 2 g and + 1 of the output.
+template <int D, int NH>
 struct Rows {
-  static constexpr int kRows = HIGH ? 2 : 1, kKeys = 32, kSteps = D / 16;
-  uint32_t qf[kSteps][4];
-  float row_scale[2], o[D / 8][4], m_run[2], l_run[2], r_run;
+  static constexpr int kKeys = 32, kSteps = D / 16;
+  uint32_t qf[NH][kSteps][2];
+  float row_scale[NH][2], o[NH][D / 16][4], m_run[NH][2], l_run[NH][2], r_run, log_r;
 
   // byte offset of 16-byte chunk c of a row of a tile as TMA lays it down
   static __device__ __forceinline__ uint32_t chunk(int row, int c) {
@@ -75,39 +101,36 @@ struct Rows {
   __device__ __forceinline__ void begin(const bf16* q, int G, float scale_log2) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = g8 + h * 8;
+    for (int n = 0; n < NH; ++n) {
+      const int r = g8 + n * 8;
+      uint2 x[kSteps];
       float mx = 0.f;
-      if ((HIGH || h == 0) && r < G) {
-        const uint2* row = reinterpret_cast<const uint2*>(q + r * D + t4 * (D / 4));
 #pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) {
-          const uint2 x = row[ks];
-          qf[ks][h] = x.x;
-          qf[ks][2 + h] = x.y;
-          const float2 a = unpack_bf16x2(x.x), b = unpack_bf16x2(x.y);
-          mx = fmaxf(fmaxf(fmaxf(mx, fabsf(a.x)), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < kSteps; ++ks) qf[ks][h] = qf[ks][2 + h] = 0u;
+      for (int ks = 0; ks < kSteps; ++ks) {
+        x[ks] = r < G ? *reinterpret_cast<const uint2*>(q + r * D + t4 * (D / 4) + ks * 4) : make_uint2(0, 0);
+        const float2 a = unpack_bf16x2(x[ks].x), b = unpack_bf16x2(x[ks].y);
+        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(a.x)), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
       }
-      if (!HIGH && h == 1) break;
       float down;
       const float up = row_up(quad_max(mx), down);
-      row_scale[h] = down * scale_log2 * kInv127;
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks)
+      for (int ks = 0; ks < kSteps; ++ks) {
+        const float2 a = unpack_bf16x2(x[ks].x), b = unpack_bf16x2(x[ks].y);
+        qf[n][ks][0] = pack_f16x2(a.x * up, a.y * up);
+        qf[n][ks][1] = pack_f16x2(b.x * up, b.y * up);
+      }
+      down *= scale_log2 * kInv127;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const float2 x = unpack_bf16x2(qf[ks][2 * p + h]);
-          qf[ks][2 * p + h] = pack_f16x2(x.x * up, x.y * up);
-        }
+      for (int e = 0; e < 2; ++e) {
+        row_scale[n][e] = __shfl_sync(0xffffffffu, down, (2 * t4 + e) * 4);
+        m_run[n][e] = -INFINITY;
+        l_run[n][e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    m_run[0] = m_run[1] = -INFINITY;
-    l_run[0] = l_run[1] = r_run = 0.f;
+    r_run = 0.f;
+    log_r = -INFINITY;
   }
 
   // Keys r0 .. r0 + 31 of a tile; the first is token tok_base. near, far: magnitudes of the pages of its first and second 16. scores: where
@@ -116,9 +139,11 @@ struct Rows {
                                        float* scores, int64_t score_stride, int G) {
     if (!(tok_base < hi && tok_base + kKeys > lo)) return;  // warp-uniform
     const int lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
-    float s[4][4];  // 8 tokens each
+    float s[NH][2][4];  // 16 keys each
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) s[n][k][0] = s[n][k][1] = s[n][k][2] = s[n][k][3] = 0.f;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) {
       uint32_t w[4][4];
@@ -130,67 +155,93 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t f = flip_codes(w[j][i]);
-          mma_m16n8k16_f16(s[j], qf[c * 4 + i], codes_f16x2<0x4140>(f), codes_f16x2<0x4342>(f));
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t x = flip_codes(w[2 * k][i]), y = flip_codes(w[2 * k + 1][i]);
+          const uint32_t a[4] = {codes_f16x2<0x4140>(x), codes_f16x2<0x4140>(y), codes_f16x2<0x4342>(x), codes_f16x2<0x4342>(y)};
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_m16n8k16_f16(s[n][k], a, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
         }
     }
     const bool whole = tok_base + kKeys <= hi && tok_base >= lo;  // every token is seen
-    float corr[2] = {1.f, 1.f};
-    // (of pages that have a token which is seen; a NaN is passed over)
-    const float r_new = fmaxf(r_run, fmaxf(tok_base + 16 > lo ? near.y : 0.f, tok_base + 16 < hi ? far.y : 0.f));
-    const float share[2] = {page_share(near.y, r_new), page_share(far.y, r_new)};
-    const float r_corr = r_new > r_run ? page_share(r_run, r_new) : 1.f;
-    r_run = r_new;
+    bool out[2][2] = {{false, false}, {false, false}};            // of this lane's keys: not seen
+    if (!whole) {
 #pragma unroll
-    for (int h = 0; h < kRows; ++h) {
-      const float scale[2] = {row_scale[h] * near.x, row_scale[h] * far.x};
-      float mx = -INFINITY;
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int r = 0; r < 2; ++r) {
+          const int tok = tok_base + k * 16 + r * 8 + g8;
+          out[k][r] = !(tok < hi && tok >= lo);
 #pragma unroll
-        for (int e = 2 * h; e < 2 * h + 2; ++e) {
-          s[j][e] *= scale[j >> 1];
-          if (!whole) {
-            const int tok = tok_base + j * 8 + 2 * t4 + (e & 1);
-            if (!(tok < hi && tok >= lo)) s[j][e] = -INFINITY;
-          }
-          mx = fmaxf(mx, s[j][e]);
+          for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[n][k][2 * r + e] = out[k][r] ? -INFINITY : s[n][k][2 * r + e];
         }
-      if (scores && g8 + 8 * h < G) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float2*>(scores + (g8 + 8 * h) * score_stride + tok_base + j * 8 + 2 * t4) = make_float2(s[j][2 * h], s[j][2 * h + 1]);
-      }
-      const float m_new = fmaxf(m_run[h], quad_max(mx));
-      const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
-      corr[h] = fast_exp2(m_run[h] - m_use);
-      m_run[h] = m_new;
-      float ps = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 2 * h; e < 2 * h + 2; ++e) {
-          const float p = fast_exp2(s[j][e] - m_use + kPUp);
-          ps += p;
-          s[j][e] = whole || s[j][e] != -INFINITY ? p * share[j >> 1] : 0.f;  // (a share that is NaN, of a token that is not seen)
-        }
-      l_run[h] = l_run[h] * corr[h] + ps;
-      corr[h] *= r_corr;
     }
-    if (__any_sync(0xffffffffu, corr[0] != 1.f || (HIGH && corr[1] != 1.f))) {
+    // R, of pages that have a token which is seen (a NaN is passed over); the maxima
+    const float most = fmaxf(tok_base + 16 > lo ? near.y : 0.f, tok_base + 16 < hi ? far.y : 0.f);
+    float mx[NH][2];
+    bool grow = most > r_run;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int e = 0; e < 2 * kRows; ++e) o[i][e] *= corr[e >> 1];
+      for (int e = 0; e < 2; ++e) {
+        mx[n][e] = fmaxf(fmaxf(s[n][0][e], s[n][0][2 + e]) * (row_scale[n][e] * near.x), fmaxf(s[n][1][e], s[n][1][2 + e]) * (row_scale[n][e] * far.x));
+        grow = grow || mx[n][e] > m_run[n][e] + kLag;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+      float r_corr = 1.f;
+      if (most > r_run) {
+        const float r_new = fminf(2.f * most, 3.3e38f);
+        r_corr = page_share(r_run, r_new);
+        r_run = r_new;
+        log_r = __log2f(r_new);
+      }
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float m_new = fmaxf(m_run[n][e], keys_max(mx[n][e]));
+          const float corr = fast_exp2(m_run[n][e] - ((m_new == -INFINITY) ? 0.f : m_new));
+          m_run[n][e] = m_new;
+          l_run[n][e] *= corr;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) o[n][i][e] *= corr * r_corr, o[n][i][2 + e] *= corr * r_corr;
+        }
+    }
+    const float up[2] = {kUp + page_log(near.y, log_r), kUp + page_log(far.y, log_r)};
+    const float down[2] = {fast_exp2(-up[0]), fast_exp2(-up[1])};
+    uint32_t pf[NH][2][2];  // [16 keys][8 of them], transposed: heads are rows
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const float m_use[2] = {m_run[n][0] == -INFINITY ? 0.f : m_run[n][0], m_run[n][1] == -INFINITY ? 0.f : m_run[n][1]};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float page = k == 0 ? near.x : far.x;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float scale = row_scale[n][e] * page, off = up[k] - m_use[e];
+          const int head = n * 8 + 2 * t4 + e;
+          if (scores && head < G) {
+            float* to = scores + head * score_stride + tok_base + k * 16 + g8;
+            to[0] = s[n][k][e] * scale;
+            to[8] = s[n][k][2 + e] * scale;
+          }
+          float p0 = fast_exp2(fmaf(s[n][k][e], scale, off)), p1 = fast_exp2(fmaf(s[n][k][2 + e], scale, off));
+          if (!whole) {  // (a magnitude that is zero, or none, of a token that is not seen)
+            p0 = out[k][0] ? 0.f : p0;
+            p1 = out[k][1] ? 0.f : p1;
+          }
+          const float both = p0 + p1;
+          l_run[n][e] += both == 0.f ? 0.f : both * down[k];
+          s[n][k][e] = p0;
+          s[n][k][2 + e] = p1;
+        }
+        pf[n][k][0] = transpose_8x8(pack_f16x2(s[n][k][0], s[n][k][1]));
+        pf[n][k][1] = transpose_8x8(pack_f16x2(s[n][k][2], s[n][k][3]));
+      }
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      uint32_t pf[4];
-      pf[0] = pack_f16x2(s[2 * k][0], s[2 * k][1]);
-      pf[1] = HIGH ? pack_f16x2(s[2 * k][2], s[2 * k][3]) : 0u;
-      pf[2] = pack_f16x2(s[2 * k + 1][0], s[2 * k + 1][1]);
-      pf[3] = HIGH ? pack_f16x2(s[2 * k + 1][2], s[2 * k + 1][3]) : 0u;
       const int mi = lane >> 3, row = r0 + k * 16 + (mi & 1) * 8 + (lane & 7);
 #pragma unroll
       for (int c = 0; c < D / 16; c += 2) {  // 16 columns per chunk; a transposed pair of bytes is two columns of a token
@@ -198,16 +249,14 @@ struct Rows {
         ldmatrix_x4_trans(r, v_smem + chunk(row, c + (mi >> 1)));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t a = flip_codes(r[2 * h]), b = flip_codes(r[2 * h + 1]);
-          mma_m16n8k16_f16(o[(c + h) * 2], pf, codes_f16x2<0x4240>(a), codes_f16x2<0x4240>(b));          // even columns
-          mma_m16n8k16_f16(o[(c + h) * 2 + 1], pf, codes_f16x2<0x4341>(a), codes_f16x2<0x4341>(b));      // odd ones
+          const uint32_t x = flip_codes(r[2 * h]), y = flip_codes(r[2 * h + 1]);
+          const uint32_t a[4] = {codes_f16x2<0x4240>(x), codes_f16x2<0x4341>(x), codes_f16x2<0x4240>(y), codes_f16x2<0x4341>(y)};
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_m16n8k16_f16(o[n][c + h], a, pf[n][k][0], pf[n][k][1]);
         }
       }
     }
   }
-
-  // columns of o[i][2 r], o[i + 1][2 r], o[i][2 r + 1], o[i + 1][2 r + 1] (i even): four in a row
-  static __device__ __forceinline__ int column(int i) { return i * 8 + 4 * (threadIdx.x & 3); }
 };
 
 // What two parts of a pair's keys have of a row: o in units of R, relative to the maximum.
@@ -223,19 +272,19 @@ struct Joined {
     fb *= page_share(r2, r_new);
   }
 };
-// 1 / sum in units of R, and log2 of the sum of exponentials, for a row with a sink or without
+// R / sum, and log2 of the sum of exponentials, for a row with a sink or without
 __device__ __forceinline__ float finish(float M, float L, float R, float sink, float& lse) {
   const float Mx = fmaxf(M, sink), Mu = Mx == -INFINITY ? 0.f : Mx;
-  const float e = fast_exp2(M - Mu), denom = L * e + fast_exp2(sink - Mu + kPUp);
-  lse = denom == 0.f ? INFINITY : Mu + log2f(denom) - kPUp;
-  return denom == 0.f ? 0.f : e / denom * (R * kInv127);
+  const float e = fast_exp2(M - Mu), denom = L * e + fast_exp2(sink - Mu);
+  lse = denom == 0.f ? INFINITY : Mu + log2f(denom);
+  return denom == 0.f ? 0.f : e / denom * (R * (kInv127 * 0x1p-11f));
 }
 
-template <int D, bool HIGH>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int D, int NH>
+__global__ void __launch_bounds__(kThreads, Shape<D, NH>::kCtas)
 attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
-  using S = Shape<D, HIGH>;
-  using R = Rows<D, HIGH>;
+  using S = Shape<D, NH>;
+  using R = Rows<D, NH>;
   constexpr int STAGES = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -337,36 +386,32 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 
       // warps 2 and 3 hand their results to 0 and 1, 1 to 0; a register goes to the same lane
       auto give = [&](int p) {
+        float* st = stats + p * S::kStats * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < S::kVecs; ++i) {
-          if constexpr (HIGH) parts[(p * S::kVecs + i) * 32 + lane] = make_float4(rows.o[i][0], rows.o[i][1], rows.o[i][2], rows.o[i][3]);
-          else parts[(p * S::kVecs + i) * 32 + lane] = make_float4(rows.o[2 * i][0], rows.o[2 * i][1], rows.o[2 * i + 1][0], rows.o[2 * i + 1][1]);
+        for (int n = 0; n < NH; ++n) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            parts[(p * S::kVecs + n * (D / 16) + i) * 32 + lane] = make_float4(rows.o[n][i][0], rows.o[n][i][1], rows.o[n][i][2], rows.o[n][i][3]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) st[(n * 4 + e) * 32] = rows.m_run[n][e], st[(n * 4 + 2 + e) * 32] = rows.l_run[n][e];
         }
-        float* st = stats + p * 5 * 32 + lane;
-        st[0] = rows.m_run[0], st[32] = rows.l_run[0], st[64] = rows.m_run[1], st[96] = rows.l_run[1], st[128] = rows.r_run;
+        st[4 * NH * 32] = rows.r_run;
       };
       auto add = [&](int p) {
-        const float* st = stats + p * 5 * 32 + lane;
-        const float r_new = fmaxf(rows.r_run, st[128]);
-        const Joined x(rows.m_run[0], rows.l_run[0], rows.r_run, r_new, st[0], st[32], st[128]);
-        if constexpr (HIGH) {
-          const Joined y(rows.m_run[1], rows.l_run[1], rows.r_run, r_new, st[64], st[96], st[128]);
+        const float* st = stats + p * S::kStats * 32 + lane;
+        const float r2 = st[4 * NH * 32], r_new = fmaxf(rows.r_run, r2);
 #pragma unroll
-          for (int i = 0; i < S::kVecs; ++i) {
-            const float4 v = parts[(p * S::kVecs + i) * 32 + lane];
-            rows.o[i][0] = rows.o[i][0] * x.fa + v.x * x.fb;
-            rows.o[i][1] = rows.o[i][1] * x.fa + v.y * x.fb;
-            rows.o[i][2] = rows.o[i][2] * y.fa + v.z * y.fb;
-            rows.o[i][3] = rows.o[i][3] * y.fa + v.w * y.fb;
-          }
-        } else {
+        for (int n = 0; n < NH; ++n) {
+          const Joined x(rows.m_run[n][0], rows.l_run[n][0], rows.r_run, r_new, st[n * 128], st[n * 128 + 64], r2);
+          const Joined y(rows.m_run[n][1], rows.l_run[n][1], rows.r_run, r_new, st[n * 128 + 32], st[n * 128 + 96], r2);
 #pragma unroll
-          for (int i = 0; i < S::kVecs; ++i) {
-            const float4 v = parts[(p * S::kVecs + i) * 32 + lane];
-            rows.o[2 * i][0] = rows.o[2 * i][0] * x.fa + v.x * x.fb;
-            rows.o[2 * i][1] = rows.o[2 * i][1] * x.fa + v.y * x.fb;
-            rows.o[2 * i + 1][0] = rows.o[2 * i + 1][0] * x.fa + v.z * x.fb;
-            rows.o[2 * i + 1][1] = rows.o[2 * i + 1][1] * x.fa + v.w * x.fb;
+          for (int i = 0; i < D / 16; ++i) {
+            const float4 v = parts[(p * S::kVecs + n * (D / 16) + i) * 32 + lane];
+            float (&o)[4] = rows.o[n][i];
+            o[0] = o[0] * x.fa + v.x * x.fb;
+            o[1] = o[1] * y.fa + v.y * y.fb;
+            o[2] = o[2] * x.fa + v.z * x.fb;
+            o[3] = o[3] * y.fa + v.w * y.fb;
           }
         }
         rows.r_run = r_new;
@@ -374,34 +419,35 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
       if (warp >= 2) give(warp - 2);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (warp < 2) add(warp);
-      if (warp == 1) give(2);
+      if (warp == 1) give(1);  // (its own place: each lane has read what it writes)
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (warp == 0) add(1);
+      // the places are free for the next pair: warps 2 and 3 write them ahead of the next barrier
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (warp == 0) {
-        add(2);
+        const int g8 = lane >> 2, t4 = lane & 3;
 #pragma unroll
-        for (int h = 0; h < (HIGH ? 2 : 1); ++h) {
-          const int r = (lane >> 2) + 8 * h;
-          const float M = rows.m_run[h], L = quad_sum(rows.l_run[h]);
-          if (r >= G || failed) continue;
-          if (walk.whole()) {
-            float lse;
-            const float f = finish(M, L, rows.r_run, a.sinks ? a.sinks[head0 + r] * kLog2e : -INFINITY, lse);
-            if (a.lse && (lane & 3) == 0) a.lse[static_cast<size_t>(walk.b) * a.Hq + head0 + r] = lse;
-            bf16* dst = a.out + walk.b * a.out_stride + (head0 + r) * D;
+        for (int n = 0; n < NH; ++n)
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 2)
-              *reinterpret_cast<uint2*>(dst + R::column(i)) = make_uint2(pack_bf16x2(rows.o[i][2 * h] * f, rows.o[i + 1][2 * h] * f),
-                                                                         pack_bf16x2(rows.o[i][2 * h + 1] * f, rows.o[i + 1][2 * h + 1] * f));
-          } else {
-            float* po = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (walk.t == 0 ? 1 : 0)) * (G * (D + 2) + 4);
+          for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + 2 * t4 + e;
+            const float M = rows.m_run[n][e], L = keys_sum(rows.l_run[n][e]);
+            if (r >= G || failed) continue;
+            if (walk.whole()) {
+              float lse;
+              const float f = finish(M, L, rows.r_run, a.sinks ? a.sinks[head0 + r] * kLog2e : -INFINITY, lse);
+              if (a.lse && g8 == 0) a.lse[static_cast<size_t>(walk.b) * a.Hq + head0 + r] = lse;
+              bf16* dst = a.out + walk.b * a.out_stride + (head0 + r) * D + 2 * g8;
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 2) {
-              float* at = po + r * D + R::column(i);
-              at[0] = rows.o[i][2 * h], at[1] = rows.o[i + 1][2 * h], at[2] = rows.o[i][2 * h + 1], at[3] = rows.o[i + 1][2 * h + 1];
+              for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint32_t*>(dst + i * 16) = pack_bf16x2(rows.o[n][i][e] * f, rows.o[n][i][2 + e] * f);
+            } else {
+              float* po = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (walk.t == 0 ? 1 : 0)) * (G * (D + 2) + 4);
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+                *reinterpret_cast<float2*>(po + r * D + i * 16 + 2 * g8) = make_float2(rows.o[n][i][e], rows.o[n][i][2 + e]);
+              if (g8 == 0) po[G * D + r] = M, po[G * D + G + r] = L, po[G * (D + 2)] = rows.r_run;
             }
-            if ((lane & 3) == 0) po[G * D + r] = M, po[G * D + G + r] = L, po[G * (D + 2)] = rows.r_run;
           }
-        }
       }
     }
   }
@@ -409,12 +455,15 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
 }
 
 // Adds up the pairs that lie in several CTAs. Block x: the pair that the border between CTAs x and x + 1 cuts, if no border before it does.
+// First a warp per query head finds the factors of all parts, then every warp adds columns of a head at a time.
+constexpr int kJoinThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(D)
+__global__ void __launch_bounds__(kJoinThreads)
 attn_i8_join_kernel(const __grid_constant__ Args a, int ctas) {
-  constexpr int R = 4;  // query heads at a time, so that their loads are in flight together
+  extern __shared__ float factor[];  // [G][parts]
+  __shared__ float final_sm[16];
   const DecodeWork work{a.ctx_lens, a.B, a.Hkv, a.window, 0};
-  const int cut = blockIdx.x + 1, d = threadIdx.x, G = a.Hq / a.Hkv;
+  const int cut = blockIdx.x + 1, G = a.Hq / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const DecodeShares at(work.total(), ctas);
   const int64_t pos = at[cut];
   int b, kvh, t;
@@ -427,41 +476,41 @@ attn_i8_join_kernel(const __grid_constant__ Args a, int ctas) {
   pdl_wait();
   pdl_launch_dependents();
   if (!mine) return;
-  const size_t place = static_cast<size_t>(G) * (D + 2) + 4;
-  auto part = [&](int x) { return a.parts + (static_cast<size_t>(x) * 2 + (x < cut ? 1 : 0)) * place; };
-  float r_all = 0.f;
-  for (int x = cut - 1; x <= last; ++x) r_all = fmaxf(r_all, part(x)[G * (D + 2)]);
-  for (int r0 = 0; r0 < G; r0 += R) {
-    float acc[R], L[R], M[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) acc[i] = L[i] = 0.f, M[i] = -INFINITY;
-    for (int x = cut - 1; x <= last; ++x) {
-      const float* p = part(x) + r0 * D + d;
-      const float *pm = part(x) + G * D + r0, *pl = pm + G;
-      const float rx = part(x)[G * (D + 2)];
-      float o[R], m[R], l[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const bool in = r0 + i < G;
-        o[i] = in ? p[i * D] : 0.f;
-        m[i] = in ? pm[i] : -INFINITY;
-        l[i] = in ? pl[i] : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const Joined f(M[i], L[i], r_all, r_all, m[i], l[i], rx);
-        acc[i] = acc[i] * f.fa + o[i] * f.fb;
-      }
+  const int place = G * (D + 2) + 4, n = last - cut + 2;
+  const float* first = a.parts + (static_cast<int64_t>(cut) * 2 - 1) * place;  // the end of CTA cut - 1; then the starts of the others
+  auto part = [&](int x) { return first + (x == 0 ? 0 : (2 * x - 1) * static_cast<int64_t>(place)); };
+  for (int g = warp; g < G; g += kJoinThreads / 32) {
+    float M = -INFINITY, R = 0.f, L = 0.f;
+    for (int x = lane; x < n; x += 32) M = fmaxf(M, part(x)[G * D + g]), R = fmaxf(R, part(x)[G * (D + 2)]);
+    M = warp_reduce_max(M);
+    R = warp_reduce_max(R);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    for (int x = lane; x < n; x += 32) {
+      const float f = fast_exp2(part(x)[G * D + g] - Mu);
+      L += part(x)[G * D + G + g] * f;
+      factor[g * n + x] = f * page_share(part(x)[G * (D + 2)], R);
     }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (r0 + i >= G) break;
-      const int head = kvh * G + r0 + i;
-      float lse;
-      const float f = finish(M[i], L[i], r_all, a.sinks ? a.sinks[head] * kLog2e : -INFINITY, lse);
-      if (a.lse && d == 0) a.lse[static_cast<size_t>(b) * a.Hq + head] = lse;
-      a.out[b * a.out_stride + head * D + d] = __float2bfloat16(acc[i] * f);
+    L = warp_reduce_sum(L);
+    const int head = kvh * G + g;
+    float lse;
+    const float f = finish(M, L, R, a.sinks ? a.sinks[head] * kLog2e : -INFINITY, lse);
+    if (lane == 0) {
+      final_sm[g] = f;
+      if (a.lse) a.lse[static_cast<size_t>(b) * a.Hq + head] = lse;
     }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * D / 2; i += kJoinThreads) {
+    const int g = i / (D / 2);
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+    for (int x = 0; x < n; ++x) {
+      const float f = factor[g * n + x];
+      const float2 v = *reinterpret_cast<const float2*>(part(x) + i * 2);
+      acc.x += v.x * f, acc.y += v.y * f;
+    }
+    const float f = final_sm[g];
+    *reinterpret_cast<uint32_t*>(a.out + b * a.out_stride + kvh * G * D + i * 2) = pack_bf16x2(acc.x * f, acc.y * f);
   }
 }
 
@@ -509,7 +558,7 @@ struct Layout {
   int ctas;
   Layout(int B, int Hq, int Hkv, int D, int max_ctx, bool weights) {
     const int64_t tiles = static_cast<int64_t>(B) * Hkv * (ceil_div64(max_ctx, kKeyTile) + 1);
-    const int full = 2 * pxl_host::num_sms();
+    const int full = (Hq / Hkv > 8 ? 2 : 3) * pxl_host::num_sms();
     ctas = tiles < full ? static_cast<int>(tiles) : full;
     lse = static_cast<int64_t>(ctas) * 2 * (Hq / Hkv * (D + 2) + 4);
     score_stride = weights ? ceil_div64(max_ctx, kKeyTile) * kKeyTile : 0;
@@ -518,19 +567,20 @@ struct Layout {
   }
 };
 
-template <int D, bool HIGH>
+template <int D, int NH>
 int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas, float* weights, int64_t W, int slots,
                   const int* seq_slots, cudaStream_t stream) {
-  constexpr int kSmem = Shape<D, HIGH>::kSmem;
+  constexpr int kSmem = Shape<D, NH>::kSmem;
   static std::atomic<bool> configured[64];  // function attributes are per device
   std::atomic<bool>& done = configured[pxl_host::current_device_slot()];
   if (!done.load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(attn_i8_decode_kernel<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(attn_i8_decode_kernel<D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
       return PXL_ERR_CUDA;
     done.store(true, std::memory_order_relaxed);
   }
-  pxl_host::launch(attn_i8_decode_kernel<D, HIGH>, dim3(ctas), dim3(kThreads), kSmem, stream, tk, tv, a);
-  if (ctas > 1) pxl_host::launch_behind(attn_i8_join_kernel<D>, dim3(ctas - 1), dim3(D), 0, stream, a, ctas);
+  pxl_host::launch(attn_i8_decode_kernel<D, NH>, dim3(ctas), dim3(kThreads), kSmem, stream, tk, tv, a);
+  if (ctas > 1)
+    pxl_host::launch_behind(attn_i8_join_kernel<D>, dim3(ctas - 1), dim3(kJoinThreads), a.Hq / a.Hkv * ctas * 4, stream, a, ctas);
   if (weights)
     pxl_host::launch_behind(attn_i8_weigh_kernel, dim3(static_cast<unsigned>(ceil_div64(a.score_stride, kWeighKeys)), a.Hkv, a.B), dim3(256), 0,
                             stream, a, weights, W, slots, seq_slots);
@@ -568,6 +618,6 @@ PXL_EXPORT int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k
                out_stride, sinks, ws, weights ? ws + at.lse : nullptr, weights ? ws + at.scores : nullptr, at.score_stride, B, Hq, Hkv, page,
                max_blocks, num_blocks, scale * kLog2e, window, status};
   auto go = [&](auto launch) { return launch(tk, tv, a, at.ctas, weights, W, slots, seq_slots, stream); };
-  if (D == 64) return Hq / Hkv > 8 ? go(launch_decode<64, true>) : go(launch_decode<64, false>);
-  return Hq / Hkv > 8 ? go(launch_decode<128, true>) : go(launch_decode<128, false>);
+  if (D == 64) return Hq / Hkv > 8 ? go(launch_decode<64, 2>) : go(launch_decode<64, 1>);
+  return Hq / Hkv > 8 ? go(launch_decode<128, 2>) : go(launch_decode<128, 1>);
 }

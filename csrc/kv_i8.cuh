@@ -35,10 +35,12 @@ __device__ __forceinline__ float row_up(float most, float& down) {
   return __uint_as_float(static_cast<uint32_t>(up) << 23);
 }
 constexpr float kInv127 = 1.f / 127.f;
-constexpr float kPUp = 15.f;  // log2 of the factor on probabilities in f16
 
 // share of a page's magnitude in the largest so far; 0 for a page of zeros, NaN for one without a magnitude
 __device__ __forceinline__ float page_share(float m, float most) { return m == 0.f ? 0.f : __fdiv_rn(m, most); }
+
+// log2 of that, from log2 of the largest; not below -40 (whose values are lost beside the others'), NaN without a magnitude
+__device__ __forceinline__ float page_log(float m, float log_most) { return m == m ? fmaxf(__log2f(m) - log_most, -40.f) : m; }
 
 }  // namespace pxl
 
