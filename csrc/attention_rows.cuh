@@ -7,22 +7,6 @@
 
 namespace pxl {
 
-__device__ __forceinline__ uint64_t pair2(float a, float b) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ float2 unpair2(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // One tile. `masked(j)`: column j is not visible (asked unless `interior`). m_run: reference maximum, in log2 units; l2: row sums
 // in two pairs. p_ready: barriers of the two halves of P, one arrival per warp. Warp-collective.
 template <int SM, typename Masked>
