@@ -1224,14 +1224,14 @@ def _head_rows(x: torch.Tensor) -> torch.Tensor:
 
 def store_kv_i8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor,
                 block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_lens: torch.Tensor, max_q_len: int) -> None:
-    N, Hkv, page, D, B, MB = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
-    k, v, dev = _head_rows(k), _head_rows(v), k_cache.device
-    if B == 0 or k.shape[0] == 0 or max_q_len == 0:
+    N, Hkv, page, D, T, B, MB = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
+    if B == 0 or T == 0 or max_q_len == 0:
         return
+    k, v, dev = _head_rows(k), _head_rows(v), k_cache.device
     with _on(dev):
         check(_lib.lib().pxl_kv_i8_store(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), block_tables.data_ptr(), cu_q.data_ptr(),
-                                         ctx_lens.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), k.shape[0], B,
-                                         min(max_q_len, k.shape[0]), Hkv, D, page, MB, N, status_tensor(dev).data_ptr(), _stream(dev)),
+                                         ctx_lens.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), T, B,
+                                         min(max_q_len, T), Hkv, D, page, MB, N, status_tensor(dev).data_ptr(), _stream(dev)),
               "pxl_kv_i8_store")
     _count()
 
@@ -1253,40 +1253,42 @@ def load_kv_i8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tenso
 
 
 def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, window, sinks, max_ctx, out, weights, seq_slots):
-    N, Hkv, page, D, B, MB, max_ctx = kv_i8.check_attention(what, q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks, out, weights,
-                                                            seq_slots, max_ctx)
-    q, dev = _head_rows(q), q.device
-    T, Hq, _ = q.shape
+    N, Hkv, page, D, T, Hq, B, MB, max_ctx, slots, W = kv_i8.check_attention(what, q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks,
+                                                                             out, weights, seq_slots, max_ctx)
+    dev = q.device
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
-    if T == 0 or B == 0 or max_q_len == 0:
+    if T == 0 or B == 0 or max_q_len <= 0:
         return out
+    q = _head_rows(q)
     k_cache, v_cache, kv_max = cache
-    W, slots = (weights.shape[2], weights.shape[0]) if weights is not None else (0, 0)
-    w = (_ptr(weights), W, slots, _ptr(seq_slots))
-    where = (Hq, Hkv, D, page, MB, N, float(scale), window, max_ctx, status_tensor(dev).data_ptr(), _stream(dev))
+    weighed = weights is not None
     with _on(dev):
         lib = _lib.lib()
+        status, stream = status_tensor(dev).data_ptr(), _stream(dev)
+        # (workspaces are of this call: calls on other streams, and graphs, have their own)
         if cu_q is None:
-            need = lib.pxl_attn_i8_decode_workspace(B, Hq, Hkv, D, max_ctx, int(weights is not None))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)      # of this call: calls on other streams and graphs have their own
+            need = lib.pxl_attn_i8_decode_workspace(B, Hq, Hkv, D, max_ctx, weighed)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
             check(lib.pxl_attn_i8_decode(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
-                                         block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks), *w,
-                                         ws.data_ptr(), need, B, *where), "pxl_attn_i8_decode")
+                                         block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks),
+                                         _ptr(weights), W, slots, _ptr(seq_slots), ws.data_ptr(), need, B, Hq, Hkv, D, page, MB, N, scale,
+                                         window, max_ctx, status, stream), "pxl_attn_i8_decode")
         else:
             need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            lse = None if weights is None else torch.empty((T, Hq), dtype=torch.float32, device=dev)
+            lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if weighed else None
+            where = (T, B, max_q_len, Hq, Hkv, D, page, MB, N, scale, window, max_ctx, status, stream)
             check(lib.pxl_attn_i8_prefill(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
                                           block_tables.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0),
-                                          _ptr(sinks), _ptr(lse), _ptr(ws), need, T, B, max_q_len, *where), "pxl_attn_i8_prefill")
-            if weights is not None:
+                                          _ptr(sinks), _ptr(lse), _ptr(ws), need, *where), "pxl_attn_i8_prefill")
+            if weighed:
                 need = lib.pxl_attn_i8_weigh_workspace(B, max_q_len, Hq, Hkv, max_ctx)
                 ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
                 check(lib.pxl_attn_i8_weigh(q.data_ptr(), q.stride(0), k_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(),
-                                            cu_q.data_ptr(), ctx_lens.data_ptr(), lse.data_ptr(), *w, _ptr(ws), need, T, B, max_q_len, *where),
-                      "pxl_attn_i8_weigh")
-    _count(1 if weights is None else 2)
+                                            cu_q.data_ptr(), ctx_lens.data_ptr(), lse.data_ptr(), weights.data_ptr(), W, slots,
+                                            _ptr(seq_slots), _ptr(ws), need, *where), "pxl_attn_i8_weigh")
+    _count(2 + weighed)
     return out
 
 
@@ -1311,16 +1313,16 @@ def attn_prefill_i8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def evict_kv_i8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor, weights: torch.Tensor, block_tables: torch.Tensor,
                 ctx_lens: torch.Tensor, new_tables: torch.Tensor, keep: int, recent: int, first: int = 0,
                 seq_slots: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
-    N, Hkv, page, D, B, MB, MN = kv_i8.check_evict("evict_kv_i8", (k_cache, v_cache, kv_max), weights, block_tables, ctx_lens, new_tables, keep,
-                                                   recent, first, seq_slots)
+    N, Hkv, page, D, B, MB, MN, slots, W = kv_i8.check_evict("evict_kv_i8", (k_cache, v_cache, kv_max), weights, block_tables, ctx_lens,
+                                                             new_tables, keep, recent, first, seq_slots)
     dev = k_cache.device
     kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty(B, dtype=torch.int32, device=dev)
     if B == 0:
         return kept, lens
     with _on(dev):
-        check(_lib.lib().pxl_kv_i8_evict(k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), weights.data_ptr(), weights.shape[2],
-                                         weights.shape[0], _ptr(seq_slots), block_tables.data_ptr(), ctx_lens.data_ptr(),
+        check(_lib.lib().pxl_kv_i8_evict(k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(), weights.data_ptr(), W, slots,
+                                         _ptr(seq_slots), block_tables.data_ptr(), ctx_lens.data_ptr(),
                                          new_tables.data_ptr(), kept.data_ptr(), lens.data_ptr(), B, Hkv, D, page, MB, MN, N, keep, recent,
                                          first, status_tensor(dev).data_ptr(), _stream(dev)), "pxl_kv_i8_evict")
     _count(2)

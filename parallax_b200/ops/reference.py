@@ -665,7 +665,7 @@ def store_kv_i8(k, v, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, ma
     """Writes the new tokens' keys and values ``[T, heads, D]`` into an 8-bit cache (see :mod:`.kv_i8`): rows ``cu_q[b]`` to ``cu_q[b + 1]``
     are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each. The pages that are written belong to one
     sequence each; what a page holds behind the last token stays."""
-    _, Hkv, page, D, B, _ = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
+    _, Hkv, page, D, _, B, _ = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
     for b in range(B):
         row, n, t = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b]), int(ctx_lens[b])
         for p in range((t - n) // page, (t - 1) // page + 1) if n > 0 else ():
@@ -752,7 +752,7 @@ def evict_kv_i8(k_cache, v_cache, kv_max, weights, block_tables, ctx_lens, new_t
     magnitudes that its tokens had. ``weights`` move along, and are zero behind what stayed. Returns the tokens that stayed, int32
     ``[B, heads, keep]`` (-1 behind the last), and the new lengths, int32 ``[B]``."""
     cache = (k_cache, v_cache, kv_max)
-    _, Hkv, page, D, B, _, _ = kv_i8.check_evict("evict_kv_i8", cache, weights, block_tables, ctx_lens, new_tables, keep, recent, first, seq_slots)
+    _, Hkv, page, D, B, *_ = kv_i8.check_evict("evict_kv_i8", cache, weights, block_tables, ctx_lens, new_tables, keep, recent, first, seq_slots)
     kept = torch.full((B, Hkv, keep), -1, dtype=torch.int32, device=k_cache.device)
     head = torch.arange(Hkv)[:, None]
     for b in range(B):
