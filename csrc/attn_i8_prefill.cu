@@ -139,24 +139,45 @@ __device__ __forceinline__ float convert_row(uint32_t row_addr, int r, bool vali
   return down;
 }
 
+// Which columns of a tile the rows of a warp see: [from, to) of this lane's row; of the 16-column groups, those that some row sees some of
+// and those that all rows see whole, a bit each.
+struct Seen {
+  int from, to;
+  uint32_t some, whole;
+  __device__ __forceinline__ Seen(int from, int to) : from(from), to(to) {
+    const int f_min = __reduce_min_sync(0xffffffffu, from), f_max = __reduce_max_sync(0xffffffffu, from);
+    const int t_min = __reduce_min_sync(0xffffffffu, to), t_max = __reduce_max_sync(0xffffffffu, to);
+    some = whole = 0;
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      some |= (g * 16 < t_max && g * 16 + 16 > f_min ? 1u : 0u) << g;
+      whole |= (g * 16 >= f_max && g * 16 + 16 <= t_min ? 1u : 0u) << g;
+    }
+  }
+};
+
 // One tile of a row: S from tensor memory, P back to its place. pages: 16 bytes for each page of the tile (key magnitude / 127, log2 of its
-// share of R plus kUp, the inverse of that power, R); shift: log2 of the 16-column groups in a page.
-template <int D, bool INTERIOR, typename Masked>
-__device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool first, Masked masked, float row_scale, const float4* pages,
+// share of R plus kUp, the inverse of that power, R); shift: log2 of the 16-column groups in a page. INTERIOR: every column is seen; else
+// columns are looked at one by one only in the groups on an edge, and those that nobody sees cost nothing.
+template <int D, bool INTERIOR>
+__device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool first, const Seen& seen, float row_scale, const float4* pages,
                                            int shift, float& m_run, float& r_run, float& l_run, uint32_t p_ready) {
   uint32_t sc[kT];
 #pragma unroll
   for (int c = 0; c < kT; c += 32) tmem_ld_32x32b_x32(my_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sc[c]));
   const float r_new = pages[0].w;
   tmem_ld_wait();
-  if constexpr (!INTERIOR) {
-#pragma unroll
-    for (int j = 0; j < kT; ++j)
-      if (masked(j)) sc[j] = 0xff800000u;  // -inf
-  }
   float mx = -INFINITY;
 #pragma unroll
   for (int g = 0; g < 8; ++g) {
+    if constexpr (!INTERIOR) {
+      if (!(seen.some >> g & 1)) continue;
+      if (!(seen.whole >> g & 1)) {
+#pragma unroll
+        for (int j = g * 16; j < g * 16 + 16; ++j)
+          if (j < seen.from || j >= seen.to) sc[j] = 0xff800000u;  // -inf
+      }
+    }
     float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
@@ -193,7 +214,14 @@ __device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool fi
       uint32_t pk[16];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const float4 page = pages[((c >> 4) + g) >> shift];
+        const int at = (c >> 4) + g;
+        if (!INTERIOR && !(seen.some >> at & 1)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pk[g * 8 + j] = 0u;
+          continue;
+        }
+        const bool edge = !INTERIOR && !(seen.whole >> at & 1);
+        const float4 page = pages[at >> shift];
         const float scale = page.x * row_scale, off = page.y - m_use;
         const uint64_t scale2 = pair2(scale, scale), off2 = pair2(off, off);
         uint64_t sum = 0ull;
@@ -202,7 +230,7 @@ __device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool fi
           const float s0 = __uint_as_float(sc[c + g * 16 + j]), s1 = __uint_as_float(sc[c + g * 16 + j + 1]);
           const float2 x = unpair2(fma2(pair2(s0, s1), scale2, off2));
           float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
-          if constexpr (!INTERIOR) {  // (a magnitude of zero, or none, of a key that is not seen)
+          if (edge) {  // (a magnitude of zero, or none, of a key that is not seen)
             p0 = s0 == -INFINITY ? 0.f : p0;
             p1 = s1 == -INFINITY ? 0.f : p1;
           }
@@ -242,11 +270,11 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   pdl_wait();
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int b = blockIdx.z, kvh = blockIdx.y % a.Hkv, split = blockIdx.y / a.Hkv, G = a.Hq / a.Hkv;
+  const int b = blockIdx.z, kvh = blockIdx.x % a.Hkv, split = blockIdx.y, G = a.Hq / a.Hkv;
   const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin, ctx = a.ctx_lens[b];
   const int per_unit = kRowsQ / G;  // tokens
-  // heavy blocks (late queries see the most keys) are scheduled first
-  const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * per_unit;
+  // heavy blocks (late queries see the most keys) are scheduled first, of all heads (head by head: 827 us for 806)
+  const int q0 = (static_cast<int>(gridDim.x) / a.Hkv - 1 - static_cast<int>(blockIdx.x) / a.Hkv) * 2 * per_unit;
   if (q0 >= L || q_begin < 0 || q_begin + L > a.T) return;  // uniform for the CTA, before any barrier or allocation
   const int units = L - q0 > per_unit ? 2 : 1, tokens = min(L - q0, 2 * per_unit);
   const int pos0 = ctx - L + q0;      // position of the first token
@@ -325,12 +353,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const int next_head = head_of(blk, it + 1);
         const float2 next = a.kv_max[next_head];  // on its way while this tile is issued
         blk = block_of(it + 2);
-        // R and the tile's pages
-        const int tok = (t_begin + it) * kT + lane * a.page;
-        float m = lane < ppt && tok < hi && tok + a.page > lo ? most.y : 0.f;
-        m = m == m ? m : 0.f;
-        m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-        if (m > r_all) r_all = fminf(2.f * m, 3.3e38f);
+        // the codes first; then R and the tile's pages, which the barrier of the keys counts
         for (int kv = 0; ok && kv < 2; ++kv, ++item) {
           const int stage = item % S::kStages;
           if (item >= S::kStages)
@@ -342,11 +365,19 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           __syncwarp();
           if (lane < ppt) {
             tma_load_2d(dst, kv ? &tm_v : &tm_k, bar, 0, head * a.page);
-            if (kv == 0) {
+            if (kv == 1) mbar_arrive(bar);
+          }
+          if (kv == 0) {
+            const int tok = (t_begin + it) * kT + lane * a.page;
+            float m = lane < ppt && tok < hi && tok + a.page > lo ? most.y : 0.f;
+            m = m == m ? m : 0.f;
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            if (m > r_all) r_all = fminf(2.f * m, 3.3e38f);
+            if (lane < ppt) {
               const float share = most.y == most.y ? fmaxf(page_share(most.y, r_all), 0x1p-40f) : most.y;
               pages_sm[(it % kRing) * 8 + lane] = make_float4(most.x * kInv127, __log2f(share) + kUp, __fdividef(0x1p-7f, share), r_all);
+              mbar_arrive(bar);
             }
-            mbar_arrive(bar);
           }
         }
         head = next_head;
@@ -424,7 +455,8 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     if (u < units) {
       const int r = q4 * 32 + lane, tok = u * per_unit + r / G, head = kvh * G + r % G;  // query row = TMEM lane
       const bool valid = r < per_unit * G && tok < tokens;
-      const int q_pos = pos0 + tok, last = pos0 + min((u + 1) * per_unit, tokens) - 1;  // the unit's last position
+      const int last = pos0 + min((u + 1) * per_unit, tokens) - 1;  // the unit's last position
+      const int q_pos = min(pos0 + tok, last);                      // (rows that are nobody's: as the last)
       const int key_lo = (a.window > 0 && q_pos - a.window + 1 > 0) ? q_pos - a.window + 1 : 0;
       const uint32_t lane_sel = static_cast<uint32_t>(q4 * 32) << 16;
       const uint32_t my_s = tm_s + u * kT + lane_sel, my_o = tm_o + u * D + lane_sel;
@@ -447,13 +479,11 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const float4* pages = pages_sm + (it % kRing) * 8;
         // every key is seen by every row of the unit
         const bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
-        if (interior) {
-          softmax_i8<D, true>(my_s, my_o, it == 0, [](int) { return false; }, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
-        } else {
-          const int from = key_lo - key0, to = (valid ? q_pos + 1 : 0) - key0;  // columns that this row sees
-          softmax_i8<D, false>(my_s, my_o, it == 0, [&](int j) { return j < from || j >= to; }, row_scale, pages, shift, m_run, r_run, l_run,
-                               p_ready + 16 * u);
-        }
+        const Seen seen(interior ? 0 : key_lo - key0, interior ? kT : q_pos + 1 - key0);
+        if (interior)
+          softmax_i8<D, true>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+        else
+          softmax_i8<D, false>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
       }
       if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);
@@ -582,7 +612,8 @@ int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
     done.store(true, std::memory_order_relaxed);
   }
   const int per = 2 * (kRowsQ / (a.Hq / a.Hkv));
-  pxl_host::launch(attn_i8_prefill_kernel<D>, dim3(ceil_div(max_q_len, per), a.Hkv * a.splits, B), dim3(kThreads), Shape<D>::kSmem, stream, tq,
+  if (static_cast<int64_t>(ceil_div(max_q_len, per)) * a.Hkv > INT32_MAX || a.splits > 65535) return PXL_ERR_TOO_LARGE;
+  pxl_host::launch(attn_i8_prefill_kernel<D>, dim3(ceil_div(max_q_len, per) * a.Hkv, a.splits, B), dim3(kThreads), Shape<D>::kSmem, stream, tq,
                    tk, tv, a);
   if (a.splits > 1)
     pxl_host::launch_behind(attn_i8_prefill_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div64(static_cast<int64_t>(a.T) * a.Hq, 4))), dim3(128),
@@ -610,7 +641,7 @@ PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* 
     return PXL_ERR_INVALID_ARG;
   const Layout at(T, B, max_q_len, Hq, Hkv, D, max_ctx);
   if (workspace_bytes < at.total * 4 || (at.total > 0 && !workspace)) return PXL_ERR_INVALID_ARG;
-  if (static_cast<int64_t>(Hkv) * at.splits > 65535 || B > 65535) return PXL_ERR_TOO_LARGE;
+  if (B > 65535) return PXL_ERR_TOO_LARGE;
   CUtensorMap tq, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * Hkv * page;
   if (!pxl_host::make_tmap_queries(&tq, q, q_stride, T, Hq, D, Hq / Hkv) || !pxl_host::make_tmap_codes(&tk, k_cache, rows, D, page) ||
