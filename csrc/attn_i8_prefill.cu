@@ -142,8 +142,9 @@ __device__ __forceinline__ float convert_row(uint32_t row_addr, int r, bool vali
 // Which columns of a tile the rows of a warp see: [from, to) of this lane's row; of the 16-column groups, those that some row sees some of
 // and those that all rows see whole, a bit each.
 struct Seen {
-  int from, to;
-  uint32_t some, whole;
+  int from = 0, to = kT;
+  uint32_t some = 0xffu, whole = 0xffu;
+  Seen() = default;
   __device__ __forceinline__ Seen(int from, int to) : from(from), to(to) {
     const int f_min = __reduce_min_sync(0xffffffffu, from), f_max = __reduce_max_sync(0xffffffffu, from);
     const int t_min = __reduce_min_sync(0xffffffffu, to), t_max = __reduce_max_sync(0xffffffffu, to);
@@ -479,11 +480,11 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const float4* pages = pages_sm + (it % kRing) * 8;
         // every key is seen by every row of the unit
         const bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
-        const Seen seen(interior ? 0 : key_lo - key0, interior ? kT : q_pos + 1 - key0);
         if (interior)
-          softmax_i8<D, true>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+          softmax_i8<D, true>(my_s, my_o, it == 0, Seen(), row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
         else
-          softmax_i8<D, false>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+          softmax_i8<D, false>(my_s, my_o, it == 0, Seen(key_lo - key0, q_pos + 1 - key0), row_scale, pages, shift, m_run, r_run, l_run,
+                               p_ready + 16 * u);
       }
       if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);
