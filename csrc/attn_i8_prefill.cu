@@ -410,7 +410,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       for (int it = 0; ok && it < n_tiles; ++it) {
         const bool more = it + 1 < n_tiles;
-        ok = full(2 * it + 1);
+        ok = full(2 * it + 1) && (!more || full(2 * it + 2));  // (there by now; waiting between the products would hold them up)
         const uint64_t dv = desc_v(sm0 + S::kOffKV + slot_of(2 * it + 1) * S::kTile);
         for (int u = 0; ok && u < units; ++u) {
 #pragma unroll
@@ -425,8 +425,6 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           if (u == units - 1) commit(kv_empty + 8 * slot_of(2 * it + 1), leader);
           if (!more) commit(o_full + 8 * u, leader);
           if (more) {
-            if (u == 0) ok = full(2 * it + 2);
-            if (!ok) break;
             issue_s(u, it + 1);
             if (u == units - 1) commit(kv_empty + 8 * slot_of(2 * it + 2), leader);
           }
@@ -472,19 +470,20 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (lane == 0) mbar_arrive(q_ready);
       }
       for (int it = 0; it < n_tiles; ++it) {
-        failed = mbar_wait_bounded(s_full + 8 * u, it & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
-        failed = __any_sync(0xffffffffu, failed);  // warp-uniform: the TMEM accesses below are warp-wide
-        if (failed) break;
-        tc_fence_after_sync();
         const int key0 = (t_begin + it) * kT;
         const float4* pages = pages_sm + (it % kRing) * 8;
         // every key is seen by every row of the unit
         const bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
+        Seen seen;
+        if (!interior) seen = Seen(key_lo - key0, q_pos + 1 - key0);
+        failed = mbar_wait_bounded(s_full + 8 * u, it & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
+        failed = __any_sync(0xffffffffu, failed);  // warp-uniform: the TMEM accesses below are warp-wide
+        if (failed) break;
+        tc_fence_after_sync();
         if (interior)
-          softmax_i8<D, true>(my_s, my_o, it == 0, Seen(), row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+          softmax_i8<D, true>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
         else
-          softmax_i8<D, false>(my_s, my_o, it == 0, Seen(key_lo - key0, q_pos + 1 - key0), row_scale, pages, shift, m_run, r_run, l_run,
-                               p_ready + 16 * u);
+          softmax_i8<D, false>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
       }
       if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);
