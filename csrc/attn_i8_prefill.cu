@@ -556,9 +556,9 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   const int token = static_cast<int>(row / a.Hq), head = static_cast<int>(row % a.Hq);
   if (row >= rows || token < a.cu_q[0] || token >= a.cu_q[B]) return;
   const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
-  float M = -INFINITY, R = 0.f;
   const float* p = a.parts + row * (D + kPartTail);
   const int64_t next = rows * (D + kPartTail);
+  float M = -INFINITY, R = 0.f;
   for (int s = lane; s < a.splits; s += 32) {
     const float4 t = *reinterpret_cast<const float4*>(p + s * next + D);
     M = fmaxf(M, t.x);
@@ -567,17 +567,33 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   M = warp_reduce_max(M);
   R = warp_reduce_max(R);
   const float top = fmaxf(M, sink), Mu = top == -INFINITY ? 0.f : top;
-  float l = fast_exp2(sink - Mu), acc[D / 32];
+  float l = 0.f, acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 t = *reinterpret_cast<const float4*>(p + s * next + D);
-    if (t.y == 0.f) continue;  // none of its keys is seen (and its output was not written)
-    const float f = fast_exp2(t.x - Mu), fr = f * page_share(t.z, R);
-    l += t.y * f;
+  for (int s0 = 0; s0 < a.splits; s0 += 32) {
+    float f = 0.f;  // of part s0 + lane; 0 where none of its keys is seen (and its output was not written)
+    bool some = false;
+    if (s0 + lane < a.splits) {
+      const float4 t = *reinterpret_cast<const float4*>(p + (s0 + lane) * next + D);
+      some = t.y != 0.f;
+      f = some ? fast_exp2(t.x - Mu) : 0.f;
+      l += some ? t.y * f : 0.f;
+      f *= page_share(t.z, R);
+    }
+    const uint32_t there = __ballot_sync(0xffffffffu, some);
+    const int n = min(32, a.splits - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      const bool in = there >> s & 1;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] += p[s * next + i * 32 + lane] * fr;
+      for (int i = 0; i < D / 32; ++i) {
+        const float o = in ? p[(s0 + s) * next + i * 32 + lane] : 0.f;
+        acc[i] += in ? o * fs : 0.f;
+      }
+    }
   }
+  l = warp_reduce_sum(l) + fast_exp2(sink - Mu);
   if (a.lse && lane == 0) a.lse[row] = l == 0.f ? INFINITY : Mu + log2f(l);
   const float inv = l == 0.f ? 0.f : R * (kInv127 * 0x1p-7f) / l;
 #pragma unroll

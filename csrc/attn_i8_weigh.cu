@@ -1,13 +1,16 @@
 // What the queries of new tokens gave to each token of a cache in 8 bits (layout: kv_i8.cu): weights[slot, head, token] += the sum over the
 // queries that see it, and over the query heads of its key head, of exp(score - log of the query's sum), on the 5th-generation tensor cores.
 //
-// A CTA has 128 keys of a key head, as the A operand: a key is a lane of tensor memory, and its sum stays in one thread's register, with no
+// A CTA has 256 keys of a key head, as two A operands: a key is a lane of tensor memory, and its sum stays in one thread's register, with no
 // exchange between threads. Its codes become bf16 once (exactly); the queries stream through as they are, 128 / G tokens of G heads at a
 // time:
-//   warp 8   : TMA producer, a ring of query boxes, and their rows' logarithms beside them
-//   warp 9   : MMA issuer, S = K Q^T into four TMEM buffers of 128 columns
-//   warps 0-7: two groups of four, one after the other's unit: exponentials of a column each, 128 of them per key
-// The bound is the exponentials: 128 x 128 per unit at 16 a clock, 1024 clocks, beside 512 of the products (D = 128).
+//   warp 16   : TMA producer, a ring of query boxes, and their rows' logarithms beside them
+//   warp 17   : MMA issuer, S = K Q^T into two TMEM buffers of 128 columns for each 128 keys
+//   warps 0-15: four groups of four, each with a buffer of its own: 128 exponentials per key and unit, 16 columns at a time with the next
+//               scores and logarithms on their way
+// 2048 tokens of 40 heads behind 14000, us: 128 keys per CTA and two groups 598; with the next 32 columns on their way 550; 256 keys per CTA,
+// which halves the queries' way through L2, and four groups 484 (391 without the exponentials).
+// The bound is the exponentials: 256 x 128 per unit at 16 a clock, 2048 clocks, beside 1024 of the products (D = 128).
 // Long units for few keys are split over CTAs, whose sums a second kernel adds in their order.
 #include <atomic>
 
@@ -21,21 +24,21 @@ namespace {
 using namespace pxl;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kKeys = 128, kCols = 128;
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr int kM = 128, kKeys = 2 * kM, kCols = 128;
+constexpr int kGroups = 4, kProducerWarp = 4 * kGroups, kMmaWarp = kProducerWarp + 1, kThreads = (kMmaWarp + 1) * 32;
 constexpr int kHalf = 128 * 128;
-constexpr int kBufs = 4;  // of S
+constexpr int kBufs = kGroups;  // of S: 2 t + (i & 1) has the scores of keys 128 t and on with unit i
+constexpr int kUnits = 4;       // in the rings of queries and of their logarithms
 
 template <int D>
 struct Shape {
   static constexpr int kTile = D / 64 * kHalf;
-  static constexpr int kSlots = 4;  // query units in the ring
-  static constexpr int kOffQ = kTile;
-  static constexpr int kOffLse = kOffQ + kSlots * kTile;  // [kBufs][128] floats
-  static constexpr int kOffSums = kOffLse + kBufs * 512;  // [128] floats
-  static constexpr int kOffBars = kOffSums + 512;
+  static constexpr int kOffQ = 2 * kTile;
+  static constexpr int kOffLse = kOffQ + kUnits * kTile;   // [kUnits][128] floats
+  static constexpr int kOffSums = kOffLse + kUnits * 512;  // [2][128] floats
+  static constexpr int kOffBars = kOffSums + 2 * 512;
   static constexpr int kSmem = 1024 + kOffBars + 256;
-  static constexpr uint32_t kIdesc = umma_idesc(kKeys, kCols, 1, 1);  // bf16
+  static constexpr uint32_t kIdesc = umma_idesc(kM, kCols, 1, 1);  // bf16
 };
 static_assert(Shape<128>::kSmem <= 232448);
 
@@ -67,9 +70,10 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   float* lse_sm = reinterpret_cast<float*>(smem + S::kOffLse);
   float* sum_sm = reinterpret_cast<float*>(smem + S::kOffSums);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
-  // q_full, q_empty [kSlots] | s_full, s_empty [kBufs]
-  const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * S::kSlots, s_full = q_empty + 8 * S::kSlots, s_empty = s_full + 8 * kBufs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kSlots + 2 * kBufs);
+  // q_full, q_empty, lse_empty [kUnits] | s_full, s_empty [kBufs]
+  const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * kUnits, lse_empty = q_empty + 8 * kUnits, s_full = lse_empty + 8 * kUnits,
+                 s_empty = s_full + 8 * kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kUnits + 2 * kBufs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   pdl_wait();
 
@@ -83,7 +87,7 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, slot < 0 || slot >= a.slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
     return;
   }
-  // units of queries that see some of the keys: positions key0 .. key0 + 127 + window - 1
+  // units of queries that see some of the keys: positions key0 .. key0 + 255 + window - 1
   const int from = key0 - pos0 > 0 ? (key0 - pos0) / per_unit : 0;
   int past = L;  // first query behind every window
   if (a.window > 0 && static_cast<int64_t>(key0) + kKeys - 1 + a.window - pos0 < L) past = key0 + kKeys - 1 + a.window - pos0;
@@ -92,9 +96,10 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < S::kSlots; ++s) {
+    for (int s = 0; s < kUnits; ++s) {
       mbar_init(q_full + 8 * s, 1 + 32);  // the bytes, and the producer's lanes
       mbar_init(q_empty + 8 * s, 1);
+      mbar_init(lse_empty + 8 * s, 8);    // the warps that take the unit
     }
     for (int s = 0; s < kBufs; ++s) {
       mbar_init(s_full + 8 * s, 1);
@@ -120,14 +125,14 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const int64_t head = head_of(key0 + r);
     uint4 x = make_uint4(0, 0, 0, 0);
     if (head >= 0) x = *reinterpret_cast<const uint4*>(a.k_cache + (head * a.page + (key0 + r) % a.page) * D + c * 16);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w}, at = sm0 + (c >> 2) * kHalf + r * 128;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w}, at = sm0 + (r / kM) * S::kTile + (c >> 2) * kHalf + r % kM * 128;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 3) * 2 + p) ^ (r & 7)) << 4)), "r"(codes_bf16x2(w[2 * p], 0)),
                    "r"(codes_bf16x2(w[2 * p], 2)), "r"(codes_bf16x2(w[2 * p + 1], 0)), "r"(codes_bf16x2(w[2 * p + 1], 2))
                    : "memory");
   }
-  for (int i = threadIdx.x; i < S::kSlots * (D / 64) * (kCols - per_unit * G) * 8; i += kThreads) {
+  for (int i = threadIdx.x; i < kUnits * (D / 64) * (kCols - per_unit * G) * 8; i += kThreads) {
     const int c = i % 8, r = per_unit * G + i / 8 % (kCols - per_unit * G), h = i / 8 / (kCols - per_unit * G);
     st_shared_zero16(sm0 + S::kOffQ + h * kHalf + r * 128 + c * 16);
   }
@@ -139,81 +144,102 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t tm_s = *tmem_slot;
 
   if (warp == kProducerWarp) {
+    // logarithms of four units are on their way
     bool ok = true;
-    float next[4];
-    auto load = [&](int i) {  // logarithms of the unit's rows; none (infinity: a weight of 0) for rows that are nobody's
+    float next[kUnits][4];
+    auto load = [&](int i, float (&to)[4]) {  // of the unit's rows; none (infinity: a weight of 0) for rows that are nobody's
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = j * 32 + lane, tok = (u_begin + i) * per_unit + r / G;
-        next[j] = i < n_units && r < per_unit * G && tok < L ? a.lse[static_cast<int64_t>(q_begin + tok) * a.Hq + kvh * G + r % G] : INFINITY;
+        to[j] = i < n_units && r < per_unit * G && tok < L ? a.lse[static_cast<int64_t>(q_begin + tok) * a.Hq + kvh * G + r % G] : INFINITY;
       }
     };
-    load(0);
-    for (int i = 0; i < n_units; ++i) {
-      const int s = i % S::kSlots, buf = i % kBufs;
-      if (i >= S::kSlots) ok = mbar_wait_bounded(q_empty + 8 * s, (i / S::kSlots - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_EMPTY);
-      if (ok && i >= kBufs) ok = mbar_wait_bounded(s_empty + 8 * buf, (i / kBufs - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_EMPTY);
-      if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lse_sm[buf * 128 + j * 32 + lane] = -next[j];
-      const uint32_t bar = q_full + 8 * s;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, (D / 64) * per_unit * G * 128);
-        for (int h = 0; h < D / 64; ++h)
-          tma_load_3d(sm0 + S::kOffQ + s * S::kTile + h * kHalf, &tm_q, bar, h * 64, kvh * G, q_begin + (u_begin + i) * per_unit);
+    for (int s = 0; s < kUnits; ++s) load(s, next[s]);
+    for (int i0 = 0; ok && i0 < n_units; i0 += kUnits) {
+#pragma unroll
+      for (int s = 0; s < kUnits; ++s) {
+        const int i = i0 + s;
+        if (!ok || i >= n_units) break;
+        if (i >= kUnits) ok = mbar_wait_bounded(q_empty + 8 * s, (i / kUnits - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_EMPTY);
+        if (ok && i >= kUnits) ok = mbar_wait_bounded(lse_empty + 8 * s, (i / kUnits - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_EMPTY);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lse_sm[s * 128 + j * 32 + lane] = -next[s][j];
+        const uint32_t bar = q_full + 8 * s;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, (D / 64) * per_unit * G * 128);
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_3d(sm0 + S::kOffQ + s * S::kTile + h * kHalf, &tm_q, bar, h * 64, kvh * G, q_begin + (u_begin + i) * per_unit);
+        }
+        mbar_arrive(bar);
+        load(i + kUnits, next[s]);
       }
-      mbar_arrive(bar);
-      load(i + 1);
     }
   } else if (warp == kMmaWarp) {
     const uint32_t leader = elect_leader();
-    for (int i = 0; i < n_units; ++i) {
-      const int s = i % S::kSlots, buf = i % kBufs;
-      bool ok = mbar_wait_bounded(q_full + 8 * s, (i / S::kSlots) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_FULL);
-      if (ok && i >= kBufs) ok = mbar_wait_bounded(s_empty + 8 * buf, (i / kBufs - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_EMPTY);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after_sync();
+    bool ok = true;
+    for (int i = 0; ok && i < n_units; ++i) {
+      const int s = i % kUnits;
+      ok = wait_warp(q_full + 8 * s, (i / kUnits) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_FULL);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
-        mma_ss(tm_s + buf * kCols, umma_desc_k_sw128(sm0 + off), umma_desc_k_sw128(sm0 + S::kOffQ + s * S::kTile + off), S::kIdesc,
-               ks > 0 ? 1u : 0u, leader);
+      for (int t = 0; t < 2; ++t) {
+        const int buf = 2 * t + (i & 1);
+        if (ok && i >= 2) ok = wait_warp(s_empty + 8 * buf, ((i >> 1) - 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
+          mma_ss(tm_s + buf * kCols, umma_desc_k_sw128(sm0 + t * S::kTile + off), umma_desc_k_sw128(sm0 + S::kOffQ + s * S::kTile + off),
+                 S::kIdesc, ks > 0 ? 1u : 0u, leader);
+        }
+        if (t == 1) commit(q_empty + 8 * s, leader);
+        commit(s_full + 8 * buf, leader);
       }
-      commit(q_empty + 8 * s, leader);
-      commit(s_full + 8 * buf, leader);
     }
   }
   float total = 0.f;
-  const int group = warp >> 2, r = (warp & 3) * 32 + lane, t = key0 + r;  // this thread's key
+  const int group = warp >> 2, r = (warp & 3) * 32 + lane, tile0 = key0 + (group >> 1) * kM, t = tile0 + r;  // this thread's key
   int failed = 0;
-  if (warp < 8) {
+  if (warp < 4 * kGroups) {
     const int64_t head = head_of(t);
     const float scale = head >= 0 ? a.kv_max[head].x * kInv127 * a.scale_log2 : 0.f;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint64_t scale2 = pair2(scale, scale);
-    for (int i = group; i < n_units; i += 2) {
-      const int buf = i % kBufs, tok0 = (u_begin + i) * per_unit;
-      failed = mbar_wait_bounded(s_full + 8 * buf, (i / kBufs) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
+    for (int i = group & 1; i < n_units; i += 2) {
+      const int buf = group, tok0 = (u_begin + i) * per_unit;
+      failed = mbar_wait_bounded(s_full + 8 * buf, (i >> 1) & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);  // warp-uniform: the TMEM loads below are warp-wide
       if (failed) break;
       tc_fence_after_sync();
       const int last = min(tok0 + per_unit, L) - 1;  // the unit's last query
-      const bool interior = key0 + kKeys - 1 <= pos0 + tok0 && (a.window <= 0 || key0 > pos0 + last - a.window) && tok0 + per_unit <= L;
+      const bool interior = tile0 + kM - 1 <= pos0 + tok0 && (a.window <= 0 || tile0 > pos0 + last - a.window) && tok0 + per_unit <= L;
       // columns whose queries see this key
       const int first_tok = max(t - pos0 - tok0, 0), end_tok = min(last + 1 - tok0, a.window > 0 ? t - pos0 - tok0 + a.window : last + 1 - tok0);
       const int c_lo = min(first_tok, per_unit) * G, c_hi = head >= 0 ? max(end_tok, 0) * G : 0;
-      const float4* neg = reinterpret_cast<const float4*>(lse_sm + buf * 128);
+      const float4* neg = reinterpret_cast<const float4*>(lse_sm + i % kUnits * 128);
       uint64_t sum[2] = {0ull, 0ull};
+      // 16 columns at a time, the next 16 scores and logarithms on their way
+      uint32_t v[2][16];
+      float4 z[2][4];
+      auto load = [&](int c, uint32_t (&to)[16], float4 (&neg_lse)[4]) {
+        tmem_ld_32x32b_x16(tm_s + buf * kCols + lane_sel + c, to);
 #pragma unroll
-      for (int c = 0; c < kCols; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tm_s + buf * kCols + lane_sel + c, v);
+        for (int j = 0; j < 4; ++j) neg_lse[j] = neg[(c >> 2) + j];
+      };
+      load(0, v[0], z[0]);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        const int at = (c >> 4) & 1;
         tmem_ld_wait();
+        if (c + 16 < kCols) load(c + 16, v[at ^ 1], z[at ^ 1]);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 z = neg[(c + j) >> 2];
-          const float2 x = unpair2(fma2(pair2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, pair2(z.x, z.y)));
-          const float2 y = unpair2(fma2(pair2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), scale2, pair2(z.z, z.w)));
+        for (int j = 0; j < 16; j += 4) {
+          const float4& n = z[at][j >> 2];
+          const float2 x = unpair2(fma2(pair2(__uint_as_float(v[at][j]), __uint_as_float(v[at][j + 1])), scale2, pair2(n.x, n.y)));
+          const float2 y = unpair2(fma2(pair2(__uint_as_float(v[at][j + 2]), __uint_as_float(v[at][j + 3])), scale2, pair2(n.z, n.w)));
           float p[4] = {fast_exp2(x.x), fast_exp2(x.y), fast_exp2(y.x), fast_exp2(y.y)};
           if (!interior) {
 #pragma unroll
@@ -225,18 +251,21 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty + 8 * buf);
+      if (lane == 0) {
+        mbar_arrive(s_empty + 8 * buf);
+        mbar_arrive(lse_empty + 8 * (i % kUnits));
+      }
       const float2 two = unpair2(add2(sum[0], sum[1]));
       total += two.x + two.y;
     }
-    if (group == 1) sum_sm[r] = total;
+    if (group & 1) sum_sm[(group >> 1) * 128 + r] = total;
   }
 
   __syncwarp();
   if (*abort_flag) __nanosleep(200000);  // loads that are still in flight must land before smem is released
   tc_fence_before_sync();
-  if (!__syncthreads_or(failed) && group == 0 && t < ctx) {
-    total += sum_sm[r];
+  if (!__syncthreads_or(failed) && warp < 4 * kGroups && !(group & 1) && t < ctx) {
+    total += sum_sm[(group >> 1) * 128 + r];
     if (a.splits == 1) a.weights[(static_cast<int64_t>(slot) * a.Hkv + kvh) * a.W + t] += total;
     else a.parts[((static_cast<int64_t>(split) * gridDim.z + b) * a.Hkv + kvh) * a.max_ctx + t] = total;
   }
