@@ -324,7 +324,7 @@ PXL_EXPORT int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_
   if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || num_blocks <= 0 || !lse || !weights)
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || window > (1 << 30) || num_blocks <= 0 || !lse || !weights)
     return PXL_ERR_INVALID_ARG;
   const int splits = splits_of(B, max_q_len, Hq, Hkv, max_ctx);
   const int64_t need = pxl_attn_i8_weigh_workspace(B, max_q_len, Hq, Hkv, max_ctx);

@@ -1253,8 +1253,8 @@ def load_kv_i8(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tenso
 
 
 def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, window, sinks, max_ctx, out, weights, seq_slots):
-    N, Hkv, page, D, T, Hq, B, MB, max_ctx, slots, W = kv_i8.check_attention(what, q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks,
-                                                                             out, weights, seq_slots, max_ctx)
+    N, Hkv, page, D, T, Hq, B, MB, window, max_ctx, slots, W = kv_i8.check_attention(what, q, cache, block_tables, cu_q, ctx_lens, scale, window,
+                                                                                     sinks, out, weights, seq_slots, max_ctx)
     dev = q.device
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
@@ -1274,6 +1274,7 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
                                          block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks),
                                          _ptr(weights), W, slots, _ptr(seq_slots), ws.data_ptr(), need, B, Hq, Hkv, D, page, MB, N, scale,
                                          window, max_ctx, status, stream), "pxl_attn_i8_decode")
+            _count(2 + weighed)
         else:
             need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -1282,13 +1283,14 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
             check(lib.pxl_attn_i8_prefill(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), kv_max.data_ptr(),
                                           block_tables.data_ptr(), cu_q.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0),
                                           _ptr(sinks), _ptr(lse), _ptr(ws), need, *where), "pxl_attn_i8_prefill")
+            _count(1 + (need > 0))
             if weighed:
                 need = lib.pxl_attn_i8_weigh_workspace(B, max_q_len, Hq, Hkv, max_ctx)
                 ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
                 check(lib.pxl_attn_i8_weigh(q.data_ptr(), q.stride(0), k_cache.data_ptr(), kv_max.data_ptr(), block_tables.data_ptr(),
                                             cu_q.data_ptr(), ctx_lens.data_ptr(), lse.data_ptr(), weights.data_ptr(), W, slots,
                                             _ptr(seq_slots), _ptr(ws), need, *where), "pxl_attn_i8_weigh")
-    _count(2 + weighed)
+                _count(1 + (need > 0))
     return out
 
 

@@ -93,8 +93,8 @@ def _rows_2d(t: torch.Tensor) -> torch.Tensor:
 def check_attention(what: str, q: torch.Tensor, cache: tuple, block_tables: torch.Tensor, cu_q: Optional[torch.Tensor],
                     ctx_lens: torch.Tensor, scale: float, window: int, sinks: Optional[torch.Tensor], out: Optional[torch.Tensor],
                     weights: Optional[torch.Tensor], seq_slots: Optional[torch.Tensor], max_ctx: int) -> tuple[int, ...]:
-    """Checks what the two attentions share; returns blocks, key heads, page, D, queries, query heads, sequences, pages of a table, longest
-    sequence, slots of the weights and tokens of a slot."""
+    """Checks what the two attentions share; returns blocks, key heads, page, D, queries, query heads, sequences, pages of a table, window,
+    longest sequence, slots of the weights and tokens of a slot."""
     N, Hkv, page, D, dev = check_cache(*cache, what)
     T, Hq = check_rows(q, "q", None, D, dev, what)
     if Hq % Hkv or not 0 < Hq // Hkv <= MAX_GROUP:
@@ -119,9 +119,13 @@ def check_attention(what: str, q: torch.Tensor, cache: tuple, block_tables: torc
             refuse(what, "out has neighbouring heads and columns, rows that start on 16 bytes and do not overlap")
         if T > 0 and q.stride(2) == 1 and q.stride(1) == D and _share_memory(_rows_2d(q), _rows_2d(out)):
             refuse(what, "out overlaps the queries")
+        lo, hi = out.data_ptr(), out.data_ptr() + 2 * ((T - 1) * out.stride(0) + Hq * D)
+        for t in (*cache, weights, sinks):
+            if T > 0 and t is not None and t.data_ptr() < hi and lo < t.data_ptr() + t.numel() * t.element_size():
+                refuse(what, "out overlaps the cache, the weights or the sinks")
     slots, W = (0, 0) if weights is None else check_weights(weights, seq_slots, B, Hkv, dev, what)
     most = MB * page
-    return N, Hkv, page, D, T, Hq, B, MB, max_ctx if 0 < max_ctx < most else most, slots, W
+    return N, Hkv, page, D, T, Hq, B, MB, min(window, 1 << 30), max_ctx if 0 < max_ctx < most else most, slots, W
 
 
 def check_store(what: str, k: torch.Tensor, v: torch.Tensor, cache: tuple, block_tables: torch.Tensor, cu_q: torch.Tensor,
@@ -158,6 +162,8 @@ def check_evict(what: str, cache: tuple, weights: torch.Tensor, block_tables: to
     slots, W = check_weights(weights, seq_slots, B, Hkv, dev, what)
     if recent < 0 or first < 0 or keep < 1 or first + recent > keep:
         refuse(what, f"keep at least one token, the first and the recent ones among them: got keep {keep}, recent {recent}, first {first}")
+    if B > 0 and new_tables.data_ptr() == block_tables.data_ptr():
+        refuse(what, "new_tables have pages of their own, not those of block_tables")
     if keep > MN * page:
         refuse(what, f"keep {keep} tokens need more than the {MN} pages of new_tables")
     return N, Hkv, page, D, B, MB, MN, slots, W

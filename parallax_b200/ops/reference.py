@@ -717,7 +717,8 @@ def attn_decode_i8(q, k_cache, v_cache, kv_max, block_tables, ctx_lens, scale, w
                    seq_slots=None):
     """One query per sequence, ``q [B, Hq, D]``, over an 8-bit cache (see :mod:`.kv_i8`): ``window`` keys per query (0: all), ``sinks [Hq]``
     beside them. ``max_ctx``: no sequence is longer (0: as long as the tables reach). ``weights [slots, heads, tokens]``: what the query
-    gave to each token, summed over the query heads of a key head, is added there, sequence b in slot ``seq_slots[b]`` (None: b)."""
+    gave to each token, summed over the query heads of a key head, is added there, sequence b in slot ``seq_slots[b]`` (None: b), each in
+    one of its own."""
     cache = (k_cache, v_cache, kv_max)
     kv_i8.check_attention("attn_decode_i8", q, cache, block_tables, None, ctx_lens, scale, window, sinks, out, weights, seq_slots, max_ctx)
     res = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
@@ -739,7 +740,9 @@ def attn_prefill_i8(q, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, m
     res = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
     for b in range(ctx_lens.shape[0]):
         lo, hi, t = int(cu_q[b]), int(cu_q[b + 1]), int(ctx_lens[b])
-        if hi > lo and t > 0:
+        if hi > lo and t <= 0:
+            res[lo:hi] = 0
+        elif hi > lo:
             slot = b if seq_slots is None else int(seq_slots[b])
             res[lo:hi] = _attend_i8(q[lo:hi], cache, block_tables[b], hi - lo, t, scale, window, sinks, None if weights is None else weights[slot])
     return res

@@ -175,6 +175,11 @@ def test_attention_refuses_results_over_queries():
     packed = torch.zeros(3, 8, 64).bfloat16()
     a["q"] = packed[:, :4]
     ops.attn_decode_i8(**a, out=packed[:, 4:])
+    for name in ("k_cache", "v_cache", "weights"):
+        a = _call(weights=torch.zeros(3, 2, 100))
+        over = a[name].flatten().view(torch.uint8)[512:2048].view(torch.bfloat16).view(3, 4, 64)
+        with pytest.raises(KernelError, match="overlaps"):
+            ops.attn_decode_i8(**a, out=over)
     with pytest.raises(KernelError, match="attn_prefill_i8"):
         b = _call()
         ops.attn_prefill_i8(b["q"], b["k_cache"], b["v_cache"], b["kv_max"], b["block_tables"], torch.zeros(3, dtype=torch.int32), b["ctx_lens"],
@@ -203,7 +208,9 @@ def test_store_and_evict_refuse():
     for keep, recent, first, weights, new in ((0, 0, 0, w, tab), (4, 3, 2, w, tab), (17, 1, 0, w, tab), (4, -1, 0, w, tab), (4, 1, -1, w, tab),
                                               (4, 1, 0, w[:, :1], tab), (4, 1, 0, w, torch.zeros(2, 1, dtype=torch.int32))):
         with pytest.raises(KernelError, match="evict_kv_i8"):
-            ops.evict_kv_i8(*cache, weights, tab, one, new, keep, recent, first)
+            ops.evict_kv_i8(*cache, weights, tab + 0, one, new, keep, recent, first)
+    with pytest.raises(KernelError, match="pages of their own"):
+        ops.evict_kv_i8(*cache, w, tab, one, tab, 4, 1)
 
 
 def test_a_prompt_steps_an_eviction_and_more_steps():

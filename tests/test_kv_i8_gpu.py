@@ -483,3 +483,80 @@ def test_store_attention_and_eviction_in_a_launch_chain():
             got = go(mine, w)
         _check()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ sizes, streams, odd lengths
+def test_more_new_tokens_than_tokens():
+    """Queries at positions below zero see nothing; the others see the tokens that are there."""
+    g = _gen(60)
+    cache = oracle.make_cache(g, 4, 1, 16, 64)
+    q = torch.randn(9, 2, 64, generator=g).bfloat16()
+    d = _dev(q, *cache, _i32([[0], [1]]), _i32([0, 5, 9]), _i32([3, 0]))
+    out = torch.full((9, 2, 64), 5.0, dtype=torch.bfloat16, device=DEV)
+    weights = torch.zeros(2, 1, 16, device=DEV)
+    ops.attn_prefill_i8(*d, 5, 0.1, out=out, weights=weights)
+    _check()
+    assert (out[:2] == 0).all() and (out[5:] == 0).all()
+    (o, mean, add, size), = oracle.attention(q[2:5], cache, _i32([[0]]), [3], [3], 0.1)
+    oracle.assert_output(out[2:5].cpu(), o, mean, size)
+    oracle.assert_weights(weights[0, :, :3].cpu(), add, torch.zeros(1, 3), size, 3)
+    assert (weights[0, :, 3:] == 0).all() and (weights[1] == 0).all()
+
+
+@pytest.mark.parametrize("page,D", [(64, 128), (16, 64)])
+def test_blocks_past_two_and_four_gigabytes(page, D):
+    """Offsets above 2^31 and 2^32 bytes in the cache: the same codes and results as at its start."""
+    heads, G = 8, 2
+    blocks = (9 << 29) // (heads * page * D)
+    g = _gen(61)
+    k, v = (torch.zeros(blocks, heads, page, D, dtype=torch.int8, device=DEV) for _ in range(2))
+    m = torch.zeros(blocks, heads, 2, device=DEV)
+    n = 3 * page + 5
+    x = torch.randn(n, 2 * heads, D, generator=g).bfloat16().to(DEV)
+    q = torch.randn(n, G * heads, D, generator=g).bfloat16().to(DEV)
+    ends, lens = _dev(_i32([0, n]), _i32([n]))
+    got = []
+    for first in (0, blocks // 2 - 2, blocks - 8):
+        tab = torch.arange(first, first + 4).int()[None].to(DEV)
+        new_tab = torch.arange(first + 4, first + 8).int()[None].to(DEV)
+        weights = torch.zeros(1, heads, n, device=DEV)
+        ops.store_kv_i8(x[:, :heads], x[:, heads:], k, v, m, tab, ends, lens, n)
+        r = [*ops.load_kv_i8(k, v, m, tab, ends, n), ops.attn_prefill_i8(q, k, v, m, tab, ends, lens, n, 0.1, weights=weights),
+             ops.attn_decode_i8(q[:1], k, v, m, tab, lens, 0.1, weights=weights)]
+        kept, n_kept = ops.evict_kv_i8(k, v, m, weights, tab, lens, new_tab, 2 * page + 1, 7)
+        r += [kept, weights, *ops.load_kv_i8(k, v, m, new_tab, _i32([0, 2 * page + 1]).to(DEV), 2 * page + 1)]
+        got.append(r)
+    _check()
+    for r in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, got[0]))
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_on_a_stream_of_its_own(decode):
+    run, d, weights = _case(62, decode)
+    want = run().clone()
+    weigh = weights.clone()
+    _check()
+    s = torch.cuda.Stream()
+    q = d[0].clone()
+    for _ in range(3):
+        with torch.cuda.stream(s):
+            d[0].zero_()
+            weights.zero_()
+            d[0].copy_(q)                 # the inputs come on this stream, right before
+            got = run()
+        s.synchronize()
+        assert torch.equal(got, want) and torch.equal(weights, weigh)
+    _check()
+
+
+@pytest.mark.parametrize("G", [1, 3, 16])
+def test_one_long_sequence(G):
+    """Many CTAs for a pair, in decoding as for a few new tokens, with sinks and weights."""
+    _compare(63 + G, [1], [20011], G, 1, 128, 64, sink=True, decode=True, weighed=True)
+    _compare(64 + G, [9], [12007], G, 1, 64, 16, sink=True, weighed=True)
+
+
+def test_many_short_sequences():
+    _compare(65, [1] * 700, [1 + 7 * i % 90 for i in range(700)], 4, 2, 64, 16, decode=True)
+    _compare(66, [1 + i % 3 for i in range(300)], [3 + 11 * i % 50 for i in range(300)], 2, 1, 128, 32, weighed=True)
