@@ -8,6 +8,9 @@
 // magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R,
 // so that what is rounded to f16 (2^-11) is the probability times the share; a factor of 2^11 keeps its bits down to 2^-25 of the row's
 // largest, and it is rounded in steps of 2^-35 below. The reference maximum may lag by 2^4 before anything is rescaled.
+// What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 306 us, 6.4 TB/s. Three CTAs per SM, since a tile's products wait
+// for its exponentials; f16 rather than 8-bit products, since q and the probabilities would lose bits. Short pairs are bound by their
+// beginning and end (203 windows of 128 keys, 64 heads of 64: 25 us).
 // A pair that lies in several CTAs is added up by a second kernel. Where the weights are wanted, the scores go to the workspace (4 bytes
 // per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are known.
 #include <atomic>

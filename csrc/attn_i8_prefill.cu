@@ -15,6 +15,9 @@
 // that what is rounded to f16 is the probability times the share (2^-11 of it, down to 2^-21 of the row's largest; 2^-32 below), and the
 // sum of a page's 16 columns is divided by the share again. Both the reference maximum (by 2^8) and R are let run ahead before O in tensor
 // memory is rescaled.
+// 8111 tokens, 32 heads, D = 128, twice: 726 us, 0.96 PFLOP/s. A tile takes 4400 clocks for both units, the chain of one unit's: product 550,
+// softmax 2700, notice and issue 1000; the tensor pipe is 41 % full. Two units of 128 rows for one conversion: with one the converting warps
+// would take as long as the softmax.
 // Few rows: the keys are split over several CTAs, whose results a second kernel adds up.
 // Every wait is bounded; on expiry the kernel records a status code, all roles unwind, tensor memory is freed.
 #include <atomic>

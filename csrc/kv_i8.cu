@@ -87,7 +87,8 @@ __device__ __forceinline__ float over_127(float x) {
 
 // ---- write ---------------------------------------------------------------------------------------------------------
 // One CTA per (page that gets tokens, key head): HALF threads for the keys and as many for the values, which keep what they read. ROWS: new
-// tokens that a page gets at most (1 in a decoding step, with a warp for each half).
+// tokens that a page gets at most (1 in a decoding step, with a warp for each half). 12000 tokens of 8 heads in prompts 21 us, 2.4 TB/s in and
+// out: load, meet, round and store follow one another in a CTA.
 template <int D, int ROWS, int HALF>
 __global__ void __launch_bounds__(2 * HALF)
 store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t k_stride, int64_t v_stride,
@@ -156,8 +157,8 @@ store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64
 
 // ---- read ----------------------------------------------------------------------------------------------------------
 // A warp takes a row of the result, all heads, keys and values: it finds the row's sequence by counting the ends at or before it, then has 8
-// codes per lane of keys and of values in four steps in flight, and its stores are whole lines. (16 rows to a CTA, found by bisection, one load behind the other:
-// 105 us for 82000 tokens of 8 heads.)
+// codes per lane of keys and of values in four steps in flight, and its stores are whole lines. 82000 tokens of 8 heads 92 us, 4.9 TB/s. (16 rows
+// to a CTA, found by bisection, one load behind the other: 105 us.)
 constexpr int kLoadWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kLoadWarps * 32)
@@ -226,7 +227,7 @@ load_kv_i8_kernel(const int8_t* __restrict__ k_cache, const int8_t* __restrict__
 // 11 and 10 of them, a histogram each), then the tokens above it and the earliest of those that have it, in order: each warp counts and
 // then writes those of its own stretch. The weights are read from memory once and kept as keys in shared memory (CACHED: up to 50000
 // tokens), or read in each of the five passes. They move to their new places chunk by chunk, the first chunk first: a token never moves
-// back, so that no chunk writes where a later one reads.
+// back, so that no chunk writes where a later one reads. 40 sequences of up to 9000 tokens, 8 heads: 24 us.
 constexpr int kPickThreads = 1024;
 constexpr int kBins = 2048;
 constexpr int kPickCache = 50000;
@@ -366,8 +367,9 @@ evict_pick_kernel(float* __restrict__ weights, int64_t W, int slots, const int* 
 }
 
 // The tokens that stay into their new pages: a warp takes 16 of a key head, with all their codes in flight (16 of them to a load). The new
-// magnitude of a page is the largest that a token of it had: a warp looks all of its page's tokens up. (CTAs of 64 tokens that met between
-// the look-up, three loads one behind the other, and the codes: 125 us for 40 x 2048 tokens of 8 heads.)
+// magnitude of a page is the largest that a token of it had: a warp looks all of its page's tokens up. 40 x 2048 tokens of 8 heads 85 us, 3.7
+// TB/s: single rows of 128 bytes and 2.5 operations per code. (CTAs of 64 tokens that met between the look-up, three loads one behind the
+// other, and the codes: 125 us.)
 constexpr int kMoveWarps = 4;
 template <int D, int PAGE>
 __global__ void __launch_bounds__(kMoveWarps * 32)

@@ -62,9 +62,9 @@ def assert_output(got, want, mean, size, steps=0.0):
     """bf16 outputs: half a step of the result; and of the mean of |v|, 2^-11 for probabilities in 16 bits and the scores' error: fp32 sums
     of D products are off by up to 2^-20 of the sum of their magnitudes (`size`, in log2 units), twice that in a quotient of two sums.
     `steps`: what small probabilities lose beside pages of far larger values. What is rounded to f16 is the probability, relative to the
-    row's largest or to one 2^8 below it, times the page's share of R <= 2 max |v|, times 2^7 (decode: 2^15, R = max |v|); f16 rounds by at
-    most 2^-25, so a key is off by 2^-32 R (2^-40 R), the sum of the probabilities is at least 1, and R is at most twice the largest: keys *
-    2^-31 (2^-40) * max |v|."""
+    row's largest or to one up to 2^8 below it, times the page's share of R, times 2^7 (decode: 2^11); f16 rounds what is too small for its
+    mantissa by at most 2^-25, so a key is off by 2^-32 R (2^-36 R). The sum of the probabilities is at least 1, and R at most twice the
+    largest magnitude: keys * 2^-31 (2^-35) * max |v|."""
     got, nan = got.double(), torch.isnan(want)
     assert torch.equal(torch.isnan(got), nan)
     far = (got - want).abs() - (2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -19 * size + 2.0 ** -14) * mean + steps + 1e-30)
