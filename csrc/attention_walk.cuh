@@ -123,25 +123,30 @@ struct DecodeShares {
   __device__ __forceinline__ int64_t operator[](int cta) const { return each * cta + min(cta, longer); }
 };
 
-// One CTA's way along the row, a pair (or the part of one that is its share) at a time.
+// One CTA's way along the row, a pair (or the part of one that is its share) at a time. Uncut: the pairs that begin in its share, whole.
 struct DecodeWalk {
   DecodeWork work;
   int left, b, kvh, t, weight, take, lo, hi;  // tiles left; of the pair, tiles t .. t + take of `weight`
   KeyTiles tiles;
+  bool uncut;
 
-  __device__ __forceinline__ DecodeWalk(const DecodeWork& w, int cta, int ctas) : work(w), tiles(0, 0, 0) {
+  __device__ __forceinline__ DecodeWalk(const DecodeWork& w, int cta, int ctas, bool uncut = false) : work(w), tiles(0, 0, 0), uncut(uncut) {
     const DecodeShares at(work.total(), ctas);
     left = static_cast<int>(at[cta + 1] - at[cta]);
     b = kvh = t = weight = take = lo = hi = 0;
     if (left > 0) {
       work.find(at[cta], b, kvh, t);
       enter();
+      if (uncut && t > 0) {
+        take = weight - t;
+        next();
+      }
     }
   }
   __device__ __forceinline__ void enter() {
     tiles = work.tiles(b, lo, hi);
     weight = tiles.total > 0 ? tiles.total : 1;
-    take = min(left, weight - t);
+    take = uncut ? weight : min(left, weight - t);
   }
   __device__ __forceinline__ int count() const { return tiles.total > 0 ? take : 0; }
   __device__ __forceinline__ bool whole() const { return take == weight; }

@@ -8,12 +8,14 @@
 // magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R,
 // so that what is rounded to f16 (2^-11) is the probability times the share; a factor of 2^11 keeps its bits down to 2^-25 of the row's
 // largest, and it is rounded in steps of 2^-35 below. The reference maximum may lag by 2^4 before anything is rescaled.
-// What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 306 us, 6.4 TB/s. Three CTAs per SM, since a tile's products wait
-// for its exponentials; f16 rather than 8-bit products, since q and the probabilities would lose bits. Short pairs are bound by their
-// beginning and end (203 windows of 128 keys, 64 heads of 64: 25 us).
-// A pair that lies in several CTAs is added up by a second kernel. Where the weights are wanted, the scores go to the workspace (4 bytes
-// per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are known.
+// What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 297 us, 6.6 TB/s. Three CTAs per SM, since a tile's
+// products wait for its exponentials; f16 rather than 8-bit products, since q and the probabilities would lose bits. Short pairs are bound
+// by their beginning and end (203 windows of 128 keys, 64 heads of 64: 21 us).
+// A pair that lies in several CTAs is added up by a second kernel; short ones are not cut. Where the weights are wanted, the scores go to
+// the workspace (4 bytes per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are
+// known.
 #include <atomic>
+#include <type_traits>
 
 #include "attention_walk.cuh"
 #include "common.cuh"
@@ -30,17 +32,20 @@ constexpr int kThreads = 160;  // four consumer warps and the producer
 constexpr float kUp = 11.f;    // log2 of the factor on probabilities in f16
 constexpr float kLag = 4.f;    // log2 of how far the reference maximum may lag
 
+// (Heads of 64, 40 sequences of up to 8000 tokens, 32 heads: three CTAs of eight stages 62 us, four of six 59.)
+constexpr int ctas_per_sm(int D, int NH) { return NH > 1 ? 2 : D == 64 ? 4 : 3; }
+
 // NH: tiles of 8 query heads
 template <int D, int NH>
 struct Shape {
-  static constexpr int kCtas = NH == 1 ? 3 : 2;                  // on an SM
+  static constexpr int kCtas = ctas_per_sm(D, NH);
   static constexpr int kTileBytes = kKeyTile * D;                // of K, or of V
-  static constexpr int kStages = D == 64 ? 8 : 4;                // even: a stage belongs to one pair of warps
+  static constexpr int kStages = D == 128 ? 4 : NH == 1 ? 6 : 8;  // even: a stage belongs to one pair of warps
   static constexpr int kVecs = NH * D / 16;                      // 16-byte vectors of a lane's output
-  static constexpr int kStats = 4 * NH + 1;                      // maxima and sums of a lane's heads, R
-  static constexpr int kOffParts = kStages * 2 * kTileBytes;     // [2][kVecs][32] float4
-  static constexpr int kOffStats = kOffParts + 2 * kVecs * 512;  // [2][kStats][32] floats
-  static constexpr int kOffMax = kOffStats + 2 * kStats * 128;   // [stages][4] magnitudes of a stage's pages
+  static constexpr int kStats = 16 * NH + 4;                     // maxima and sums of a warp's heads, R
+  static constexpr int kOffParts = kStages * 2 * kTileBytes;     // [4][kVecs / 2][32] float4
+  static constexpr int kOffStats = kOffParts + 2 * kVecs * 512;  // [4][kStats] floats
+  static constexpr int kOffMax = kOffStats + 4 * kStats * 4;     // [stages][4] magnitudes of a stage's pages
   static constexpr int kOffBars = kOffMax + kStages * 32;
   static constexpr int kSmem = 1024 + kOffBars + kStages * 16 + 16;
   static_assert(kCtas * (kSmem + 1024) <= 233472);
@@ -60,6 +65,7 @@ struct Args {
   int64_t num_blocks;
   float scale_log2;
   int window;
+  bool uncut;
   int* status;
 };
 
@@ -315,7 +321,7 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
   }
   // the lengths and the tables of a step are there before its first kernel, the queries and the new keys after the wait
   const DecodeWork work{a.ctx_lens, a.B, a.Hkv, a.window, 0};
-  DecodeWalk walk(work, blockIdx.x, gridDim.x);
+  DecodeWalk walk(work, blockIdx.x, gridDim.x, a.uncut);
   auto blocks_of = [&](const DecodeWalk& w) {
     return TileBlocks{a.block_tables + static_cast<size_t>(w.left > 0 ? w.b : 0) * a.max_blocks, w.tiles, w.t, w.left > 0 ? w.count() : 0,
                       a.page, shift, w.hi, a.max_blocks, a.num_blocks, a.status};
@@ -387,29 +393,42 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         if (lane == 0) mbar_arrive(empty0 + 8 * stage);
       }
 
-      // warps 2 and 3 hand their results to 0 and 1, 1 to 0; a register goes to the same lane
-      auto give = [&](int p) {
-        float* st = stats + p * S::kStats * 32 + lane;
+      // The four warps' results, each of some keys, become a quarter of the columns of all keys each: half of them change hands with the warp
+      // that had the other tiles, half of the rest with the one that had the other 32 keys of these. A warp writes its second gift where it
+      // has read the first one.
+      float sums[NH][2];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) sums[n][0] = keys_sum(rows.l_run[n][0]), sums[n][1] = keys_sum(rows.l_run[n][1]);
+      const int t4 = lane & 3;
+      auto exchange = [&](auto half, int at, int from, bool upper) {  // keeps `half` of 2 * half vectors
+        constexpr int N = decltype(half)::value;
+        float4* to = parts + at * (S::kVecs / 2) * 32 + lane;
+        float* st = stats + at * S::kStats;
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            parts[(p * S::kVecs + n * (D / 16) + i) * 32 + lane] = make_float4(rows.o[n][i][0], rows.o[n][i][1], rows.o[n][i][2], rows.o[n][i][3]);
+          for (int i = 0; i < N; ++i) {
+            float (&lo)[4] = rows.o[n][i], (&hi)[4] = rows.o[n][i + N];
+            to[(n * N + i) * 32] = upper ? make_float4(lo[0], lo[1], lo[2], lo[3]) : make_float4(hi[0], hi[1], hi[2], hi[3]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) st[(n * 4 + e) * 32] = rows.m_run[n][e], st[(n * 4 + 2 + e) * 32] = rows.l_run[n][e];
+            for (int j = 0; j < 4; ++j) lo[j] = upper ? hi[j] : lo[j];
+          }
+          if (lane < 4)
+            *reinterpret_cast<float4*>(st + n * 16 + lane * 4) = make_float4(rows.m_run[n][0], sums[n][0], rows.m_run[n][1], sums[n][1]);
         }
-        st[4 * NH * 32] = rows.r_run;
-      };
-      auto add = [&](int p) {
-        const float* st = stats + p * S::kStats * 32 + lane;
-        const float r2 = st[4 * NH * 32], r_new = fmaxf(rows.r_run, r2);
+        if (lane == 0) st[16 * NH] = rows.r_run;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const float4* of = parts + from * (S::kVecs / 2) * 32 + lane;
+        const float* os = stats + from * S::kStats;
+        const float r2 = os[16 * NH], r_new = fmaxf(rows.r_run, r2);
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
-          const Joined x(rows.m_run[n][0], rows.l_run[n][0], rows.r_run, r_new, st[n * 128], st[n * 128 + 64], r2);
-          const Joined y(rows.m_run[n][1], rows.l_run[n][1], rows.r_run, r_new, st[n * 128 + 32], st[n * 128 + 96], r2);
+          const float4 other = *reinterpret_cast<const float4*>(os + n * 16 + t4 * 4);
+          const Joined x(rows.m_run[n][0], sums[n][0], rows.r_run, r_new, other.x, other.y, r2);
+          const Joined y(rows.m_run[n][1], sums[n][1], rows.r_run, r_new, other.z, other.w, r2);
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const float4 v = parts[(p * S::kVecs + n * (D / 16) + i) * 32 + lane];
+          for (int i = 0; i < N; ++i) {
+            const float4 v = of[(n * N + i) * 32];
             float (&o)[4] = rows.o[n][i];
             o[0] = o[0] * x.fa + v.x * x.fb;
             o[1] = o[1] * y.fa + v.y * y.fb;
@@ -418,40 +437,34 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
           }
         }
         rows.r_run = r_new;
+        __syncwarp();  // all lanes have read the sums
       };
-      if (warp >= 2) give(warp - 2);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (warp < 2) add(warp);
-      if (warp == 1) give(1);  // (its own place: each lane has read what it writes)
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (warp == 0) add(1);
-      // the places are free for the next pair: warps 2 and 3 write them ahead of the next barrier
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (warp == 0) {
-        const int g8 = lane >> 2, t4 = lane & 3;
+      exchange(std::integral_constant<int, D / 32>(), warp, warp ^ 2, (warp & 2) != 0);
+      exchange(std::integral_constant<int, D / 64>(), warp ^ 2, warp ^ 3, (warp & 1) != 0);
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the places are free for the next pair
+      const int g8 = lane >> 2, col = ((warp >> 1) * 2 + (warp & 1)) * (D / 4) + 2 * g8;
 #pragma unroll
-        for (int n = 0; n < NH; ++n)
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = n * 8 + 2 * t4 + e;
-            const float M = rows.m_run[n][e], L = keys_sum(rows.l_run[n][e]);
-            if (r >= G || failed) continue;
-            if (walk.whole()) {
-              float lse;
-              const float f = finish(M, L, rows.r_run, a.sinks ? a.sinks[head0 + r] * kLog2e : -INFINITY, lse);
-              if (a.lse && g8 == 0) a.lse[static_cast<size_t>(walk.b) * a.Hq + head0 + r] = lse;
-              bf16* dst = a.out + walk.b * a.out_stride + (head0 + r) * D + 2 * g8;
+        for (int e = 0; e < 2; ++e) {
+          const int r = n * 8 + 2 * t4 + e;
+          const float M = rows.m_run[n][e], L = sums[n][e];
+          if (r >= G || failed) continue;
+          if (walk.whole()) {
+            float lse;
+            const float f = finish(M, L, rows.r_run, a.sinks ? a.sinks[head0 + r] * kLog2e : -INFINITY, lse);
+            if (a.lse && warp == 0 && g8 == 0) a.lse[static_cast<size_t>(walk.b) * a.Hq + head0 + r] = lse;
+            bf16* dst = a.out + walk.b * a.out_stride + (head0 + r) * D + col;
 #pragma unroll
-              for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint32_t*>(dst + i * 16) = pack_bf16x2(rows.o[n][i][e] * f, rows.o[n][i][2 + e] * f);
-            } else {
-              float* po = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (walk.t == 0 ? 1 : 0)) * (G * (D + 2) + 4);
+            for (int i = 0; i < D / 64; ++i) *reinterpret_cast<uint32_t*>(dst + i * 16) = pack_bf16x2(rows.o[n][i][e] * f, rows.o[n][i][2 + e] * f);
+          } else {
+            float* po = a.parts + (static_cast<size_t>(blockIdx.x) * 2 + (walk.t == 0 ? 1 : 0)) * (G * (D + 2) + 4);
 #pragma unroll
-              for (int i = 0; i < D / 16; ++i)
-                *reinterpret_cast<float2*>(po + r * D + i * 16 + 2 * g8) = make_float2(rows.o[n][i][e], rows.o[n][i][2 + e]);
-              if (g8 == 0) po[G * D + r] = M, po[G * D + G + r] = L, po[G * (D + 2)] = rows.r_run;
-            }
+            for (int i = 0; i < D / 64; ++i)
+              *reinterpret_cast<float2*>(po + r * D + i * 16 + col) = make_float2(rows.o[n][i][e], rows.o[n][i][2 + e]);
+            if (warp == 0 && g8 == 0) po[G * D + r] = M, po[G * D + G + r] = L, po[G * (D + 2)] = rows.r_run;
           }
-      }
+        }
     }
   }
   if (__syncthreads_or(failed)) __nanosleep(200000);  // loads that are still in flight must land before the shared memory is released
@@ -555,13 +568,21 @@ attn_i8_weigh_kernel(const __grid_constant__ Args a, float* __restrict__ weights
   }
 }
 
+// Whether pairs are left whole, so that no second kernel has to add their parts up (4 to 7 us), although a CTA may get the tiles of almost
+// a pair more than its even share. us, cut / whole, 32 heads of 128: 8 pairs of up to 4 tiles 8.9 / 7.7, of up to 8 8.2 / 10.2; 64 pairs of up to 8
+// 11.7 / 11.3, of up to 16 14.0 / 16.4; 1624 pairs of up to 8 47.8 / 44.3, of up to 16 69.7 / 65.4.
+bool uncut(int64_t pairs, int window, int max_ctx) {
+  const int tiles = window > 0 && window < max_ctx ? ceil_div(window - 1, kKeyTile) + 1 : ceil_div(max_ctx, kKeyTile);
+  return tiles <= (pairs >= 1024 ? 16 : pairs >= 64 ? 8 : 4);
+}
+
 // floats of the workspace: partial results, log2 of the sums, scores
 struct Layout {
   int64_t lse, scores, score_stride, total;
   int ctas;
   Layout(int B, int Hq, int Hkv, int D, int max_ctx, bool weights) {
     const int64_t tiles = static_cast<int64_t>(B) * Hkv * (ceil_div64(max_ctx, kKeyTile) + 1);
-    const int full = (Hq / Hkv > 8 ? 2 : 3) * pxl_host::num_sms();
+    const int full = ctas_per_sm(D, Hq / Hkv > 8 ? 2 : 1) * pxl_host::num_sms();
     ctas = tiles < full ? static_cast<int>(tiles) : full;
     lse = static_cast<int64_t>(ctas) * 2 * (Hq / Hkv * (D + 2) + 4);
     score_stride = weights ? ceil_div64(max_ctx, kKeyTile) * kKeyTile : 0;
@@ -582,7 +603,7 @@ int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, i
     done.store(true, std::memory_order_relaxed);
   }
   pxl_host::launch(attn_i8_decode_kernel<D, NH>, dim3(ctas), dim3(kThreads), kSmem, stream, tk, tv, a);
-  if (ctas > 1)
+  if (ctas > 1 && !a.uncut)
     pxl_host::launch_behind(attn_i8_join_kernel<D>, dim3(ctas - 1), dim3(kJoinThreads), a.Hq / a.Hkv * ctas * 4, stream, a, ctas);
   if (weights)
     pxl_host::launch_behind(attn_i8_weigh_kernel, dim3(static_cast<unsigned>(ceil_div64(a.score_stride, kWeighKeys)), a.Hkv, a.B), dim3(256), 0,
@@ -619,7 +640,7 @@ PXL_EXPORT int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k
   float* ws = static_cast<float*>(workspace);
   const Args a{static_cast<const bf16*>(q), q_stride, reinterpret_cast<const float2*>(kv_max), block_tables, ctx_lens, static_cast<bf16*>(out),
                out_stride, sinks, ws, weights ? ws + at.lse : nullptr, weights ? ws + at.scores : nullptr, at.score_stride, B, Hq, Hkv, page,
-               max_blocks, num_blocks, scale * kLog2e, window, status};
+               max_blocks, num_blocks, scale * kLog2e, window, uncut(static_cast<int64_t>(B) * Hkv, window, max_ctx), status};
   auto go = [&](auto launch) { return launch(tk, tv, a, at.ctas, weights, W, slots, seq_slots, stream); };
   if (D == 64) return Hq / Hkv > 8 ? go(launch_decode<64, 2>) : go(launch_decode<64, 1>);
   return Hq / Hkv > 8 ? go(launch_decode<128, 2>) : go(launch_decode<128, 1>);

@@ -560,3 +560,18 @@ def test_one_long_sequence(G):
 def test_many_short_sequences():
     _compare(65, [1] * 700, [1 + 7 * i % 90 for i in range(700)], 4, 2, 64, 16, decode=True)
     _compare(66, [1 + i % 3 for i in range(300)], [3 + 11 * i % 50 for i in range(300)], 2, 1, 128, 32, weighed=True)
+
+
+@pytest.mark.parametrize("seqs,heads,most", [(5, 2, 256), (5, 2, 257), (40, 2, 512), (40, 2, 513), (300, 4, 1024), (300, 4, 1025)])
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 2), (64, 9)])
+def test_sequences_that_are_cut_and_that_are_not(seqs, heads, most, D, G):
+    """On both sides of the lengths up to which a (sequence, key head) pair stays in one CTA, lengths of all kinds."""
+    g = _gen(67 + seqs + most)
+    ctx = [most] + torch.randint(1, most + 1, (seqs - 1,), generator=g).tolist()
+    _compare(68 + most, [1] * seqs, ctx, G, heads, D, 16, sink=True, decode=True, weighed=seqs == 40)
+
+
+@pytest.mark.parametrize("window", [129, 193, 194, 400])
+def test_windows_that_are_cut_and_that_are_not(window):
+    ctx = [1, 64, 3000, 129, 700, 193, 2047, 385, 2048, 1000]
+    _compare(window, [1] * 10, ctx, 8, 2, 64, 32, window=window, sink=True, decode=True, weighed=True)
