@@ -87,10 +87,10 @@ __device__ __forceinline__ float over_127(float x) {
 
 // ---- write ---------------------------------------------------------------------------------------------------------
 // One CTA per (page that gets tokens, key head): HALF threads for the keys and as many for the values, which keep what they read. ROWS: new
-// tokens that a page gets at most (1 in a decoding step, with a warp for each half). 12000 tokens of 8 heads in prompts 21 us, 2.4 TB/s in and
-// out: load, meet, round and store follow one another in a CTA.
+// tokens that a page gets at most (1 in a decoding step, with a warp for each half). 12000 tokens of 8 heads in prompts 19 us, 2.6 TB/s in and
+// out: load, meet, round and store follow one another in a CTA. (Four CTAs on an SM for pages of 64: 21 -> 19.)
 template <int D, int ROWS, int HALF>
-__global__ void __launch_bounds__(2 * HALF)
+__global__ void __launch_bounds__(2 * HALF, D == 128 && ROWS == 64 ? 4 : 0)
 store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t k_stride, int64_t v_stride,
                    const int* __restrict__ block_tables, const int* __restrict__ cu_q, const int* __restrict__ ctx_lens,
                    int8_t* __restrict__ k_cache, int8_t* __restrict__ v_cache, float* __restrict__ kv_max, int T, int Hkv, int page,
@@ -157,11 +157,11 @@ store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64
 
 // ---- read ----------------------------------------------------------------------------------------------------------
 // A warp takes a row of the result, all heads, keys and values: it finds the row's sequence by counting the ends at or before it, then has 8
-// codes per lane of keys and of values in four steps in flight, and its stores are whole lines. 82000 tokens of 8 heads 92 us, 4.9 TB/s. (16 rows
-// to a CTA, found by bisection, one load behind the other: 105 us.)
+// codes per lane of keys and of values in four steps in flight, and its stores are whole lines. 82000 tokens of 8 heads 88 us, 5.0 TB/s. (16 rows
+// to a CTA, found by bisection, one load behind the other: 105 us; two rows to a warp 100; five CTAs on an SM 92.)
 constexpr int kLoadWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kLoadWarps * 32)
+__global__ void __launch_bounds__(kLoadWarps * 32, 6)
 load_kv_i8_kernel(const int8_t* __restrict__ k_cache, const int8_t* __restrict__ v_cache, const float* __restrict__ kv_max,
                   const int* __restrict__ block_tables, const int* __restrict__ cu_k, bf16* __restrict__ k_out, bf16* __restrict__ v_out, int rows,
                   int B, int Hkv, int page, int max_blocks, int64_t num_blocks, int* status) {
@@ -367,12 +367,12 @@ evict_pick_kernel(float* __restrict__ weights, int64_t W, int slots, const int* 
 }
 
 // The tokens that stay into their new pages: a warp takes 16 of a key head, with all their codes in flight (16 of them to a load). The new
-// magnitude of a page is the largest that a token of it had: a warp looks all of its page's tokens up. 40 x 2048 tokens of 8 heads 85 us, 3.7
-// TB/s: single rows of 128 bytes and 2.5 operations per code. (CTAs of 64 tokens that met between the look-up, three loads one behind the
-// other, and the codes: 125 us.)
+// magnitude of a page is the largest that a token of it had: a warp looks all of its page's tokens up. 40 x 2048 tokens of 8 heads 88 us, 3.4
+// TB/s: single rows of 128 bytes and 2.5 operations per code; eight CTAs on an SM for heads of 128: 92. (CTAs of 64 tokens that met between
+// the look-up, three loads one behind the other, and the codes: 125 us.)
 constexpr int kMoveWarps = 4;
 template <int D, int PAGE>
-__global__ void __launch_bounds__(kMoveWarps * 32)
+__global__ void __launch_bounds__(kMoveWarps * 32, D == 128 ? 9 : 0)
 evict_move_kernel(int8_t* __restrict__ k_cache, int8_t* __restrict__ v_cache, float* __restrict__ kv_max, const int* __restrict__ block_tables,
                   const int* __restrict__ new_tables, const int* __restrict__ kept, const int* __restrict__ new_lens, int Hkv, int max_blocks,
                   int max_new, int64_t num_blocks, int keep, int* status) {
