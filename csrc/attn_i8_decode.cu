@@ -627,7 +627,8 @@ PXL_EXPORT int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
       ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || window > (1 << 30) || num_blocks <= 0 ||
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
+      window < 0 || window > (1 << 30) || num_blocks <= 0 ||
       num_blocks * Hkv * page >= (1ll << 31))
     return PXL_ERR_INVALID_ARG;
   const Layout at(B, Hq, Hkv, D, max_ctx, weights != nullptr);

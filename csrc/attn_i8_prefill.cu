@@ -280,7 +280,11 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const int per_unit = kRowsQ / G;  // tokens
   // heavy blocks (late queries see the most keys) are scheduled first, of all heads (head by head: 827 us for 806)
   const int q0 = (static_cast<int>(gridDim.x) / a.Hkv - 1 - static_cast<int>(blockIdx.x) / a.Hkv) * 2 * per_unit;
-  if (q0 >= L || q_begin < 0 || q_begin + L > a.T) return;  // uniform for the CTA, before any barrier or allocation
+  if (q0 >= L) return;  // uniform for the CTA, before any barrier or allocation
+  if (q_begin < 0 || q_begin > a.T - L) {
+    if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, PXL_DEV_BAD_INDEX);
+    return;
+  }
   const int units = L - q0 > per_unit ? 2 : 1, tokens = min(L - q0, 2 * per_unit);
   const int pos0 = ctx - L + q0;      // position of the first token
   const int hi = pos0 + tokens;       // keys [lo, hi) are seen by some row
@@ -651,12 +655,14 @@ PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, in
 PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max,
                                    const int* block_tables, const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride,
                                    const float* sinks, float* lse, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len,
-                                   int Hq, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx, int* status, cudaStream_t stream) {
+                                   int Hq, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx,
+                                   int* status, cudaStream_t stream) {
   if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
       ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || window > (1 << 30) || num_blocks <= 0 ||
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
+      window < 0 || window > (1 << 30) || num_blocks <= 0 ||
       num_blocks * Hkv * page >= (1ll << 31))
     return PXL_ERR_INVALID_ARG;
   const Layout at(T, B, max_q_len, Hq, Hkv, D, max_ctx);

@@ -82,7 +82,7 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin, ctx = a.ctx_lens[b], slot = a.seq_slots ? a.seq_slots[b] : b;
   const int per_unit = kCols / G;
   const int key0 = blockIdx.x * kKeys, pos0 = ctx - L;  // position of the first query
-  if (L <= 0 || key0 >= ctx || q_begin < 0 || q_begin + L > a.T) return;  // uniform for the CTA, before any barrier or allocation
+  if (L <= 0 || key0 >= ctx || q_begin < 0 || q_begin > a.T - L) return;  // uniform for the CTA, before any barrier or allocation
   if (slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) {
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, slot < 0 || slot >= a.slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
     return;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(256) attn_i8_weigh_join_kernel(const __grid_co
   pdl_launch_dependents();
   const int b = blockIdx.z, h = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = a.ctx_lens[b], slot = a.seq_slots ? a.seq_slots[b] : b;
   const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin;
-  if (t >= ctx || L <= 0 || q_begin < 0 || q_begin + L > a.T || slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) return;
+  if (t >= ctx || L <= 0 || q_begin < 0 || q_begin > a.T - L || slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) return;
   float sum = 0.f;
   for (int s = 0; s < a.splits; ++s) sum += a.parts[((static_cast<int64_t>(s) * gridDim.z + b) * a.Hkv + h) * a.max_ctx + t];
   a.weights[(static_cast<int64_t>(slot) * a.Hkv + h) * a.W + t] += sum;
@@ -324,7 +324,9 @@ PXL_EXPORT int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_
   if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || window < 0 || window > (1 << 30) || num_blocks <= 0 || !lse || !weights)
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
+      window < 0 || window > (1 << 30) || num_blocks <= 0 ||
+      !lse || !weights)
     return PXL_ERR_INVALID_ARG;
   const int splits = splits_of(B, max_q_len, Hq, Hkv, max_ctx);
   const int64_t need = pxl_attn_i8_weigh_workspace(B, max_q_len, Hq, Hkv, max_ctx);

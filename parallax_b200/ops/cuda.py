@@ -1260,7 +1260,7 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
     if T == 0 or B == 0 or max_q_len <= 0:
         return out
-    q = _head_rows(q)
+    q, max_q_len = _head_rows(q), min(max_q_len, T)
     k_cache, v_cache, kv_max = cache
     weighed = weights is not None
     with _on(dev):
@@ -1274,7 +1274,7 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
                                          block_tables.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), out.stride(0), _ptr(sinks),
                                          _ptr(weights), W, slots, _ptr(seq_slots), ws.data_ptr(), need, B, Hq, Hkv, D, page, MB, N, scale,
                                          window, max_ctx, status, stream), "pxl_attn_i8_decode")
-            _count(2 + weighed)
+            _count(1 + weighed)  # (and one more where pairs are cut)
         else:
             need = lib.pxl_attn_i8_prefill_workspace(T, B, max_q_len, Hq, Hkv, D, max_ctx)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

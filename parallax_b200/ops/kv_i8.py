@@ -125,7 +125,11 @@ def check_attention(what: str, q: torch.Tensor, cache: tuple, block_tables: torc
                 refuse(what, "out overlaps the cache, the weights or the sinks")
     slots, W = (0, 0) if weights is None else check_weights(weights, seq_slots, B, Hkv, dev, what)
     most = MB * page
-    return N, Hkv, page, D, T, Hq, B, MB, min(window, 1 << 30), max_ctx if 0 < max_ctx < most else most, slots, W
+    if 0 < max_ctx < most:
+        most = max_ctx
+    if most >= 1 << 30:
+        refuse(what, f"sequences stay below 2^30 tokens, got {most}")
+    return N, Hkv, page, D, T, Hq, B, MB, min(window, 1 << 30), most, slots, W
 
 
 def check_store(what: str, k: torch.Tensor, v: torch.Tensor, cache: tuple, block_tables: torch.Tensor, cu_q: torch.Tensor,

@@ -91,7 +91,7 @@ P = 1 << 20        # an address that nothing reads: every call below is refused
 @pytest.mark.parametrize("change", [dict(D=96), dict(page=8), dict(page=128), dict(Hq=5), dict(Hq=34), dict(Hkv=0), dict(scale=0.0), dict(scale=-1.0),
                                     dict(window=-1), dict(window=(1 << 30) + 1), dict(q_stride=100), dict(out_stride=100), dict(q=P + 2),
                                     dict(out=P + 4), dict(k=P + 8), dict(v=P + 8), dict(m=P + 4), dict(blocks=0), dict(blocks=1 << 40),
-                                    dict(max_blocks=0), dict(max_ctx=0), dict(ws=0), dict(ws_bytes=8)])
+                                    dict(max_blocks=0), dict(max_ctx=0), dict(max_ctx=1 << 30), dict(ws=0), dict(ws_bytes=8)])
 @pytest.mark.parametrize("decode", [True, False])
 def test_attention_refused_by_the_library(change, decode):
     a = dict(q=P, q_stride=256, k=P, v=P, m=P, out=P, out_stride=256, ws=P, ws_bytes=1 << 30, Hq=4, Hkv=2, D=64, page=16, max_blocks=2048, blocks=4096,

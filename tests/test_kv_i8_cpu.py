@@ -186,6 +186,13 @@ def test_attention_refuses_results_over_queries():
                             1, 0.125)
 
 
+def test_tables_that_are_too_long():
+    a = _call(ctx_lens=torch.ones(1, dtype=torch.int32), block_tables=torch.empty(1, (1 << 30) // 16, dtype=torch.int32))
+    a["q"] = a["q"][:1]
+    with pytest.raises(KernelError, match="2\\^30"):
+        ops.attn_decode_i8(**a)
+
+
 @pytest.mark.parametrize("shape", [(4, 2, 8, 64), (4, 2, 128, 64), (4, 2, 16, 96), (4, 2, 16, 256)])
 def test_pages_and_heads_that_are_refused(shape):
     c = torch.zeros(shape, dtype=torch.int8)

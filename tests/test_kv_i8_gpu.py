@@ -315,6 +315,26 @@ def test_blocks_off_the_cache_and_slots_off_the_weights_are_reported(decode):
     assert all(torch.equal(a, b) for a, b in zip(before, cache))
 
 
+@pytest.mark.parametrize("ends", [[0, 2, 5], [-1, 1, 2], [0, 3, 2]])
+def test_ends_off_the_queries(ends):
+    """Sequences whose rows are not all there are reported and left out; one that ends before it begins has none."""
+    from parallax_b200.ops import cuda as cu
+
+    g = _gen(25)
+    cache = _dev(*oracle.make_cache(g, 4, 1, 16, 64))
+    q = torch.randn(2, 2, 64, generator=g).bfloat16().to(DEV)
+    tab, lens = _dev(_i32([[1, 2], [3, 0]]), _i32([30, 30]))
+    out, weights = torch.full((2, 2, 64), 7, dtype=torch.bfloat16, device=DEV), torch.zeros(2, 1, 32, device=DEV)
+    ops.attn_prefill_i8(q, *cache, tab, _i32(ends).to(DEV), lens, 1 << 40, 0.1, out=out, weights=weights)
+    with pytest.raises(ops.KernelError, match="index"):
+        cu.check_status(torch.device(DEV))
+    b = 0 if ends == [0, 2, 5] else 1 if ends[0] < 0 else None
+    for s in range(2):
+        assert abs(float(weights[s].sum()) - (0 if b != s else 2 * (ends[s + 1] - ends[s]))) < 1e-2
+    for r in range(2):
+        assert bool((out[r] == 7).all()) == (b is None or not ends[b] <= r < ends[b + 1])
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @pytest.mark.parametrize("page,D", [(16, 128), (32, 64), (64, 128), (16, 64), (64, 64)])
 @pytest.mark.parametrize("keep,recent,first", [(64, 20, 4), (64, 64, 0), (33, 0, 0), (40, 0, 40), (300, 7, 1), (1, 0, 0)])
