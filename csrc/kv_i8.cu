@@ -250,6 +250,14 @@ evict_pick_kernel(float* __restrict__ weights, int64_t W, int slots, const int* 
   const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slot = seq_slots ? seq_slots[b] : b;
   int n = max(ctx_lens[b], 0);
+  bool twice = false;  // another sequence has the slot
+  if (seq_slots)
+    for (int i = threadIdx.x; i < static_cast<int>(gridDim.y); i += kPickThreads)
+      twice = twice || (i != b && seq_slots[i] == slot && n > 0 && ctx_lens[i] > 0);
+  if (__syncthreads_or(twice)) {
+    if (threadIdx.x == 0 && status) atomicCAS(status, 0, PXL_DEV_BAD_SLOT);
+    n = 0;
+  }
   if (slot < 0 || slot >= slots || n > W || n > capacity) {
     if (threadIdx.x == 0 && status) atomicCAS(status, 0, slot < 0 || slot >= slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
     n = 0;
@@ -341,7 +349,8 @@ evict_pick_kernel(float* __restrict__ weights, int64_t W, int slots, const int* 
       const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && key == prefix), below = (1u << lane) - 1;
       const bool take = i < hi && (key > prefix || (key == prefix && ties + __popc(eq & below) < left));
       const uint32_t all = __ballot_sync(0xffffffffu, take);
-      if (take) out[first + at + __popc(all & below)] = first + i;
+      const int place = at + __popc(all & below);
+      if (take && place < want) out[first + place] = first + i;  // (they are `want`, unless the weights change meanwhile)
       at += __popc(all);
       ties += __popc(eq);
     }
@@ -353,7 +362,7 @@ evict_pick_kernel(float* __restrict__ weights, int64_t W, int slots, const int* 
 #pragma unroll
     for (int j = 0; j < kMove; ++j) {
       const int i = i0 + j * kPickThreads + threadIdx.x;
-      x[j] = i < keep ? w[out[i]] : 0.f;
+      x[j] = i < keep ? w[min(max(out[i], 0), n - 1)] : 0.f;
     }
     __syncthreads();
 #pragma unroll
@@ -387,7 +396,7 @@ evict_move_kernel(int8_t* __restrict__ k_cache, int8_t* __restrict__ v_cache, fl
   auto look = [&](int r, float2& m) {  // row of token r of those that stay, in the cache; -1 for none
     m = make_float2(0.f, 0.f);
     if (r >= n) return -1;
-    const int i = of[r], blk = i / PAGE < max_blocks ? bt[i / PAGE] : -1;
+    const int i = of[r], blk = i >= 0 && i / PAGE < max_blocks ? bt[i / PAGE] : -1;
     if (blk < 0 || blk >= num_blocks) {
       if (status) atomicCAS(status, 0, PXL_DEV_BAD_SLOT);
       return -1;

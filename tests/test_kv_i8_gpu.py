@@ -335,6 +335,24 @@ def test_ends_off_the_queries(ends):
         assert bool((out[r] == 7).all()) == (b is None or not ends[b] <= r < ends[b + 1])
 
 
+def test_evictions_from_one_slot_are_reported():
+    """Two sequences with tokens in it; not those without any, as they fill a batch up."""
+    from parallax_b200.ops import cuda as cu
+
+    g = _gen(26)
+    cache = _dev(*oracle.make_cache(g, 8, 1, 16, 64))
+    tab, new = _dev(_i32([[1, 2], [3, 0], [-1, -1]]), _i32([[4], [5], [6]]))
+    weights, slots = torch.rand(3, 1, 32, generator=g).to(DEV), _i32([1, 1, 1]).to(DEV)
+    run = lambda lens: ops.evict_kv_i8(*cache, weights, tab, _i32(lens).to(DEV), new, 12, 3, seq_slots=slots)
+    assert run([0, 30, 0])[1].tolist() == [0, 12, 0]
+    _check()
+    before = weights.clone()
+    kept, lens = run([30, 30, 0])
+    with pytest.raises(ops.KernelError, match="slot"):
+        cu.check_status(torch.device(DEV))
+    assert (kept == -1).all() and (lens == 0).all() and torch.equal(weights, before)
+
+
 # ------------------------------------------------------------------------------------------------ evict
 @pytest.mark.parametrize("page,D", [(16, 128), (32, 64), (64, 128), (16, 64), (64, 64)])
 @pytest.mark.parametrize("keep,recent,first", [(64, 20, 4), (64, 64, 0), (33, 0, 0), (40, 0, 40), (300, 7, 1), (1, 0, 0)])
