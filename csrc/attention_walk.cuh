@@ -123,6 +123,11 @@ struct DecodeShares {
   __device__ __forceinline__ int64_t operator[](int cta) const { return each * cta + min(cta, longer); }
 };
 
+// The share of CTA `rank` of the 2^log that have a pair to themselves.
+struct PairShare {
+  int pair, rank, log;
+};
+
 // One CTA's way along the row, a pair (or the part of one that is its share) at a time. Uncut: the pairs that begin in its share, whole.
 struct DecodeWalk {
   DecodeWork work;
@@ -142,6 +147,13 @@ struct DecodeWalk {
         next();
       }
     }
+  }
+  __device__ __forceinline__ DecodeWalk(const DecodeWork& w, const PairShare& of)
+      : work(w), b(of.pair / w.Hkv), kvh(of.pair % w.Hkv), tiles(0, 0, 0), uncut(false) {
+    tiles = work.tiles(b, lo, hi);
+    weight = tiles.total > 0 ? tiles.total : 1;
+    t = weight * of.rank >> of.log;
+    left = take = (weight * (of.rank + 1) >> of.log) - t;
   }
   __device__ __forceinline__ void enter() {
     tiles = work.tiles(b, lo, hi);

@@ -11,8 +11,9 @@
 // What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 297 us, 6.6 TB/s. Three CTAs per SM, since a tile's
 // products wait for its exponentials; f16 rather than 8-bit products, since q and the probabilities would lose bits. Short pairs are bound
 // by their beginning and end (203 windows of 128 keys, 64 heads of 64: 21 us).
-// A pair that lies in several CTAs is added up by a second kernel; short ones are not cut. Where the weights are wanted, the scores go to
-// the workspace (4 bytes per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are
+// A pair that lies in several CTAs is added up by a second kernel; short ones are not cut, and few pairs get a cluster each, whose CTAs add
+// up from each other's shared memory (one sequence of up to 776 tokens, 32 heads of 128: 9.9 -> 6.7 us). Where the weights are wanted, the
+// scores go to the workspace (4 bytes per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are
 // known.
 #include <atomic>
 #include <type_traits>
@@ -66,6 +67,7 @@ struct Args {
   float scale_log2;
   int window;
   bool uncut;
+  int log_ranks;  // of the CTAs of a cluster that has a pair to itself; 0: none
   int* status;
 };
 
@@ -289,7 +291,9 @@ __device__ __forceinline__ float finish(float M, float L, float R, float sink, f
   return denom == 0.f ? 0.f : __fdividef(e, denom) * (R * (kInv127 * 0x1p-11f));
 }
 
-template <int D, int NH>
+// TOGETHER: a cluster of 2^a.log_ranks CTAs has a pair, and adds its parts up from shared memory.
+constexpr int kLogRanks = 3, kRanks = 1 << kLogRanks;  // at most
+template <int D, int NH, bool TOGETHER>
 __global__ void __launch_bounds__(kThreads, Shape<D, NH>::kCtas)
 attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
   using S = Shape<D, NH>;
@@ -321,7 +325,13 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
   }
   // the lengths and the tables of a step are there before its first kernel, the queries and the new keys after the wait
   const DecodeWork work{a.ctx_lens, a.B, a.Hkv, a.window, 0};
-  DecodeWalk walk(work, blockIdx.x, gridDim.x, a.uncut);
+  const int rank = static_cast<int>(blockIdx.x) & ((1 << a.log_ranks) - 1);
+  DecodeWalk walk = [&] {
+    if constexpr (TOGETHER) return DecodeWalk(work, PairShare{static_cast<int>(blockIdx.x) >> a.log_ranks, rank, a.log_ranks});
+    else return DecodeWalk(work, blockIdx.x, gridDim.x, a.uncut);
+  }();
+  const int pair_b = walk.b, pair_kvh = walk.kvh;
+  const bool idle = walk.left <= 0;
   auto blocks_of = [&](const DecodeWalk& w) {
     return TileBlocks{a.block_tables + static_cast<size_t>(w.left > 0 ? w.b : 0) * a.max_blocks, w.tiles, w.t, w.left > 0 ? w.count() : 0,
                       a.page, shift, w.hi, a.max_blocks, a.num_blocks, a.status};
@@ -450,7 +460,12 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
           const int r = n * 8 + 2 * t4 + e;
           const float M = rows.m_run[n][e], L = sums[n][e];
           if (r >= G || failed) continue;
-          if (walk.whole()) {
+          if constexpr (TOGETHER) {
+            float* po = reinterpret_cast<float*>(parts) + r * D + col;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) *reinterpret_cast<float2*>(po + i * 16) = make_float2(rows.o[n][i][e], rows.o[n][i][2 + e]);
+            if (warp == 0 && g8 == 0) reinterpret_cast<float4*>(stats)[r] = make_float4(M, L, rows.r_run, 1.f);
+          } else if (walk.whole()) {
             float lse;
             const float f = finish(M, L, rows.r_run, a.sinks ? a.sinks[head0 + r] * kLog2e : -INFINITY, lse);
             if (a.lse && warp == 0 && g8 == 0) a.lse[static_cast<size_t>(walk.b) * a.Hq + head0 + r] = lse;
@@ -466,6 +481,45 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
           }
         }
     }
+  }
+  if constexpr (TOGETHER) {
+    static_assert(4 * S::kStats >= 64 && S::kStats % 4 == 0 && 2 * S::kVecs * 128 >= 8 * NH * D);
+    if (idle && threadIdx.x < G) reinterpret_cast<float4*>(stats)[threadIdx.x] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    __syncwarp();
+    cluster_sync_all();
+    // a rank's share of the results, four columns per thread
+    const int ranks = 1 << a.log_ranks, all = G * D / 4, each = (all + ranks - 1) >> a.log_ranks;
+    for (int i = threadIdx.x; i < each && rank * each + i < all; i += kThreads) {
+      const int at = rank * each + i;
+      const int r = at / (D / 4);
+      float4 st[kRanks], o[kRanks];
+      float M = -INFINITY, L = 0.f, top = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRanks; ++k) {
+        const uint32_t from = k < ranks ? k : 0;
+        st[k] = ld_shared_cluster_f32x4(cluster_map_shared(smem_u32(stats) + r * 16, from));
+        o[k] = ld_shared_cluster_f32x4(cluster_map_shared(smem_u32(parts) + at * 16, from));
+        if (k >= ranks) st[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < kRanks; ++k) M = fmaxf(M, st[k].x), top = fmaxf(top, st[k].z);
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kRanks; ++k) {
+        const float e = fast_exp2(st[k].x - Mu), f = e * page_share(st[k].z, top);
+        L += st[k].y * e;
+        if (st[k].w != 0.f) acc.x += o[k].x * f, acc.y += o[k].y * f, acc.z += o[k].z * f, acc.w += o[k].w * f;
+      }
+      const int head = pair_kvh * G + r;
+      float lse;
+      const float f = finish(M, L, top, a.sinks ? a.sinks[head] * kLog2e : -INFINITY, lse);
+      if (a.lse && at % (D / 4) == 0) a.lse[static_cast<size_t>(pair_b) * a.Hq + head] = lse;
+      *reinterpret_cast<uint2*>(a.out + pair_b * a.out_stride + head * D + at % (D / 4) * 4) =
+          make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+    }
+    __syncwarp();
+    cluster_sync_all();  // nobody's shared memory goes before it has been read
   }
   if (__syncthreads_or(failed)) __nanosleep(200000);  // loads that are still in flight must land before the shared memory is released
 }
@@ -571,10 +625,10 @@ attn_i8_weigh_kernel(const __grid_constant__ Args a, float* __restrict__ weights
 // Whether pairs are left whole, so that no second kernel has to add their parts up (4 to 7 us), although a CTA may get the tiles of almost
 // a pair more than its even share. us, cut / whole, 32 heads of 128: 8 pairs of up to 4 tiles 8.9 / 7.7, of up to 8 8.2 / 10.2; 64 pairs of up to 8
 // 11.7 / 11.3, of up to 16 14.0 / 16.4; 1624 pairs of up to 8 47.8 / 44.3, of up to 16 69.7 / 65.4.
-bool uncut(int64_t pairs, int window, int max_ctx) {
-  const int tiles = window > 0 && window < max_ctx ? ceil_div(window - 1, kKeyTile) + 1 : ceil_div(max_ctx, kKeyTile);
-  return tiles <= (pairs >= 1024 ? 16 : pairs >= 64 ? 8 : 4);
+int most_tiles(int window, int max_ctx) {  // of a pair
+  return window > 0 && window < max_ctx ? ceil_div(window - 1, kKeyTile) + 1 : ceil_div(max_ctx, kKeyTile);
 }
+bool uncut(int64_t pairs, int tiles) { return tiles <= (pairs >= 1024 ? 16 : pairs >= 64 ? 8 : 4); }
 
 // floats of the workspace: partial results, log2 of the sums, scores
 struct Layout {
@@ -591,20 +645,75 @@ struct Layout {
   }
 };
 
+// How many CTAs share a pair, as a power of two, so that all pairs are on the chip at once; 0: pairs are dealt out. us, dealt out / eight, four or
+// two CTAs, 32 heads of 128 on 8: one sequence of up to 776 tokens 9.9 / 6.9, of up to 6000 19.0 / 12.8, of up to 12000 18.5 / 20.0; 12 of up to
+// 1500 16.0 / 12.3 (four), of up to 6000 28.6 / 31.1; 27 of up to 1500 19.5 / 17.3 (two), of up to 6000 47.1 / 51.8.
 template <int D, int NH>
-int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas, float* weights, int64_t W, int slots,
+int log_ranks_of(int64_t pairs, int tiles) {
+  static std::atomic<int> known[64][kLogRanks + 1];  // clusters that are on the chip at once + 1
+  for (int log = kLogRanks; log > 0; --log) {
+    if (tiles > (log == kLogRanks ? 128 : 32)) continue;
+    std::atomic<int>& entry = known[pxl_host::current_device_slot()][log];
+    int n = entry.load(std::memory_order_relaxed) - 1;
+    if (n < 0) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(1 << log);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = Shape<D, NH>::kSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << log;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, attn_i8_decode_kernel<D, NH, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      entry.store(n + 1, std::memory_order_relaxed);
+    }
+    if (pairs <= n) return log;
+  }
+  return 0;
+}
+
+template <int D, int NH>
+int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, Args a, int ctas, int tiles, float* weights, int64_t W, int slots,
                   const int* seq_slots, cudaStream_t stream) {
   constexpr int kSmem = Shape<D, NH>::kSmem;
   static std::atomic<bool> configured[64];  // function attributes are per device
   std::atomic<bool>& done = configured[pxl_host::current_device_slot()];
   if (!done.load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(attn_i8_decode_kernel<D, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(attn_i8_decode_kernel<D, NH, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(attn_i8_decode_kernel<D, NH, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
       return PXL_ERR_CUDA;
     done.store(true, std::memory_order_relaxed);
   }
-  pxl_host::launch(attn_i8_decode_kernel<D, NH>, dim3(ctas), dim3(kThreads), kSmem, stream, tk, tv, a);
-  if (ctas > 1 && !a.uncut)
-    pxl_host::launch_behind(attn_i8_join_kernel<D>, dim3(ctas - 1), dim3(kJoinThreads), a.Hq / a.Hkv * ctas * 4, stream, a, ctas);
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.Hkv;
+  if (!a.uncut) a.log_ranks = log_ranks_of<D, NH>(pairs, tiles);
+  if (a.log_ranks) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(pairs << a.log_ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << a.log_ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pxl_host::chained() ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, attn_i8_decode_kernel<D, NH, true>, tk, tv, a) != cudaSuccess) {
+      cudaGetLastError();
+      return PXL_ERR_CUDA;
+    }
+  } else {
+    pxl_host::launch(attn_i8_decode_kernel<D, NH, false>, dim3(ctas), dim3(kThreads), kSmem, stream, tk, tv, a);
+    if (ctas > 1 && !a.uncut)
+      pxl_host::launch_behind(attn_i8_join_kernel<D>, dim3(ctas - 1), dim3(kJoinThreads), a.Hq / a.Hkv * ctas * 4, stream, a, ctas);
+  }
   if (weights)
     pxl_host::launch_behind(attn_i8_weigh_kernel, dim3(static_cast<unsigned>(ceil_div64(a.score_stride, kWeighKeys)), a.Hkv, a.B), dim3(256), 0,
                             stream, a, weights, W, slots, seq_slots);
@@ -639,10 +748,11 @@ PXL_EXPORT int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k
   if (!pxl_host::make_tmap_codes(&tk, k_cache, rows, D, page) || !pxl_host::make_tmap_codes(&tv, v_cache, rows, D, page))
     return PXL_ERR_TENSORMAP;
   float* ws = static_cast<float*>(workspace);
+  const int tiles = most_tiles(window, max_ctx);
   const Args a{static_cast<const bf16*>(q), q_stride, reinterpret_cast<const float2*>(kv_max), block_tables, ctx_lens, static_cast<bf16*>(out),
                out_stride, sinks, ws, weights ? ws + at.lse : nullptr, weights ? ws + at.scores : nullptr, at.score_stride, B, Hq, Hkv, page,
-               max_blocks, num_blocks, scale * kLog2e, window, uncut(static_cast<int64_t>(B) * Hkv, window, max_ctx), status};
-  auto go = [&](auto launch) { return launch(tk, tv, a, at.ctas, weights, W, slots, seq_slots, stream); };
+               max_blocks, num_blocks, scale * kLog2e, window, uncut(static_cast<int64_t>(B) * Hkv, tiles), 0, status};
+  auto go = [&](auto launch) { return launch(tk, tv, a, at.ctas, tiles, weights, W, slots, seq_slots, stream); };
   if (D == 64) return Hq / Hkv > 8 ? go(launch_decode<64, 2>) : go(launch_decode<64, 1>);
   return Hq / Hkv > 8 ? go(launch_decode<128, 2>) : go(launch_decode<128, 1>);
 }

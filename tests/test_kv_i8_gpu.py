@@ -613,3 +613,13 @@ def test_sequences_that_are_cut_and_that_are_not(seqs, heads, most, D, G):
 def test_windows_that_are_cut_and_that_are_not(window):
     ctx = [1, 64, 3000, 129, 700, 193, 2047, 385, 2048, 1000]
     _compare(window, [1] * 10, ctx, 8, 2, 64, 32, window=window, sink=True, decode=True, weighed=True)
+
+
+@pytest.mark.parametrize("seqs,heads,most", [(3, 4, 2048), (24, 4, 1500), (27, 8, 700), (40, 8, 700), (12, 8, 2049), (1, 1, 8193), (2, 2, 9000)])
+@pytest.mark.parametrize("D,G,weighed", [(64, 4, True), (128, 5, False), (128, 16, True), (64, 1, False), (64, 12, False)])
+def test_pairs_that_ctas_share(seqs, heads, most, D, G, weighed):
+    """Eight, four and two CTAs in a cluster for each pair, and pairs that are dealt out to all; some sequences shorter than the CTAs are many."""
+    g = _gen(69 + seqs + most)
+    ctx = [most] + torch.randint(0, most + 1, (seqs - 1,), generator=g).tolist()
+    ctx[-1] = ctx[-1] if seqs < 3 else 100
+    _compare(70 + most, [1] * seqs, ctx, G, heads, D, 32, sink=True, decode=True, weighed=weighed)
