@@ -452,6 +452,7 @@ bool cache_ok(int Hkv, int D, int page, int max_blocks, int64_t num_blocks, cons
   return Hkv > 0 && (D == 64 || D == 128) && (page == 16 || page == 32 || page == 64) && max_blocks > 0 && num_blocks > 0 &&
          num_blocks * Hkv * page < (1ll << 31) && !((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15);
 }
+bool pairs_ok(const float* kv_max) { return !(reinterpret_cast<uintptr_t>(kv_max) & 7); }  // (where they are read as such)
 int done() { return cudaGetLastError() == cudaSuccess ? PXL_OK : PXL_ERR_CUDA; }
 
 }  // namespace
@@ -485,7 +486,7 @@ PXL_EXPORT int pxl_kv_i8_load(const void* k_cache, const void* v_cache, const fl
                               void* v, int rows, int B, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, int* status,
                               cudaStream_t stream) {
   if (rows <= 0) return PXL_OK;
-  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || B < 0 ||
+  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || !pairs_ok(kv_max) || B < 0 ||
       ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15))
     return PXL_ERR_INVALID_ARG;
   auto go = [&](auto kernel) {
@@ -502,7 +503,7 @@ PXL_EXPORT int pxl_kv_i8_evict(void* k_cache, void* v_cache, float* kv_max, floa
                                int D, int page, int max_blocks, int max_new, int64_t num_blocks, int keep, int recent, int first, int* status,
                                cudaStream_t stream) {
   if (B <= 0) return PXL_OK;
-  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || max_new <= 0 || W <= 0 || keep < 1 || recent < 0 || first < 0 ||
+  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || !pairs_ok(kv_max) || max_new <= 0 || W <= 0 || keep < 1 || recent < 0 || first < 0 ||
       static_cast<int64_t>(recent) + first > keep || keep > static_cast<int64_t>(max_new) * page || static_cast<int64_t>(max_blocks) * page > INT32_MAX)
     return PXL_ERR_INVALID_ARG;
   if (B > 65535 || Hkv > 65535) return PXL_ERR_TOO_LARGE;

@@ -570,7 +570,8 @@ int pxl_act_rows(const void* x, int64_t ldx, int x_f32, int act, const void* tab
 
 // ---- kv_i8.cu, attn_i8_decode.cu, attn_i8_prefill.cu, attn_i8_weigh.cu: keys and values in 8 bits ---------------------------------------------
 // k_cache, v_cache: int8 codes [num_blocks, Hkv, page, D], D 64 or 128, page 16, 32 or 64; kv_max [num_blocks, Hkv, 2]: the largest
-// magnitude of a page's keys and of its values. A code stands for code * (kv_max / 127). Block tables [B, max_blocks].
+// magnitude of a page's keys and of its values, on 8 bytes (for the write, on 4). A code stands for code * (kv_max / 127). Block tables
+// [B, max_blocks].
 // New tokens into the cache: rows cu_q[b] .. cu_q[b + 1] of k and v [T, Hkv, D] (heads side by side, strides in elements) are the last
 // of the ctx_lens[b] tokens of sequence b, at most max_q_len of each.
 int pxl_kv_i8_store(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int* block_tables, const int* cu_q,
