@@ -562,7 +562,13 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   pdl_wait();
   pdl_launch_dependents();
   const int token = static_cast<int>(row / a.Hq), head = static_cast<int>(row % a.Hq);
-  if (row >= rows || token < a.cu_q[0] || token >= a.cu_q[B]) return;
+  bool there = false;  // in a sequence that has parts; one that was reported has none
+  if (row < rows)
+    for (int b = lane; b < B; b += 32) {
+      const int begin = a.cu_q[b], end = a.cu_q[b + 1];
+      there = there || (begin >= 0 && end <= a.T && token >= begin && token < end);
+    }
+  if (!__any_sync(0xffffffffu, there)) return;
   const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
   const float* p = a.parts + row * (D + kPartTail);
   const int64_t next = rows * (D + kPartTail);
@@ -588,12 +594,12 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
       l += some ? t.y * f : 0.f;
       f *= page_share(t.z, R);
     }
-    const uint32_t there = __ballot_sync(0xffffffffu, some);
+    const uint32_t written = __ballot_sync(0xffffffffu, some);
     const int n = min(32, a.splits - s0);
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
       const float fs = __shfl_sync(0xffffffffu, f, s);
-      const bool in = there >> s & 1;
+      const bool in = written >> s & 1;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const float o = in ? p[(s0 + s) * next + i * 32 + lane] : 0.f;
