@@ -64,7 +64,7 @@ struct Args {
   int64_t out_stride;
   const float* sinks;
   float *lse, *parts;  // log2 of the sums [T, Hq] (null: not wanted); partial results [splits][T * Hq][D + 4]
-  int T, Hq, Hkv, page, max_blocks;
+  int T, max_q_len, Hq, Hkv, page, max_blocks;
   int64_t num_blocks;
   float scale_log2;
   int window, splits;
@@ -281,7 +281,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   // heavy blocks (late queries see the most keys) are scheduled first, of all heads (head by head: 827 us for 806)
   const int q0 = (static_cast<int>(gridDim.x) / a.Hkv - 1 - static_cast<int>(blockIdx.x) / a.Hkv) * 2 * per_unit;
   if (q0 >= L) return;  // uniform for the CTA, before any barrier or allocation
-  if (q_begin < 0 || q_begin > a.T - L) {
+  if (q_begin < 0 || q_begin > a.T - L || L > a.max_q_len) {  // rows that are not there, or more than the grid has CTAs for
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, PXL_DEV_BAD_INDEX);
     return;
   }
@@ -566,7 +566,7 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   if (row < rows)
     for (int b = lane; b < B; b += 32) {
       const int begin = a.cu_q[b], end = a.cu_q[b + 1];
-      there = there || (begin >= 0 && end <= a.T && token >= begin && token < end);
+      there = there || (begin >= 0 && end <= a.T && end - begin <= a.max_q_len && token >= begin && token < end);
     }
   if (!__any_sync(0xffffffffu, there)) return;
   const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
@@ -616,7 +616,7 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
 
 // CTAs that share a block of queries' keys: as many as fill the chip, each with at least four tiles.
 int splits_of(int B, int max_q_len, int Hq, int Hkv, int max_ctx) {
-  const int64_t blocks = static_cast<int64_t>(ceil_div(max_q_len, 2 * (kRowsQ / (Hq / Hkv)))) * Hkv * B;
+  const int64_t blocks = static_cast<int64_t>(ceil_div(max_q_len > 0 ? max_q_len : 1, 2 * (kRowsQ / (Hq / Hkv)))) * Hkv * B;
   const int64_t fill = pxl_host::num_sms() / (blocks > 0 ? blocks : 1), most = max_ctx / (4 * kT);
   const int64_t s = fill < most ? fill : most;
   return s < 1 ? 1 : static_cast<int>(s);
@@ -641,10 +641,9 @@ int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
       return PXL_ERR_CUDA;
     done.store(true, std::memory_order_relaxed);
   }
-  const int per = 2 * (kRowsQ / (a.Hq / a.Hkv));
-  if (static_cast<int64_t>(ceil_div(max_q_len, per)) * a.Hkv > INT32_MAX || a.splits > 65535) return PXL_ERR_TOO_LARGE;
-  pxl_host::launch(attn_i8_prefill_kernel<D>, dim3(ceil_div(max_q_len, per) * a.Hkv, a.splits, B), dim3(kThreads), Shape<D>::kSmem, stream, tq,
-                   tk, tv, a);
+  const int blocks = ceil_div(max_q_len > 0 ? max_q_len : 1, 2 * (kRowsQ / (a.Hq / a.Hkv)));
+  if (static_cast<int64_t>(blocks) * a.Hkv > INT32_MAX || a.splits > 65535) return PXL_ERR_TOO_LARGE;
+  pxl_host::launch(attn_i8_prefill_kernel<D>, dim3(blocks * a.Hkv, a.splits, B), dim3(kThreads), Shape<D>::kSmem, stream, tq, tk, tv, a);
   if (a.splits > 1)
     pxl_host::launch_behind(attn_i8_prefill_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div64(static_cast<int64_t>(a.T) * a.Hq, 4))), dim3(128),
                             0, stream, a, B);
@@ -654,7 +653,7 @@ int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 }  // namespace
 
 PXL_EXPORT int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx) {
-  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len <= 0) return 0;
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len < 0) return 0;
   return Layout(T, B, max_q_len, Hq, Hkv, D, max_ctx).total * 4;
 }
 
@@ -663,11 +662,11 @@ PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* 
                                    const float* sinks, float* lse, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len,
                                    int Hq, int Hkv, int D, int page, int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx,
                                    int* status, cudaStream_t stream) {
-  if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
+  if (T <= 0 || B <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || (out_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
       ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_q_len < 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
       window < 0 || window > (1 << 30) || num_blocks <= 0 ||
       num_blocks * Hkv * page >= (1ll << 31))
     return PXL_ERR_INVALID_ARG;
@@ -680,6 +679,6 @@ PXL_EXPORT int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* 
       !pxl_host::make_tmap_codes(&tv, v_cache, rows, D, page))
     return PXL_ERR_TENSORMAP;
   const Args a{reinterpret_cast<const float2*>(kv_max), block_tables, cu_q, ctx_lens, static_cast<bf16*>(out), out_stride, sinks, lse,
-               static_cast<float*>(workspace), T, Hq, Hkv, page, max_blocks, num_blocks, scale * kLog2e, window, at.splits, status};
+               static_cast<float*>(workspace), T, max_q_len, Hq, Hkv, page, max_blocks, num_blocks, scale * kLog2e, window, at.splits, status};
   return D == 64 ? launch_prefill<64>(tq, tk, tv, a, B, max_q_len, stream) : launch_prefill<128>(tq, tk, tv, a, B, max_q_len, stream);
 }

@@ -49,7 +49,7 @@ struct Args {
   const float* lse;  // log2 of the sums, [T, Hq]
   float *weights, *parts;
   int64_t W;
-  int slots, T, Hq, Hkv, page, max_blocks, max_ctx, splits;
+  int slots, T, max_q_len, Hq, Hkv, page, max_blocks, max_ctx, splits;
   int64_t num_blocks;
   float scale_log2;
   int window;
@@ -82,7 +82,8 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin, ctx = a.ctx_lens[b], slot = a.seq_slots ? a.seq_slots[b] : b;
   const int per_unit = kCols / G;
   const int key0 = blockIdx.x * kKeys, pos0 = ctx - L;  // position of the first query
-  if (L <= 0 || key0 >= ctx || q_begin < 0 || q_begin > a.T - L) return;  // uniform for the CTA, before any barrier or allocation
+  // uniform for the CTA, before any barrier or allocation; of a sequence that the attention reported there are no logarithms
+  if (L <= 0 || key0 >= ctx || q_begin < 0 || q_begin > a.T - L || L > a.max_q_len) return;
   if (slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) {
     if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, slot < 0 || slot >= a.slots ? PXL_DEV_BAD_SLOT : PXL_DEV_BAD_INDEX);
     return;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(256) attn_i8_weigh_join_kernel(const __grid_co
   pdl_launch_dependents();
   const int b = blockIdx.z, h = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x, ctx = a.ctx_lens[b], slot = a.seq_slots ? a.seq_slots[b] : b;
   const int q_begin = a.cu_q[b], L = a.cu_q[b + 1] - q_begin;
-  if (t >= ctx || L <= 0 || q_begin < 0 || q_begin > a.T - L || slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) return;
+  if (t >= ctx || L <= 0 || q_begin < 0 || q_begin > a.T - L || L > a.max_q_len || slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) return;
   float sum = 0.f;
   for (int s = 0; s < a.splits; ++s) sum += a.parts[((static_cast<int64_t>(s) * gridDim.z + b) * a.Hkv + h) * a.max_ctx + t];
   a.weights[(static_cast<int64_t>(slot) * a.Hkv + h) * a.W + t] += sum;
@@ -311,7 +312,7 @@ int launch_weigh(const CUtensorMap& tq, const Args& a, int B, cudaStream_t strea
 }  // namespace
 
 PXL_EXPORT int64_t pxl_attn_i8_weigh_workspace(int B, int max_q_len, int Hq, int Hkv, int max_ctx) {
-  if (B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len <= 0 || max_ctx <= 0) return 0;
+  if (B <= 0 || Hkv <= 0 || Hq < Hkv || max_q_len < 0 || max_ctx <= 0) return 0;
   const int s = splits_of(B, max_q_len, Hq, Hkv, max_ctx);
   return s > 1 ? static_cast<int64_t>(s) * B * Hkv * max_ctx * 4 : 0;
 }
@@ -321,10 +322,10 @@ PXL_EXPORT int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_
                                  const int* seq_slots, void* workspace, int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv,
                                  int D, int page, int max_blocks, int64_t num_blocks, float scale, int window, int max_ctx, int* status,
                                  cudaStream_t stream) {
-  if (T <= 0 || B <= 0 || max_q_len <= 0) return PXL_OK;
+  if (T <= 0 || B <= 0) return PXL_OK;
   if ((D != 64 && D != 128) || (page != 16 && page != 32 && page != 64) || Hkv <= 0 || Hq % Hkv || Hq / Hkv < 1 || Hq / Hkv > 16 ||
       !(scale > 0.f) || (q_stride & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache)) & 15) ||
-      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
+      (reinterpret_cast<uintptr_t>(kv_max) & 7) || max_blocks <= 0 || max_q_len < 0 || max_ctx <= 0 || max_ctx >= (1 << 30) ||
       window < 0 || window > (1 << 30) || num_blocks <= 0 ||
       !lse || !weights)
     return PXL_ERR_INVALID_ARG;
@@ -335,7 +336,7 @@ PXL_EXPORT int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_
   CUtensorMap tq;
   if (!pxl_host::make_tmap_queries(&tq, q, q_stride, T, Hq, D, Hq / Hkv)) return PXL_ERR_TENSORMAP;
   const Args a{static_cast<const int8_t*>(k_cache), reinterpret_cast<const float2*>(kv_max), block_tables, cu_q, ctx_lens, seq_slots, lse,
-               weights, static_cast<float*>(workspace), W, slots, T, Hq, Hkv, page, max_blocks, max_ctx, splits, num_blocks, scale * kLog2e,
+               weights, static_cast<float*>(workspace), W, slots, T, max_q_len, Hq, Hkv, page, max_blocks, max_ctx, splits, num_blocks, scale * kLog2e,
                window, status};
   return D == 64 ? launch_weigh<64>(tq, a, B, stream) : launch_weigh<128>(tq, a, B, stream);
 }

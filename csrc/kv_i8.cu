@@ -93,8 +93,8 @@ template <int D, int ROWS, int HALF>
 __global__ void __launch_bounds__(2 * HALF, D == 128 && ROWS == 64 ? 4 : 0)
 store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t k_stride, int64_t v_stride,
                    const int* __restrict__ block_tables, const int* __restrict__ cu_q, const int* __restrict__ ctx_lens,
-                   int8_t* __restrict__ k_cache, int8_t* __restrict__ v_cache, float* __restrict__ kv_max, int T, int Hkv, int page,
-                   int max_blocks, int64_t num_blocks, int* status) {
+                   int8_t* __restrict__ k_cache, int8_t* __restrict__ v_cache, float* __restrict__ kv_max, int T, int max_q_len, int Hkv,
+                   int page, int max_blocks, int64_t num_blocks, int* status) {
   constexpr int C = D / 8, kSteps = ceil_div(ROWS * C, HALF);  // chunks of 8 values in a row; of a thread
   pdl_wait();
   pdl_launch_dependents();
@@ -102,6 +102,10 @@ store_kv_i8_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64
   const int row0 = cu_q[b], n = cu_q[b + 1] - row0, t = ctx_lens[b];
   const int begin = t - n, from = begin > 0 ? begin : 0;
   const int p = from / page + static_cast<int>(blockIdx.x);
+  if (n > max_q_len) {  // the grid has no CTAs for all its pages: none of them
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0 && status) atomicCAS(status, 0, PXL_DEV_BAD_INDEX);
+    return;
+  }
   if (n <= 0 || t <= 0 || p > (t - 1) / page) return;
   const int lo = from > p * page ? from - p * page : 0, hi = min(page, t - p * page), rows = hi - lo;
   const int first = row0 + p * page + lo - begin;  // row of token lo of the page
@@ -460,19 +464,19 @@ int done() { return cudaGetLastError() == cudaSuccess ? PXL_OK : PXL_ERR_CUDA; }
 PXL_EXPORT int pxl_kv_i8_store(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int* block_tables, const int* cu_q,
                                const int* ctx_lens, void* k_cache, void* v_cache, float* kv_max, int T, int B, int max_q_len, int Hkv, int D,
                                int page, int max_blocks, int64_t num_blocks, int* status, cudaStream_t stream) {
-  if (B <= 0 || T <= 0 || max_q_len <= 0) return PXL_OK;
-  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || Hkv > 65535 || (k_stride & 7) || (v_stride & 7) ||
+  if (B <= 0 || T <= 0) return PXL_OK;
+  if (!cache_ok(Hkv, D, page, max_blocks, num_blocks, k_cache, v_cache) || max_q_len < 0 || Hkv > 65535 || (k_stride & 7) || (v_stride & 7) ||
       ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15))
     return PXL_ERR_INVALID_ARG;
   if (B > 65535) return PXL_ERR_TOO_LARGE;
   const dim3 grid((max_q_len + page - 2) / page + 1, Hkv, B);
   auto go = [&](auto kernel, int threads) {
     pxl_host::launch(kernel, grid, dim3(threads), 0, stream, static_cast<const bf16*>(k), static_cast<const bf16*>(v), k_stride, v_stride,
-                     block_tables, cu_q, ctx_lens, static_cast<int8_t*>(k_cache), static_cast<int8_t*>(v_cache), kv_max, T, Hkv, page,
-                     max_blocks, num_blocks, status);
+                     block_tables, cu_q, ctx_lens, static_cast<int8_t*>(k_cache), static_cast<int8_t*>(v_cache), kv_max, T, max_q_len, Hkv,
+                     page, max_blocks, num_blocks, status);
     return done();
   };
-  if (max_q_len == 1) return D == 64 ? go(store_kv_i8_kernel<64, 1, 32>, 64) : go(store_kv_i8_kernel<128, 1, 32>, 64);
+  if (max_q_len <= 1) return D == 64 ? go(store_kv_i8_kernel<64, 1, 32>, 64) : go(store_kv_i8_kernel<128, 1, 32>, 64);
   if (D == 64)
     return page == 16   ? go(store_kv_i8_kernel<64, 16, 64>, 128)
            : page == 32 ? go(store_kv_i8_kernel<64, 32, 128>, 256)

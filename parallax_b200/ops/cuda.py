@@ -1225,7 +1225,7 @@ def _head_rows(x: torch.Tensor) -> torch.Tensor:
 def store_kv_i8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_max: torch.Tensor,
                 block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_lens: torch.Tensor, max_q_len: int) -> None:
     N, Hkv, page, D, T, B, MB = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
-    if B == 0 or T == 0 or max_q_len == 0:
+    if B == 0 or T == 0:
         return
     k, v, dev = _head_rows(k), _head_rows(v), k_cache.device
     with _on(dev):
@@ -1258,7 +1258,7 @@ def _attn_i8(what, q, cache, block_tables, cu_q, ctx_lens, max_q_len, scale, win
     dev = q.device
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
-    if T == 0 or B == 0 or max_q_len <= 0:
+    if T == 0 or B == 0:
         return out
     q, max_q_len = _head_rows(q), min(max_q_len, T)
     k_cache, v_cache, kv_max = cache
@@ -1308,6 +1308,8 @@ def attn_prefill_i8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     weights: Optional[torch.Tensor] = None, seq_slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     if cu_q is None:
         kv_i8.refuse("attn_prefill_i8", "cu_q is int32 [sequences + 1]")
+    if max_q_len < 0:
+        kv_i8.refuse("attn_prefill_i8", f"max_q_len is not negative, got {max_q_len}")
     return _attn_i8("attn_prefill_i8", q, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len, scale, window, sinks, max_ctx,
                     out, weights, seq_slots)
 

@@ -661,11 +661,19 @@ def _kv_i8_sequence(k_cache, v_cache, kv_max, table, n):
     return [(c[blocks].float() * scale[..., j, None, None]).transpose(0, 1).flatten(1, 2)[:, :n] for j, c in enumerate((k_cache, v_cache))]
 
 
+def _kv_i8_new_tokens(what, cu_q, max_q_len):
+    """Refuses sequences with more new tokens than the call says; the kernels leave them out and report them."""
+    most = int((cu_q[1:] - cu_q[:-1]).amax()) if cu_q.shape[0] > 1 else 0
+    if most > max_q_len:
+        kv_i8.refuse(what, f"at most max_q_len = {max_q_len} new tokens of each sequence, got {most}")
+
+
 def store_kv_i8(k, v, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, max_q_len):
     """Writes the new tokens' keys and values ``[T, heads, D]`` into an 8-bit cache (see :mod:`.kv_i8`): rows ``cu_q[b]`` to ``cu_q[b + 1]``
-    are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each. The pages that are written belong to one
-    sequence each; what a page holds behind the last token stays."""
+    are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each (one with more is reported and not written).
+    The pages that are written belong to one sequence each; what a page holds behind the last token stays."""
     _, Hkv, page, D, _, B, _ = kv_i8.check_store("store_kv_i8", k, v, (k_cache, v_cache, kv_max), block_tables, cu_q, ctx_lens, max_q_len)
+    _kv_i8_new_tokens("store_kv_i8", cu_q, max_q_len)
     for b in range(B):
         row, n, t = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b]), int(ctx_lens[b])
         for p in range((t - n) // page, (t - 1) // page + 1) if n > 0 else ():
@@ -734,9 +742,15 @@ def attn_prefill_i8(q, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, m
                     weights=None, seq_slots=None):
     """The queries of new tokens, ``q [T, Hq, D]``, over an 8-bit cache that holds their keys and values already: rows ``cu_q[b]`` to
     ``cu_q[b + 1]`` are the last of the ``ctx_lens[b]`` tokens of sequence b, at most ``max_q_len`` of each, and see the tokens up to their
-    own. The other arguments are those of ``attn_decode_i8``; rows behind the last sequence stay as they are."""
+    own. The other arguments are those of ``attn_decode_i8``; rows behind the last sequence stay as they are, and so do rows and weights of
+    a sequence that is reported: one with more new tokens than ``max_q_len``, or with rows that are not there."""
     cache = (k_cache, v_cache, kv_max)
+    if cu_q is None:
+        kv_i8.refuse("attn_prefill_i8", "cu_q is int32 [sequences + 1]")
+    if max_q_len < 0:
+        kv_i8.refuse("attn_prefill_i8", f"max_q_len is not negative, got {max_q_len}")
     kv_i8.check_attention("attn_prefill_i8", q, cache, block_tables, cu_q, ctx_lens, scale, window, sinks, out, weights, seq_slots, max_ctx)
+    _kv_i8_new_tokens("attn_prefill_i8", cu_q, max_q_len)
     res = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if out is None else out
     for b in range(ctx_lens.shape[0]):
         lo, hi, t = int(cu_q[b]), int(cu_q[b + 1]), int(ctx_lens[b])

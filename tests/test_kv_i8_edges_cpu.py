@@ -24,3 +24,55 @@ def test_magnitudes_that_start_on_no_8_bytes_are_refused(D, page):
     tail = (2, D, page, 4, 64, None, None)
     assert lib.pxl_kv_i8_load(P, P, P + 4, P, P, P, P, 3, 1, *tail) == INVALID_ARG
     assert lib.pxl_kv_i8_evict(P, P, P + 4, P, 64, 1, None, P, P, P, P, P, 1, 2, D, page, 4, 2, 64, 30, 2, 2, None, None) == INVALID_ARG
+
+
+# ------------------------------------------------------------------------------------------------ more new tokens than a call says
+@pytest.mark.parametrize("most", [0, 4])
+def test_more_new_tokens_than_the_call_says_are_refused(most):
+    """The forms that know the lengths when they are called refuse them before anything is written; the kernels report them."""
+    g = torch.Generator().manual_seed(1)
+    cache = oracle.make_cache(g, 4, 2, 16, 64)
+    before = [c.clone() for c in cache]
+    tab, ends, lens = torch.tensor([[0], [1]]).int(), torch.tensor([0, 2, 7]).int(), torch.tensor([9, 5]).int()
+    x = torch.randn(7, 2, 64, generator=g).bfloat16()
+    with pytest.raises(KernelError, match="max_q_len"):
+        ops.store_kv_i8(x, x, *cache, tab, ends, lens, most)
+    assert all(torch.equal(a, b) for a, b in zip(cache, before))
+    weights, out = torch.zeros(2, 2, 16), torch.full((7, 2, 64), 7.0).bfloat16()
+    with pytest.raises(KernelError, match="max_q_len"):
+        ops.attn_prefill_i8(x, *cache, tab, ends, lens, most, 0.1, out=out, weights=weights)
+    assert (weights == 0).all() and (out == 7).all()
+    with pytest.raises(KernelError, match="max_q_len"):
+        ops.attn_prefill_i8(x, *cache, tab, ends, lens, -1, 0.1)
+
+
+def test_calls_that_allow_no_new_tokens_reach_the_library(monkeypatch):
+    """Sequences that have some all the same are reported there."""
+    import contextlib
+
+    calls = []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return lambda *args: calls.append(name) or 0
+
+    monkeypatch.setattr(_lib, "lib", lambda: Recorder())
+    monkeypatch.setattr(cu, "_on", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(cu, "_stream", lambda device: 0)
+    monkeypatch.setattr(cu, "status_tensor", lambda device: torch.zeros(1, dtype=torch.int32))
+    cache = oracle.make_cache(torch.Generator().manual_seed(2), 4, 2, 16, 64)
+    x, tab, ends, lens = torch.zeros(3, 2, 64).bfloat16(), torch.zeros(1, 1).int(), torch.tensor([0, 3]).int(), torch.tensor([5]).int()
+    cu.store_kv_i8(x, x, *cache, tab, ends, lens, 0)
+    cu.attn_prefill_i8(x, *cache, tab, ends, lens, 0, 0.1)
+    assert "pxl_kv_i8_store" in calls and "pxl_attn_i8_prefill" in calls
+    with pytest.raises(KernelError, match="max_q_len"):
+        cu.attn_prefill_i8(x, *cache, tab, ends, lens, -1, 0.1)
+
+
+def test_a_negative_number_of_new_tokens_is_refused_by_the_library():
+    lib = _library()
+    sizes = (4, 2, 64, 16, 8, 8, 0.1, 0, 100, None, None)
+    assert lib.pxl_kv_i8_store(P, P, 128, 128, P, P, P, P, P, P, 3, 1, -1, 2, 64, 16, 4, 4, None, None) == INVALID_ARG
+    assert lib.pxl_attn_i8_prefill(P, 256, P, P, P, P, P, P, P, 256, None, None, P, 1 << 30, 2, 1, -1, *sizes) == INVALID_ARG
+    assert lib.pxl_attn_i8_weigh(P, 256, P, P, P, P, P, P, P, 100, 1, None, P, 1 << 30, 2, 1, -1, *sizes) == INVALID_ARG
+    assert lib.pxl_attn_i8_prefill_workspace(3, 1, 0, 4, 2, 64, 4096) >= lib.pxl_attn_i8_prefill_workspace(3, 1, 1, 4, 2, 64, 4096) > 0

@@ -72,3 +72,49 @@ def test_ends_off_the_queries_of_long_sequences(ends):
         assert abs(float(weights[s].sum()) - (0 if b != s else 2 * (ends[s + 1] - ends[s]))) < 1e-2
     for r in range(2):
         assert bool((out[r] == 7).all()) == (b is None or not ends[b] <= r < ends[b + 1])
+
+
+# ------------------------------------------------------------------------------------------------ more new tokens than a call says
+@pytest.mark.parametrize("ctx", [60, 4000])
+@pytest.mark.parametrize("G", [2, 16])
+def test_prompts_of_more_new_tokens_than_the_call_says(ctx, G):
+    """Reported and left out, by the outputs and by the weights; the sequence beside them is not touched by that. 4000 tokens: keys are
+    split over CTAs."""
+    g = _gen(1)
+    new, D = [40, 3], 64
+    blocks = 2 * -(-ctx // 16)
+    cache = oracle.make_cache(g, blocks, 1, 16, D)
+    tables = oracle.tables_for(g, [ctx, ctx], 16, blocks)
+    q = torch.randn(43, G, D, generator=g).bfloat16()
+    before = torch.rand(2, 1, ctx, generator=g)
+    d = _dev(q, *cache, tables, _cu(new), _i32([ctx, ctx]), before)
+    out = torch.full((43, G, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.attn_prefill_i8(*d[:7], 39, 0.1, out=out, weights=d[7])
+    _reported("index")
+    (_, _, _, _), (o, mean, add, size) = oracle.attention(q, cache, tables, new, [ctx, ctx], 0.1)
+    assert (out[:40] == 7).all() and torch.equal(d[7][0].cpu(), before[0])
+    oracle.assert_output(out[40:].cpu(), o, mean, size)
+    oracle.assert_weights(d[7][1].cpu(), before[1].double() + add, before[1], size, 3)
+    ops.attn_prefill_i8(*d[:7], 0, 0.1, out=out, weights=d[7])
+    _reported("index")
+    assert (out[:40] == 7).all()
+    ops.attn_prefill_i8(*d[:7], 40, 0.1, out=out)
+    _check()
+    assert not (out[:40] == 7).all()
+
+
+@pytest.mark.parametrize("most", [0, 1, 16, 39])
+@pytest.mark.parametrize("page", [16, 64])
+def test_store_of_more_new_tokens_than_the_call_says(most, page):
+    g = _gen(2)
+    cache = _dev(*oracle.make_cache(g, 12, 2, page, 64))
+    tables = oracle.tables_for(g, [70, 50], page, 12).to(DEV)
+    x = torch.randn(40 + most, 4, 64, generator=g).bfloat16().to(DEV)
+    want = [c.clone() for c in cache]
+    ends, lens = _dev(_i32([0, 40, 40 + most]), _i32([70, 50]))
+    if most > 0:
+        ops.store_kv_i8(x[40:, :2], x[40:, 2:], *want, tables[1:], _i32([0, most]).to(DEV), lens[1:], most)
+    _check()
+    ops.store_kv_i8(x[:, :2], x[:, 2:], *cache, tables, ends, lens, most)
+    _reported("index")
+    assert all(torch.equal(a, b) for a, b in zip(cache, want))
