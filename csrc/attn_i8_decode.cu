@@ -102,6 +102,7 @@ struct Rows {
   static constexpr int kKeys = 32, kSteps = D / 16;
   uint32_t qf[NH][kSteps][2];
   float row_scale[NH][2], o[NH][D / 16][4], m_run[NH][2], l_run[NH][2], r_run, log_r;
+  bool none;  // values without a magnitude were seen
 
   // byte offset of 16-byte chunk c of a row of a tile as TMA lays it down
   static __device__ __forceinline__ uint32_t chunk(int row, int c) {
@@ -142,6 +143,7 @@ struct Rows {
     }
     r_run = 0.f;
     log_r = -INFINITY;
+    none = false;
   }
 
   // Keys r0 .. r0 + 31 of a tile; the first is token tok_base. near, far: magnitudes of the pages of its first and second 16. scores: where
@@ -188,8 +190,9 @@ struct Rows {
             for (int e = 0; e < 2; ++e) s[n][k][2 * r + e] = out[k][r] ? -INFINITY : s[n][k][2 * r + e];
         }
     }
-    // R, of pages that have a token which is seen (a NaN is passed over); the maxima
-    const float most = fmaxf(tok_base + 16 > lo ? near.y : 0.f, tok_base + 16 < hi ? far.y : 0.f);
+    // R, of pages that have a token which is seen (a NaN is passed over: it is for the output, not for the sum); the maxima
+    const float near_y = tok_base + 16 > lo ? near.y : 0.f, far_y = tok_base + 16 < hi ? far.y : 0.f, most = fmaxf(near_y, far_y);
+    none = none || near_y + far_y != near_y + far_y;
     float mx[NH][2];
     bool grow = most > r_run;
 #pragma unroll
@@ -403,6 +406,12 @@ attn_i8_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         if (lane == 0) mbar_arrive(empty0 + 8 * stage);
       }
 
+      if (rows.none) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) rows.o[n][i][0] = rows.o[n][i][1] = rows.o[n][i][2] = rows.o[n][i][3] = NAN;
+      }
       // The four warps' results, each of some keys, become a quarter of the columns of all keys each: half of them change hands with the warp
       // that had the other tiles, half of the rest with the one that had the other 32 keys of these. A warp writes its second gift where it
       // has read the first one.

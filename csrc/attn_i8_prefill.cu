@@ -71,7 +71,7 @@ struct Args {
   int* status;
 };
 
-// What a row's keys gave: maximum (log2), sum, output in units of R times 2^kUp.
+// What a row's keys gave: output in units of R times 2^kUp, maximum (log2), sum, R, whether it saw values without a magnitude.
 constexpr int kPartTail = 4;
 
 // V tile as B operand of all its columns: 64-column chunks kHalf apart
@@ -269,9 +269,10 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t q_full = smem_u32(bars), q_ready = q_full + 8, codes_full = q_full + 16, codes_empty = codes_full + 8 * S::kStages,
                  kv_full = codes_empty + 8 * S::kStages, kv_empty = kv_full + 8 * S::kSlots, s_full = kv_empty + 8 * S::kSlots,
                  o_full = s_full + 16, p_ready = o_full + 16;
-  static_assert((2 + 2 * S::kStages + 2 * S::kSlots + 8) * 8 + 8 <= 256);
+  static_assert((2 + 2 * S::kStages + 2 * S::kSlots + 8) * 8 + 12 <= 256);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 + 2 * S::kStages + 2 * S::kSlots + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* none_flag = abort_flag + 1;  // some page's values have no magnitude
   pdl_wait();
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -294,7 +295,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const int n_tiles = __shfl_sync(0xffffffffu, min(t_each, t_first + t_all - t_begin), 0);
 
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
+    *abort_flag = *none_flag = 0;
     const int ppt = kT / a.page;
     mbar_init(q_full, 1);
     mbar_init(q_ready, 4 * units);
@@ -383,7 +384,9 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
             if (m > r_all) r_all = fminf(2.f * m, 3.3e38f);
             if (lane < ppt) {
-              const float share = most.y == most.y ? fmaxf(page_share(most.y, r_all), 0x1p-40f) : most.y;
+              // (any share does for values without a magnitude: the sum of exponentials depends on the keys alone)
+              const float share = most.y == most.y ? fmaxf(page_share(most.y, r_all), 0x1p-40f) : 1.f;
+              if (most.y != most.y) *none_flag = 1;
               pages_sm[(it % kRing) * 8 + lane] = make_float4(most.x * kInv127, __log2f(share) + kUp, __fdividef(0x1p-7f, share), r_all);
               mbar_arrive(bar);
             }
@@ -495,13 +498,23 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
       if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);
+      bool none = false;  // the row sees values without a magnitude: its output is no number. Looked up here, and not tile by tile: a
+                          // register more in the loop is a tenth of the time
+      if (!failed && n_tiles > 0 && *none_flag) {
+        const int end = min(q_pos, (t_begin + n_tiles) * kT - 1);
+        for (int p = max(key_lo, t_begin * kT) / a.page; p < a.max_blocks && p * a.page <= end; ++p) {
+          const int blk = a.block_tables[static_cast<size_t>(b) * a.max_blocks + p];
+          const float m = blk >= 0 && blk < a.num_blocks ? a.kv_max[blk * a.Hkv + kvh].y : 0.f;
+          none = none || m != m;
+        }
+      }
       const int64_t row = static_cast<int64_t>(q_begin + q0 + tok) * a.Hq + head;
       if (!failed && a.splits == 1) {
         const float sink = a.sinks && valid ? a.sinks[head] * kLog2e : -INFINITY;
         const float M = fmaxf(m_run, sink), Mu = M == -INFINITY ? 0.f : M, f = fast_exp2(m_run - Mu);
         const float denom = l_run * f + fast_exp2(sink - Mu);
         if (a.lse && valid) a.lse[row] = denom == 0.f ? INFINITY : Mu + log2f(denom);
-        const float inv = denom == 0.f ? 0.f : f / denom * (r_run * (kInv127 * 0x1p-7f));
+        const float inv = none ? NAN : denom == 0.f ? 0.f : f / denom * (r_run * (kInv127 * 0x1p-7f));
         bf16* dst = a.out + static_cast<int64_t>(q_begin + q0 + tok) * a.out_stride + head * D;
         if (n_tiles > 0) tc_fence_after_sync();
 #pragma unroll
@@ -526,7 +539,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
       } else if (!failed) {
         float* po = a.parts + (split * static_cast<int64_t>(a.T) * a.Hq + row) * (D + kPartTail);
-        if (valid) *reinterpret_cast<float4*>(po + D) = make_float4(m_run, l_run, r_run, 0.f);
+        if (valid) *reinterpret_cast<float4*>(po + D) = make_float4(m_run, l_run, r_run, none ? 1.f : 0.f);
         if (n_tiles > 0) {
           tc_fence_after_sync();
 #pragma unroll
@@ -573,8 +586,10 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   const float* p = a.parts + row * (D + kPartTail);
   const int64_t next = rows * (D + kPartTail);
   float M = -INFINITY, R = 0.f;
+  bool none = false;
   for (int s = lane; s < a.splits; s += 32) {
     const float4 t = *reinterpret_cast<const float4*>(p + s * next + D);
+    none = none || t.w != 0.f;
     M = fmaxf(M, t.x);
     R = fmaxf(R, t.z);
   }
@@ -609,7 +624,7 @@ attn_i8_prefill_join_kernel(const __grid_constant__ Args a, int B) {
   }
   l = warp_reduce_sum(l) + fast_exp2(sink - Mu);
   if (a.lse && lane == 0) a.lse[row] = l == 0.f ? INFINITY : Mu + log2f(l);
-  const float inv = l == 0.f ? 0.f : R * (kInv127 * 0x1p-7f) / l;
+  const float inv = __any_sync(0xffffffffu, none) ? NAN : l == 0.f ? 0.f : R * (kInv127 * 0x1p-7f) / l;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) a.out[token * a.out_stride + head * D + i * 32 + lane] = __float2bfloat16(acc[i] * inv);
 }

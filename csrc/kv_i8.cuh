@@ -36,14 +36,15 @@ __device__ __forceinline__ float row_up(float most, float& down) {
 }
 constexpr float kInv127 = 1.f / 127.f;
 
-// share of a page's magnitude in the largest so far; 0 for a page of zeros, NaN for one without a magnitude
+// share of a magnitude in the largest so far; 0 of none
 __device__ __forceinline__ float page_share(float m, float most) {
   if (most > 1e-30f && most < 1e30f) return __fdividef(m, most);  // (which is 0 for a divisor above 2^126)
   return m == 0.f ? 0.f : __fdiv_rn(m, most);
 }
 
-// log2 of that, from log2 of the largest; not below -40 (whose values are lost beside the others'), NaN without a magnitude
-__device__ __forceinline__ float page_log(float m, float log_most) { return m == m ? fmaxf(__log2f(m) - log_most, -40.f) : m; }
+// log2 of that, from log2 of the largest; not below -40 (whose values are lost beside the others'); 0 without a magnitude, so that the sums
+// of exponentials, and the weights with them, depend on the keys alone
+__device__ __forceinline__ float page_log(float m, float log_most) { return m == m ? fmaxf(__log2f(m) - log_most, -40.f) : 0.f; }
 
 }  // namespace pxl
 

@@ -118,3 +118,65 @@ def test_store_of_more_new_tokens_than_the_call_says(most, page):
     ops.store_kv_i8(x[:, :2], x[:, 2:], *cache, tables, ends, lens, most)
     _reported("index")
     assert all(torch.equal(a, b) for a, b in zip(cache, want))
+
+
+# ------------------------------------------------------------------------------------------------ pages without a magnitude
+FORMS = [([1] * 3, [2048, 1500, 31], 4),                  # single queries: a cluster for each pair
+         ([1] * 12, [2049] + [300] * 11, 8),              # pairs dealt out
+         ([1] * 40, [200] * 40, 2),                       # pairs left whole
+         ([300, 17], [1000, 17], 2),                      # prompts
+         ([37], [2100], 2)]                               # keys split over CTAs
+
+
+@pytest.mark.parametrize("new,ctx,heads", FORMS)
+@pytest.mark.parametrize("page,D,G", [(16, 128, 4), (64, 64, 9), (32, 64, 1)])
+@pytest.mark.parametrize("window", [0, 150])
+def test_values_without_a_magnitude_leave_the_weights_as_they_should_be(new, ctx, heads, page, D, G, window):
+    """What a token got depends on keys alone: outputs are no numbers for those who see it, weights and the other outputs are right."""
+    g = _gen(4)
+    blocks = sum(-(-t // page) for t in ctx)
+    cache = oracle.make_cache(g, blocks, heads, page, D)
+    tables = oracle.tables_for(g, ctx, page, blocks)
+    for b, t in enumerate(ctx):                            # a page in the middle of head 0's, the last one of head 1's
+        if b % 3 < 2:
+            cache[2][int(tables[b, (t - 1) // 2 // page]), 0, 1] = math.nan
+            cache[2][int(tables[b, (t - 1) // page]), 1, 1] = math.nan
+    q = torch.randn(sum(new), G * heads, D, generator=g).bfloat16()
+    weights, scale = torch.rand(len(ctx), heads, max(ctx), generator=g), D ** -0.5
+    out, w = _attend(q, cache, tables, new, ctx, scale, window, weights=weights, max_ctx=max(ctx))
+    row = 0
+    for b, (o, mean, add, size) in enumerate(oracle.attention(q, cache, tables, new, ctx, scale, window)):
+        assert torch.isfinite(add).all() and (b % 3 == 2 or torch.isnan(o).any())
+        oracle.assert_output(out[row:row + new[b]], o, mean, size)
+        want = weights[b].double()
+        want[:, :ctx[b]] += add
+        oracle.assert_weights(w[b], want, weights[b], size, new[b])
+        row += new[b]
+
+
+@pytest.mark.parametrize("new,ctx,heads", FORMS)
+def test_keys_without_a_magnitude(new, ctx, heads):
+    """Scores that are no numbers: neither outputs nor weights are numbers for those who see the page, all others are right."""
+    g = _gen(5)
+    blocks = sum(-(-t // 16) for t in ctx)
+    cache = oracle.make_cache(g, blocks, heads, 16, 64)
+    tables = oracle.tables_for(g, ctx, 16, blocks)
+    cache[2][int(tables[0, ctx[0] // 2 // 16]), 0, 0] = math.nan
+    q = torch.randn(sum(new), 4 * heads, 64, generator=g).bfloat16()
+    weights = torch.rand(len(ctx), heads, max(ctx), generator=g)
+    out, w = _attend(q, cache, tables, new, ctx, 0.125, weights=weights, max_ctx=max(ctx))
+    whole = [c.clone() for c in cache]
+    whole[2][int(tables[0, ctx[0] // 2 // 16]), 0, 0] = 1.0
+    row = 0
+    first = ctx[0] // 2 // 16 * 16 - (ctx[0] - new[0])     # the first query of sequence 0 that sees the page
+    for b, (o, mean, add, size) in enumerate(oracle.attention(q, whole, tables, new, ctx, 0.125)):
+        if b == 0:
+            o[max(first, 0):, :4] = math.nan
+            assert torch.isnan(w[0, 0, :ctx[0]]).all()
+        oracle.assert_output(out[row:row + new[b]], o, mean, size)
+        want = weights[b].double()
+        want[:, :ctx[b]] += add
+        for h in range(heads):
+            if b or h:
+                oracle.assert_weights(w[b, h], want[h], weights[b, h], size, new[b])
+        row += new[b]
