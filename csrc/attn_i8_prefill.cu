@@ -14,7 +14,8 @@
 // magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R, so
 // that what is rounded to f16 is the probability times the share (2^-11 of it, down to 2^-21 of the row's largest; 2^-32 below), and the
 // sum of a page's 16 columns is divided by the share again. Both the reference maximum (by 2^8) and R are let run ahead before O in tensor
-// memory is rescaled.
+// memory is rescaled. R is one for the CTA, unless that is more than 16 times what a row has seen of its own (a page that only others see is far
+// above the rest): then the row keeps one for itself.
 // 8111 tokens, 32 heads, D = 128, twice: 726 us, 0.96 PFLOP/s. A tile takes 4400 clocks for both units, the chain of one unit's: product 550,
 // softmax 2700, notice and issue 1000; the tensor pipe is 41 % full. Two units of 128 rows for one conversion: with one the converting warps
 // would take as long as the softmax. (Heads of 64: CTAs of one unit, two on an SM, take longer too, 288 us for 239 of 5 x 3001 tokens with
@@ -50,7 +51,8 @@ struct Shape {
   static constexpr int kOffKV = 2 * kTile;             // behind the two units of Q
   static constexpr int kOffCodes = kOffKV + kSlots * kTile;
   static constexpr int kOffPages = kOffCodes + kStages * kCodes;  // [kRing][8] float4
-  static constexpr int kOffBars = kOffPages + kRing * 8 * 16;
+  static constexpr int kOffMags = kOffPages + kRing * 8 * 16;     // [kRing][8] magnitudes of values
+  static constexpr int kOffBars = kOffMags + kRing * 8 * 4;
   static constexpr int kSmem = 1024 + kOffBars + 256;
   static constexpr uint32_t kIdescS = umma_idesc(kRowsQ, kT, 0, 0);
   static constexpr uint32_t kIdescPV = umma_idesc(kRowsQ, D, 0, 0) | (1u << 16);  // B (V) is MN-major
@@ -161,16 +163,127 @@ struct Seen {
   }
 };
 
+// What the softmax knows of a row so far: maximum (log2), R, sum of exponentials.
+struct RowState {
+  float m_run = -INFINITY, r_run = 0.f, l_run = 0.f;
+};
+
+// O in tensor memory for another maximum and another R.
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t my_o, float m_new, float r_new, RowState& row) {
+  const float grown = fast_exp2(row.m_run - (m_new == -INFINITY ? 0.f : m_new)), corr = grown * (r_new == row.r_run ? 1.f : page_share(row.r_run, r_new));
+  row.m_run = m_new;
+  row.r_run = r_new;
+  row.l_run *= grown;
+#pragma unroll
+  for (int c = 0; c < D; c += 16) {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(my_o + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
+    tmem_st_32x32b_x16(my_o + c, v);
+  }
+}
+
+// R of a row for a tile of which it sees the columns [from, to): that of the CTA, unless it is more than 16 times the largest magnitude the row
+// sees there. One that was taken once is never too large later on, since what a row has seen only grows.
+__device__ __forceinline__ float row_share(int from, int to, float r_all, const float* mags, int shift, float r_run) {
+  float top = 0.f;
+  bool sees = false;
+#pragma unroll
+  for (int g = 0; g < 8; ++g)
+    if (to > g * 16 && from < g * 16 + 16) {
+      sees = true;
+      top = fmaxf(top, mags[g >> shift]);
+    }
+  if (!sees) return r_run;
+  return r_all == r_run || r_all <= 16.f * top ? r_all : top > r_run ? fminf(2.f * top, 3.3e38f) : r_run;
+}
+
+// One tile, as below, of rows that have an R of their own among them; 32 columns at a time, for it is not called where values are alike.
+template <int D>
+__device__ __noinline__ RowState softmax_apart(uint32_t my_s, uint32_t my_o, bool first, int from, int to, float row_scale, const float4* pages,
+                                               const float* mags, int shift, RowState row, uint32_t p_ready) {
+  const float r_new = row_share(from, to, pages[0].w, mags, shift, row.r_run);
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kT; c += 16) {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(my_s + c, v);
+    tmem_ld_wait();
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + j >= from && c + j < to) m = fmaxf(m, __uint_as_float(v[j]));
+    mx = fmaxf(mx, m * (pages[c >> 4 >> shift].x * row_scale));
+  }
+  const float m_new = fmaxf(row.m_run, mx);
+  if (first) {
+    row.m_run = m_new;
+    row.r_run = r_new;
+  } else if (__any_sync(0xffffffffu, m_new > row.m_run + 8.f || r_new != row.r_run)) {
+    rescale<D>(my_o, m_new, r_new, row);
+  }
+  const float m_use = row.m_run == -INFINITY ? 0.f : row.m_run, log_r = __log2f(row.r_run);
+#pragma unroll 1
+  for (int c = 0; c < kT; c += 32) {
+    uint32_t v[32], pk[16];
+    tmem_ld_32x32b_x32(my_s + c, v);  // (P takes the places of scores that have been read)
+    tmem_ld_wait();
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int at = ((c >> 4) + g) >> shift;
+      const float scale = pages[at].x * row_scale, up = kUp + page_log(mags[at], log_r);
+      float both = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        float p[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int col = c + g * 16 + j + k;
+          p[k] = fast_exp2(fmaf(__uint_as_float(v[g * 16 + j + k]), scale, up - m_use));
+          p[k] = col >= from && col < to ? p[k] : 0.f;
+          both += p[k];
+        }
+        pk[g * 8 + (j >> 1)] = pack_f16x2(p[0], p[1]);
+      }
+      row.l_run += both == 0.f ? 0.f : both * fast_exp2(-up);
+    }
+    tmem_st_32x32b_x16(my_s + c / 2, pk);
+    if (c & 32) {
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(p_ready + (c >> 6) * 8);
+    }
+  }
+  return row;
+}
+
 // One tile of a row: S from tensor memory, P back to its place. pages: 16 bytes for each page of the tile (key magnitude / 127, log2 of its
-// share of R plus kUp, the inverse of that power, R); shift: log2 of the 16-column groups in a page. INTERIOR: every column is seen; else
-// columns are looked at one by one only in the groups on an edge, and those that nobody sees cost nothing.
+// share of R plus kUp, the inverse of that power, R; for the second page, of which every tile has one, the smallest magnitude of values in the
+// tile instead); shift: log2 of the 16-column groups in a page. INTERIOR: every column is seen, and R is the CTA's; else columns are looked
+// at one by one only in the groups on an edge, and those that nobody sees cost nothing.
 template <int D, bool INTERIOR>
 __device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool first, const Seen& seen, float row_scale, const float4* pages,
-                                           int shift, float& m_run, float& r_run, float& l_run, uint32_t p_ready) {
+                                           const float* mags, int shift, RowState& row, uint32_t p_ready) {
+  float &m_run = row.m_run, &r_run = row.r_run, &l_run = row.l_run;
   uint32_t sc[kT];
 #pragma unroll
   for (int c = 0; c < kT; c += 32) tmem_ld_32x32b_x32(my_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sc[c]));
-  const float r_new = pages[0].w;
+  float r_new = pages[0].w;
+  if constexpr (!INTERIOR) {
+    bool own = false;
+    if (r_new > 16.f * pages[1].w)  // (the same for all threads)
+      own = r_new != r_run && (seen.to > 0 && seen.from < kT) && row_share(seen.from, seen.to, r_new, mags, shift, r_run) != r_new;
+    if (__any_sync(0xffffffffu, own)) {
+      tmem_ld_wait();
+      row = softmax_apart<D>(my_s, my_o, first, seen.from, seen.to, row_scale, pages, mags, shift, row, p_ready);
+      return;
+    }
+    if (!(seen.to > 0 && seen.from < kT)) r_new = r_run;  // what a row does not see leaves its R alone
+  }
   tmem_ld_wait();
   float mx = -INFINITY;
 #pragma unroll
@@ -197,19 +310,7 @@ __device__ __forceinline__ void softmax_i8(uint32_t my_s, uint32_t my_o, bool fi
     m_run = m_new;
     r_run = r_new;
   } else if (__any_sync(0xffffffffu, m_new > m_run + 8.f || r_new != r_run)) {
-    const float grown = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new)), corr = grown * page_share(r_run, r_new);
-    m_run = m_new;
-    r_run = r_new;
-    l_run *= grown;
-#pragma unroll
-    for (int c = 0; c < D; c += 16) {
-      uint32_t v[16];
-      tmem_ld_32x32b_x16(my_o + c, v);
-      tmem_ld_wait();
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
-      tmem_st_32x32b_x16(my_o + c, v);
-    }
+    rescale<D>(my_o, m_new, r_new, row);
   }
   const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
 #pragma unroll
@@ -264,6 +365,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sm0 = smem_u32(smem);
   float4* pages_sm = reinterpret_cast<float4*>(smem + S::kOffPages);
+  float* mags_sm = reinterpret_cast<float*>(smem + S::kOffMags);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
   // q_full, q_ready | codes_full, codes_empty [kStages] | kv_full, kv_empty [kSlots] | s_full, o_full [2] | p_ready [2][2]
   const uint32_t q_full = smem_u32(bars), q_ready = q_full + 8, codes_full = q_full + 16, codes_empty = codes_full + 8 * S::kStages,
@@ -381,13 +483,15 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const int tok = (t_begin + it) * kT + lane * a.page;
             float m = lane < ppt && tok < hi && tok + a.page > lo ? most.y : 0.f;
             m = m == m ? m : 0.f;
+            const float low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(m > 0.f || (lane < ppt && most.y == 0.f) ? m : INFINITY)));
             m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
             if (m > r_all) r_all = fminf(2.f * m, 3.3e38f);
             if (lane < ppt) {
               // (any share does for values without a magnitude: the sum of exponentials depends on the keys alone)
               const float share = most.y == most.y ? fmaxf(page_share(most.y, r_all), 0x1p-40f) : 1.f;
               if (most.y != most.y) *none_flag = 1;
-              pages_sm[(it % kRing) * 8 + lane] = make_float4(most.x * kInv127, __log2f(share) + kUp, __fdividef(0x1p-7f, share), r_all);
+              pages_sm[(it % kRing) * 8 + lane] = make_float4(most.x * kInv127, __log2f(share) + kUp, __fdividef(0x1p-7f, share), lane == 1 ? low : r_all);
+              mags_sm[(it % kRing) * 8 + lane] = most.y;
               mbar_arrive(bar);
             }
           }
@@ -471,7 +575,8 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const uint32_t lane_sel = static_cast<uint32_t>(q4 * 32) << 16;
       const uint32_t my_s = tm_s + u * kT + lane_sel, my_o = tm_o + u * D + lane_sel;
       const int shift = a.page == 16 ? 0 : a.page == 32 ? 1 : 2;
-      float m_run = -INFINITY, r_run = 0.f, l_run = 0.f, row_scale = 0.f;
+      RowState row;
+      float row_scale = 0.f;
       int failed = 0;
       if (n_tiles > 0) {
         failed = mbar_wait_bounded(q_full, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_FULL) ? 0 : 1;
@@ -483,18 +588,20 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       for (int it = 0; it < n_tiles; ++it) {
         const int key0 = (t_begin + it) * kT;
         const float4* pages = pages_sm + (it % kRing) * 8;
-        // every key is seen by every row of the unit
-        const bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
+        const float* mags = mags_sm + (it % kRing) * 8;
+        // every key is seen by every row of the unit, and no row has an R of its own (nor can it, unless a window hid keys before)
+        bool interior = key0 + kT - 1 <= pos0 + u * per_unit && (a.window <= 0 || key0 > last - a.window);
         Seen seen;
         if (!interior) seen = Seen(key_lo - key0, q_pos + 1 - key0);
+        else if (a.window > 0 && it > 0) interior = !__any_sync(0xffffffffu, row.r_run != pages_sm[((it - 1) % kRing) * 8].w);
         failed = mbar_wait_bounded(s_full + 8 * u, it & 1, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
         failed = __any_sync(0xffffffffu, failed);  // warp-uniform: the TMEM accesses below are warp-wide
         if (failed) break;
         tc_fence_after_sync();
         if (interior)
-          softmax_i8<D, true>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+          softmax_i8<D, true>(my_s, my_o, it == 0, seen, row_scale, pages, mags, shift, row, p_ready + 16 * u);
         else
-          softmax_i8<D, false>(my_s, my_o, it == 0, seen, row_scale, pages, shift, m_run, r_run, l_run, p_ready + 16 * u);
+          softmax_i8<D, false>(my_s, my_o, it == 0, seen, row_scale, pages, mags, shift, row, p_ready + 16 * u);
       }
       if (!failed && n_tiles > 0) failed = mbar_wait_bounded(o_full + 8 * u, 0, abort_flag, a.status, PXL_DEV_TIMEOUT_TMEM_FULL) ? 0 : 1;
       failed = __any_sync(0xffffffffu, failed);
@@ -508,12 +615,13 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           none = none || m != m;
         }
       }
-      const int64_t row = static_cast<int64_t>(q_begin + q0 + tok) * a.Hq + head;
+      const auto [m_run, r_run, l_run] = row;
+      const int64_t place = static_cast<int64_t>(q_begin + q0 + tok) * a.Hq + head;
       if (!failed && a.splits == 1) {
         const float sink = a.sinks && valid ? a.sinks[head] * kLog2e : -INFINITY;
         const float M = fmaxf(m_run, sink), Mu = M == -INFINITY ? 0.f : M, f = fast_exp2(m_run - Mu);
         const float denom = l_run * f + fast_exp2(sink - Mu);
-        if (a.lse && valid) a.lse[row] = denom == 0.f ? INFINITY : Mu + log2f(denom);
+        if (a.lse && valid) a.lse[place] = denom == 0.f ? INFINITY : Mu + log2f(denom);
         const float inv = none ? NAN : denom == 0.f ? 0.f : f / denom * (r_run * (kInv127 * 0x1p-7f));
         bf16* dst = a.out + static_cast<int64_t>(q_begin + q0 + tok) * a.out_stride + head * D;
         if (n_tiles > 0) tc_fence_after_sync();
@@ -538,7 +646,7 @@ attn_i8_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           }
         }
       } else if (!failed) {
-        float* po = a.parts + (split * static_cast<int64_t>(a.T) * a.Hq + row) * (D + kPartTail);
+        float* po = a.parts + (split * static_cast<int64_t>(a.T) * a.Hq + place) * (D + kPartTail);
         if (valid) *reinterpret_cast<float4*>(po + D) = make_float4(m_run, l_run, r_run, none ? 1.f : 0.f);
         if (n_tiles > 0) {
           tc_fence_after_sync();

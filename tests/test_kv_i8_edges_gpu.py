@@ -180,3 +180,39 @@ def test_keys_without_a_magnitude(new, ctx, heads):
             if b or h:
                 oracle.assert_weights(w[b, h], want[h], weights[b, h], size, new[b])
         row += new[b]
+
+
+# ------------------------------------------------------------------------------------------------ magnitudes far apart
+@pytest.mark.parametrize("big", [2.0 ** 30, 1e30, 3e38])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("new,ctx", [(200, 200), (80, 400), (80, 3000)])
+@pytest.mark.parametrize("page,D,G", [(16, 128, 4), (64, 64, 1), (32, 64, 16)])
+def test_values_that_only_other_queries_see(big, window, new, ctx, page, D, G):
+    """A page whose values are far above the others': those who do not see it have their results as exactly as ever. What is rounded to
+    f16 is a probability (relative to the row's largest) times its page's share of R times 2^7, f16 rounds by at most 2^-25 there, and R
+    is at most 16 times the largest magnitude that the row sees: keys * 2^-28 * that. (3000 tokens: keys are split over CTAs.)"""
+    g = _gen(6)
+    heads, blocks = 2, -(-ctx // page)
+    cache = oracle.make_cache(g, blocks, heads, page, D)
+    tables = oracle.tables_for(g, [ctx], page, blocks)
+    first_pos = ctx - new
+    at = (ctx - 1) // page                                 # a page that the last queries see
+    early = max(0, first_pos - window // 2) // page        # with a window: one that only the first queries see
+    cache[2][int(tables[0, at]), 0, 1] = torch.tensor(big).bfloat16().float()
+    if window:
+        cache[2][int(tables[0, early]), 1, 1] = torch.tensor(big).bfloat16().float()
+    q = torch.randn(new, G * heads, D, generator=g).bfloat16()
+    scale = D ** -0.5
+    out, _ = _attend(q, cache, tables, [new], [ctx], scale, window, max_ctx=ctx)
+    (o, mean, _, size), = oracle.attention(q, cache, tables, [new], [ctx], scale, window)
+    m = cache[2][tables[0].long()][:, :, 1].double()       # [pages, heads]
+    calm = [0, 0]
+    for i in range(new):
+        pos = first_pos + i
+        lo = max(0, pos - window + 1) // page if window else 0
+        for h in range(heads):
+            seen = float(m[lo:pos // page + 1, h].max())
+            calm[h] += seen < big / 2
+            part = slice(h * G, h * G + G)
+            oracle.assert_output(out[i:i + 1, part], o[i:i + 1, part], mean[i:i + 1, part], size, ctx * 2.0 ** -28 * seen)
+    assert min(calm) > 0
