@@ -627,7 +627,7 @@ attn_i8_weigh_kernel(const __grid_constant__ Args a, float* __restrict__ weights
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int t = t0 + j * 256;
-    if (t >= lo && t < ctx) w[t] += sum[j];
+    if (t >= lo && t < ctx) atomicAdd(w + t, sum[j]);  // (another sequence may have the slot; its own tokens get one sum each)
   }
 }
 

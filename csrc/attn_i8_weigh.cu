@@ -267,7 +267,7 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   tc_fence_before_sync();
   if (!__syncthreads_or(failed) && warp < 4 * kGroups && !(group & 1) && t < ctx) {
     total += sum_sm[(group >> 1) * 128 + r];
-    if (a.splits == 1) a.weights[(static_cast<int64_t>(slot) * a.Hkv + kvh) * a.W + t] += total;
+    if (a.splits == 1) atomicAdd(a.weights + (static_cast<int64_t>(slot) * a.Hkv + kvh) * a.W + t, total);  // (another may have the slot)
     else a.parts[((static_cast<int64_t>(split) * gridDim.z + b) * a.Hkv + kvh) * a.max_ctx + t] = total;
   }
   tc_fence_after_sync();
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) attn_i8_weigh_join_kernel(const __grid_co
   if (t >= ctx || L <= 0 || q_begin < 0 || q_begin > a.T - L || L > a.max_q_len || slot < 0 || slot >= a.slots || ctx > a.W || ctx > a.max_ctx) return;
   float sum = 0.f;
   for (int s = 0; s < a.splits; ++s) sum += a.parts[((static_cast<int64_t>(s) * gridDim.z + b) * a.Hkv + h) * a.max_ctx + t];
-  a.weights[(static_cast<int64_t>(slot) * a.Hkv + h) * a.W + t] += sum;
+  atomicAdd(a.weights + (static_cast<int64_t>(slot) * a.Hkv + h) * a.W + t, sum);
 }
 
 // CTAs that share the queries of a tile of keys: enough to fill the chip, each with at least eight units.

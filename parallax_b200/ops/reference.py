@@ -725,8 +725,8 @@ def attn_decode_i8(q, k_cache, v_cache, kv_max, block_tables, ctx_lens, scale, w
                    seq_slots=None):
     """One query per sequence, ``q [B, Hq, D]``, over an 8-bit cache (see :mod:`.kv_i8`): ``window`` keys per query (0: all), ``sinks [Hq]``
     beside them. ``max_ctx``: no sequence is longer (0: as long as the tables reach). ``weights [slots, heads, tokens]``: what the query
-    gave to each token, summed over the query heads of a key head, is added there, sequence b in slot ``seq_slots[b]`` (None: b), each in
-    one of its own."""
+    gave to each token, summed over the query heads of a key head, is added there, sequence b in slot ``seq_slots[b]`` (None: b). Sequences
+    that share a slot add up there, in any order; an eviction needs slots of their own."""
     cache = (k_cache, v_cache, kv_max)
     kv_i8.check_attention("attn_decode_i8", q, cache, block_tables, None, ctx_lens, scale, window, sinks, out, weights, seq_slots, max_ctx)
     res = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out

@@ -216,3 +216,22 @@ def test_values_that_only_other_queries_see(big, window, new, ctx, page, D, G):
             part = slice(h * G, h * G + G)
             oracle.assert_output(out[i:i + 1, part], o[i:i + 1, part], mean[i:i + 1, part], size, ctx * 2.0 ** -28 * seen)
     assert min(calm) > 0
+
+
+# ------------------------------------------------------------------------------------------------ slots that sequences share
+@pytest.mark.parametrize("new,ctx", [([1] * 200, [90] * 200), ([5] * 60, [90] * 60), ([600, 600], [700, 640])])
+def test_weights_of_sequences_in_one_slot_add_up(new, ctx):
+    g = _gen(7)
+    heads, G, D = 2, 4, 64
+    blocks = sum(-(-t // 16) for t in ctx)
+    cache = oracle.make_cache(g, blocks, heads, 16, D)
+    tables = oracle.tables_for(g, ctx, 16, blocks)
+    q = torch.randn(sum(new), G * heads, D, generator=g).bfloat16()
+    slots = _i32([1 + i % 2 for i in range(len(ctx))])
+    before = torch.rand(3, heads, max(ctx), generator=g)
+    _, w = _attend(q, cache, tables, new, ctx, 0.125, weights=before, slots=slots, max_ctx=max(ctx))
+    want, size = before.double(), 0.0
+    for b, (_, _, add, s) in enumerate(oracle.attention(q, cache, tables, new, ctx, 0.125)):
+        want[int(slots[b]), :, :ctx[b]] += add
+        size = max(size, s)
+    oracle.assert_weights(w, want, before, size, sum(new))
