@@ -676,8 +676,9 @@ def store_kv_i8(k, v, k_cache, v_cache, kv_max, block_tables, cu_q, ctx_lens, ma
     _kv_i8_new_tokens("store_kv_i8", cu_q, max_q_len)
     for b in range(B):
         row, n, t = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b]), int(ctx_lens[b])
-        for p in range((t - n) // page, (t - 1) // page + 1) if n > 0 else ():
-            lo, hi = max(0, t - n - p * page), min(page, t - p * page)
+        begin = max(0, t - n)                    # (rows of tokens before the sequence's first are left out)
+        for p in range(begin // page, (t - 1) // page + 1) if n > 0 else ():
+            lo, hi = max(0, begin - p * page), min(page, t - p * page)
             blk, r = int(block_tables[b, p]), row + p * page + lo - (t - n)
             for j, (x, cache) in enumerate(((k, k_cache), (v, v_cache))):
                 x = x[r:r + hi - lo].float().transpose(0, 1)                                  # [heads, tokens, D]

@@ -76,3 +76,16 @@ def test_a_negative_number_of_new_tokens_is_refused_by_the_library():
     assert lib.pxl_attn_i8_prefill(P, 256, P, P, P, P, P, P, P, 256, None, None, P, 1 << 30, 2, 1, -1, *sizes) == INVALID_ARG
     assert lib.pxl_attn_i8_weigh(P, 256, P, P, P, P, P, P, P, 100, 1, None, P, 1 << 30, 2, 1, -1, *sizes) == INVALID_ARG
     assert lib.pxl_attn_i8_prefill_workspace(3, 1, 0, 4, 2, 64, 4096) >= lib.pxl_attn_i8_prefill_workspace(3, 1, 1, 4, 2, 64, 4096) > 0
+
+
+# ------------------------------------------------------------------------------------------------ more new tokens than tokens
+@pytest.mark.parametrize("n,t", [(5, 3), (5, 0), (40, 20), (33, 32)])
+def test_store_of_more_new_tokens_than_tokens(n, t):
+    """Those at positions below zero are left out; nothing but the sequence's pages is written."""
+    g = torch.Generator().manual_seed(3)
+    cache = oracle.make_cache(g, 5, 2, 16, 64)
+    want = [c.clone() for c in cache]
+    tab, k, v = torch.tensor([[0, 1, 2, 3]]).int(), torch.randn(n, 2, 64, generator=g).bfloat16(), torch.randn(n, 2, 64, generator=g).bfloat16()
+    ops.store_kv_i8(k, v, *cache, tab, torch.tensor([0, n]).int(), torch.tensor([t]).int(), n)
+    ops.store_kv_i8(k[n - t:], v[n - t:], *want, tab, torch.tensor([0, t]).int(), torch.tensor([t]).int(), n)
+    assert all(torch.equal(a, b) for a, b in zip(cache, want))

@@ -235,3 +235,19 @@ def test_weights_of_sequences_in_one_slot_add_up(new, ctx):
         want[int(slots[b]), :, :ctx[b]] += add
         size = max(size, s)
     oracle.assert_weights(w, want, before, size, sum(new))
+
+
+# ------------------------------------------------------------------------------------------------ more new tokens than tokens
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_store_of_more_new_tokens_than_tokens(page):
+    g = _gen(8)
+    cache = oracle.make_cache(g, 12, 2, page, 64)
+    new, ctx = [5, 7, 90, 65], [3, 0, 70, 64]
+    tables = torch.randperm(12, generator=g).int().view(4, 3)
+    lens = _i32([min(t, 3 * page) for t in ctx])
+    x = torch.randn(sum(new), 4, 64, generator=g).bfloat16()
+    dev, xd = _dev(*cache), x.to(DEV)
+    ops.store_kv_i8(xd[:, :2], xd[:, 2:], *dev, *_dev(tables, _cu(new), lens), 90)
+    _check()
+    ops.store_kv_i8(x[:, :2], x[:, 2:], *cache, tables, _cu(new), lens, 90)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
