@@ -2,10 +2,12 @@
 //
 // A cache holds pages [blocks, Hkv, page, D] of int8 codes for K and as many for V, and kv_max fp32 [blocks, Hkv, 2]: the largest
 // magnitude m of a page's keys and of its values. A code c stands for c * (m / 127). Codes are round(127 x / m), ties to even: 127 x is
-// exact in fp32 for bf16 x and the quotient of two such numbers is no nearer than 2^-9 to a tie that it is not, so that the rounded
-// quotient gives the code of the exact one. Tokens behind a page's first may raise m; the codes that are there become
-// round(c * m_old / m_new), also from an exact product. m is NaN once a page was given a number that is not finite, until its first
-// token is written again.
+// exact in fp32 for bf16 x, and m is a bf16 number too. With x / m = X / (M 2^k), X and M whole numbers of 8 bits, the quotient is off a
+// tie j / 2 by |254 X - j M 2^k| / (2 M 2^k): not at all, or by at least 1 / (254 X + 1) > 2^-16 of the tie (16383 / 32768 for
+// x = 129 / 32768 and m = 1). The rounded quotient is off by 2^-24 of itself and gives the code of the exact one. Tokens behind a page's
+// first may raise m; the codes that are there become round(c * m_old / m_new), also from an exact product and as far from ties. m is NaN
+// once a page was given a number that is not finite, until its first token is written again. (Magnitudes of a caller's own that are no
+// bf16 numbers do as well, but for codes that are written again from within 2^-16 of a tie, which may be the neighbour of the nearest.)
 #include <atomic>
 
 #include "common.cuh"

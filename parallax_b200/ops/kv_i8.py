@@ -1,10 +1,10 @@
 """Keys and values in 8 bits with a magnitude for each page and key head: the checks that the kernels' wrappers and the CPU forms share.
 
 A cache is ``k_cache`` and ``v_cache``, int8 ``[blocks, key heads, page, D]``, and ``kv_max``, fp32 ``[blocks, key heads, 2]``: the largest
-magnitude of a page's keys and of its values. A code stands for ``code * (kv_max / 127)``. The magnitude of a page grows with what is written
-behind its first tokens (the codes that are there are rounded again) and begins anew with its first token. A page that was given a number
-that is not finite has NaN there, and gives NaN to whoever sees one of its tokens: among the keys to outputs and weights, among the values to
-outputs alone.
+magnitude of a page's keys and of its values, a bf16 number as they are. A code stands for ``code * (kv_max / 127)``. The magnitude of a page
+grows with what is written behind its first tokens (the codes that are there are rounded again) and begins anew with its first token. A page
+that was given a number that is not finite has NaN there, and gives NaN to whoever sees one of its tokens: among the keys to outputs and
+weights, among the values to outputs alone.
 """
 
 from __future__ import annotations

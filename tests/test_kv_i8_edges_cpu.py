@@ -89,3 +89,16 @@ def test_store_of_more_new_tokens_than_tokens(n, t):
     ops.store_kv_i8(k, v, *cache, tab, torch.tensor([0, n]).int(), torch.tensor([t]).int(), n)
     ops.store_kv_i8(k[n - t:], v[n - t:], *want, tab, torch.tensor([0, t]).int(), torch.tensor([t]).int(), n)
     assert all(torch.equal(a, b) for a, b in zip(cache, want))
+
+
+# ------------------------------------------------------------------------------------------------ codes next to a tie
+@pytest.mark.parametrize("x,m,want", [(129 / 32768, 1.0, 0), (1.0, 254.0, 0), (129 / 128, 254.0, 1), (3.0, 254.0, 2), (255 / 512, 127.0, 0),
+                                      (64.0, 128.0, 64), (127.0, 254.0, 64), (129 / 256, 127.0, 1)])
+def test_codes_of_numbers_next_to_a_tie(x, m, want):
+    """127 x / m: 0.49998, 0.5, 0.504, 1.5, 0.498, 63.5, 63.5, 0.504."""
+    cache = [torch.zeros(1, 1, 16, 64, dtype=torch.int8), torch.zeros(1, 1, 16, 64, dtype=torch.int8), torch.zeros(1, 1, 2)]
+    k = torch.zeros(1, 1, 64)
+    k[0, 0, :3] = torch.tensor([m, x, -x])
+    assert torch.equal(k.bfloat16().float(), k)
+    ops.store_kv_i8(k.bfloat16(), -k.bfloat16(), *cache, torch.zeros(1, 1).int(), torch.tensor([0, 1]).int(), torch.tensor([1]).int(), 1)
+    assert cache[0][0, 0, 0, :3].tolist() == [127, want, -want] and cache[1][0, 0, 0, :3].tolist() == [-127, -want, want]

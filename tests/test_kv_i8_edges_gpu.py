@@ -251,3 +251,44 @@ def test_store_of_more_new_tokens_than_tokens(page):
     _check()
     ops.store_kv_i8(x[:, :2], x[:, 2:], *cache, tables, _cu(new), lens, 90)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
+
+
+# ------------------------------------------------------------------------------------------------ codes next to a tie
+def _near_ties(M, per_page):
+    """Numbers x = X / 2^k whose 127 x / M is a tie or next to one, and their codes, in whole numbers: twice the quotient is 254 X over
+    M 2^k, and how far it is from an odd number j is |254 X - j M 2^k| / (M 2^k)."""
+    found = []
+    for k in range(-1, 10):
+        for X in range(128, 256):
+            num, den = (254 * X, M << k) if k >= 0 else (508 * X, M)
+            if num > 254 * den:
+                continue
+            j = num // den | 1
+            j = j if abs(num - j * den) <= abs(num - (j - 2) * den) else j - 2
+            off, near = num - j * den, (j - 1) // 2
+            code = near + (near & 1) if off == 0 else near + (off > 0)
+            found.append((abs(off) / den, X / 2.0 ** k, code))
+    found.sort()
+    return found[:per_page]
+
+
+def test_codes_of_numbers_next_to_a_tie():
+    """The nearest to ties, of all significands of 8 bits: 129 / 32768 of 1 is 16383 / 32768, 2^-15 below one half."""
+    assert min(abs(129 / 32768 - x / 128) for _, x, _ in _near_ties(128, 500)) == 0
+    x, want = torch.zeros(128, 16, 64), torch.zeros(128, 16, 64)
+    for i in range(128):
+        page = _near_ties(128 + i, 510)
+        v, c = torch.tensor([p[1] for p in page]), torch.tensor([float(p[2]) for p in page])
+        x[i].view(-1)[:1021] = torch.cat([torch.tensor([128.0 + i]), v, -v])
+        want[i].view(-1)[:1021] = torch.cat([torch.tensor([127.0]), c, -c])
+    x = x.flatten(0, 1)[:, None] * 2.0 ** -7
+    assert torch.equal(x.bfloat16().float(), x)
+    cache = [torch.zeros(128, 1, 16, 64, dtype=torch.int8), torch.zeros(128, 1, 16, 64, dtype=torch.int8), torch.zeros(128, 1, 2)]
+    args = (torch.arange(128).int()[None], _cu([2048]), _i32([2048]))
+    dev = _dev(*cache)
+    xd = x.bfloat16().to(DEV)
+    ops.store_kv_i8(xd, -xd, *dev, *_dev(*args), 2048)
+    _check()
+    assert torch.equal(dev[0][:, 0].cpu().float(), want) and torch.equal(dev[1][:, 0].cpu().float(), -want)
+    ops.store_kv_i8(x.bfloat16(), -x.bfloat16(), *cache, *args, 2048)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
