@@ -118,7 +118,7 @@ def check_attention(what: str, q: torch.Tensor, cache: tuple, block_tables: torc
             refuse(what, f"out has the rows of q, got {out.shape[0]} and {T}")
         if out.stride(2) != 1 or out.stride(1) != D or out.stride(0) & 7 or out.data_ptr() & 15 or T > 1 and out.stride(0) < Hq * D:
             refuse(what, "out has neighbouring heads and columns, rows that start on 16 bytes and do not overlap")
-        if T > 0 and q.stride(2) == 1 and q.stride(1) == D and _share_memory(_rows_2d(q), _rows_2d(out)):
+        if T > 0 and q.stride(2) == 1 and (q.stride(1) == D or Hq == 1) and _share_memory(_rows_2d(q), _rows_2d(out)):
             refuse(what, "out overlaps the queries")
         lo, hi = out.data_ptr(), out.data_ptr() + 2 * ((T - 1) * out.stride(0) + Hq * D)
         for t in (*cache, weights, sinks):

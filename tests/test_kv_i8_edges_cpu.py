@@ -102,3 +102,18 @@ def test_codes_of_numbers_next_to_a_tie(x, m, want):
     assert torch.equal(k.bfloat16().float(), k)
     ops.store_kv_i8(k.bfloat16(), -k.bfloat16(), *cache, torch.zeros(1, 1).int(), torch.tensor([0, 1]).int(), torch.tensor([1]).int(), 1)
     assert cache[0][0, 0, 0, :3].tolist() == [127, want, -want] and cache[1][0, 0, 0, :3].tolist() == [-127, -want, want]
+
+
+# ------------------------------------------------------------------------------------------------ results over queries
+@pytest.mark.parametrize("shift", [0, 8, 128])
+def test_results_over_the_queries_of_a_single_head_are_refused(shift):
+    """Whatever the stride of a dimension of one says."""
+    g = torch.Generator().manual_seed(4)
+    cache = oracle.make_cache(g, 4, 1, 16, 64)
+    flat = torch.randn(4 * 128, generator=g).bfloat16()
+    tab, lens = torch.zeros(3, 1).int(), torch.ones(3).int()
+    for stride in (64, 7, 3 * 128):
+        q = flat.as_strided((3, 1, 64), (128, stride, 1))
+        with pytest.raises(KernelError, match="overlaps the queries"):
+            ops.attn_decode_i8(q, *cache, tab, lens, 0.1, out=flat.as_strided((3, 1, 64), (128, 64, 1), shift))
+        ops.attn_decode_i8(q.clone(), *cache, tab, lens, 0.1, out=flat.as_strided((3, 1, 64), (128, 64, 1), 64))
