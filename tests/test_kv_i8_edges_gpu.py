@@ -292,3 +292,34 @@ def test_codes_of_numbers_next_to_a_tie():
     assert torch.equal(dev[0][:, 0].cpu().float(), want) and torch.equal(dev[1][:, 0].cpu().float(), -want)
     ops.store_kv_i8(x.bfloat16(), -x.bfloat16(), *cache, *args, 2048)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
+
+
+# ------------------------------------------------------------------------------------------------ prompts in a launch chain
+@pytest.mark.parametrize("ctx,new", [([300, 170], [90, 170]), ([4000, 2500], [30, 3])])
+def test_prompts_and_their_weights_in_a_launch_chain(ctx, new):
+    """Written, attended to, thinned out and attended to again without a wait in between; the second with keys split over CTAs."""
+    from parallax_b200.ops import cuda as cu
+
+    g = _gen(9)
+    width = -(-max(ctx) // 16)
+    cache = _dev(*oracle.make_cache(g, 2 * width + 20, 2, 16, 128))
+    tab, new_tab = _dev(torch.arange(2 * width).int().view(2, width), (torch.arange(20) + 2 * width).int().view(2, 10))
+    x = torch.randn(sum(new), 4, 128, generator=g).bfloat16().to(DEV)
+    q = torch.randn(sum(new), 8, 128, generator=g).bfloat16().to(DEV)
+    ends, lens, single = _dev(_cu(new), _i32(ctx), _i32([0, 1, 2]))
+
+    def go(cache, weights):
+        ops.store_kv_i8(x[:, :2], x[:, 2:], *cache, tab, ends, lens, max(new))
+        out = ops.attn_prefill_i8(q, *cache, tab, ends, lens, max(new), 0.1, weights=weights)
+        _, n = ops.evict_kv_i8(*cache, weights, tab, lens, new_tab, 150, 10)
+        again = ops.attn_prefill_i8(q[:2], *cache, new_tab, single, n, 1, 0.1, weights=weights)
+        return out, again, weights, *cache
+
+    want = go([c.clone() for c in cache], torch.zeros(2, 2, max(ctx), device=DEV))
+    _check()
+    for _ in range(10):
+        mine, w = [c.clone() for c in cache], torch.zeros(2, 2, max(ctx), device=DEV)
+        with cu.launch_chain():
+            got = go(mine, w)
+        _check()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
