@@ -8,9 +8,9 @@
 // magnitude so far and at most twice as much when it was chosen: an exponential is taken of the score plus log2 of the page's share of R,
 // so that what is rounded to f16 (2^-11) is the probability times the share; a factor of 2^11 keeps its bits down to 2^-25 of the row's
 // largest, and it is rounded in steps of 2^-35 below. The reference maximum may lag by 2^4 before anything is rescaled.
-// What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 297 us, 6.6 TB/s. Three CTAs per SM, since a tile's
-// products wait for its exponentials; f16 rather than 8-bit products, since q and the probabilities would lose bits. Short pairs are bound
-// by their beginning and end (203 windows of 128 keys, 64 heads of 64: 21 us).
+// What bounds it is memory: 128 sequences of up to 12000 tokens, 40 heads on 8, 305 us with the join, 6.5 TB/s (calls one behind the other 308
+// to 361 on four cards). Two to four CTAs per SM, since a tile's products wait for its exponentials; f16 rather than 8-bit products, since q
+// and the probabilities would lose bits. Short pairs are bound by their beginning and end (203 windows of 128 keys, 64 heads of 64: 22 us).
 // A pair that lies in several CTAs is added up by a second kernel; short ones are not cut, and few pairs get a cluster each, whose CTAs add
 // up from each other's shared memory (one sequence of up to 776 tokens, 32 heads of 128: 9.9 -> 6.7 us). Where the weights are wanted, the
 // scores go to the workspace (4 bytes per query head and key beside 2 D per key head) and a third kernel adds their exponentials once the sums are
@@ -633,7 +633,8 @@ attn_i8_weigh_kernel(const __grid_constant__ Args a, float* __restrict__ weights
 
 // Whether pairs are left whole, so that no second kernel has to add their parts up (4 to 7 us), although a CTA may get the tiles of almost
 // a pair more than its even share. us, cut / whole, 32 heads of 128: 8 pairs of up to 4 tiles 8.9 / 7.7, of up to 8 8.2 / 10.2; 64 pairs of up to 8
-// 11.7 / 11.3, of up to 16 14.0 / 16.4; 1624 pairs of up to 8 47.8 / 44.3, of up to 16 69.7 / 65.4.
+// 11.7 / 11.3, of up to 16 14.0 / 16.4; 1624 pairs of up to 8 47.8 / 44.3, of up to 16 69.7 / 65.4. (Heads of 64 and groups of more than 8 heads
+// have the same limits, with other CTAs per SM; there they are right by tests, not by times.)
 int most_tiles(int window, int max_ctx) {  // of a pair
   return window > 0 && window < max_ctx ? ceil_div(window - 1, kKeyTile) + 1 : ceil_div(max_ctx, kKeyTile);
 }

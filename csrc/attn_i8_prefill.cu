@@ -16,10 +16,10 @@
 // sum of a page's 16 columns is divided by the share again. Both the reference maximum (by 2^8) and R are let run ahead before O in tensor
 // memory is rescaled. R is one for the CTA, unless that is more than 16 times what a row has seen of its own (a page that only others see is far
 // above the rest): then the row keeps one for itself.
-// 8111 tokens, 32 heads, D = 128, twice: 726 us, 0.96 PFLOP/s. A tile takes 4400 clocks for both units, the chain of one unit's: product 550,
+// 8111 tokens, 32 heads, D = 128, twice: 757 us, 0.92 PFLOP/s (739 to 787 by run and card). A tile takes 4400 clocks for both units, the chain of one unit's: product 550,
 // softmax 2700, notice and issue 1000; the tensor pipe is 41 % full. Two units of 128 rows for one conversion: with one the converting warps
 // would take as long as the softmax. (Heads of 64: CTAs of one unit, two on an SM, take longer too, 288 us for 239 of 5 x 3001 tokens with
-// windows of 128, 802 for 674 of the two prompts.)
+// windows of 128, 802 for 674 of the two prompts. Since rows have an R of their own where that is needed, 238 and 677.)
 // Few rows: the keys are split over several CTAs, whose results a second kernel adds up.
 // Every wait is bounded; on expiry the kernel records a status code, all roles unwind, tensor memory is freed.
 #include <atomic>

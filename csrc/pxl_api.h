@@ -573,7 +573,7 @@ int pxl_act_rows(const void* x, int64_t ldx, int x_f32, int act, const void* tab
 // magnitude of a page's keys and of its values, on 8 bytes (for the write, on 4). A code stands for code * (kv_max / 127). Block tables
 // [B, max_blocks].
 // New tokens into the cache: rows cu_q[b] .. cu_q[b + 1] of k and v [T, Hkv, D] (heads side by side, strides in elements) are the last
-// of the ctx_lens[b] tokens of sequence b, at most max_q_len of each.
+// of the ctx_lens[b] tokens of sequence b, at most max_q_len of each: a sequence with more is reported (index) and not written.
 int pxl_kv_i8_store(const void* k, const void* v, int64_t k_stride, int64_t v_stride, const int* block_tables, const int* cu_q,
                     const int* ctx_lens, void* k_cache, void* v_cache, float* kv_max, int T, int B, int max_q_len, int Hkv, int D, int page,
                     int max_blocks, int64_t num_blocks, int* status, pxl_stream_t stream);
@@ -587,21 +587,22 @@ int pxl_kv_i8_evict(void* k_cache, void* v_cache, float* kv_max, float* weights,
                     int page, int max_blocks, int max_new, int64_t num_blocks, int keep, int recent, int first, int* status,
                     pxl_stream_t stream);
 // Attention of one query per sequence, q [B, Hq, D] (heads side by side), over the cache, no sequence longer than max_ctx. weights (null:
-// none) [slots, Hkv, W]: what a token got, summed over the query heads of its key head, is added there, a sequence's in slot
-// seq_slots[b] (null: b). workspace: as many bytes as asked for, on 16.
+// none) [slots, Hkv, W]: what a token got, summed over the query heads of its key head, is added there (atomically: sequences may share a
+// slot), a sequence's in slot seq_slots[b] (null: b). workspace: as many bytes as asked for, on 16.
 int64_t pxl_attn_i8_decode_workspace(int B, int Hq, int Hkv, int D, int max_ctx, int with_weights);
 int pxl_attn_i8_decode(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max, const int* block_tables,
                        const int* ctx_lens, void* out, int64_t out_stride, const float* sinks, float* weights, int64_t W, int slots,
                        const int* seq_slots, void* workspace, int64_t workspace_bytes, int B, int Hq, int Hkv, int D, int page, int max_blocks,
                        int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
 // The same of the queries of new tokens, rows cu_q[b] .. cu_q[b + 1] of q [T, Hq, D], the last of the ctx_lens[b] tokens of sequence b, at
-// most max_q_len of each. lse (null: not wanted) [T, Hq]: log2 of the sums of exponentials.
+// most max_q_len of each: a sequence with more, or with rows off q, is reported (index), its rows stay as they are. lse (null: not
+// wanted) [T, Hq]: log2 of the sums of exponentials.
 int64_t pxl_attn_i8_prefill_workspace(int T, int B, int max_q_len, int Hq, int Hkv, int D, int max_ctx);
 int pxl_attn_i8_prefill(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache, const float* kv_max, const int* block_tables,
                         const int* cu_q, const int* ctx_lens, void* out, int64_t out_stride, const float* sinks, float* lse, void* workspace,
                         int64_t workspace_bytes, int T, int B, int max_q_len, int Hq, int Hkv, int D, int page, int max_blocks,
                         int64_t num_blocks, float scale, int window, int max_ctx, int* status, pxl_stream_t stream);
-// What these queries gave to each token, from their sums: added to weights [slots, Hkv, W].
+// What these queries gave to each token, from their sums: added to weights [slots, Hkv, W], but for the sequences that were reported.
 int64_t pxl_attn_i8_weigh_workspace(int B, int max_q_len, int Hq, int Hkv, int max_ctx);
 int pxl_attn_i8_weigh(const void* q, int64_t q_stride, const void* k_cache, const float* kv_max, const int* block_tables, const int* cu_q,
                       const int* ctx_lens, const float* lse, float* weights, int64_t W, int slots, const int* seq_slots, void* workspace,
