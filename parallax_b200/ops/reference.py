@@ -648,9 +648,9 @@ def _kv_i8_codes(x, most):
 
 
 def _kv_i8_again(codes, old, new):
-    """Codes for another magnitude: round(code * old / new); as they are where that is none."""
+    """Codes for another magnitude: round(code * old / new); as they are where that is none, or the same."""
     c = torch.round(codes.double() * old.double() / torch.where(new > 0, new, torch.ones_like(new)).double())
-    return torch.where(new.isnan(), codes.double(), c).to(torch.int8)
+    return torch.where(new.isnan() | (new == old), codes.double(), c).to(torch.int8)
 
 
 def _kv_i8_sequence(k_cache, v_cache, kv_max, table, n):

@@ -117,3 +117,18 @@ def test_results_over_the_queries_of_a_single_head_are_refused(shift):
         with pytest.raises(KernelError, match="overlaps the queries"):
             ops.attn_decode_i8(q, *cache, tab, lens, 0.1, out=flat.as_strided((3, 1, 64), (128, 64, 1), shift))
         ops.attn_decode_i8(q.clone(), *cache, tab, lens, 0.1, out=flat.as_strided((3, 1, 64), (128, 64, 1), 64))
+
+
+# ------------------------------------------------------------------------------------------------ pages of zeros
+def test_codes_of_a_page_whose_magnitude_stays_are_left_as_they_are():
+    """Of a magnitude of zero too, where a caller's codes are any: they stand for zeros."""
+    g = torch.Generator().manual_seed(5)
+    cache = oracle.make_cache(g, 4, 2, 16, 64)
+    cache[2][0] = 0.0
+    before = [c.clone() for c in cache]
+    x, ends = torch.zeros(1, 2, 64).bfloat16(), torch.tensor([0, 1]).int()
+    ops.store_kv_i8(x, x, *cache, torch.zeros(1, 1).int(), ends, torch.tensor([6]).int(), 1)
+    for c, was in zip(cache[:2], before):
+        assert torch.equal(c[0, :, :5], was[0, :, :5]) and (c[0, :, 5] == 0).all() and torch.equal(c[0, :, 6:], was[0, :, 6:])
+    ops.evict_kv_i8(*cache, torch.rand(1, 2, 16, generator=g), torch.zeros(1, 1).int(), torch.tensor([16]).int(), torch.ones(1, 1).int(), 16, 2)
+    assert torch.equal(cache[0][1], cache[0][0]) and torch.equal(cache[1][1], cache[1][0]) and (cache[2][1] == 0).all()

@@ -323,3 +323,20 @@ def test_prompts_and_their_weights_in_a_launch_chain(ctx, new):
             got = go(mine, w)
         _check()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ pages of zeros
+def test_codes_of_a_page_whose_magnitude_stays_are_left_as_they_are():
+    """Of a magnitude of zero too: by the write and by the eviction, as the CPU forms have it."""
+    g = _gen(10)
+    cache = oracle.make_cache(g, 8, 2, 32, 128)
+    cache[2][0] = cache[2][1, 0] = 0.0
+    dev = _dev(*cache)
+    x, ends, lens = torch.zeros(1, 2, 128).bfloat16(), _i32([0, 1]), _i32([40])
+    tab, new_tab, weights = _i32([[1, 0]]), _i32([[2, 3]]), torch.rand(1, 2, 40, generator=g)
+    d = _dev(x, tab, ends, lens, weights, new_tab)
+    for c, a in ((dev, d), (cache, [x, tab, ends, lens, weights, new_tab])):
+        ops.store_kv_i8(a[0], a[0], *c, *a[1:4], 1)
+        ops.evict_kv_i8(*c, a[4], a[1], a[3], a[5], 35, 3)
+    _check()
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
