@@ -2,8 +2,8 @@
 // queries that see it, and over the query heads of its key head, of exp(score - log of the query's sum), on the 5th-generation tensor cores.
 //
 // A CTA has 256 keys of a key head, as two A operands: a key is a lane of tensor memory, and its sum stays in one thread's register, with no
-// exchange between threads. Its codes become bf16 once (exactly); the queries stream through as they are, 128 / G tokens of G heads at a
-// time:
+// exchange between threads. Its codes become bf16 once (exactly), times the power of two in its page's magnitude and the softmax scale, so that
+// the products are of the scores' size whatever that of the queries; these stream through as they are, 128 / G tokens of G heads at a time:
 //   warp 16   : TMA producer, a ring of query boxes, and their rows' logarithms beside them
 //   warp 17   : MMA issuer, S = K Q^T into two TMEM buffers of 128 columns for each 128 keys
 //   warps 0-15: four groups of four, each with a buffer of its own: 128 exponentials per key and unit, 16 columns at a time with the next
@@ -56,8 +56,14 @@ struct Args {
   int* status;
 };
 
-__device__ __forceinline__ uint32_t codes_bf16x2(uint32_t four, int at) {
-  return pack_bf16x2(static_cast<int8_t>(four >> (8 * at)), static_cast<int8_t>(four >> (8 * at + 8)));
+__device__ __forceinline__ uint32_t codes_bf16x2(uint32_t four, int at, float unit) {
+  return pack_bf16x2(static_cast<int8_t>(four >> (8 * at)) * unit, static_cast<int8_t>(four >> (8 * at + 8)) * unit);
+}
+// the power of two in what a code is multiplied by (within 2^100 of 1: 2^7 times it, and its inverse, are numbers), and the inverse of that
+__device__ __forceinline__ float unit_of(float factor, float& inverse) {
+  const uint32_t e = min(max(__float_as_uint(factor) >> 23 & 255u, 27u), 227u);
+  inverse = __uint_as_float((254u - e) << 23);
+  return __uint_as_float(e << 23);
 }
 
 template <int D>
@@ -125,12 +131,16 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const int r = i / (D / 16), c = i % (D / 16);
     const int64_t head = head_of(key0 + r);
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (head >= 0) x = *reinterpret_cast<const uint4*>(a.k_cache + (head * a.page + (key0 + r) % a.page) * D + c * 16);
+    float unit = 0.f, inverse;
+    if (head >= 0) {
+      x = *reinterpret_cast<const uint4*>(a.k_cache + (head * a.page + (key0 + r) % a.page) * D + c * 16);
+      unit = unit_of(a.kv_max[head].x * kInv127 * a.scale_log2, inverse);
+    }
     const uint32_t w[4] = {x.x, x.y, x.z, x.w}, at = sm0 + (r / kM) * S::kTile + (c >> 2) * kHalf + r % kM * 128;
 #pragma unroll
     for (int p = 0; p < 2; ++p)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 3) * 2 + p) ^ (r & 7)) << 4)), "r"(codes_bf16x2(w[2 * p], 0)),
-                   "r"(codes_bf16x2(w[2 * p], 2)), "r"(codes_bf16x2(w[2 * p + 1], 0)), "r"(codes_bf16x2(w[2 * p + 1], 2))
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 3) * 2 + p) ^ (r & 7)) << 4)), "r"(codes_bf16x2(w[2 * p], 0, unit)),
+                   "r"(codes_bf16x2(w[2 * p], 2, unit)), "r"(codes_bf16x2(w[2 * p + 1], 0, unit)), "r"(codes_bf16x2(w[2 * p + 1], 2, unit))
                    : "memory");
   }
   for (int i = threadIdx.x; i < kUnits * (D / 64) * (kCols - per_unit * G) * 8; i += kThreads) {
@@ -206,7 +216,9 @@ attn_i8_weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   int failed = 0;
   if (warp < 4 * kGroups) {
     const int64_t head = head_of(t);
-    const float scale = head >= 0 ? a.kv_max[head].x * kInv127 * a.scale_log2 : 0.f;
+    float scale = head >= 0 ? a.kv_max[head].x * kInv127 * a.scale_log2 : 0.f, inverse;  // what the power of two leaves of it
+    unit_of(scale, inverse);
+    scale *= inverse;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint64_t scale2 = pair2(scale, scale);
     for (int i = group & 1; i < n_units; i += 2) {

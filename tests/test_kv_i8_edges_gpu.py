@@ -340,3 +340,25 @@ def test_codes_of_a_page_whose_magnitude_stays_are_left_as_they_are():
         ops.evict_kv_i8(*c, a[4], a[1], a[3], a[5], 35, 3)
     _check()
     assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, cache))
+
+
+# ------------------------------------------------------------------------------------------------ numbers of any size
+@pytest.mark.parametrize("queries,keys", [(118, 0), (-118, 0), (120, -120), (-100, 100), (60, 40)])
+@pytest.mark.parametrize("new,ctx", [([1, 1], [300, 65]), ([70, 9], [300, 65]), ([20], [3000])])
+def test_weights_of_queries_and_keys_of_any_size(queries, keys, new, ctx):
+    """Scores of ordinary size from numbers that are not."""
+    g = _gen(11)
+    blocks = sum(-(-t // 16) for t in ctx)
+    cache = oracle.make_cache(g, blocks, 2, 16, 128)
+    cache[2][..., 0] *= 2.0 ** keys
+    tables = oracle.tables_for(g, ctx, 16, blocks)
+    q = (torch.randn(sum(new), 6, 128, generator=g) * 2.0 ** queries).bfloat16()
+    weights, scale = torch.rand(len(ctx), 2, max(ctx), generator=g), 0.125 * 2.0 ** -(queries + keys)
+    out, w = _attend(q, cache, tables, new, ctx, scale, weights=weights, max_ctx=max(ctx))
+    row = 0
+    for b, (o, mean, add, size) in enumerate(oracle.attention(q, cache, tables, new, ctx, scale)):
+        oracle.assert_output(out[row:row + new[b]], o, mean, size)
+        want = weights[b].double()
+        want[:, :ctx[b]] += add
+        oracle.assert_weights(w[b], want, weights[b], size, new[b])
+        row += new[b]
